@@ -11,6 +11,7 @@ import re
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "include", "mkda.h")
+BLOCK_HEADER = os.path.join(HERE, "..", "include", "mkda_block.h")      # the operators around the layer
 ENTRY_POINTS = (
     "mkda_gate_cumsum_fwd", "mkda_gate_bwd", "mkda_reduce_partials", "mkda_reduce_multi", "mkda_step_fwd", "mkda_chain_fwd", "mkda_l2norm_rstd", "mkda_intra_fwd",
     "mkda_recur_fwd", "mkda_out_fwd", "mkda_epilogue_bwd", "mkda_epilogue_bwd_tiles", "mkda_bwd_dh", "mkda_bwd_chunk",
@@ -19,6 +20,8 @@ ENTRY_POINTS = (
 # with more arguments than the struct and the stream: the order of the segments, a second struct, dO, dq and dk as rows
 LONGER_ENTRY_POINTS = {"mkda_recur_fwd_ordered": 3, "mkda_chain_fwd_ordered": 3, "mkda_bwd_dh_ordered": 3, "mkda_gate_intra_fwd": 3, "mkda_bwd_dh_rows": 3,
                        "mkda_bwd_chunk_rows": 5}
+BLOCK_ENTRY_POINTS = ("mkda_conv_fwd", "mkda_conv_bwd", "mkda_conv_step", "mkda_scan_fwd", "mkda_scan_bwd", "mkda_scan_step", "mkda_norm_fwd",
+                      "mkda_norm_bwd", "mkda_sum_rows")
 ENUMS = {}
 STRUCTS = {}
 
@@ -45,6 +48,8 @@ def _parse_header(path=HEADER):
             count = int(m.group(3) or 0)
             if "*" in ctype_s:
                 ct = ctypes.c_void_p
+            elif ctype_s == "long long":
+                ct = ctypes.c_longlong
             elif ctype_s == "int":
                 ct = ctypes.c_int
             elif ctype_s == "float":
@@ -52,7 +57,7 @@ def _parse_header(path=HEADER):
             elif ctype_s in STRUCTS:
                 ct = STRUCTS[ctype_s]
             else:
-                raise RuntimeError(f"mkda.h: cannot map type {ctype_s!r} of field {fname}")
+                raise RuntimeError(f"{os.path.basename(path)}: cannot map type {ctype_s!r} of field {fname}")
             fields.append((fname, ct * count if count else ct))
         STRUCTS[name] = type(name, (ctypes.Structure,), {"_fields_": fields})
         order.append(name)
@@ -60,6 +65,7 @@ def _parse_header(path=HEADER):
 
 
 STRUCT_ORDER = _parse_header()
+BLOCK_STRUCT_ORDER = _parse_header(BLOCK_HEADER)
 globals().update(ENUMS)
 
 
@@ -81,15 +87,17 @@ def load():
         raise MkdaError(f"{path} is missing: build it with `python -m mogankda_b200.build` (no CPU or library fallback exists)")
     lib = ctypes.CDLL(path)
     lib.mkda_last_error.restype = ctypes.c_char_p
-    for name in (*ENTRY_POINTS, *LONGER_ENTRY_POINTS):
+    for name in (*ENTRY_POINTS, *LONGER_ENTRY_POINTS, *BLOCK_ENTRY_POINTS):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p] * LONGER_ENTRY_POINTS.get(name, 2)
-    n = len(STRUCT_ORDER)
-    sizes = (ctypes.c_int * n)()
-    cnt = lib.mkda_struct_sizes(sizes, n)
-    if cnt != n or any(sizes[i] != ctypes.sizeof(STRUCTS[s]) for i, s in enumerate(STRUCT_ORDER)):
-        raise MkdaError(f"{path} does not match include/mkda.h (struct sizes differ): rebuild with `python -m mogankda_b200.build --force`")
+    for order, sizes_of, header in ((STRUCT_ORDER, lib.mkda_struct_sizes, HEADER), (BLOCK_STRUCT_ORDER, lib.mkda_block_struct_sizes, BLOCK_HEADER)):
+        n = len(order)
+        sizes = (ctypes.c_int * n)()
+        cnt = sizes_of(sizes, n)
+        if cnt != n or any(sizes[i] != ctypes.sizeof(STRUCTS[s]) for i, s in enumerate(order)):
+            raise MkdaError(f"{path} does not match include/{os.path.basename(header)} (struct sizes differ): rebuild with "
+                            "`python -m mogankda_b200.build --force`")
     _libs[variant] = lib
     return lib
 

@@ -14,8 +14,9 @@ import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ("host.cu", "entry.cu", "prologue.cu", "combine.cu", "step.cu", "selftest.cu", "tc_chunk.cu", "tc_recur.cu", "tc_intra.cu", "tc_bwd_chunk.cu")
-HOST_SOURCES = ("layer.cpp", "binding.cpp")
+SOURCES = ("host.cu", "entry.cu", "prologue.cu", "combine.cu", "step.cu", "selftest.cu", "tc_chunk.cu", "tc_recur.cu", "tc_intra.cu", "tc_bwd_chunk.cu",
+           "conv.cu", "scan.cu", "norm.cu")
+HOST_SOURCES = ("layer.cpp", "binding.cpp", "block.cpp")
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-w"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Wno-deprecated-gpu-targets"]
@@ -36,7 +37,7 @@ def build(force=False, verbose=False):
     """Compiles (only what is stale) and links; returns the library path."""
     nvcc = os.environ.get("NVCC", "nvcc")
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
-    headers.append(os.path.join(HERE, "..", "include", "mkda.h"))
+    headers += [os.path.join(HERE, "..", "include", h) for h in ("mkda.h", "mkda_block.h")]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     jobs, objs = [], []

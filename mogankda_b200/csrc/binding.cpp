@@ -6,11 +6,9 @@
 // differentiation are seen to below.
 #include <Python.h>
 
-#include "layer.h"
+#include "binding.h"
 
 #include <c10/cuda/CUDAGuard.h>
-#include <pybind11/pybind11.h>
-#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/edge.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -27,24 +25,6 @@ using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 namespace {
-
-// An error of the library is a mogankda_b200._lib.MkdaError, in the forward call and out of the autograd engine.  Called without the GIL.
-template <typename F>
-auto library_call(F f) {
-    try {
-        return f();
-    } catch (const LibraryError& e) {
-        pybind11::gil_scoped_acquire gil;
-        PyObject* mod = PyImport_ImportModule("mogankda_b200._lib");
-        PyObject* type = mod ? PyObject_GetAttrString(mod, "MkdaError") : nullptr;
-        if (type) PyErr_SetString(type, e.what());
-        Py_XDECREF(type);
-        Py_XDECREF(mod);
-        python_error err;
-        err.persist();
-        throw err;
-    }
-}
 
 // Inputs and intermediates are saved as variables: in-place changes are detected, a second backward pass is refused once the buffers are gone,
 // and saved-tensor hooks (activation checkpointing, offloading) get all of it.  The blocks that hold the intermediates may come back from a hook
@@ -108,20 +88,6 @@ struct DeltaRuleBackward : public torch::autograd::Node {
         return out;
     }
 };
-
-PyObject* fail(PyObject* type, const std::string& msg) {
-    PyErr_SetString(type, msg.c_str());
-    return nullptr;
-}
-#define REQUIRE(cond, msg) do { if (!(cond)) return fail(PyExc_AssertionError, msg); } while (0)
-
-bool tensor_arg(PyObject* o, Tensor& t) {
-    if (o == Py_None) return true;
-    if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "expected a tensor, got %s", Py_TYPE(o)->tp_name); return false; }
-    t = THPVariable_Unpack(o);
-    return true;
-}
-const char NEED_CUDA[] = "mogankda_b200 kernels need CUDA tensors (there is no CPU fallback)";
 
 // check(q, k, v, g, beta, initial_state, cu_seqlens) -> (B, T, HV, device index); raises what the call has to raise
 PyObject* check(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -280,6 +246,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "host path of a layer call
 PyMODINIT_FUNC PyInit__host() {
 #define MKDA_SIZE(S) (int)sizeof(S),
     const int built[] = {MKDA_STRUCTS(MKDA_SIZE)};
+    const int built_block[] = {MKDA_BLOCK_STRUCTS(MKDA_SIZE)};
     constexpr int n = sizeof(built) / sizeof(built[0]);
     int have[n];
     if (mkda_struct_sizes(have, n) != n || !std::equal(have, have + n, built)) {
@@ -287,5 +254,17 @@ PyMODINIT_FUNC PyInit__host() {
                                            "`python -m mogankda_b200.build --force`");
         return nullptr;
     }
-    return PyModule_Create(&module);
+    constexpr int nb = sizeof(built_block) / sizeof(built_block[0]);
+    int have_block[nb];
+    if (mkda_block_struct_sizes(have_block, nb) != nb || !std::equal(have_block, have_block + nb, built_block)) {
+        PyErr_SetString(PyExc_ImportError, "_host.so and libmkda.so were built from different include/mkda_block.h (struct sizes differ): rebuild with "
+                                           "`python -m mogankda_b200.build --force`");
+        return nullptr;
+    }
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddFunctions(m, block_methods) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
 }

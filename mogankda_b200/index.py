@@ -165,3 +165,34 @@ def get_layout(B, T, cu_seqlens, device, seg_chunks=0, auto_heads=0, cost_ratio=
             _cache.pop(0)
         _cache.append((key, cu_seqlens, ver, lay))
     return lay
+
+
+@dataclass
+class Bounds:
+    """Packed sequences as the operators around the layer take them: boundaries, first checkpoint of a scan and order, longest first."""
+    table: torch.Tensor         # int32: cu [N+1], first checkpoints [N], order [N]
+    dims: tuple                 # (N, covers_all, some sequence is empty, checkpoints)
+
+
+def bounds_table(T, cu, step):
+    """(table as a list, dims); ``cu`` is a list of ints, ``step`` the tokens per checkpoint."""
+    if len(cu) < 1 or cu[0] != 0 or any(cu[i + 1] < cu[i] for i in range(len(cu) - 1)) or cu[-1] > T:
+        raise ValueError("cu_seqlens must start at 0, be non-decreasing and end within T")
+    lens = np.diff(np.array(cu, dtype=np.int64))
+    first = np.concatenate([[0], np.cumsum(-(-lens // step))])
+    table = cu + first[:-1].tolist() + np.argsort(-lens, kind="stable").tolist()
+    return table, (len(lens), int(cu[-1] == T), int(bool((lens == 0).any())), int(first[-1]))
+
+
+def get_bounds(T, cu_seqlens, device):
+    """Cached like ``get_layout``; a miss reads ``cu_seqlens`` back to the host."""
+    key, ver = ("bounds", T, device), cu_seqlens._version
+    b = _cached(key, cu_seqlens, ver)
+    if b is None:
+        table, dims = bounds_table(T, [int(x) for x in cu_seqlens.tolist()], ENUMS["MKDA_SCAN_CHECKPOINT"])
+        b = Bounds(torch.tensor(table, dtype=torch.int32, device=device), dims)
+        with _cache_lock:
+            if len(_cache) >= _CACHE_MAX:
+                _cache.pop(0)
+            _cache.append((key, cu_seqlens, ver, b))
+    return b
