@@ -50,10 +50,11 @@ typedef struct {
     const void* dlast;         /* [N,W-1,D] or NULL */
     void* dx;                  /* [TT,D] */
     void* dstate;              /* [N,W-1,D] or NULL */
-    int part_rows;             /* R >= 1: the tokens are cut into R runs, each with a row of partial sums */
+    int part_rows;             /* R, what mkda_conv_bwd_part_rows says: the tokens are cut into R runs, each with a row of partial sums */
     float* part;               /* [R][W+1][D]: of the weight's W columns, then of the bias */
 } MkdaConvBwd;
 int mkda_conv_bwd(const MkdaConvBwd* p, void* stream);
+int mkda_conv_bwd_part_rows(int TT, int D);
 
 /* One token of each of N sequences; the state is shifted in place. */
 typedef struct {
@@ -109,7 +110,7 @@ typedef struct {
 } MkdaScanStep;
 int mkda_scan_step(const MkdaScanStep* p, void* stream);
 
-/* s = x + residual, held in the residual's type; y = s / sqrt(mean s^2 + eps) * weight, rows of `width` channels.
+/* s = x + residual, held in the residual's type, which is x's or fp32; y = s / sqrt(mean s^2 + eps) * weight, rows of `width` channels.
  * Without a residual s = x.  out_e4m3: y leaves as e4m3 with scales such that a row (group = 0) or each `group` = 128 channels of it reach 448. */
 typedef struct {
     int rows; int width; int dtype; int res_dtype; float eps;
@@ -124,13 +125,13 @@ typedef struct {
 int mkda_norm_fwd(const MkdaNormFwd* p, void* stream);
 
 typedef struct {
-    int rows; int width; int dtype; int res_dtype; float eps;
-    const void* s; long long s_stride; int s_dtype;       /* what was normalised */
+    int rows; int width; int dtype; float eps;
+    const void* s; long long s_stride; int s_dtype;       /* what was normalised, in dtype or fp32 */
     const void* weight; int weight_dtype;
     const void* dy;            /* [rows,width] in dtype, contiguous */
-    const void* dsum;          /* [rows,width] in res_dtype, or NULL */
+    const void* dsum;          /* [rows,width] in s_dtype, or NULL */
     void* dx;                  /* [rows,width] in dtype */
-    void* dres;                /* [rows,width] in res_dtype, or NULL */
+    void* dres;                /* [rows,width] in s_dtype, or NULL */
     int part_rows;             /* what mkda_norm_bwd_part_rows says */
     float* part;               /* [part_rows,width] partial sums of the weight's gradient, or NULL */
 } MkdaNormBwd;

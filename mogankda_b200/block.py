@@ -68,7 +68,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, *, 
 
 def rms_norm(x, weight=None, *, residual=None, eps=1e-6, out_dtype=None, scale_group=None):
     """RMS norm of the rows of x [..,H], H up to 32768: ``y = s / sqrt(mean s^2 + eps) * weight`` with s = x, or with ``residual`` s = x + residual as the
-    residual's type holds it (the residual stream may be wider than x).  Statistics in 32 bits, y rounded once.
+    residual's type holds it (that of x, or float32).  Statistics in 32 bits, y rounded once.
 
     Returns y; with ``residual`` ``(y, s)``.  ``out_dtype=torch.float8_e4m3fn`` returns ``(y8, scale)`` or ``(y8, scale, s)``: y8 * scale is y, with one scale
     per row ([..,1]) or with ``scale_group=128`` per 128 channels ([..,H/128]), max |y| / 448 (at least 2^-126); it has no gradient."""

@@ -217,8 +217,7 @@ variable_list conv_backward(const Sequences& q, int silu, const variable_list& s
     const int64_t D = w.size(0), W = w.size(1), TT = q.s.TT;
     const Tensor dy = grads[0].defined() ? aligned(grads[0]) : at::zeros_like(x0, at::MemoryFormat::Contiguous);
     const Tensor dlast = grads.size() > 1 && grads[1].defined() ? aligned(grads[1]) : Tensor();
-    // runs of tokens: two blocks per SM and more, at least 16 tokens (each run reads W - 1 rows on both sides again, and leaves a row of sums)
-    const int64_t blocks = (D + 511) / 512, run = std::max<int64_t>(16, (TT * blocks + 8 * sms() - 1) / (8 * sms())), rows = std::max<int64_t>(1, (TT + run - 1) / run);
+    const int64_t rows = mkda_conv_bwd_part_rows((int)TT, (int)D);
     const Tensor part = new_cuda({rows, (W + 1) * D}, at::kFloat, x0.device());
     variable_list out(4);
     out[0] = out_like(x0, q.covers_all);
@@ -546,7 +545,7 @@ variable_list norm_backward(double eps, at::ScalarType dt, bool residual, at::Sc
         if (need(1)) part = new_cuda({mkda_norm_bwd_part_rows((int)rows, (int)H), H}, at::kFloat, dev);
     }
     MkdaNormBwd p{};
-    p.rows = (int)rows; p.width = (int)H; p.dtype = dtype_code(out[0]); p.res_dtype = residual ? dtype_code(out[2]) : MKDA_F32; p.eps = (float)eps;
+    p.rows = (int)rows; p.width = (int)H; p.dtype = dtype_code(out[0]); p.eps = (float)eps;
     p.s = r.t.data_ptr(); p.s_stride = r.stride; p.s_dtype = dtype_code(r.t); p.weight = cptr(wc); p.weight_dtype = w.defined() ? dtype_code(w) : MKDA_F32;
     p.dy = dy.data_ptr(); p.dsum = cptr(dsum); p.dx = out[0].data_ptr(); p.dres = residual && res_dt != dt ? out[2].data_ptr() : nullptr;
     p.part_rows = part.defined() ? (int)part.size(0) : 0; p.part = fmptr(part);
@@ -572,7 +571,8 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     REQUIRE(H >= 1 && H <= MKDA_NORM_MAX_WIDTH, "rows of 1 to 32768 channels");
     REQUIRE(rows <= MOST_TOKENS, "less than 2^31 rows");
     REQUIRE(!w.defined() || (w.dim() == 1 && w.size(0) == H && float_type(w)), "weight must be [H]");
-    REQUIRE(!res.defined() || (res.sizes() == x.sizes() && float_type(res)), "residual must have the shape of x");
+    REQUIRE(!res.defined() || res.sizes() == x.sizes(), "residual must have the shape of x");
+    REQUIRE(!res.defined() || res.scalar_type() == x.scalar_type() || res.scalar_type() == at::kFloat, "residual must have the type of x, or be float32");
     const double eps = PyFloat_AsDouble(a[3]);
     const int e4m3 = PyObject_IsTrue(a[4]), group = (int)PyLong_AsLong(a[5]);
     if (PyErr_Occurred()) return nullptr;

@@ -60,7 +60,7 @@ __device__ __forceinline__ int sequence_of(const MkdaSeqs& s, int t) {
     return lo;
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Calls f with the dtype as a compile-time constant; false for another one.
 template <typename F>
 inline bool with_dtype(int dtype, F f) {

@@ -76,7 +76,7 @@ def test_entry_points_refuse_without_launching(lib):
     conv = [("W", 1), ("W", 5), ("D", 0), ("dtype", 3), ("dtype", -1), ("weight", 0)]
     seqs = [("S.N", 3), ("S.T", -1)]
     for name, struct, ptrs, more in (("mkda_conv_fwd", "MkdaConvFwd", ("x", "weight", "y"), [("x", 0), ("y", 0)]),
-                                     ("mkda_conv_bwd", "MkdaConvBwd", ("x", "weight", "dy", "dx", "part"), [("dy", 0), ("dx", 0), ("part", 0), ("part_rows", 0), ("part_rows", 65536)])):
+                                     ("mkda_conv_bwd", "MkdaConvBwd", ("x", "weight", "dy", "dx", "part"), [("dy", 0), ("dx", 0), ("part", 0), ("part_rows", 0), ("part_rows", 2)])):
         p = _filled(S[struct](), ptrs, D=8, W=4, dtype=1, x_stride=8)
         p.S.TT, p.S.N, p.S.T = 4, 2, 2
         if struct == "MkdaConvBwd":
@@ -98,7 +98,7 @@ def test_entry_points_refuse_without_launching(lib):
     p = _filled(S["MkdaNormFwd"](), ("x", "y"), rows=2, width=64, dtype=1, x_stride=64)
     _refused(lib, "mkda_norm_fwd", p, [("x", 0), ("y", 0), ("residual", 0x30000), ("out_e4m3", 1), ("width", 0), ("width", 32769), ("rows", -1), ("dtype", 9), ("group", 64), ("group", 128)])
     p = _filled(S["MkdaNormBwd"](), ("s", "dy", "dx"), rows=2, width=64, dtype=1, s_dtype=1, s_stride=64)
-    _refused(lib, "mkda_norm_bwd", p, [("s", 0), ("dy", 0), ("dx", 0), ("width", 0), ("dtype", 9), ("s_dtype", -1), ("part", 0x30000)])
+    _refused(lib, "mkda_norm_bwd", p, [("s", 0), ("dy", 0), ("dx", 0), ("width", 0), ("dtype", 9), ("s_dtype", -1), ("s_dtype", 2), ("part", 0x30000)])
     p = S["MkdaSumRows"]()
     j = p.job[0]
     j.out, j.rows, j.groups, j.pitch, j.cols, j.inner, j.valid = 0x30000, 2, 1, 8, 8, 8, 8

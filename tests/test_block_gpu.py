@@ -543,7 +543,8 @@ def test_refusals_on_the_gpu():
         (AssertionError, lambda: mk.selective_scan(x, x, A, bc, bc, initial_state=torch.zeros(2, 16, 8, device="cuda").bfloat16())),
         (TypeError, lambda: mk.selective_scan(x, None, A, bc, bc)), (TypeError, lambda: mk.selective_scan_step(x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], None)),
         (AssertionError, lambda: mk.selective_scan_step(x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], torch.zeros(2, 16, 8, device="cuda").bfloat16())),
-        (AssertionError, lambda: mk.rms_norm(x, w)), (AssertionError, lambda: mk.rms_norm(x, residual=x[:1])), (ValueError, lambda: mk.rms_norm(x, out_dtype=torch.float16)),
+        (AssertionError, lambda: mk.rms_norm(x, w)), (AssertionError, lambda: mk.rms_norm(x, residual=x[:1])), (AssertionError, lambda: mk.rms_norm(x, residual=x.bfloat16())),
+        (AssertionError, lambda: mk.rms_norm(x.half(), residual=x.bfloat16())), (ValueError, lambda: mk.rms_norm(x, out_dtype=torch.float16)),
         (ValueError, lambda: mk.rms_norm(x, scale_group=128)), (AssertionError, lambda: mk.rms_norm(x, out_dtype=torch.float8_e4m3fn, scale_group=128)),
         (ValueError, lambda: mk.rms_norm(x, out_dtype=torch.float8_e4m3fn, scale_group=64)), (AssertionError, lambda: mk.rms_norm(torch.zeros(1, 32769, device="cuda"))),
         (RuntimeError, lambda: mk.rms_norm(x.clone().requires_grad_(True), out_dtype=torch.float8_e4m3fn)),
