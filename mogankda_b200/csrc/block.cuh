@@ -43,6 +43,68 @@ __device__ __forceinline__ void store8(void* base, size_t idx, int valid, bool v
     }
 }
 
+// The same for four elements, 8-byte (fp32: 16-byte) accesses
+template <int DT>
+struct alignas(DT == MKDA_F32 ? 16 : 8) Raw4 { uint32_t w[DT == MKDA_F32 ? 4 : 2]; };
+template <int DT>
+__device__ __forceinline__ Raw4<DT> load4(const void* base, size_t idx, int valid, bool vec) {
+    Raw4<DT> r;
+#pragma unroll
+    for (uint32_t& w : r.w) w = 0u;
+    if (valid <= 0) return r;
+    if (vec) {
+        if constexpr (DT == MKDA_F32) {
+            const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const float*>(base) + idx);
+            r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + idx);
+            r.w[0] = v.x; r.w[1] = v.y;
+        }
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = e >= valid ? 0u : DT == MKDA_F32 ? static_cast<const uint32_t*>(base)[idx + e] : static_cast<const uint16_t*>(base)[idx + e];
+        if constexpr (DT == MKDA_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.w[e] = w[e];
+        } else {
+            r.w[0] = w[0] | w[1] << 16;
+            r.w[1] = w[2] | w[3] << 16;
+        }
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void unpack4(const Raw4<DT>& r, float (&v)[4]) {
+    if constexpr (DT == MKDA_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(r.w[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if constexpr (DT == MKDA_BF16) {
+                v[2 * e] = __uint_as_float(r.w[e] << 16);
+                v[2 * e + 1] = __uint_as_float(r.w[e] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[e]));
+                v[2 * e] = f.x; v[2 * e + 1] = f.y;
+            }
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* base, size_t idx, int valid, bool vec, const float (&v)[4]) {
+    if (valid <= 0) return;
+    if (vec) {
+        st4(base, DT, idx, make_float4(v[0], v[1], v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < valid) st1(base, DT, idx + e, v[e]);
+    }
+}
+
 struct Span { int start, end; };
 __device__ __forceinline__ Span sequence(const MkdaSeqs& s, int n) {
     if (!s.cu) return Span{n * s.T, (n + 1) * s.T};

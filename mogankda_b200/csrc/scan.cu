@@ -97,167 +97,208 @@ __device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB)
     return Channels{g, g * per + b * CB, min(CB, per - b * CB)};
 }
 
-template <int DT, int LPC, int CPT>
-__global__ void __launch_bounds__(SCAN_THREADS) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
+// Forward.  Four warps walk the recurrence and four beside them do the elementwise part, a tile ahead (loads, softplus) and a tile behind (skip, gate, stores); the block's
+// barrier joins them once a tile.  A channel's chain is short and there are few warps of it (4096 channels are 512), so what counts is how many cycles a token takes a warp that
+// has a scheduler to itself: with the elementwise part in the same warps 168, of which 32 are the exponentials of the special function unit.
+constexpr int SCAN_HELPERS = 256;
+template <int LPC, int TILE>
+struct ScanFwdShared {
+    using Sh = ScanShape<LPC, 1, TILE>;
+    float2 d[2][TILE][Sh::CB];             // d, d x
+    float B[2][TILE][Sh::NP], C[2][TILE][Sh::NP], y[2][TILE][Sh::YROW];
+};
+
+template <int DT, int LPC>
+__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
     follow_stream();
     constexpr int TILE = 32;
-    using Sh = ScanShape<LPC, CPT, TILE>;
-    constexpr int NP = Sh::NP, CB = Sh::CB, ROW = Sh::ROW, PIECES = Sh::PIECES, BC = Sh::BC, YROW = Sh::YROW;
-    __shared__ __align__(16) float2 s_d[TILE][CB];         // d, d x
-    __shared__ __align__(16) float s_B[TILE][NP], s_C[TILE][NP], s_y[TILE][YROW];
-    __shared__ __align__(16) float s_bias[CB], s_skip[CB];
-    const int tid = threadIdx.x, D = p.D, NST = p.NST;
+    using Sh = ScanShape<LPC, 1, TILE>;
+    constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    auto& sh = *reinterpret_cast<ScanFwdShared<LPC, TILE>*>(raw_shared);
+    const int D = p.D, NST = p.NST;
     const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
-    for (int c = tid; c < CB; c += SCAN_THREADS) {
-        s_bias[c] = p.dt_bias && c < cs.count ? p.dt_bias[cs.first + c] : 0.f;
-        s_skip[c] = p.skip && c < cs.count ? p.skip[cs.first + c] : 0.f;
-    }
-    // layout of the recurrence
-    const int q = tid % LPC, c0 = tid / LPC * CPT, n0 = 4 * q;
-    f32x2 A[CPT][2], h[CPT][2];
+    if (threadIdx.x < SCAN_THREADS) {
+        const int tid = threadIdx.x, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q;
+        const bool there = c0 < cs.count;
+        const size_t ch = cs.first + c0;
+        const float4 a = there ? ld_states(p.A, ch, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const f32x2 A0 = mul2(lo2(a), both(RCP_LN2)), A1 = mul2(hi2(a), both(RCP_LN2));
+        for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
+            const int n = p.S.order ? p.S.order[slot] : slot;
+            const Span sq = sequence(p.S, n);
+            const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+            const float4 v = p.h0 && there ? ld_states(p.h0, (size_t)n * D + ch, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
+            f32x2 h0 = lo2(v), h1 = hi2(v);
+            const size_t ck0 = p.ckpt ? (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) : 0;
+            float* ck = p.ckpt ? p.ckpt + (ck0 * D + ch) * NP + n0 : nullptr;
+            __syncthreads();                               // the first tile is there
+            for (int k = 0; k < tiles; ++k) {
+                const int buf = k & 1, t0 = k * TILE;
+                const float2* sd = &sh.d[buf][0][c0];
+                const float* sB = &sh.B[buf][0][n0];
+                const float* sC = &sh.C[buf][0][n0];
+                float* sy = &sh.y[buf][0][0];
+                // Four tokens at a time, three groups in flight: what a token reads is requested two groups ahead, its decays are formed one group ahead, between the
+                // steps of the chain (the special function unit takes one of them every eight cycles), and the sums of a group are finished in the next one.
+                struct Token { float2 d; float4 B, C; };
+                auto fetch = [&](int t) {
+                    Token x;
+                    x.d = sd[t * CB];
+                    x.B = *reinterpret_cast<const float4*>(sB + t * NP);
+                    x.C = *reinterpret_cast<const float4*>(sC + t * NP);
+                    return x;
+                };
+                Token now[4], next[4];
+                f32x2 e[4][2], en[4][2];
+                float ys[4];
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-        const float4 a = c0 + c < cs.count ? ld_states(p.A, cs.first + c0 + c, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-        A[c][0] = mul2(lo2(a), both(RCP_LN2));
-        A[c][1] = mul2(hi2(a), both(RCP_LN2));
-    }
-    // layout of the elementwise part: this thread's eight channels, the same in all its pieces
-    const int ec = tid % ROW * 8, et = tid / ROW, valid = cs.count - ec;
-    constexpr int STEP = SCAN_THREADS / ROW;
-    const int bn = tid % (NP / 8) * 8, bt = tid / (NP / 8), bvalid = NST - bn;
-    constexpr int BSTEP = SCAN_THREADS / (NP / 8);
-    __syncthreads();
-
-    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-        const int n = p.S.order ? p.S.order[slot] : slot;
-        const Span sq = sequence(p.S, n);
-        const int len = sq.end - sq.start;
+                for (int u = 0; u < 4; ++u) now[u] = fetch(u);
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-            const float4 v = p.h0 && c0 + c < cs.count ? ld_states(p.h0, (size_t)n * D + cs.first + c0 + c, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-            h[c][0] = lo2(v);
-            h[c][1] = hi2(v);
+                for (int u = 0; u < 4; ++u) next[u] = fetch(4 + u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    e[u][0] = ex2f2_(mul2(A0, both(now[u].d.x)));
+                    e[u][1] = ex2f2_(mul2(A1, both(now[u].d.x)));
+                }
+#pragma unroll
+                for (int t4 = 0; t4 < TILE; t4 += 4) {
+                    if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) {
+                        float4 w;
+                        unpack2(h0, w.x, w.y);
+                        unpack2(h1, w.z, w.w);
+                        *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = w;
+                    }
+                    float yn[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if (t4 + 4 < TILE) {
+                            en[u][0] = ex2f2_(mul2(A0, both(next[u].d.x)));
+                            en[u][1] = ex2f2_(mul2(A1, both(next[u].d.x)));
+                        }
+                        const f32x2 dx = both(now[u].d.y);
+                        h0 = fma2(e[u][0], h0, mul2(dx, lo2(now[u].B)));
+                        h1 = fma2(e[u][1], h1, mul2(dx, hi2(now[u].B)));
+                        yn[u] = sum2(fma2(h1, hi2(now[u].C), mul2(h0, lo2(now[u].C))));
+                        now[u] = next[u];
+                        if (t4 + 8 < TILE) next[u] = fetch(t4 + 8 + u);
+                        e[u][0] = en[u][0];
+                        e[u][1] = en[u][1];
+                    }
+                    if (t4) {
+                        lanes_sum4<LPC>(ys, q);
+                        put_sums<LPC, YROW>(sy, t4 - 4, c0, ys, q);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) ys[u] = yn[u];
+                }
+                lanes_sum4<LPC>(ys, q);
+                put_sums<LPC, YROW>(sy, TILE - 4, c0, ys, q);
+                __syncthreads();
+            }
+            if (p.ht && there) {
+                float4 w;
+                unpack2(h0, w.x, w.y);
+                unpack2(h1, w.z, w.w);
+                st_states(p.ht, (size_t)n * D + ch, n0, NST, w);
+            }
+            __syncthreads();                               // the last tile has been stored
         }
-        const size_t ck0 = p.ckpt ? (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) : 0;
-        Raw8 rx[PIECES], rd[PIECES], rz[PIECES], rB[BC], rC[BC];
-        auto request = [&](int t0) {
+        return;
+    }
+
+    // the elementwise part: four channels of a token in a piece, the same channels in all pieces of a thread; half of the threads bring B, half C
+    constexpr int HELPERS = SCAN_HELPERS, ROW = CB / 4, STEP = HELPERS / ROW, PIECES = (TILE * ROW + HELPERS - 1) / HELPERS;
+    constexpr int BROW = NP / 4, BSTEP = HELPERS / 2 / BROW, BC = (TILE * BROW * 2 + HELPERS - 1) / HELPERS;
+    const int tid = threadIdx.x - SCAN_THREADS, ec = tid % ROW * 4, et = tid / ROW, valid = cs.count - ec;
+    const int half = tid / (HELPERS / 2), bn = tid % BROW * 4, bt = tid % (HELPERS / 2) / BROW, bvalid = NST - bn;
+    const void* const bc = half ? p.C : p.B;
+    const long long bc_stride = half ? p.C_stride : p.B_stride;
+    float bias[4], skip[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bias[e] = p.dt_bias && ec + e < cs.count ? p.dt_bias[cs.first + ec + e] : 0.f;
+        skip[e] = p.skip && ec + e < cs.count ? p.skip[cs.first + ec + e] : 0.f;
+    }
+    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
+        const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
+        const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+        Raw4<DT> rx[PIECES], rd[PIECES], rz[PIECES], rb[BC];                             // of the tile that is formed next
+        Raw4<DT> x1[PIECES], z1[PIECES], x2[PIECES], z2[PIECES];                         // of the tiles one and two behind it
+        auto request = [&](int k) {
+            const int t0 = k * TILE;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int t = t0 + et + i * STEP;
                 const int ok = et + i * STEP < TILE && t < len ? valid : 0;
                 const size_t tok = (size_t)(sq.start + t);
-                rx[i] = load8<DT>(p.x, tok * p.x_stride + cs.first + ec, ok, vec);
-                rd[i] = load8<DT>(p.dt, tok * p.dt_stride + cs.first + ec, ok, vec);
-                if (p.z) rz[i] = load8<DT>(p.z, tok * p.z_stride + cs.first + ec, ok, vec);
+                rx[i] = load4<DT>(p.x, tok * p.x_stride + cs.first + ec, ok, vec);
+                rd[i] = load4<DT>(p.dt, tok * p.dt_stride + cs.first + ec, ok, vec);
+                if (p.z) rz[i] = load4<DT>(p.z, tok * p.z_stride + cs.first + ec, ok, vec);
             }
 #pragma unroll
             for (int i = 0; i < BC; ++i) {
                 const int t = t0 + bt + i * BSTEP;
                 const int ok = bt + i * BSTEP < TILE && t < len ? bvalid : 0;
-                const size_t tok = (size_t)(sq.start + t);
-                rB[i] = load8<DT>(p.B, tok * p.B_stride + cs.group * NST + bn, ok, bvec);
-                rC[i] = load8<DT>(p.C, tok * p.C_stride + cs.group * NST + bn, ok, bvec);
+                rb[i] = load4<DT>(bc, (size_t)(sq.start + t) * bc_stride + cs.group * NST + bn, ok, bvec);
             }
         };
         request(0);
-        for (int t0 = 0; t0 < len; t0 += TILE) {
-            float x[PIECES][8], z[PIECES][8];
+        for (int k = -1; k <= tiles; ++k) {                // forms tile k + 1, stores tile k - 1
+            if (k + 1 < tiles) {
+                const int buf = (k + 1) & 1, t0 = (k + 1) * TILE;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                float d[8];
-                unpack8<DT>(rx[i], x[i]);
-                unpack8<DT>(rd[i], d);
-                if (p.z) unpack8<DT>(rz[i], z[i]);
-                const int t = et + i * STEP;
-                if (t >= TILE) continue;
-                const bool there = t0 + t < len;
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = et + i * STEP;
+                    if (t >= TILE) continue;
+                    const bool there = t0 + t < len;       // d = 0 behind the last token: the state stays as it is
+                    float x[4], d[4];
+                    unpack4<DT>(rx[i], x);
+                    unpack4<DT>(rd[i], d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    d[e] += s_bias[ec + e];
-                    if (p.softplus) d[e] = scan_softplus(d[e]);
-                    if (!there) d[e] = 0.f;                // the state stays as it is behind the last token
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {              // in an order that keeps the eight threads of a store apart
-                    const int e = 2 * ((k + (tid >> 1)) & 3);
-                    float4 w;
-                    w.x = e == 0 ? d[0] : e == 2 ? d[2] : e == 4 ? d[4] : d[6];
-                    w.z = e == 0 ? d[1] : e == 2 ? d[3] : e == 4 ? d[5] : d[7];
-                    w.y = w.x * (e == 0 ? x[i][0] : e == 2 ? x[i][2] : e == 4 ? x[i][4] : x[i][6]);
-                    w.w = w.z * (e == 0 ? x[i][1] : e == 2 ? x[i][3] : e == 4 ? x[i][5] : x[i][7]);
-                    if (!there) w = make_float4(0.f, 0.f, 0.f, 0.f);
-                    *reinterpret_cast<float4*>(&s_d[t][ec + e]) = w;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < BC; ++i) {
-                const int t = bt + i * BSTEP;
-                if (t >= TILE) continue;
-                float b[8], c[8];
-                unpack8<DT>(rB[i], b);
-                unpack8<DT>(rC[i], c);
-                st4(&s_B[t][bn], MKDA_F32, 0, make_float4(b[0], b[1], b[2], b[3]));
-                st4(&s_B[t][bn], MKDA_F32, 4, make_float4(b[4], b[5], b[6], b[7]));
-                st4(&s_C[t][bn], MKDA_F32, 0, make_float4(c[0], c[1], c[2], c[3]));
-                st4(&s_C[t][bn], MKDA_F32, 4, make_float4(c[4], c[5], c[6], c[7]));
-            }
-            __syncthreads();
-            if (t0 + TILE < len) request(t0 + TILE);
-#pragma unroll 2
-            for (int t4 = 0; t4 < TILE; t4 += 4) {
-                if (p.ckpt && t4 % CKPT == 0 && t0 + t4 < len) {
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c)
-                        if (c0 + c < cs.count) {
-                            float4 v;
-                            unpack2(h[c][0], v.x, v.y);
-                            unpack2(h[c][1], v.z, v.w);
-                            *reinterpret_cast<float4*>(p.ckpt + ((ck0 + (t0 + t4) / CKPT) * D + cs.first + c0 + c) * NP + n0) = v;
-                        }
-                }
-                float ys[CPT][4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float4 B = *reinterpret_cast<const float4*>(&s_B[t4 + u][n0]), C = *reinterpret_cast<const float4*>(&s_C[t4 + u][n0]);
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        const float2 d = s_d[t4 + u][c0 + c];
-                        const f32x2 dd = both(d.x), dx = both(d.y);
-                        h[c][0] = fma2(ex2f2_(mul2(A[c][0], dd)), h[c][0], mul2(dx, lo2(B)));
-                        h[c][1] = fma2(ex2f2_(mul2(A[c][1], dd)), h[c][1], mul2(dx, hi2(B)));
-                        ys[c][u] = sum2(fma2(h[c][1], hi2(C), mul2(h[c][0], lo2(C))));
+                    for (int e = 0; e < 4; ++e) {
+                        d[e] += bias[e];
+                        if (p.softplus) d[e] = scan_softplus(d[e]);
+                        d[e] = there ? d[e] : 0.f;
+                        x[e] = there ? d[e] * x[e] : 0.f;
                     }
+                    // two pairs at a time, in an order that keeps the eight threads of a store apart
+                    const float4 w0 = make_float4(d[0], x[0], d[1], x[1]), w1 = make_float4(d[2], x[2], d[3], x[3]);
+                    const int r = (tid >> 2) & 1;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 * r]) = r ? w1 : w0;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 - 2 * r]) = r ? w0 : w1;
                 }
 #pragma unroll
-                for (int c = 0; c < CPT; ++c) {
-                    lanes_sum4<LPC>(ys[c], q);
-                    put_sums<LPC, YROW>(&s_y[0][0], t4, c0 + c, ys[c], q);
+                for (int i = 0; i < BC; ++i) {
+                    const int t = bt + i * BSTEP;
+                    if (t >= TILE) continue;
+                    float v[4];
+                    unpack4<DT>(rb[i], v);
+                    *reinterpret_cast<float4*>(half ? &sh.C[buf][t][bn] : &sh.B[buf][t][bn]) = make_float4(v[0], v[1], v[2], v[3]);
                 }
             }
+            if (k >= 1) {
+                const int buf = (k - 1) & 1, t0 = (k - 1) * TILE;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = et + i * STEP;
+                    if (t >= TILE || t0 + t >= len) continue;
+                    const float4 s = *reinterpret_cast<const float4*>(&sh.y[buf][t][ec]);
+                    float y[4] = {s.x, s.y, s.z, s.w}, x[4], z[4];
+                    unpack4<DT>(x2[i], x);
+                    if (p.z) unpack4<DT>(z2[i], z);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (p.skip) y[e] = fmaf(skip[e], x[e], y[e]);
+                        if (p.z) y[e] *= z[e] * sigmoidf_(z[e]);
+                    }
+                    store4<DT>(p.y, (size_t)(sq.start + t0 + t) * D + cs.first + ec, min(valid, 4), vec, y);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) { x2[i] = x1[i]; z2[i] = z1[i]; x1[i] = rx[i]; z1[i] = rz[i]; }
+            if (k + 2 < tiles) request(k + 2);
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int t = et + i * STEP;
-                if (t >= TILE || t0 + t >= len) continue;
-                float y[8];
-                ld8(&s_y[t][ec], MKDA_F32, 0, y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (p.skip) y[e] = fmaf(s_skip[ec + e], x[i][e], y[e]);
-                    if (p.z) y[e] *= z[i][e] * sigmoidf_(z[i][e]);
-                }
-                store8<DT>(p.y, (size_t)(sq.start + t0 + t) * D + cs.first + ec, min(valid, 8), vec, y);
-            }
-        }
-        if (p.ht) {
-#pragma unroll
-            for (int c = 0; c < CPT; ++c)
-                if (c0 + c < cs.count) {
-                    float4 v;
-                    unpack2(h[c][0], v.x, v.y);
-                    unpack2(h[c][1], v.z, v.w);
-                    st_states(p.ht, (size_t)n * D + cs.first + c0 + c, n0, NST, v);
-                }
         }
     }
 }
@@ -607,10 +648,11 @@ static int bad_scan(int D, int NST, int G, int dtype) {
     if (dtype < MKDA_F32 || dtype > MKDA_F16) return set_error(MKDA_ERR_ARG, "scan: unsupported dtype");
     return MKDA_OK;
 }
-static bool wide_rows(const MkdaScanFwd& f) {
-    return f.D / f.G % 8 == 0 && f.x_stride % 8 == 0 && f.dt_stride % 8 == 0 && (!f.z || f.z_stride % 8 == 0) && aligned16(f.x) && aligned16(f.dt) && aligned16(f.z);
+// rows of channels, and of B and C, that can be read `w` elements at a time
+static bool wide_rows(const MkdaScanFwd& f, int w) {
+    return f.D / f.G % w == 0 && f.x_stride % w == 0 && f.dt_stride % w == 0 && (!f.z || f.z_stride % w == 0) && aligned16(f.x) && aligned16(f.dt) && aligned16(f.z);
 }
-static bool wide_states(const MkdaScanFwd& f) { return f.NST % 8 == 0 && f.B_stride % 8 == 0 && f.C_stride % 8 == 0 && aligned16(f.B) && aligned16(f.C); }
+static bool wide_states(const MkdaScanFwd& f, int w) { return f.NST % w == 0 && f.B_stride % w == 0 && f.C_stride % w == 0 && aligned16(f.B) && aligned16(f.C); }
 static int blocks_of_channels(int D, int G, int CB) { return G * ((D / G + CB - 1) / CB); }
 
 }  // namespace mkda
@@ -625,14 +667,19 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
     if (!good_sequences(p->S) || (p->ckpt && p->S.cu && !p->S.ckpt_off)) return set_error(MKDA_ERR_ARG, "scan_fwd: bad sequences");
     if (!aligned16(p->A) || !aligned16(p->h0) || !aligned16(p->ht) || !aligned16(p->ckpt)) return set_error(MKDA_ERR_ARG, "scan_fwd: A and states must be 16-byte aligned");
     if (p->S.N == 0) return MKDA_OK;
+    int rc = MKDA_OK;
     with_dtype(p->dtype, [&](auto dt) {
         with_lanes(p->NST, [&](auto l) {
-            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
-            const bool vec = wide_rows(*p) && p->D % 8 == 0 && aligned16(p->y);
+            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value, smem = (int)sizeof(ScanFwdShared<LPC, 32>);
+            const bool vec = wide_rows(*p, 4) && aligned16(p->y);
             const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC, 1, 32>::CB);
-            launch(scan_fwd_kernel<DT, LPC, 1>, dim3(blocks, p->S.N < 65535 ? p->S.N : 65535), SCAN_THREADS, 0, (cudaStream_t)stream, *p, vec, wide_states(*p));
+            auto* kern = scan_fwd_kernel<DT, LPC>;
+            rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_fwd");
+            if (rc == MKDA_OK)
+                launch(kern, dim3(blocks, p->S.N < 65535 ? p->S.N : 65535), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
         });
     });
+    if (rc != MKDA_OK) return rc;
     return check_launch("scan_fwd");
 }
 
@@ -662,11 +709,11 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
         with_lanes(p->f.NST, [&](auto l) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value, CPT = bwd_cpt<LPC>();
             const MkdaScanFwd& f = p->f;
-            const bool vec = wide_rows(f) && f.D % 8 == 0 && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
+            const bool vec = wide_rows(f, 8) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
             auto* kern = scan_bwd_kernel<DT, LPC, CPT>;
             constexpr int smem = (int)sizeof(ScanBwdShared<LPC, CPT>);
             rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
-            if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_THREADS, smem, (cudaStream_t)stream, *p, vec, wide_states(f));
+            if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_THREADS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 8));
         });
     });
     return rc != MKDA_OK ? rc : check_launch("scan_bwd");
