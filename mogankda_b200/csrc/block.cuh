@@ -94,6 +94,13 @@ __device__ __forceinline__ void unpack4(const Raw4<DT>& r, float (&v)[4]) {
     }
 }
 template <int DT>
+__device__ __forceinline__ void unpack4_2(const Raw4<DT>& r, f32x2 (&v)[2]) {
+    float f[4];
+    unpack4<DT>(r, f);
+    v[0] = pack2(f[0], f[1]);
+    v[1] = pack2(f[2], f[3]);
+}
+template <int DT>
 __device__ __forceinline__ void store4(void* base, size_t idx, int valid, bool vec, const float (&v)[4]) {
     if (valid <= 0) return;
     if (vec) {

@@ -28,16 +28,24 @@ struct ScanShape {
 };
 
 // softplus with its relative error small everywhere: log(1 + u) = 2 artanh(u / (2 + u)), u = exp(-|s|) in (0, 1], by the series of artanh
-// (argument at most 1/3: seven terms leave 2e-8).  A dt of 1e-3 is a small u; the logarithm of 1 + u would lose its digits.
+// (argument at most 1/3: six terms leave 1.4e-7).  A dt of 1e-3 is a small u; the logarithm of 1 + u would lose its digits.
+__device__ __forceinline__ f32x2 scan_softplus2(f32x2 s) {
+    float a, b, c, d;
+    unpack2(s, a, b);
+    const f32x2 u = ex2f2_(pack2(-fabsf(a) * RCP_LN2, -fabsf(b) * RCP_LN2));
+    unpack2(add2(u, both(2.f)), c, d);
+    const f32x2 w = mul2(u, pack2(rcpf_(c), rcpf_(d))), q = mul2(w, w);
+    f32x2 r = fma2(q, both(1.f / 11.f), both(1.f / 9.f));
+    r = fma2(q, r, both(1.f / 7.f));
+    r = fma2(q, r, both(1.f / 5.f));
+    r = fma2(q, r, both(1.f / 3.f));
+    r = fma2(q, r, both(1.f));
+    return fma2(mul2(w, both(2.f)), r, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
+}
 __device__ __forceinline__ float scan_softplus(float s) {
-    const float u = expf_(-fabsf(s)), w = __fdividef(u, 2.f + u), q = w * w;
-    float r = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-    r = fmaf(q, r, 1.f / 9.f);
-    r = fmaf(q, r, 1.f / 7.f);
-    r = fmaf(q, r, 1.f / 5.f);
-    r = fmaf(q, r, 1.f / 3.f);
-    r = fmaf(q, r, 1.f);
-    return fmaxf(s, 0.f) + 2.f * w * r;
+    float a, b;
+    unpack2(scan_softplus2(both(s)), a, b);
+    return a;
 }
 
 // Sums over the LPC lanes of a channel of four values each: v[0..3] of lane q become one (LPC >= 4: of token q & 3, in v[0]; LPC = 2: of
@@ -100,18 +108,31 @@ __device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB)
 // Forward.  Four warps walk the recurrence and four beside them do the elementwise part, a tile ahead (loads, softplus) and a tile behind (skip, gate, stores); the block's
 // barrier joins them once a tile.  A channel's chain is short and there are few warps of it (4096 channels are 512), so what counts is how many cycles a token takes a warp that
 // has a scheduler to itself: with the elementwise part in the same warps 168, of which 32 are the exponentials of the special function unit.
-constexpr int SCAN_HELPERS = 256;
+constexpr int SCAN_HELPERS = 256, SCAN_LONG = 256;
+// registers of the backward kernel's two roles, out of 168 for each of 384 threads: 128 x 240 + 256 x 128 = 63 488 of 64 512
+constexpr int SCAN_BWD_WALK_REGS = 240, SCAN_BWD_HELP_REGS = 128, SCAN_BWD_LAUNCH_REGS = 168;
+static_assert(SCAN_THREADS * SCAN_BWD_WALK_REGS + SCAN_HELPERS * SCAN_BWD_HELP_REGS <= (SCAN_THREADS + SCAN_HELPERS) * SCAN_BWD_LAUNCH_REGS, "register split");
 template <int LPC, int TILE>
 struct ScanFwdShared {
     using Sh = ScanShape<LPC, 1, TILE>;
-    float2 d[2][TILE][Sh::CB];             // d, d x
-    float B[2][TILE][Sh::NP], C[2][TILE][Sh::NP], y[2][TILE][Sh::YROW];
+    static constexpr int AHEAD = 8;        // rows behind the last one that are read and not used
+    float2 d[2][TILE + AHEAD][Sh::CB];     // d, d x
+    float B[2][TILE + AHEAD][Sh::NP], C[2][TILE + AHEAD][Sh::NP], y[2][TILE][Sh::YROW];
 };
+// four states of a channel
+struct Four { f32x2 v[2]; };
+__device__ __forceinline__ Four four(const float4& f) { return Four{{lo2(f), hi2(f)}}; }
+__device__ __forceinline__ float4 flat(const Four& s) {
+    float4 f;
+    unpack2(s.v[0], f.x, f.y);
+    unpack2(s.v[1], f.z, f.w);
+    return f;
+}
 
-template <int DT, int LPC>
+// (Two states a lane and twice the warps on the chain: 302 us where this takes 275.)
+template <int DT, int LPC, int TILE>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
     follow_stream();
-    constexpr int TILE = 32;
     using Sh = ScanShape<LPC, 1, TILE>;
     constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
     extern __shared__ __align__(16) unsigned char raw_shared[];
@@ -122,14 +143,15 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
         const int tid = threadIdx.x, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q;
         const bool there = c0 < cs.count;
         const size_t ch = cs.first + c0;
-        const float4 a = there ? ld_states(p.A, ch, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const f32x2 A0 = mul2(lo2(a), both(RCP_LN2)), A1 = mul2(hi2(a), both(RCP_LN2));
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
         for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
             const int n = p.S.order ? p.S.order[slot] : slot;
             const Span sq = sequence(p.S, n);
             const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
-            const float4 v = p.h0 && there ? ld_states(p.h0, (size_t)n * D + ch, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-            f32x2 h0 = lo2(v), h1 = hi2(v);
+            Four h = four(p.h0 && there ? ld_states(p.h0, (size_t)n * D + ch, n0, NST) : zero);
             const size_t ck0 = p.ckpt ? (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) : 0;
             float* ck = p.ckpt ? p.ckpt + (ck0 * D + ch) * NP + n0 : nullptr;
             __syncthreads();                               // the first tile is there
@@ -141,49 +163,43 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 float* sy = &sh.y[buf][0][0];
                 // Four tokens at a time, three groups in flight: what a token reads is requested two groups ahead, its decays are formed one group ahead, between the
                 // steps of the chain (the special function unit takes one of them every eight cycles), and the sums of a group are finished in the next one.
-                struct Token { float2 d; float4 B, C; };
+                struct Token { float2 d; Four B, C; };
                 auto fetch = [&](int t) {
                     Token x;
                     x.d = sd[t * CB];
-                    x.B = *reinterpret_cast<const float4*>(sB + t * NP);
-                    x.C = *reinterpret_cast<const float4*>(sC + t * NP);
+                    x.B = four(*reinterpret_cast<const float4*>(sB + t * NP));
+                    x.C = four(*reinterpret_cast<const float4*>(sC + t * NP));
                     return x;
                 };
                 Token now[4], next[4];
-                f32x2 e[4][2], en[4][2];
+                Four e[4];
                 float ys[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) now[u] = fetch(u);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) next[u] = fetch(4 + u);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    e[u][0] = ex2f2_(mul2(A0, both(now[u].d.x)));
-                    e[u][1] = ex2f2_(mul2(A1, both(now[u].d.x)));
-                }
+                for (int u = 0; u < 4; ++u)
 #pragma unroll
+                    for (int i = 0; i < 2; ++i) e[u].v[i] = ex2f2_(mul2(A.v[i], both(now[u].d.x)));
+#pragma unroll                                             // unrolled by 2, 4 or 8 groups 413, 341 and 315 us where wholly 275
                 for (int t4 = 0; t4 < TILE; t4 += 4) {
-                    if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) {
-                        float4 w;
-                        unpack2(h0, w.x, w.y);
-                        unpack2(h1, w.z, w.w);
-                        *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = w;
-                    }
+                    if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = flat(h);
                     float yn[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        if (t4 + 4 < TILE) {
-                            en[u][0] = ex2f2_(mul2(A0, both(next[u].d.x)));
-                            en[u][1] = ex2f2_(mul2(A1, both(next[u].d.x)));
-                        }
                         const f32x2 dx = both(now[u].d.y);
-                        h0 = fma2(e[u][0], h0, mul2(dx, lo2(now[u].B)));
-                        h1 = fma2(e[u][1], h1, mul2(dx, hi2(now[u].B)));
-                        yn[u] = sum2(fma2(h1, hi2(now[u].C), mul2(h0, lo2(now[u].C))));
+                        f32x2 y;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x2 d = e[u].v[i];
+                            e[u].v[i] = ex2f2_(mul2(A.v[i], both(next[u].d.x)));
+                            h.v[i] = fma2(d, h.v[i], mul2(dx, now[u].B.v[i]));
+                            y = i ? fma2(h.v[i], now[u].C.v[i], y) : mul2(h.v[i], now[u].C.v[i]);
+                        }
+                        yn[u] = sum2(y);
                         now[u] = next[u];
-                        if (t4 + 8 < TILE) next[u] = fetch(t4 + 8 + u);
-                        e[u][0] = en[u][0];
-                        e[u][1] = en[u][1];
+                        next[u] = fetch(t4 + 8 + u);
                     }
                     if (t4) {
                         lanes_sum4<LPC>(ys, q);
@@ -196,12 +212,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 put_sums<LPC, YROW>(sy, TILE - 4, c0, ys, q);
                 __syncthreads();
             }
-            if (p.ht && there) {
-                float4 w;
-                unpack2(h0, w.x, w.y);
-                unpack2(h1, w.z, w.w);
-                st_states(p.ht, (size_t)n * D + ch, n0, NST, w);
-            }
+            if (p.ht && there) st_states(p.ht, (size_t)n * D + ch, n0, NST, flat(h));
             __syncthreads();                               // the last tile has been stored
         }
         return;
@@ -212,385 +223,520 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
     constexpr int BROW = NP / 4, BSTEP = HELPERS / 2 / BROW, BC = (TILE * BROW * 2 + HELPERS - 1) / HELPERS;
     const int tid = threadIdx.x - SCAN_THREADS, ec = tid % ROW * 4, et = tid / ROW, valid = cs.count - ec;
     const int half = tid / (HELPERS / 2), bn = tid % BROW * 4, bt = tid % (HELPERS / 2) / BROW, bvalid = NST - bn;
-    const void* const bc = half ? p.C : p.B;
-    const long long bc_stride = half ? p.C_stride : p.B_stride;
-    float bias[4], skip[4];
+    constexpr int SIZE = DT == MKDA_F32 ? 4 : 2;
+    const size_t x_pitch = (size_t)p.x_stride * SIZE, d_pitch = (size_t)p.dt_stride * SIZE, z_pitch = (size_t)p.z_stride * SIZE, y_pitch = (size_t)D * SIZE,
+                 b_pitch = (size_t)(half ? p.C_stride : p.B_stride) * SIZE;
+    float fb[4], fs[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        bias[e] = p.dt_bias && ec + e < cs.count ? p.dt_bias[cs.first + ec + e] : 0.f;
-        skip[e] = p.skip && ec + e < cs.count ? p.skip[cs.first + ec + e] : 0.f;
+        fb[e] = p.dt_bias && ec + e < cs.count ? p.dt_bias[cs.first + ec + e] : 0.f;
+        fs[e] = p.skip && ec + e < cs.count ? p.skip[cs.first + ec + e] : 0.f;
     }
+    const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}, skip[2] = {pack2(fs[0], fs[1]), pack2(fs[2], fs[3])};
+    const bool whole = STEP * PIECES == TILE && BSTEP * BC == TILE;      // every piece of every thread lies in the tile
     for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
         const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
         const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
-        Raw4<DT> rx[PIECES], rd[PIECES], rz[PIECES], rb[BC];                             // of the tile that is formed next
-        Raw4<DT> x1[PIECES], z1[PIECES], x2[PIECES], z2[PIECES];                         // of the tiles one and two behind it
-        auto request = [&](int k) {
-            const int t0 = k * TILE;
+        struct Rows { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], b[BC]; };
+        Rows even, odd;                                    // rows on their way, of every other tile: requested two steps before they are used
+        Raw4<DT> x1[PIECES], z1[PIECES], x2[PIECES], z2[PIECES];      // of the two tiles behind the one that is formed
+        // where this thread's first piece of the next tile to be requested, and to be stored, lies
+        const size_t row = (size_t)sq.start + et, col = (size_t)(cs.first + ec) * SIZE;
+        const char *px = static_cast<const char*>(p.x) + row * x_pitch + col, *pd = static_cast<const char*>(p.dt) + row * d_pitch + col,
+                   *pz = static_cast<const char*>(p.z) + row * z_pitch + col,
+                   *pb = static_cast<const char*>(half ? p.C : p.B) + ((size_t)sq.start + bt) * b_pitch + (size_t)(cs.group * NST + bn) * SIZE;
+        char* py = static_cast<char*>(p.y) + row * y_pitch + col;
+        auto request = [&](Rows& r, int k) {
+            const int left = len - k * TILE;               // tokens from the tile's first on
+            const bool inside = whole && left >= TILE;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const int t = t0 + et + i * STEP;
-                const int ok = et + i * STEP < TILE && t < len ? valid : 0;
-                const size_t tok = (size_t)(sq.start + t);
-                rx[i] = load4<DT>(p.x, tok * p.x_stride + cs.first + ec, ok, vec);
-                rd[i] = load4<DT>(p.dt, tok * p.dt_stride + cs.first + ec, ok, vec);
-                if (p.z) rz[i] = load4<DT>(p.z, tok * p.z_stride + cs.first + ec, ok, vec);
+                const int t = et + i * STEP, ok = inside || (t < TILE && t < left) ? valid : 0;
+                r.x[i] = load4<DT>(px + i * STEP * x_pitch, 0, ok, vec);
+                r.d[i] = load4<DT>(pd + i * STEP * d_pitch, 0, ok, vec);
+                if (p.z) r.z[i] = load4<DT>(pz + i * STEP * z_pitch, 0, ok, vec);
             }
 #pragma unroll
             for (int i = 0; i < BC; ++i) {
-                const int t = t0 + bt + i * BSTEP;
-                const int ok = bt + i * BSTEP < TILE && t < len ? bvalid : 0;
-                rb[i] = load4<DT>(bc, (size_t)(sq.start + t) * bc_stride + cs.group * NST + bn, ok, bvec);
+                const int t = bt + i * BSTEP;
+                r.b[i] = load4<DT>(pb + i * BSTEP * b_pitch, 0, inside || (t < TILE && t < left) ? bvalid : 0, bvec);
+            }
+            px += TILE * x_pitch; pd += TILE * d_pitch; pz += TILE * z_pitch; pb += TILE * b_pitch;
+        };
+        auto step = [&](Rows& r, int k) {                  // forms tile k + 1, stores tile k - 1
+            if (k + 1 < tiles) {
+                const int buf = (k + 1) & 1, left = len - (k + 1) * TILE;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = et + i * STEP;
+                    if (!whole && t >= TILE) continue;
+                    f32x2 x[2], d[2];
+                    unpack4_2<DT>(r.x[i], x);
+                    unpack4_2<DT>(r.d[i], d);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        d[e] = add2(d[e], bias[e]);
+                        if (p.softplus) d[e] = scan_softplus2(d[e]);
+                        x[e] = mul2(d[e], x[e]);
+                    }
+                    float4 w0, w1;
+                    unpack2(d[0], w0.x, w0.z);
+                    unpack2(x[0], w0.y, w0.w);
+                    unpack2(d[1], w1.x, w1.z);
+                    unpack2(x[1], w1.y, w1.w);
+                    if (left < TILE && t >= left) w0 = w1 = make_float4(0.f, 0.f, 0.f, 0.f);      // d = 0 behind the last token: the state stays as it is
+                    // two pairs at a time, in an order that keeps the eight threads of a store apart
+                    const int o = (tid >> 2) & 1;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 * o]) = o ? w1 : w0;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 - 2 * o]) = o ? w0 : w1;
+                }
+#pragma unroll
+                for (int i = 0; i < BC; ++i) {
+                    const int t = bt + i * BSTEP;
+                    if (!whole && t >= TILE) continue;
+                    float v[4];
+                    unpack4<DT>(r.b[i], v);
+                    *reinterpret_cast<float4*>(half ? &sh.C[buf][t][bn] : &sh.B[buf][t][bn]) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+            if (k >= 1) {
+                const int buf = (k - 1) & 1, left = len - (k - 1) * TILE;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = et + i * STEP;
+                    if ((!whole && t >= TILE) || t >= left) continue;
+                    const float4 f = *reinterpret_cast<const float4*>(&sh.y[buf][t][ec]);
+                    f32x2 y[2] = {lo2(f), hi2(f)}, x[2], z[2];
+                    unpack4_2<DT>(x2[i], x);
+                    if (p.z) unpack4_2<DT>(z2[i], z);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (p.skip) y[e] = fma2(skip[e], x[e], y[e]);
+                        if (p.z) y[e] = mul2(y[e], mul2(z[e], sigmoidf2_(z[e])));
+                    }
+                    float v[4];
+                    unpack2(y[0], v[0], v[1]);
+                    unpack2(y[1], v[2], v[3]);
+                    store4<DT>(py + i * STEP * y_pitch, 0, min(valid, 4), vec, v);
+                }
+                py += TILE * y_pitch;
+            }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) { x2[i] = x1[i]; z2[i] = z1[i]; x1[i] = r.x[i]; z1[i] = r.z[i]; }
+            if (k + 3 < tiles) request(r, k + 3);
+            __syncthreads();
+        };
+        request(even, 0);
+        if (tiles > 1) request(odd, 1);
+        for (int k = -1; k <= tiles; k += 2) {
+            step(even, k);
+            if (k + 1 <= tiles) step(odd, k + 1);
+        }
+    }
+}
+
+// Backward: tiles of one checkpoint, from the last to the first, with the same two roles.  A tile is run forward from its checkpoint (a_n h_n[t - 1], from which h_n follows with
+// one operation, stays in the registers of the lane), then backward, where the decays are formed again.  dB and dC are summed over the channels of a thread, then over
+// the lanes of a warp by a butterfly that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by
+// mkda_sum_rows: in a fixed order.  Two channels per thread where there are enough of them: B, C and those sums are shared by both.
+template <int LPC, int CPT>
+struct ScanBwdShared {
+    using Sh = ScanShape<LPC, CPT, CKPT>;
+    float2 d[2][CKPT][Sh::CB];                             // d, d x
+    float dy[2][CKPT][Sh::CB];
+    float B[2][CKPT][Sh::NP], C[2][CKPT][Sh::NP];
+    float y[2][CKPT][Sh::YROW], gB[2][CKPT][Sh::YROW], eA[2][CKPT][Sh::YROW];
+    float red[2][SCAN_WARPS][CKPT][2 * Sh::NP];            // dB and dC of each warp
+};
+
+template <int DT, int LPC, int CPT>
+__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kernel(const MkdaScanBwd a, const bool vec, const bool bvec) {
+    follow_stream();
+    constexpr int TILE = CKPT;
+    using Sh = ScanShape<LPC, CPT, TILE>;
+    constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    auto& sh = *reinterpret_cast<ScanBwdShared<LPC, CPT>*>(raw_shared);
+    const MkdaScanFwd& p = a.f;
+    const int D = p.D, NST = p.NST;
+    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
+    if (threadIdx.x < SCAN_THREADS) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(SCAN_BWD_WALK_REGS));
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = tid % LPC, c0 = tid / LPC * CPT, n0 = 4 * q, cl = lane / LPC;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool z = p.z;
+        bool there[CPT];
+        Four A[CPT], dA[CPT];
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) {
+            there[c] = c0 + c < cs.count;
+            A[c] = four(there[c] ? ld_states(p.A, cs.first + c0 + c, n0, NST) : zero);
+            dA[c] = four(zero);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) A[c].v[i] = mul2(A[c].v[i], both(RCP_LN2));
+        }
+        for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
+            const int n = p.S.order ? p.S.order[slot] : slot;
+            const Span sq = sequence(p.S, n);
+            const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+            const size_t ck0 = p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT);
+            Four G[CPT];                                   // a[t + 1] g[t + 1]
+            float4 rh[CPT];
+            auto request = [&](int k) {
+#pragma unroll
+                for (int c = 0; c < CPT; ++c)
+                    rh[c] = there[c] ? *reinterpret_cast<const float4*>(p.ckpt + ((ck0 + k) * D + cs.first + c0 + c) * NP + n0) : zero;
+            };
+#pragma unroll
+            for (int c = 0; c < CPT; ++c) G[c] = four(a.dht && there[c] ? ld_states(a.dht, (size_t)n * D + cs.first + c0 + c, n0, NST) : zero);
+            if (tiles) request(tiles - 1);
+            __syncthreads();                               // the first tile is there
+            for (int j = 0; j < tiles; ++j) {
+                const int buf = j & 1;
+                const float* sd = &sh.d[buf][0][c0].x;
+                const float* sdy = &sh.dy[buf][0][c0];
+                const float* sB = &sh.B[buf][0][n0];
+                const float* sC = &sh.C[buf][0][n0];
+                auto fetch_d = [&](int t, float (&d)[CPT], float (&dx)[CPT]) {
+                    if constexpr (CPT == 2) {
+                        const float4 v = *reinterpret_cast<const float4*>(sd + t * 2 * CB);
+                        d[0] = v.x; dx[0] = v.y; d[1] = v.z; dx[1] = v.w;
+                    } else {
+                        const float2 v = *reinterpret_cast<const float2*>(sd + t * 2 * CB);
+                        d[0] = v.x; dx[0] = v.y;
+                    }
+                };
+                Four h[CPT], P[TILE][CPT];
+#pragma unroll
+                for (int c = 0; c < CPT; ++c) h[c] = four(rh[c]);
+                float ysum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)];      // sums wait in registers: a store in between would keep reads behind it
+#pragma unroll
+                for (int t4 = 0; t4 < TILE; t4 += 4) {
+                    float ys[CPT][4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        float d[CPT], dx[CPT];
+                        fetch_d(t4 + u, d, dx);
+                        const Four B = four(*reinterpret_cast<const float4*>(sB + (t4 + u) * NP)), C = four(*reinterpret_cast<const float4*>(sC + (t4 + u) * NP));
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) {
+                            f32x2 y;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const f32x2 v = mul2(ex2f2_(mul2(A[c].v[i], both(d[c]))), h[c].v[i]);
+                                P[t4 + u][c].v[i] = v;
+                                h[c].v[i] = fma2(both(dx[c]), B.v[i], v);
+                                y = i ? fma2(h[c].v[i], C.v[i], y) : mul2(h[c].v[i], C.v[i]);
+                            }
+                            ys[c][u] = sum2(y);
+                        }
+                    }
+                    if (z) {
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) {
+                            lanes_sum4<LPC>(ys[c], q);
+                            ysum[c][t4 / 4] = ys[c][0];
+                            if constexpr (LPC == 2) ysum[c][TILE / 4 + t4 / 4] = ys[c][1];
+                        }
+                    }
+                }
+                if (tiles - 2 - j >= 0) request(tiles - 2 - j);
+                asm volatile("" ::: "memory");             // what the first pass has read is read again: kept for sixteen tokens it would not fit into the registers
+                constexpr int KEEP = LPC >= 4 ? LPC / 4 : 1;      // sums of dB and dC per lane: 1, 1, 2 or 4
+                float gsum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)], esum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)], red[TILE][KEEP];
+                int first = 0;                             // of the sums of dB and dC that this lane ends with
+#pragma unroll
+                for (int t4 = TILE - 4; t4 >= 0; t4 -= 4) {
+                    __syncwarp();                          // reads of the next tokens stay behind it, or their number takes the registers
+                    float gBs[CPT][4], eAs[CPT][4];
+#pragma unroll
+                    for (int u = 3; u >= 0; --u) {
+                        const int t = t4 + u;
+                        float d[CPT], dx[CPT], dy[CPT];
+                        fetch_d(t, d, dx);
+                        if constexpr (CPT == 2) {
+                            const float2 v = *reinterpret_cast<const float2*>(sdy + t * CB);
+                            dy[0] = v.x; dy[1] = v.y;
+                        } else {
+                            dy[0] = sdy[t * CB];
+                        }
+                        const Four B = four(*reinterpret_cast<const float4*>(sB + t * NP)), C = four(*reinterpret_cast<const float4*>(sC + t * NP));
+                        f32x2 dB[2], dC[2];
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) {
+                            f32x2 gb, ea;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const f32x2 v = P[t][c].v[i], hh = fma2(both(dx[c]), B.v[i], v), g = fma2(both(dy[c]), C.v[i], G[c].v[i]);
+                                dC[i] = c ? fma2(both(dy[c]), hh, dC[i]) : mul2(both(dy[c]), hh);
+                                dB[i] = c ? fma2(both(dx[c]), g, dB[i]) : mul2(both(dx[c]), g);
+                                const f32x2 e = mul2(g, v);
+                                gb = i ? fma2(g, B.v[i], gb) : mul2(g, B.v[i]);
+                                ea = i ? fma2(e, A[c].v[i], ea) : mul2(e, A[c].v[i]);
+                                dA[c].v[i] = fma2(e, both(d[c]), dA[c].v[i]);
+                                G[c].v[i] = mul2(ex2f2_(mul2(A[c].v[i], both(d[c]))), g);
+                            }
+                            gBs[c][u] = sum2(gb);
+                            eAs[c][u] = sum2(ea);
+                        }
+                        // over the lanes of other channels: eight sums over 32 / LPC lanes, halved as long as there are lanes to share them
+                        float v[8];
+                        unpack2(dB[0], v[0], v[1]);
+                        unpack2(dB[1], v[2], v[3]);
+                        unpack2(dC[0], v[4], v[5]);
+                        unpack2(dC[1], v[6], v[7]);
+                        int at = 0;
+#pragma unroll
+                        for (int b = 0, w = 4; (LPC << b) < 32; ++b, w >>= 1) {
+                            if (w >= 1) {
+                                const bool up = cl >> b & 1;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if (i >= w) break;
+                                    const float give = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+                                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, LPC << b);
+                                }
+                                at += up ? w : 0;
+                            } else {
+                                v[0] += __shfl_xor_sync(0xffffffffu, v[0], LPC << b);
+                            }
+                        }
+                        first = at;
+#pragma unroll
+                        for (int i = 0; i < KEEP; ++i) red[t][i] = v[i];
+                    }
+#pragma unroll
+                    for (int c = 0; c < CPT; ++c) {
+                        lanes_sum4<LPC>(gBs[c], q);
+                        lanes_sum4<LPC>(eAs[c], q);
+                        gsum[c][t4 / 4] = gBs[c][0];
+                        esum[c][t4 / 4] = eAs[c][0];
+                        if constexpr (LPC == 2) {
+                            gsum[c][TILE / 4 + t4 / 4] = gBs[c][1];
+                            esum[c][TILE / 4 + t4 / 4] = eAs[c][1];
+                        }
+                    }
+                }
+                auto put = [&](float* to, const float (&v)[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)]) {
+#pragma unroll
+                    for (int i = 0; i < TILE / 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < CPT; ++c) {
+                            if constexpr (LPC == 2) {
+                                to[(4 * i + q) * YROW + c0 + c] = v[c][i];
+                                to[(4 * i + q + 2) * YROW + c0 + c] = v[c][TILE / 4 + i];
+                            } else if (LPC == 4 || q < 4) {
+                                to[(4 * i + (q & 3)) * YROW + c0 + c] = v[c][i];
+                            }
+                        }
+                };
+                if (z) put(&sh.y[buf][0][0], ysum);
+                put(&sh.gB[buf][0][0], gsum);
+                put(&sh.eA[buf][0][0], esum);
+                if (LPC > 2 || cl < 8) {
+#pragma unroll
+                    for (int t = 0; t < TILE; ++t)
+#pragma unroll
+                        for (int i = 0; i < KEEP; ++i) sh.red[buf][warp][t][(first + i >= 4 ? NP : 0) + n0 + ((first + i) & 3)] = red[t][i];
+                }
+                __syncthreads();
+            }
+            if (a.dh0) {
+#pragma unroll
+                for (int c = 0; c < CPT; ++c)
+                    if (there[c]) st_states(a.dh0, (size_t)n * D + cs.first + c0 + c, n0, NST, flat(G[c]));
+            }
+            __syncthreads();                               // the last tile has been stored
+        }
+#pragma unroll
+        for (int c = 0; c < CPT; ++c)
+            if (there[c]) *reinterpret_cast<float4*>(a.part_A + ((size_t)blockIdx.y * D + cs.first + c0 + c) * NP + n0) = flat(dA[c]);
+        __syncthreads();
+        __syncthreads();                                   // the elementwise part's sums over tokens
+        return;
+    }
+
+    // the elementwise part, laid out as in the forward kernel
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(SCAN_BWD_HELP_REGS));
+    constexpr int HELPERS = SCAN_HELPERS, ROW = CB / 4, STEP = HELPERS / ROW, PIECES = (TILE * ROW + HELPERS - 1) / HELPERS;
+    constexpr int BROW = NP / 4, BSTEP = HELPERS / 2 / BROW, BC = (TILE * BROW * 2 + HELPERS - 1) / HELPERS;
+    const int tid = threadIdx.x - SCAN_THREADS, ec = tid % ROW * 4, et = tid / ROW, valid = cs.count - ec;
+    const int half = tid / (HELPERS / 2), bn = tid % BROW * 4, bt = tid % (HELPERS / 2) / BROW, bvalid = NST - bn;
+    constexpr int SIZE = DT == MKDA_F32 ? 4 : 2;
+    const size_t x_pitch = (size_t)p.x_stride * SIZE, d_pitch = (size_t)p.dt_stride * SIZE, z_pitch = (size_t)p.z_stride * SIZE, y_pitch = (size_t)D * SIZE,
+                 b_pitch = (size_t)(half ? p.C_stride : p.B_stride) * SIZE;
+    float fb[4], fs[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        fb[e] = p.dt_bias && ec + e < cs.count ? p.dt_bias[cs.first + ec + e] : 0.f;
+        fs[e] = p.skip && ec + e < cs.count ? p.skip[cs.first + ec + e] : 0.f;
+    }
+    const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}, skip[2] = {pack2(fs[0], fs[1]), pack2(fs[2], fs[3])};
+    f32x2 acc_skip[2] = {both(0.f), both(0.f)}, acc_bias[2] = {both(0.f), both(0.f)};
+    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
+        const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
+        const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+        struct Rows { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], y[PIECES], b[BC]; };
+        struct Kept { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], y[PIECES]; };
+        Rows even, odd;                                    // rows on their way, of every other tile: requested two steps before they are used
+        Kept k1, k2;                                       // of the two tiles behind the one that is formed
+        const size_t col = (size_t)(cs.first + ec) * SIZE;
+        auto request = [&](Rows& r, int j) {               // the j-th tile from the end
+            const int t0 = (tiles - 1 - j) * TILE, left = len - t0;
+            const size_t row = (size_t)(sq.start + t0 + et), brow = (size_t)(sq.start + t0 + bt);
+            const char *px = static_cast<const char*>(p.x) + row * x_pitch + col, *pd = static_cast<const char*>(p.dt) + row * d_pitch + col,
+                       *pz = static_cast<const char*>(p.z) + row * z_pitch + col, *py = static_cast<const char*>(a.dy) + row * y_pitch + col,
+                       *pb = static_cast<const char*>(half ? p.C : p.B) + brow * b_pitch + (size_t)(cs.group * NST + bn) * SIZE;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int t = et + i * STEP, ok = t < TILE && t < left ? valid : 0;
+                r.x[i] = load4<DT>(px + i * STEP * x_pitch, 0, ok, vec);
+                r.d[i] = load4<DT>(pd + i * STEP * d_pitch, 0, ok, vec);
+                if (p.z) r.z[i] = load4<DT>(pz + i * STEP * z_pitch, 0, ok, vec);
+                r.y[i] = load4<DT>(py + i * STEP * y_pitch, 0, ok, vec);
+            }
+#pragma unroll
+            for (int i = 0; i < BC; ++i) {
+                const int t = bt + i * BSTEP;
+                r.b[i] = load4<DT>(pb + i * BSTEP * b_pitch, 0, t < TILE && t < left ? bvalid : 0, bvec);
             }
         };
-        request(0);
-        for (int k = -1; k <= tiles; ++k) {                // forms tile k + 1, stores tile k - 1
-            if (k + 1 < tiles) {
-                const int buf = (k + 1) & 1, t0 = (k + 1) * TILE;
+        auto step = [&](Rows& r, int j) {                  // forms tile j + 1, stores tile j - 1, both from the end
+            if (j + 1 < tiles) {
+                const int buf = (j + 1) & 1, left = len - (tiles - 2 - j) * TILE;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     const int t = et + i * STEP;
                     if (t >= TILE) continue;
-                    const bool there = t0 + t < len;       // d = 0 behind the last token: the state stays as it is
-                    float x[4], d[4];
-                    unpack4<DT>(rx[i], x);
-                    unpack4<DT>(rd[i], d);
+                    f32x2 x[2], d[2], dy[2];
+                    unpack4_2<DT>(r.x[i], x);
+                    unpack4_2<DT>(r.d[i], d);
+                    unpack4_2<DT>(r.y[i], dy);
+                    if (p.z) {
+                        f32x2 z[2];
+                        unpack4_2<DT>(r.z[i], z);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        d[e] += bias[e];
-                        if (p.softplus) d[e] = scan_softplus(d[e]);
-                        d[e] = there ? d[e] : 0.f;
-                        x[e] = there ? d[e] * x[e] : 0.f;
+                        for (int e = 0; e < 2; ++e) dy[e] = mul2(dy[e], mul2(z[e], sigmoidf2_(z[e])));
                     }
-                    // two pairs at a time, in an order that keeps the eight threads of a store apart
-                    const float4 w0 = make_float4(d[0], x[0], d[1], x[1]), w1 = make_float4(d[2], x[2], d[3], x[3]);
-                    const int r = (tid >> 2) & 1;
-                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 * r]) = r ? w1 : w0;
-                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 - 2 * r]) = r ? w0 : w1;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        d[e] = add2(d[e], bias[e]);
+                        if (p.softplus) d[e] = scan_softplus2(d[e]);
+                        x[e] = mul2(d[e], x[e]);
+                    }
+                    float4 w0, w1, g;
+                    unpack2(d[0], w0.x, w0.z);
+                    unpack2(x[0], w0.y, w0.w);
+                    unpack2(d[1], w1.x, w1.z);
+                    unpack2(x[1], w1.y, w1.w);
+                    unpack2(dy[0], g.x, g.y);
+                    unpack2(dy[1], g.z, g.w);
+                    if (t >= left) w0 = w1 = g = make_float4(0.f, 0.f, 0.f, 0.f);      // nothing behind the last token: states and their gradients stay as they are
+                    const int o = (tid >> 2) & 1;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 * o]) = o ? w1 : w0;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 - 2 * o]) = o ? w0 : w1;
+                    *reinterpret_cast<float4*>(&sh.dy[buf][t][ec]) = g;
                 }
 #pragma unroll
                 for (int i = 0; i < BC; ++i) {
                     const int t = bt + i * BSTEP;
                     if (t >= TILE) continue;
                     float v[4];
-                    unpack4<DT>(rb[i], v);
+                    unpack4<DT>(r.b[i], v);
                     *reinterpret_cast<float4*>(half ? &sh.C[buf][t][bn] : &sh.B[buf][t][bn]) = make_float4(v[0], v[1], v[2], v[3]);
                 }
             }
-            if (k >= 1) {
-                const int buf = (k - 1) & 1, t0 = (k - 1) * TILE;
+            if (j >= 1) {
+                const int buf = (j - 1) & 1, t0 = (tiles - j) * TILE, left = len - t0;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     const int t = et + i * STEP;
-                    if (t >= TILE || t0 + t >= len) continue;
-                    const float4 s = *reinterpret_cast<const float4*>(&sh.y[buf][t][ec]);
-                    float y[4] = {s.x, s.y, s.z, s.w}, x[4], z[4];
-                    unpack4<DT>(x2[i], x);
-                    if (p.z) unpack4<DT>(z2[i], z);
+                    if (t >= TILE || t >= left) continue;
+                    const float4 fg = *reinterpret_cast<const float4*>(&sh.gB[buf][t][ec]), fe = *reinterpret_cast<const float4*>(&sh.eA[buf][t][ec]);
+                    f32x2 x[2], s[2], dy[2], ox[2], od[2], oz[2];
+                    const f32x2 gB[2] = {lo2(fg), hi2(fg)}, eA[2] = {lo2(fe), hi2(fe)};
+                    unpack4_2<DT>(k2.x[i], x);
+                    unpack4_2<DT>(k2.d[i], s);
+                    unpack4_2<DT>(k2.y[i], dy);
+                    if (p.z) {
+                        f32x2 z[2];
+                        const float4 fy = *reinterpret_cast<const float4*>(&sh.y[buf][t][ec]);
+                        const f32x2 y[2] = {lo2(fy), hi2(fy)};
+                        unpack4_2<DT>(k2.z[i], z);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (p.skip) y[e] = fmaf(skip[e], x[e], y[e]);
-                        if (p.z) y[e] *= z[e] * sigmoidf_(z[e]);
-                    }
-                    store4<DT>(p.y, (size_t)(sq.start + t0 + t) * D + cs.first + ec, min(valid, 4), vec, y);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) { x2[i] = x1[i]; z2[i] = z1[i]; x1[i] = rx[i]; z1[i] = rz[i]; }
-            if (k + 2 < tiles) request(k + 2);
-            __syncthreads();
-        }
-    }
-}
-
-// Backward: tiles of one checkpoint, from the last to the first.  Each is run forward from its checkpoint (a_n h_n[t - 1], from which h_n follows with one
-// operation, goes to shared memory), then backward.  dB and dC are summed over the channels of a thread, then over the lanes of a warp by a
-// butterfly that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by mkda_sum_rows: in a fixed order.
-template <int LPC, int CPT>
-struct ScanBwdShared {
-    using Sh = ScanShape<LPC, CPT, CKPT>;
-    float4 p[CKPT][CPT][SCAN_THREADS];                     // a h[t - 1]
-    float2 d[CKPT][Sh::CB];                                // d, d x
-    float dy[CKPT][Sh::CB];
-    float B[CKPT][Sh::NP], C[CKPT][Sh::NP];
-    float y[CKPT][Sh::YROW], gB[CKPT][Sh::YROW], eA[CKPT][Sh::YROW];
-    float red[SCAN_WARPS][CKPT][2 * Sh::NP];               // dB and dC of each warp
-    float bias[Sh::CB], skip[Sh::CB];
-};
-
-template <int DT, int LPC, int CPT>
-__global__ void __launch_bounds__(SCAN_THREADS) scan_bwd_kernel(const MkdaScanBwd a, const bool vec, const bool bvec) {
-    follow_stream();
-    constexpr int TILE = CKPT;
-    using Sh = ScanShape<LPC, CPT, TILE>;
-    constexpr int NP = Sh::NP, CB = Sh::CB, ROW = Sh::ROW, PIECES = Sh::PIECES, BC = Sh::BC, YROW = Sh::YROW;
-    extern __shared__ __align__(16) unsigned char raw_shared[];
-    ScanBwdShared<LPC, CPT>& sh = *reinterpret_cast<ScanBwdShared<LPC, CPT>*>(raw_shared);
-    const MkdaScanFwd& p = a.f;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.D, NST = p.NST;
-    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
-    for (int c = tid; c < CB; c += SCAN_THREADS) {
-        sh.bias[c] = p.dt_bias && c < cs.count ? p.dt_bias[cs.first + c] : 0.f;
-        sh.skip[c] = p.skip && c < cs.count ? p.skip[cs.first + c] : 0.f;
-    }
-    const int q = tid % LPC, c0 = tid / LPC * CPT, n0 = 4 * q;
-    f32x2 A[CPT][2], dA[CPT][2];
-#pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-        const float4 v = c0 + c < cs.count ? ld_states(p.A, cs.first + c0 + c, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-        A[c][0] = mul2(lo2(v), both(RCP_LN2));
-        A[c][1] = mul2(hi2(v), both(RCP_LN2));
-        dA[c][0] = dA[c][1] = both(0.f);
-    }
-    const int ec = tid % ROW * 8, et = tid / ROW, valid = cs.count - ec;
-    constexpr int STEP = SCAN_THREADS / ROW;
-    const int bn = tid % (NP / 8) * 8, bt = tid / (NP / 8), bvalid = NST - bn;
-    constexpr int BSTEP = SCAN_THREADS / (NP / 8);
-    float acc_skip[8], acc_bias[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc_skip[e] = acc_bias[e] = 0.f;
-    __syncthreads();
-
-    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-        const int n = p.S.order ? p.S.order[slot] : slot;
-        const Span sq = sequence(p.S, n);
-        const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
-        const size_t ck0 = p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT);
-        f32x2 G[CPT][2], h[CPT][2];                        // G: a[t + 1] g[t + 1]
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-            const float4 v = a.dht && c0 + c < cs.count ? ld_states(a.dht, (size_t)n * D + cs.first + c0 + c, n0, NST) : make_float4(0.f, 0.f, 0.f, 0.f);
-            G[c][0] = lo2(v);
-            G[c][1] = hi2(v);
-        }
-        Raw8 rx[PIECES], rd[PIECES], rz[PIECES], ry[PIECES], rB[BC], rC[BC];
-        float4 rh[CPT];
-        auto request = [&](int k) {
-            const int t0 = k * TILE;
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int t = t0 + et + i * STEP;
-                const int ok = et + i * STEP < TILE && t < len ? valid : 0;
-                const size_t tok = (size_t)(sq.start + t);
-                rx[i] = load8<DT>(p.x, tok * p.x_stride + cs.first + ec, ok, vec);
-                rd[i] = load8<DT>(p.dt, tok * p.dt_stride + cs.first + ec, ok, vec);
-                if (p.z) rz[i] = load8<DT>(p.z, tok * p.z_stride + cs.first + ec, ok, vec);
-                ry[i] = load8<DT>(a.dy, tok * D + cs.first + ec, ok, vec);
-            }
-#pragma unroll
-            for (int i = 0; i < BC; ++i) {
-                const int t = t0 + bt + i * BSTEP;
-                const int ok = bt + i * BSTEP < TILE && t < len ? bvalid : 0;
-                const size_t tok = (size_t)(sq.start + t);
-                rB[i] = load8<DT>(p.B, tok * p.B_stride + cs.group * NST + bn, ok, bvec);
-                rC[i] = load8<DT>(p.C, tok * p.C_stride + cs.group * NST + bn, ok, bvec);
-            }
-#pragma unroll
-            for (int c = 0; c < CPT; ++c)
-                rh[c] = c0 + c < cs.count ? *reinterpret_cast<const float4*>(p.ckpt + ((ck0 + k) * D + cs.first + c0 + c) * NP + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        if (tiles) request(tiles - 1);
-        for (int k = tiles - 1; k >= 0; --k) {
-            const int t0 = k * TILE;
-            float x[PIECES][8], z[PIECES][8], up[PIECES][8], s[PIECES][8];      // s: dt with its bias
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                unpack8<DT>(rx[i], x[i]);
-                unpack8<DT>(rd[i], s[i]);
-                if (p.z) unpack8<DT>(rz[i], z[i]);
-                unpack8<DT>(ry[i], up[i]);
-                const int t = et + i * STEP;
-                if (t >= TILE) continue;
-                const bool there = t0 + t < len;
-                float dy[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    s[i][e] += sh.bias[ec + e];
-                    const float d = there ? p.softplus ? scan_softplus(s[i][e]) : s[i][e] : 0.f;
-                    sh.d[t][ec + e] = make_float2(d, there ? d * x[i][e] : 0.f);
-                    dy[e] = p.z ? up[i][e] * z[i][e] * sigmoidf_(z[i][e]) : up[i][e];
-                }
-                st8<MKDA_F32>(&sh.dy[t][ec], 0, dy);
-            }
-#pragma unroll
-            for (int i = 0; i < BC; ++i) {
-                const int t = bt + i * BSTEP;
-                if (t >= TILE) continue;
-                float b[8], c[8];
-                unpack8<DT>(rB[i], b);
-                unpack8<DT>(rC[i], c);
-                st8<MKDA_F32>(&sh.B[t][bn], 0, b);
-                st8<MKDA_F32>(&sh.C[t][bn], 0, c);
-            }
-#pragma unroll
-            for (int c = 0; c < CPT; ++c) {
-                h[c][0] = lo2(rh[c]);
-                h[c][1] = hi2(rh[c]);
-            }
-            __syncthreads();
-            if (k > 0) request(k - 1);
-#pragma unroll 1
-            for (int t4 = 0; t4 < TILE; t4 += 4) {
-                float ys[CPT][4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int t = t4 + u;
-                    const float4 B = *reinterpret_cast<const float4*>(&sh.B[t][n0]), C = *reinterpret_cast<const float4*>(&sh.C[t][n0]);
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        const float2 d = sh.d[t][c0 + c];
-                        const f32x2 dd = both(d.x), dx = both(d.y);
-                        const f32x2 p0 = mul2(ex2f2_(mul2(A[c][0], dd)), h[c][0]), p1 = mul2(ex2f2_(mul2(A[c][1], dd)), h[c][1]);
-                        float4 v;
-                        unpack2(p0, v.x, v.y);
-                        unpack2(p1, v.z, v.w);
-                        sh.p[t][c][tid] = v;
-                        h[c][0] = fma2(dx, lo2(B), p0);
-                        h[c][1] = fma2(dx, hi2(B), p1);
-                        ys[c][u] = p.z ? sum2(fma2(h[c][1], hi2(C), mul2(h[c][0], lo2(C)))) : 0.f;
-                    }
-                }
-                if (p.z) {
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        lanes_sum4<LPC>(ys[c], q);
-                        put_sums<LPC, YROW>(&sh.y[0][0], t4, c0 + c, ys[c], q);
-                    }
-                }
-            }
-#pragma unroll 1
-            for (int t4 = TILE - 4; t4 >= 0; t4 -= 4) {
-                float gBs[CPT][4], eAs[CPT][4];
-#pragma unroll
-                for (int u = 3; u >= 0; --u) {
-                    const int t = t4 + u;
-                    const float4 B = *reinterpret_cast<const float4*>(&sh.B[t][n0]), C = *reinterpret_cast<const float4*>(&sh.C[t][n0]);
-                    f32x2 dB0 = both(0.f), dB1 = dB0, dC0 = dB0, dC1 = dB0;
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        const float2 d = sh.d[t][c0 + c];
-                        const f32x2 dd = both(d.x), dx = both(d.y), dy = both(sh.dy[t][c0 + c]);
-                        const float4 v = sh.p[t][c][tid];
-                        const f32x2 p0 = lo2(v), p1 = hi2(v);
-                        dC0 = fma2(dy, fma2(dx, lo2(B), p0), dC0);
-                        dC1 = fma2(dy, fma2(dx, hi2(B), p1), dC1);
-                        const f32x2 g0 = fma2(dy, lo2(C), G[c][0]), g1 = fma2(dy, hi2(C), G[c][1]);
-                        dB0 = fma2(dx, g0, dB0);
-                        dB1 = fma2(dx, g1, dB1);
-                        gBs[c][u] = sum2(fma2(g1, hi2(B), mul2(g0, lo2(B))));
-                        const f32x2 e0 = mul2(g0, p0), e1 = mul2(g1, p1);
-                        eAs[c][u] = sum2(fma2(e1, A[c][1], mul2(e0, A[c][0])));
-                        dA[c][0] = fma2(e0, dd, dA[c][0]);
-                        dA[c][1] = fma2(e1, dd, dA[c][1]);
-                        G[c][0] = mul2(ex2f2_(mul2(A[c][0], dd)), g0);
-                        G[c][1] = mul2(ex2f2_(mul2(A[c][1], dd)), g1);
-                    }
-                    // over the lanes of other channels: eight sums over 32 / LPC lanes, halved as long as there are lanes to share them
-                    float v[8];
-                    unpack2(dB0, v[0], v[1]);
-                    unpack2(dB1, v[2], v[3]);
-                    unpack2(dC0, v[4], v[5]);
-                    unpack2(dC1, v[6], v[7]);
-                    const int cl = lane / LPC;
-                    int first = 0;                         // of the sums that this lane ends with
-#pragma unroll
-                    for (int b = 0, w = 4; (LPC << b) < 32; ++b, w >>= 1) {
-                        if (w >= 1) {
-                            const bool up_ = cl >> b & 1;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (i >= w) break;
-                                const float give = up_ ? v[i] : v[i + w], keep = up_ ? v[i + w] : v[i];
-                                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, LPC << b);
-                            }
-                            first += up_ ? w : 0;
-                        } else {
-                            v[0] += __shfl_xor_sync(0xffffffffu, v[0], LPC << b);
+                        for (int e = 0; e < 2; ++e) {      // silu' = sg (1 + z (1 - sg))
+                            const f32x2 sg = sigmoidf2_(z[e]);
+                            oz[e] = mul2(mul2(dy[e], fma2(skip[e], x[e], y[e])), mul2(sg, fma2(z[e], fma2(sg, both(-1.f), both(1.f)), both(1.f))));
+                            dy[e] = mul2(dy[e], mul2(z[e], sg));
                         }
                     }
-                    constexpr int KEEP = LPC >= 4 ? LPC / 4 : 1;      // sums per lane: 1, 1, 2 or 4
-                    if (LPC > 2 || cl < 8) {
 #pragma unroll
-                        for (int i = 0; i < KEEP; ++i) sh.red[warp][t][(first + i >= 4 ? NP : 0) + n0 + ((first + i) & 3)] = v[i];
+                    for (int e = 0; e < 2; ++e) {
+                        s[e] = add2(s[e], bias[e]);
+                        const f32x2 d = p.softplus ? scan_softplus2(s[e]) : s[e];
+                        ox[e] = fma2(skip[e], dy[e], mul2(d, gB[e]));
+                        od[e] = fma2(x[e], gB[e], mul2(eA[e], both(LN2)));
+                        if (p.softplus) od[e] = mul2(od[e], sigmoidf2_(s[e]));
+                        acc_skip[e] = fma2(dy[e], x[e], acc_skip[e]);
+                        acc_bias[e] = add2(acc_bias[e], od[e]);
                     }
+                    const size_t at = (size_t)(sq.start + t0 + t) * D + cs.first + ec;
+                    const int ok = min(valid, 4);
+                    float v[4];
+                    auto store = [&](void* to, const f32x2 (&o)[2]) {
+                        unpack2(o[0], v[0], v[1]);
+                        unpack2(o[1], v[2], v[3]);
+                        store4<DT>(to, at, ok, vec, v);
+                    };
+                    store(a.dx, ox);
+                    store(a.ddt, od);
+                    if (p.z) store(a.dz, oz);
                 }
+                for (int i = tid; i < TILE * NP / 2; i += HELPERS) {      // four sums at a time: of dB the first half of a row, of dC the second
+                    const int t = i / (NP / 2), o = i % (NP / 2) * 4;
+                    if (t >= left) break;
+                    float4 v = *reinterpret_cast<const float4*>(&sh.red[buf][0][t][o]);
 #pragma unroll
-                for (int c = 0; c < CPT; ++c) {
-                    lanes_sum4<LPC>(gBs[c], q);
-                    put_sums<LPC, YROW>(&sh.gB[0][0], t4, c0 + c, gBs[c], q);
-                    lanes_sum4<LPC>(eAs[c], q);
-                    put_sums<LPC, YROW>(&sh.eA[0][0], t4, c0 + c, eAs[c], q);
+                    for (int w = 1; w < SCAN_WARPS; ++w) {
+                        const float4 u = *reinterpret_cast<const float4*>(&sh.red[buf][w][t][o]);
+                        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+                    }
+                    float* to = (o < NP ? a.part_B : a.part_C) + ((size_t)blockIdx.x * p.S.TT + sq.start + t0 + t) * NP + o % NP;
+                    *reinterpret_cast<float4*>(to) = v;
                 }
             }
-            __syncthreads();
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const int t = et + i * STEP;
-                if (t >= TILE || t0 + t >= len) continue;
-                float y[8], gB[8], eA[8], ox[8], od[8], oz[8];
-                if (p.z) ld8(&sh.y[t][ec], MKDA_F32, 0, y);
-                ld8(&sh.gB[t][ec], MKDA_F32, 0, gB);
-                ld8(&sh.eA[t][ec], MKDA_F32, 0, eA);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float dy = up[i][e];
-                    if (p.z) {
-                        const float sg = sigmoidf_(z[i][e]), act = z[i][e] * sg;
-                        oz[e] = dy * fmaf(sh.skip[ec + e], x[i][e], y[e]) * sg * fmaf(z[i][e], 1.f - sg, 1.f);
-                        dy *= act;
-                    }
-                    ox[e] = fmaf(sh.skip[ec + e], dy, sh.d[t][ec + e].x * gB[e]);
-                    od[e] = fmaf(x[i][e], gB[e], eA[e] * LN2);
-                    if (p.softplus) od[e] *= sigmoidf_(s[i][e]);
-                    acc_skip[e] = fmaf(dy, x[i][e], acc_skip[e]);
-                    acc_bias[e] += od[e];
-                }
-                const size_t at = (size_t)(sq.start + t0 + t) * D + cs.first + ec;
-                const int ok = min(valid, 8);
-                store8<DT>(a.dx, at, ok, vec, ox);
-                store8<DT>(a.ddt, at, ok, vec, od);
-                if (p.z) store8<DT>(a.dz, at, ok, vec, oz);
+                k2.x[i] = k1.x[i]; k2.d[i] = k1.d[i]; k2.z[i] = k1.z[i]; k2.y[i] = k1.y[i];
+                k1.x[i] = r.x[i]; k1.d[i] = r.d[i]; k1.z[i] = r.z[i]; k1.y[i] = r.y[i];
             }
-            for (int i = tid; i < TILE * NP * 2; i += SCAN_THREADS) {
-                const int t = i / (2 * NP), o = i % (2 * NP);
-                if (t0 + t >= len) break;
-                const float v = (sh.red[0][t][o] + sh.red[1][t][o]) + (sh.red[2][t][o] + sh.red[3][t][o]);
-                const size_t at = ((size_t)blockIdx.x * p.S.TT + sq.start + t0 + t) * NP;
-                if (o < NP) a.part_B[at + o] = v;
-                else a.part_C[at + o - NP] = v;
-            }
-            __syncthreads();                               // the shared tile may be written again
-        }
-        if (a.dh0) {
-#pragma unroll
-            for (int c = 0; c < CPT; ++c)
-                if (c0 + c < cs.count) {
-                    float4 v;
-                    unpack2(G[c][0], v.x, v.y);
-                    unpack2(G[c][1], v.z, v.w);
-                    st_states(a.dh0, (size_t)n * D + cs.first + c0 + c, n0, NST, v);
-                }
+            if (j + 3 < tiles) request(r, j + 3);
+            __syncthreads();
+        };
+        if (tiles > 0) request(even, 0);
+        if (tiles > 1) request(odd, 1);
+        for (int j = -1; j <= tiles; j += 2) {
+            step(even, j);
+            if (j + 1 <= tiles) step(odd, j + 1);
         }
     }
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-        if (c0 + c < cs.count) {
-            float4 v;
-            unpack2(dA[c][0], v.x, v.y);
-            unpack2(dA[c][1], v.z, v.w);
-            *reinterpret_cast<float4*>(a.part_A + ((size_t)blockIdx.y * D + cs.first + c0 + c) * NP + n0) = v;
-        }
-    // the threads that share eight channels, in order
-    float* all = reinterpret_cast<float*>(&sh.p[0][0][0]);      // [2][threads][8]
+    // the threads that share four channels, in order
+    float* all = reinterpret_cast<float*>(raw_shared);     // [2][HELPERS][4]: no tile is left
+    static_assert(sizeof(ScanBwdShared<LPC, CPT>) >= 2 * HELPERS * 16, "sums of all threads");
+    float v[4];
     __syncthreads();
-    st8<MKDA_F32>(all, tid * 8, acc_skip);
-    st8<MKDA_F32>(all, (SCAN_THREADS + tid) * 8, acc_bias);
+    unpack2(acc_skip[0], v[0], v[1]);
+    unpack2(acc_skip[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(all + tid * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    unpack2(acc_bias[0], v[0], v[1]);
+    unpack2(acc_bias[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(all + (HELPERS + tid) * 4) = make_float4(v[0], v[1], v[2], v[3]);
     __syncthreads();
-    for (int c = tid; c < cs.count; c += SCAN_THREADS) {
+    for (int c = tid; c < cs.count; c += HELPERS) {
         float s0 = 0.f, s1 = 0.f;
-        for (int i = c / 8; i < SCAN_THREADS; i += ROW) {
-            s0 += all[i * 8 + c % 8];
-            s1 += all[(SCAN_THREADS + i) * 8 + c % 8];
+        for (int i = c / 4; i < HELPERS; i += ROW) {
+            s0 += all[i * 4 + c % 4];
+            s1 += all[(HELPERS + i) * 4 + c % 4];
         }
         if (a.part_skip) a.part_skip[(size_t)blockIdx.y * D + cs.first + c] = s0;
         if (a.part_bias) a.part_bias[(size_t)blockIdx.y * D + cs.first + c] = s1;
@@ -670,27 +816,34 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
     int rc = MKDA_OK;
     with_dtype(p->dtype, [&](auto dt) {
         with_lanes(p->NST, [&](auto l) {
-            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value, smem = (int)sizeof(ScanFwdShared<LPC, 32>);
+            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const bool vec = wide_rows(*p, 4) && aligned16(p->y);
             const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC, 1, 32>::CB);
-            auto* kern = scan_fwd_kernel<DT, LPC>;
-            rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_fwd");
-            if (rc == MKDA_OK)
-                launch(kern, dim3(blocks, p->S.N < 65535 ? p->S.N : 65535), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
+            auto run = [&](auto tile) {
+                constexpr int TILE = decltype(tile)::value, smem = (int)sizeof(ScanFwdShared<LPC, TILE>);
+                auto* kern = scan_fwd_kernel<DT, LPC, TILE>;
+                rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_fwd");
+                if (rc == MKDA_OK)
+                    launch(kern, dim3(blocks, p->S.N < 65535 ? p->S.N : 65535), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
+            };
+            if ((long long)p->S.TT < SCAN_LONG * (long long)p->S.N) run(std::integral_constant<int, 32>());
+            else run(std::integral_constant<int, 64>());
         });
     });
     if (rc != MKDA_OK) return rc;
     return check_launch("scan_fwd");
 }
 
-template <int LPC>
-static constexpr int bwd_cpt() { return LPC <= 4 ? 2 : 2; }
+// Channels per thread of the backward kernel: two where that leaves a block for most SMs
+static bool two_channels(int D, int G, int LPC, int N) { return 2ll * blocks_of_channels(D, G, SCAN_THREADS / LPC * 2) * N > sm_count(); }
 
 extern "C" int mkda_scan_bwd_channel_blocks(int D, int G, int NST, int N) {
-    (void)N;
     int r = 0;
     if (D > 0 && G > 0 && NST > 0 && NST <= MKDA_SCAN_MAX_STATES)
-        with_lanes(NST, [&](auto l) { r = blocks_of_channels(D, G, ScanShape<decltype(l)::value, bwd_cpt<decltype(l)::value>(), CKPT>::CB); });
+        with_lanes(NST, [&](auto l) {
+            constexpr int LPC = decltype(l)::value;
+            r = blocks_of_channels(D, G, SCAN_THREADS / LPC * (two_channels(D, G, LPC, N) ? 2 : 1));
+        });
     return r;
 }
 
@@ -700,20 +853,26 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
         return set_error(MKDA_ERR_ARG, "scan_bwd: null argument");
     if (int e = bad_scan(p->f.D, p->f.NST, p->f.G, p->f.dtype)) return e;
     if (!good_sequences(p->f.S) || (p->f.S.cu && !p->f.S.ckpt_off)) return set_error(MKDA_ERR_ARG, "scan_bwd: bad sequences");
-    if (!aligned16(p->f.A) || !aligned16(p->f.ckpt) || !aligned16(p->dht) || !aligned16(p->dh0) || !aligned16(p->part_A))
+    if (!aligned16(p->f.A) || !aligned16(p->f.ckpt) || !aligned16(p->dht) || !aligned16(p->dh0) || !aligned16(p->part_A) || !aligned16(p->part_B) || !aligned16(p->part_C))
         return set_error(MKDA_ERR_ARG, "scan_bwd: A, states and partial sums must be 16-byte aligned");
     if (p->slots < 1 || p->slots > 65535 || p->channel_blocks != mkda_scan_bwd_channel_blocks(p->f.D, p->f.G, p->f.NST, p->f.S.N))
         return set_error(MKDA_ERR_ARG, "scan_bwd: 1 to 65535 slots, and as many blocks of channels as mkda_scan_bwd_channel_blocks says");
     int rc = MKDA_OK;
     with_dtype(p->f.dtype, [&](auto dt) {
         with_lanes(p->f.NST, [&](auto l) {
-            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value, CPT = bwd_cpt<LPC>();
+            constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const MkdaScanFwd& f = p->f;
-            const bool vec = wide_rows(f, 8) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
-            auto* kern = scan_bwd_kernel<DT, LPC, CPT>;
-            constexpr int smem = (int)sizeof(ScanBwdShared<LPC, CPT>);
-            rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
-            if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_THREADS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 8));
+            const bool vec = wide_rows(f, 4) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
+            auto run = [&](auto c) {
+                constexpr int CPT = decltype(c)::value, smem = (int)sizeof(ScanBwdShared<LPC, CPT>);
+                auto* kern = scan_bwd_kernel<DT, LPC, CPT>;
+                static const int regs = kernel_registers(reinterpret_cast<const void*>(kern));
+                if (regs < SCAN_BWD_LAUNCH_REGS) { rc = set_error(MKDA_ERR_LAUNCH, "scan_bwd: built with fewer registers than its roles share"); return; }
+                rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
+                if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 4));
+            };
+            if (two_channels(f.D, f.G, LPC, f.S.N)) run(std::integral_constant<int, 2>());
+            else run(std::integral_constant<int, 1>());
         });
     });
     return rc != MKDA_OK ? rc : check_launch("scan_bwd");
