@@ -96,8 +96,8 @@ typedef struct {
     float* part_bias;          /* [slots][D] or NULL */
 } MkdaScanBwd;
 int mkda_scan_bwd(const MkdaScanBwd* p, void* stream);
-/* Blocks of channels of the backward kernel for D channels in G groups (each group has as many) and NST states, over the given number of sequences; the padded number of states P. */
-int mkda_scan_bwd_channel_blocks(int D, int G, int NST, int N);
+/* Blocks of channels of the backward kernel for D channels in G groups (each group has as many) and NST states; the padded number of states P. */
+int mkda_scan_bwd_channel_blocks(int D, int G, int NST);
 int mkda_scan_padded_states(int NST);
 
 typedef struct {

@@ -389,7 +389,7 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
     for (int i : {SA, SB, SC, SSKIP, SBIAS, SH0})
         if (in[i].defined()) out[i] = new_cuda(in[i].sizes(), in[i].scalar_type(), dev);
     p.dx = out[SX].data_ptr(); p.ddt = out[SDT].data_ptr(); p.dz = mptr(out[SZ]); p.dh0 = fmptr(out[SH0]);
-    p.channel_blocks = mkda_scan_bwd_channel_blocks((int)D, (int)G, (int)N, q.s.N);
+    p.channel_blocks = mkda_scan_bwd_channel_blocks((int)D, (int)G, (int)N);
     // sequences are dealt to rows of blocks: enough of them for 16 blocks per SM; each leaves a row of sums for A, D and dt_bias
     p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(q.s.N, (16 * sms() + p.channel_blocks - 1) / p.channel_blocks));
     const std::vector<int64_t> part_size{p.channel_blocks, TT * P};

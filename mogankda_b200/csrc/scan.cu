@@ -109,9 +109,10 @@ __device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB)
 // barrier joins them once a tile.  A channel's chain is short and there are few warps of it (4096 channels are 512), so what counts is how many cycles a token takes a warp that
 // has a scheduler to itself: with the elementwise part in the same warps 168, of which 32 are the exponentials of the special function unit.
 constexpr int SCAN_HELPERS = 256, SCAN_LONG = 256;
-// registers of the backward kernel's two roles, out of 168 for each of 384 threads: 128 x 240 + 256 x 128 = 63 488 of 64 512
-constexpr int SCAN_BWD_WALK_REGS = 240, SCAN_BWD_HELP_REGS = 128, SCAN_BWD_LAUNCH_REGS = 168;
-static_assert(SCAN_THREADS * SCAN_BWD_WALK_REGS + SCAN_HELPERS * SCAN_BWD_HELP_REGS <= (SCAN_THREADS + SCAN_HELPERS) * SCAN_BWD_LAUNCH_REGS, "register split");
+// The backward kernel: threads beside those on the chain, blocks per SM, and the registers of the two roles out of those of the launch
+constexpr int SCAN_BWD_HELPERS = 128, SCAN_BWD_THREADS = SCAN_THREADS + SCAN_BWD_HELPERS, SCAN_BWD_BLOCKS = 2, SCAN_BWD_WALK_REGS = 152, SCAN_BWD_HELP_REGS = 104, SCAN_BWD_LAUNCH_REGS = 128;
+static_assert(SCAN_THREADS * SCAN_BWD_WALK_REGS + SCAN_BWD_HELPERS * SCAN_BWD_HELP_REGS <= SCAN_BWD_THREADS * SCAN_BWD_LAUNCH_REGS &&
+              SCAN_BWD_THREADS * SCAN_BWD_LAUNCH_REGS * SCAN_BWD_BLOCKS <= 65536, "register split");
 template <int LPC, int TILE>
 struct ScanFwdShared {
     using Sh = ScanShape<LPC, 1, TILE>;
@@ -335,13 +336,16 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
     }
 }
 
-// Backward: tiles of one checkpoint, from the last to the first, with the same two roles.  A tile is run forward from its checkpoint (a_n h_n[t - 1], from which h_n follows with
-// one operation, stays in the registers of the lane), then backward, where the decays are formed again.  dB and dC are summed over the channels of a thread, then over
-// the lanes of a warp by a butterfly that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by
-// mkda_sum_rows: in a fixed order.  Two channels per thread where there are enough of them: B, C and those sums are shared by both.
-template <int LPC, int CPT>
+// Backward: tiles of one checkpoint, from the last to the first, with the same two roles.  A tile is run forward from its checkpoint, then backward:
+// a_n h_n[t - 1], from which h_n follows with one operation, stays in the registers of the lane in between (the decays beside it, not formed twice, left the rest too few:
+// 406 us where this takes 400).  dB and dC are summed over the lanes of a warp by a butterfly
+// that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by mkda_sum_rows: in a fixed order.  Two blocks per SM: the
+// chain and the butterflies are latency, and two channels per thread, which halve the butterflies but take the registers of the second block, were slower (525 us).
+template <int DT, int LPC>
 struct ScanBwdShared {
-    using Sh = ScanShape<LPC, CPT, CKPT>;
+    static constexpr int PIECES = (CKPT * SCAN_THREADS / LPC / 4 + SCAN_BWD_HELPERS - 1) / SCAN_BWD_HELPERS;
+    Raw4<DT> kept[4][4][PIECES][SCAN_BWD_HELPERS];         // x, dt, z and dy of the last tiles, each thread's own: registers are what the second block needs
+    using Sh = ScanShape<LPC, 1, CKPT>;
     float2 d[2][CKPT][Sh::CB];                             // d, d x
     float dy[2][CKPT][Sh::CB];
     float B[2][CKPT][Sh::NP], C[2][CKPT][Sh::NP];
@@ -349,186 +353,138 @@ struct ScanBwdShared {
     float red[2][SCAN_WARPS][CKPT][2 * Sh::NP];            // dB and dC of each warp
 };
 
-template <int DT, int LPC, int CPT>
-__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kernel(const MkdaScanBwd a, const bool vec, const bool bvec) {
+template <int DT, int LPC>
+__global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_kernel(const MkdaScanBwd a, const bool vec, const bool bvec) {
     follow_stream();
     constexpr int TILE = CKPT;
-    using Sh = ScanShape<LPC, CPT, TILE>;
+    using Sh = ScanShape<LPC, 1, TILE>;
     constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
     extern __shared__ __align__(16) unsigned char raw_shared[];
-    auto& sh = *reinterpret_cast<ScanBwdShared<LPC, CPT>*>(raw_shared);
+    auto& sh = *reinterpret_cast<ScanBwdShared<DT, LPC>*>(raw_shared);
     const MkdaScanFwd& p = a.f;
     const int D = p.D, NST = p.NST;
     const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
     if (threadIdx.x < SCAN_THREADS) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(SCAN_BWD_WALK_REGS));
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = tid % LPC, c0 = tid / LPC * CPT, n0 = 4 * q, cl = lane / LPC;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q, cl = lane / LPC;
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool z = p.z;
-        bool there[CPT];
-        Four A[CPT], dA[CPT];
+        const bool z = p.z, there = c0 < cs.count;
+        const size_t ch = cs.first + c0;
+        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero), dA = four(zero);
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-            there[c] = c0 + c < cs.count;
-            A[c] = four(there[c] ? ld_states(p.A, cs.first + c0 + c, n0, NST) : zero);
-            dA[c] = four(zero);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) A[c].v[i] = mul2(A[c].v[i], both(RCP_LN2));
-        }
+        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
         for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
             const int n = p.S.order ? p.S.order[slot] : slot;
             const Span sq = sequence(p.S, n);
             const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
             const size_t ck0 = p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT);
-            Four G[CPT];                                   // a[t + 1] g[t + 1]
-            float4 rh[CPT];
-            auto request = [&](int k) {
-#pragma unroll
-                for (int c = 0; c < CPT; ++c)
-                    rh[c] = there[c] ? *reinterpret_cast<const float4*>(p.ckpt + ((ck0 + k) * D + cs.first + c0 + c) * NP + n0) : zero;
-            };
-#pragma unroll
-            for (int c = 0; c < CPT; ++c) G[c] = four(a.dht && there[c] ? ld_states(a.dht, (size_t)n * D + cs.first + c0 + c, n0, NST) : zero);
-            if (tiles) request(tiles - 1);
+            auto checkpoint = [&](int k) { return there ? *reinterpret_cast<const float4*>(p.ckpt + ((ck0 + k) * D + ch) * NP + n0) : zero; };
+            Four G = four(a.dht && there ? ld_states(a.dht, (size_t)n * D + ch, n0, NST) : zero);      // a[t + 1] g[t + 1]
+            float4 rh = tiles ? checkpoint(tiles - 1) : zero;
             __syncthreads();                               // the first tile is there
             for (int j = 0; j < tiles; ++j) {
                 const int buf = j & 1;
-                const float* sd = &sh.d[buf][0][c0].x;
+                const float2* sd = &sh.d[buf][0][c0];
                 const float* sdy = &sh.dy[buf][0][c0];
                 const float* sB = &sh.B[buf][0][n0];
                 const float* sC = &sh.C[buf][0][n0];
-                auto fetch_d = [&](int t, float (&d)[CPT], float (&dx)[CPT]) {
-                    if constexpr (CPT == 2) {
-                        const float4 v = *reinterpret_cast<const float4*>(sd + t * 2 * CB);
-                        d[0] = v.x; dx[0] = v.y; d[1] = v.z; dx[1] = v.w;
-                    } else {
-                        const float2 v = *reinterpret_cast<const float2*>(sd + t * 2 * CB);
-                        d[0] = v.x; dx[0] = v.y;
-                    }
-                };
-                Four h[CPT], P[TILE][CPT];
-#pragma unroll
-                for (int c = 0; c < CPT; ++c) h[c] = four(rh[c]);
-                float ysum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)];      // sums wait in registers: a store in between would keep reads behind it
+                constexpr int SUMS = TILE / 4 * (LPC == 2 ? 2 : 1);      // sums over states that a lane ends with
+                Four h = four(rh), P[TILE], dAt = four(zero);
+                float ysum[SUMS];                          // they wait in registers: a store in between would keep reads behind it
 #pragma unroll
                 for (int t4 = 0; t4 < TILE; t4 += 4) {
-                    float ys[CPT][4];
+                    float ys[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        float d[CPT], dx[CPT];
-                        fetch_d(t4 + u, d, dx);
+                        const float2 d = sd[(t4 + u) * CB];
                         const Four B = four(*reinterpret_cast<const float4*>(sB + (t4 + u) * NP)), C = four(*reinterpret_cast<const float4*>(sC + (t4 + u) * NP));
+                        f32x2 y;
 #pragma unroll
-                        for (int c = 0; c < CPT; ++c) {
-                            f32x2 y;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const f32x2 v = mul2(ex2f2_(mul2(A[c].v[i], both(d[c]))), h[c].v[i]);
-                                P[t4 + u][c].v[i] = v;
-                                h[c].v[i] = fma2(both(dx[c]), B.v[i], v);
-                                y = i ? fma2(h[c].v[i], C.v[i], y) : mul2(h[c].v[i], C.v[i]);
-                            }
-                            ys[c][u] = sum2(y);
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x2 v = mul2(ex2f2_(mul2(A.v[i], both(d.x))), h.v[i]);
+                            P[t4 + u].v[i] = v;
+                            h.v[i] = fma2(both(d.y), B.v[i], v);
+                            y = i ? fma2(h.v[i], C.v[i], y) : mul2(h.v[i], C.v[i]);
                         }
+                        ys[u] = sum2(y);
                     }
                     if (z) {
-#pragma unroll
-                        for (int c = 0; c < CPT; ++c) {
-                            lanes_sum4<LPC>(ys[c], q);
-                            ysum[c][t4 / 4] = ys[c][0];
-                            if constexpr (LPC == 2) ysum[c][TILE / 4 + t4 / 4] = ys[c][1];
-                        }
+                        lanes_sum4<LPC>(ys, q);
+                        ysum[t4 / 4] = ys[0];
+                        if constexpr (LPC == 2) ysum[TILE / 4 + t4 / 4] = ys[1];
                     }
                 }
-                if (tiles - 2 - j >= 0) request(tiles - 2 - j);
+                if (tiles - 2 - j >= 0) rh = checkpoint(tiles - 2 - j);
                 asm volatile("" ::: "memory");             // what the first pass has read is read again: kept for sixteen tokens it would not fit into the registers
                 constexpr int KEEP = LPC >= 4 ? LPC / 4 : 1;      // sums of dB and dC per lane: 1, 1, 2 or 4
-                float gsum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)], esum[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)], red[TILE][KEEP];
+                float gsum[SUMS], esum[SUMS], red[TILE][KEEP];
                 int first = 0;                             // of the sums of dB and dC that this lane ends with
 #pragma unroll
                 for (int t4 = TILE - 4; t4 >= 0; t4 -= 4) {
                     __syncwarp();                          // reads of the next tokens stay behind it, or their number takes the registers
-                    float gBs[CPT][4], eAs[CPT][4];
+                    float gBs[4], eAs[4];
 #pragma unroll
                     for (int u = 3; u >= 0; --u) {
                         const int t = t4 + u;
-                        float d[CPT], dx[CPT], dy[CPT];
-                        fetch_d(t, d, dx);
-                        if constexpr (CPT == 2) {
-                            const float2 v = *reinterpret_cast<const float2*>(sdy + t * CB);
-                            dy[0] = v.x; dy[1] = v.y;
-                        } else {
-                            dy[0] = sdy[t * CB];
-                        }
+                        const float2 d = sd[t * CB];
+                        const float dy = sdy[t * CB];
                         const Four B = four(*reinterpret_cast<const float4*>(sB + t * NP)), C = four(*reinterpret_cast<const float4*>(sC + t * NP));
-                        f32x2 dB[2], dC[2];
+                        f32x2 v[4], gb, ea;
 #pragma unroll
-                        for (int c = 0; c < CPT; ++c) {
-                            f32x2 gb, ea;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const f32x2 v = P[t][c].v[i], hh = fma2(both(dx[c]), B.v[i], v), g = fma2(both(dy[c]), C.v[i], G[c].v[i]);
-                                dC[i] = c ? fma2(both(dy[c]), hh, dC[i]) : mul2(both(dy[c]), hh);
-                                dB[i] = c ? fma2(both(dx[c]), g, dB[i]) : mul2(both(dx[c]), g);
-                                const f32x2 e = mul2(g, v);
-                                gb = i ? fma2(g, B.v[i], gb) : mul2(g, B.v[i]);
-                                ea = i ? fma2(e, A[c].v[i], ea) : mul2(e, A[c].v[i]);
-                                dA[c].v[i] = fma2(e, both(d[c]), dA[c].v[i]);
-                                G[c].v[i] = mul2(ex2f2_(mul2(A[c].v[i], both(d[c]))), g);
-                            }
-                            gBs[c][u] = sum2(gb);
-                            eAs[c][u] = sum2(ea);
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x2 g = fma2(both(dy), C.v[i], G.v[i]), e = mul2(g, P[t].v[i]);
+                            v[i] = mul2(both(d.y), g);
+                            v[i + 2] = mul2(both(dy), fma2(both(d.y), B.v[i], P[t].v[i]));
+                            gb = i ? fma2(g, B.v[i], gb) : mul2(g, B.v[i]);
+                            ea = i ? fma2(e, A.v[i], ea) : mul2(e, A.v[i]);
+                            dAt.v[i] = fma2(e, both(d.x), dAt.v[i]);
+                            G.v[i] = mul2(ex2f2_(mul2(A.v[i], both(d.x))), g);
                         }
+                        gBs[u] = sum2(gb);
+                        eAs[u] = sum2(ea);
                         // over the lanes of other channels: eight sums over 32 / LPC lanes, halved as long as there are lanes to share them
-                        float v[8];
-                        unpack2(dB[0], v[0], v[1]);
-                        unpack2(dB[1], v[2], v[3]);
-                        unpack2(dC[0], v[4], v[5]);
-                        unpack2(dC[1], v[6], v[7]);
+                        float w[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) unpack2(v[i], w[2 * i], w[2 * i + 1]);
                         int at = 0;
 #pragma unroll
-                        for (int b = 0, w = 4; (LPC << b) < 32; ++b, w >>= 1) {
-                            if (w >= 1) {
+                        for (int b = 0, k = 4; (LPC << b) < 32; ++b, k >>= 1) {
+                            if (k >= 1) {
                                 const bool up = cl >> b & 1;
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    if (i >= w) break;
-                                    const float give = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
-                                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, LPC << b);
+                                    if (i >= k) break;
+                                    const float give = up ? w[i] : w[i + k], keep = up ? w[i + k] : w[i];
+                                    w[i] = keep + __shfl_xor_sync(0xffffffffu, give, LPC << b);
                                 }
-                                at += up ? w : 0;
+                                at += up ? k : 0;
                             } else {
-                                v[0] += __shfl_xor_sync(0xffffffffu, v[0], LPC << b);
+                                w[0] += __shfl_xor_sync(0xffffffffu, w[0], LPC << b);
                             }
                         }
                         first = at;
 #pragma unroll
-                        for (int i = 0; i < KEEP; ++i) red[t][i] = v[i];
+                        for (int i = 0; i < KEEP; ++i) red[t][i] = w[i];
                     }
-#pragma unroll
-                    for (int c = 0; c < CPT; ++c) {
-                        lanes_sum4<LPC>(gBs[c], q);
-                        lanes_sum4<LPC>(eAs[c], q);
-                        gsum[c][t4 / 4] = gBs[c][0];
-                        esum[c][t4 / 4] = eAs[c][0];
-                        if constexpr (LPC == 2) {
-                            gsum[c][TILE / 4 + t4 / 4] = gBs[c][1];
-                            esum[c][TILE / 4 + t4 / 4] = eAs[c][1];
-                        }
+                    lanes_sum4<LPC>(gBs, q);
+                    lanes_sum4<LPC>(eAs, q);
+                    gsum[t4 / 4] = gBs[0];
+                    esum[t4 / 4] = eAs[0];
+                    if constexpr (LPC == 2) {
+                        gsum[TILE / 4 + t4 / 4] = gBs[1];
+                        esum[TILE / 4 + t4 / 4] = eAs[1];
                     }
                 }
-                auto put = [&](float* to, const float (&v)[CPT][TILE / 4 * (LPC == 2 ? 2 : 1)]) {
+                auto put = [&](float* to, const float (&v)[SUMS]) {
 #pragma unroll
-                    for (int i = 0; i < TILE / 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < CPT; ++c) {
-                            if constexpr (LPC == 2) {
-                                to[(4 * i + q) * YROW + c0 + c] = v[c][i];
-                                to[(4 * i + q + 2) * YROW + c0 + c] = v[c][TILE / 4 + i];
-                            } else if (LPC == 4 || q < 4) {
-                                to[(4 * i + (q & 3)) * YROW + c0 + c] = v[c][i];
-                            }
+                    for (int i = 0; i < TILE / 4; ++i) {
+                        if constexpr (LPC == 2) {
+                            to[(4 * i + q) * YROW + c0] = v[i];
+                            to[(4 * i + q + 2) * YROW + c0] = v[TILE / 4 + i];
+                        } else if (LPC == 4 || q < 4) {
+                            to[(4 * i + (q & 3)) * YROW + c0] = v[i];
                         }
+                    }
                 };
                 if (z) put(&sh.y[buf][0][0], ysum);
                 put(&sh.gB[buf][0][0], gsum);
@@ -539,18 +495,14 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
 #pragma unroll
                         for (int i = 0; i < KEEP; ++i) sh.red[buf][warp][t][(first + i >= 4 ? NP : 0) + n0 + ((first + i) & 3)] = red[t][i];
                 }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) dA.v[i] = add2(dA.v[i], dAt.v[i]);      // tile by tile: the sum over thousands of tokens loses less
                 __syncthreads();
             }
-            if (a.dh0) {
-#pragma unroll
-                for (int c = 0; c < CPT; ++c)
-                    if (there[c]) st_states(a.dh0, (size_t)n * D + cs.first + c0 + c, n0, NST, flat(G[c]));
-            }
+            if (a.dh0 && there) st_states(a.dh0, (size_t)n * D + ch, n0, NST, flat(G));
             __syncthreads();                               // the last tile has been stored
         }
-#pragma unroll
-        for (int c = 0; c < CPT; ++c)
-            if (there[c]) *reinterpret_cast<float4*>(a.part_A + ((size_t)blockIdx.y * D + cs.first + c0 + c) * NP + n0) = flat(dA[c]);
+        if (there) *reinterpret_cast<float4*>(a.part_A + ((size_t)blockIdx.y * D + ch) * NP + n0) = flat(dA);
         __syncthreads();
         __syncthreads();                                   // the elementwise part's sums over tokens
         return;
@@ -558,7 +510,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
 
     // the elementwise part, laid out as in the forward kernel
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(SCAN_BWD_HELP_REGS));
-    constexpr int HELPERS = SCAN_HELPERS, ROW = CB / 4, STEP = HELPERS / ROW, PIECES = (TILE * ROW + HELPERS - 1) / HELPERS;
+    constexpr int HELPERS = SCAN_BWD_HELPERS, ROW = CB / 4, STEP = HELPERS / ROW, PIECES = (TILE * ROW + HELPERS - 1) / HELPERS;
     constexpr int BROW = NP / 4, BSTEP = HELPERS / 2 / BROW, BC = (TILE * BROW * 2 + HELPERS - 1) / HELPERS;
     const int tid = threadIdx.x - SCAN_THREADS, ec = tid % ROW * 4, et = tid / ROW, valid = cs.count - ec;
     const int half = tid / (HELPERS / 2), bn = tid % BROW * 4, bt = tid % (HELPERS / 2) / BROW, bvalid = NST - bn;
@@ -577,9 +529,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
         const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
         const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
         struct Rows { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], y[PIECES], b[BC]; };
-        struct Kept { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], y[PIECES]; };
         Rows even, odd;                                    // rows on their way, of every other tile: requested two steps before they are used
-        Kept k1, k2;                                       // of the two tiles behind the one that is formed
         const size_t col = (size_t)(cs.first + ec) * SIZE;
         auto request = [&](Rows& r, int j) {               // the j-th tile from the end
             const int t0 = (tiles - 1 - j) * TILE, left = len - t0;
@@ -608,6 +558,11 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
                 for (int i = 0; i < PIECES; ++i) {
                     const int t = et + i * STEP;
                     if (t >= TILE) continue;
+                    auto& kept = sh.kept[(j + 1) & 3];
+                    kept[0][i][tid] = r.x[i];
+                    kept[1][i][tid] = r.d[i];
+                    if (p.z) kept[2][i][tid] = r.z[i];
+                    kept[3][i][tid] = r.y[i];
                     f32x2 x[2], d[2], dy[2];
                     unpack4_2<DT>(r.x[i], x);
                     unpack4_2<DT>(r.d[i], d);
@@ -655,14 +610,15 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
                     const float4 fg = *reinterpret_cast<const float4*>(&sh.gB[buf][t][ec]), fe = *reinterpret_cast<const float4*>(&sh.eA[buf][t][ec]);
                     f32x2 x[2], s[2], dy[2], ox[2], od[2], oz[2];
                     const f32x2 gB[2] = {lo2(fg), hi2(fg)}, eA[2] = {lo2(fe), hi2(fe)};
-                    unpack4_2<DT>(k2.x[i], x);
-                    unpack4_2<DT>(k2.d[i], s);
-                    unpack4_2<DT>(k2.y[i], dy);
+                    auto& kept = sh.kept[(j - 1) & 3];
+                    unpack4_2<DT>(kept[0][i][tid], x);
+                    unpack4_2<DT>(kept[1][i][tid], s);
+                    unpack4_2<DT>(kept[3][i][tid], dy);
                     if (p.z) {
                         f32x2 z[2];
                         const float4 fy = *reinterpret_cast<const float4*>(&sh.y[buf][t][ec]);
                         const f32x2 y[2] = {lo2(fy), hi2(fy)};
-                        unpack4_2<DT>(k2.z[i], z);
+                        unpack4_2<DT>(kept[2][i][tid], z);
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {      // silu' = sg (1 + z (1 - sg))
                             const f32x2 sg = sigmoidf2_(z[e]);
@@ -705,11 +661,6 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
                     *reinterpret_cast<float4*>(to) = v;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                k2.x[i] = k1.x[i]; k2.d[i] = k1.d[i]; k2.z[i] = k1.z[i]; k2.y[i] = k1.y[i];
-                k1.x[i] = r.x[i]; k1.d[i] = r.d[i]; k1.z[i] = r.z[i]; k1.y[i] = r.y[i];
-            }
             if (j + 3 < tiles) request(r, j + 3);
             __syncthreads();
         };
@@ -722,7 +673,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_bwd_kerne
     }
     // the threads that share four channels, in order
     float* all = reinterpret_cast<float*>(raw_shared);     // [2][HELPERS][4]: no tile is left
-    static_assert(sizeof(ScanBwdShared<LPC, CPT>) >= 2 * HELPERS * 16, "sums of all threads");
+    static_assert(sizeof(ScanBwdShared<DT, LPC>) >= 2 * HELPERS * 16, "sums of all threads");
     float v[4];
     __syncthreads();
     unpack2(acc_skip[0], v[0], v[1]);
@@ -834,16 +785,10 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
     return check_launch("scan_fwd");
 }
 
-// Channels per thread of the backward kernel: two where that leaves a block for most SMs
-static bool two_channels(int D, int G, int LPC, int N) { return 2ll * blocks_of_channels(D, G, SCAN_THREADS / LPC * 2) * N > sm_count(); }
-
-extern "C" int mkda_scan_bwd_channel_blocks(int D, int G, int NST, int N) {
+extern "C" int mkda_scan_bwd_channel_blocks(int D, int G, int NST) {
     int r = 0;
     if (D > 0 && G > 0 && NST > 0 && NST <= MKDA_SCAN_MAX_STATES)
-        with_lanes(NST, [&](auto l) {
-            constexpr int LPC = decltype(l)::value;
-            r = blocks_of_channels(D, G, SCAN_THREADS / LPC * (two_channels(D, G, LPC, N) ? 2 : 1));
-        });
+        with_lanes(NST, [&](auto l) { r = blocks_of_channels(D, G, ScanShape<decltype(l)::value, 1, CKPT>::CB); });
     return r;
 }
 
@@ -855,7 +800,7 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
     if (!good_sequences(p->f.S) || (p->f.S.cu && !p->f.S.ckpt_off)) return set_error(MKDA_ERR_ARG, "scan_bwd: bad sequences");
     if (!aligned16(p->f.A) || !aligned16(p->f.ckpt) || !aligned16(p->dht) || !aligned16(p->dh0) || !aligned16(p->part_A) || !aligned16(p->part_B) || !aligned16(p->part_C))
         return set_error(MKDA_ERR_ARG, "scan_bwd: A, states and partial sums must be 16-byte aligned");
-    if (p->slots < 1 || p->slots > 65535 || p->channel_blocks != mkda_scan_bwd_channel_blocks(p->f.D, p->f.G, p->f.NST, p->f.S.N))
+    if (p->slots < 1 || p->slots > 65535 || p->channel_blocks != mkda_scan_bwd_channel_blocks(p->f.D, p->f.G, p->f.NST))
         return set_error(MKDA_ERR_ARG, "scan_bwd: 1 to 65535 slots, and as many blocks of channels as mkda_scan_bwd_channel_blocks says");
     int rc = MKDA_OK;
     with_dtype(p->f.dtype, [&](auto dt) {
@@ -863,16 +808,12 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const MkdaScanFwd& f = p->f;
             const bool vec = wide_rows(f, 4) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
-            auto run = [&](auto c) {
-                constexpr int CPT = decltype(c)::value, smem = (int)sizeof(ScanBwdShared<LPC, CPT>);
-                auto* kern = scan_bwd_kernel<DT, LPC, CPT>;
-                static const int regs = kernel_registers(reinterpret_cast<const void*>(kern));
-                if (regs < SCAN_BWD_LAUNCH_REGS) { rc = set_error(MKDA_ERR_LAUNCH, "scan_bwd: built with fewer registers than its roles share"); return; }
-                rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
-                if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 4));
-            };
-            if (two_channels(f.D, f.G, LPC, f.S.N)) run(std::integral_constant<int, 2>());
-            else run(std::integral_constant<int, 1>());
+            constexpr int smem = (int)sizeof(ScanBwdShared<DT, LPC>);
+            auto* kern = scan_bwd_kernel<DT, LPC>;
+            static const int regs = kernel_registers(reinterpret_cast<const void*>(kern));
+            if (regs != SCAN_BWD_LAUNCH_REGS) { rc = set_error(MKDA_ERR_LAUNCH, "scan_bwd: built with other registers than its roles share"); return; }
+            rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
+            if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_BWD_THREADS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 4));
         });
     });
     return rc != MKDA_OK ? rc : check_launch("scan_bwd");

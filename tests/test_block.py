@@ -89,7 +89,7 @@ def test_entry_points_refuse_without_launching(lib):
     f = _filled(S["MkdaScanFwd"](), ("x", "dt", "B", "C", "A", "y", "ckpt"), **numbers)
     f.S.TT, f.S.N, f.S.T = 4, 2, 2
     _refused(lib, "mkda_scan_fwd", f, scan + seqs + [("y", 0), ("h0", 0x30008), ("ht", 0x30008), ("ckpt", 0x30008), ("S.cu", 0x30000)])
-    b = _filled(S["MkdaScanBwd"](), ("dy", "dx", "ddt", "part_A", "part_B", "part_C"), slots=1, channel_blocks=lib.mkda_scan_bwd_channel_blocks(8, 2, 16, 2))
+    b = _filled(S["MkdaScanBwd"](), ("dy", "dx", "ddt", "part_A", "part_B", "part_C"), slots=1, channel_blocks=lib.mkda_scan_bwd_channel_blocks(8, 2, 16))
     b.f = f
     _refused(lib, "mkda_scan_bwd", b, [("f." + n, v) for n, v in scan + seqs] + [("f.ckpt", 0), ("f.z", 0x30000), ("dy", 0), ("part_A", 0), ("part_B", 0), ("slots", 0),
                                       ("slots", 65536), ("channel_blocks", 1), ("dht", 0x30004), ("dh0", 0x30004)])
