@@ -694,41 +694,78 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
     }
 }
 
-// One token of each sequence.  Bound by HBM: the states are read and written.  A thread has four states of a channel, as above.
-template <int DT, int LPC>
-__global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p) {
+// One token of each sequence.  Bound by HBM: the states are read and written.  A thread has four states of a channel, as above, of ROWS = 4 or 1 sequences, whose states
+// are requested together and share A.  With four the lanes of a channel share the rest: a lane reads x, dt and z of one of the sequences (two lanes: of two) and ends with its sum.
+template <int DT, int LPC, int ROWS>
+__global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, const bool bvec) {
     follow_stream();
-    const int q = threadIdx.x % LPC, c = blockIdx.x * (128 / LPC) + threadIdx.x / LPC, n = blockIdx.y, n0 = 4 * q, D = p.D, NST = p.NST;
+    constexpr int MINE = ROWS == 1 ? 1 : LPC == 2 ? 2 : 1;      // sequences whose elementwise part this lane has: q & 3, or q and q + 2
+    const int q = threadIdx.x % LPC, c = blockIdx.x * (128 / LPC) + threadIdx.x / LPC, first = blockIdx.y * ROWS, n0 = 4 * q, D = p.D, NST = p.NST;
     const bool there = c < D;
-    float y = 0.f;
-    if (there) {
-        const size_t row = (size_t)n * D + c;
-        const float4 h = ld_states(p.state, row, n0, NST), A = ld_states(p.A, c, n0, NST);
-        const float x = ld1(p.x, DT, (size_t)n * p.x_stride + c);
-        float d = ld1(p.dt, DT, (size_t)n * p.dt_stride + c) + (p.dt_bias ? p.dt_bias[c] : 0.f);
-        if (p.softplus) d = scan_softplus(d);
-        const float hs[4] = {h.x, h.y, h.z, h.w}, As[4] = {A.x, A.y, A.z, A.w};
-        float o[4];
-        const int g = c / (D / p.G);
+    const int rows = there ? min(ROWS, p.N - first) : 0, g = there && p.G > 1 ? c / (D / p.G) : 0, mine = ROWS == 1 ? 0 : q & 3;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 h[ROWS];
+    Raw4<DT> rB[ROWS], rC[ROWS];
+    const size_t row = (size_t)first * D + c, at = (size_t)g * NST + n0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool ok = n0 + i < NST;
-            const float B = ok ? ld1(p.B, DT, (size_t)n * p.B_stride + g * NST + n0 + i) : 0.f, C = ok ? ld1(p.C, DT, (size_t)n * p.C_stride + g * NST + n0 + i) : 0.f;
-            o[i] = fmaf(ex2f_(As[i] * RCP_LN2 * d), hs[i], d * x * B);
-            y = fmaf(C, o[i], y);
-        }
-        st_states(p.state, row, n0, NST, make_float4(o[0], o[1], o[2], o[3]));
-        if (q == 0 && p.skip) y = fmaf(p.skip[c], x, y);
+    for (int r = 0; r < ROWS; ++r) {
+        h[r] = r < rows ? ld_states(p.state, row + (size_t)r * D, n0, NST) : zero;
+        rB[r] = load4<DT>(p.B, (size_t)(first + r) * p.B_stride + at, r < rows ? NST - n0 : 0, bvec);
+        rC[r] = load4<DT>(p.C, (size_t)(first + r) * p.C_stride + at, r < rows ? NST - n0 : 0, bvec);
     }
+    float x[MINE], d[MINE], z[MINE];
 #pragma unroll
-    for (int b = 1; b < LPC; b <<= 1) y += __shfl_xor_sync(0xffffffffu, y, b);
-    if (there && q == 0) {
-        if (p.z) {
-            const float z = ld1(p.z, DT, (size_t)n * p.z_stride + c);
-            y *= z * sigmoidf_(z);
-        }
-        st1(p.y, DT, (size_t)n * D + c, y);
+    for (int i = 0; i < MINE; ++i) {
+        const bool ok = mine + 2 * i < rows;
+        const size_t n = (size_t)(first + mine + 2 * i);
+        x[i] = ok ? ld1(p.x, DT, n * p.x_stride + c) : 0.f;
+        d[i] = ok ? ld1(p.dt, DT, n * p.dt_stride + c) : 0.f;
+        z[i] = ok && p.z ? ld1(p.z, DT, n * p.z_stride + c) : 0.f;
     }
+    Four A = four(there ? ld_states(p.A, c, n0, NST) : zero);
+    const float bias = there && p.dt_bias ? p.dt_bias[c] : 0.f, skip = there && p.skip ? p.skip[c] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        d[i] += bias;
+        if (p.softplus) d[i] = scan_softplus(d[i]);
+    }
+    float y[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        f32x2 B[2], C[2], s;
+        unpack4_2<DT>(rB[r], B);
+        unpack4_2<DT>(rC[r], C);
+        float dr = d[0], dx = d[0] * x[0];
+        if constexpr (ROWS > 1) {
+            const int i = LPC == 2 ? r / 2 : 0;
+            dr = __shfl_sync(0xffffffffu, d[i < MINE ? i : 0], LPC == 2 ? r & 1 : r, LPC);
+            dx = __shfl_sync(0xffffffffu, d[i < MINE ? i : 0] * x[i < MINE ? i : 0], LPC == 2 ? r & 1 : r, LPC);
+        }
+        Four o = four(h[r]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            o.v[i] = fma2(ex2f2_(mul2(A.v[i], both(dr))), o.v[i], mul2(both(dx), B[i]));
+            s = i ? fma2(C[i], o.v[i], s) : mul2(C[i], o.v[i]);
+        }
+        if (r < rows) st_states(p.state, row + (size_t)r * D, n0, NST, flat(o));
+        y[r] = sum2(s);
+    }
+    if constexpr (ROWS > 1) {
+        lanes_sum4<LPC>(y, q);
+    } else {
+#pragma unroll
+        for (int b = 1; b < LPC; b <<= 1) y[0] += __shfl_xor_sync(0xffffffffu, y[0], b);
+    }
+    if (q > (ROWS == 1 ? 0 : 3)) return;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i)
+        if (mine + 2 * i < rows) {
+            float v = fmaf(skip, x[i], y[i]);
+            if (p.z) v *= z[i] * sigmoidf_(z[i]);
+            st1(p.y, DT, row + (size_t)(mine + 2 * i) * D, v);
+        }
 }
 
 // lanes per channel for NST states
@@ -828,7 +865,11 @@ extern "C" int mkda_scan_step(const MkdaScanStep* p, void* stream) {
     with_dtype(p->dtype, [&](auto dt) {
         with_lanes(p->NST, [&](auto l) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
-            launch(scan_step_kernel<DT, LPC>, dim3((p->D + 128 / LPC - 1) / (128 / LPC), p->N), 128, 0, (cudaStream_t)stream, *p);
+            const bool bvec = p->NST % 4 == 0 && p->B_stride % 4 == 0 && p->C_stride % 4 == 0 && aligned16(p->B) && aligned16(p->C);
+            const int blocks = (p->D + 128 / LPC - 1) / (128 / LPC);
+            // four sequences a thread where that leaves eight blocks per SM
+            if ((long long)blocks * p->N >= 32ll * sm_count()) launch(scan_step_kernel<DT, LPC, 4>, dim3(blocks, (p->N + 3) / 4), 128, 0, (cudaStream_t)stream, *p, bvec);
+            else launch(scan_step_kernel<DT, LPC, 1>, dim3(blocks, p->N), 128, 0, (cudaStream_t)stream, *p, bvec);
         });
     });
     return check_launch("scan_step");
