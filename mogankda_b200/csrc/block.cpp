@@ -201,6 +201,7 @@ std::string count_error(int64_t want, int64_t got) {
     return "The number of initial states is expected to be equal to the number of input sequences, i.e., " + std::to_string(want) + " rather than " +
            std::to_string(got) + ".";
 }
+constexpr int64_t MOST_CHANNELS = 1 << 24;
 constexpr int64_t MOST_TOKENS = std::numeric_limits<int>::max() - 65536;      // tokens are counted in 32 bits, a run past the end included
 
 // ---- convolution ---------------------------------------------------------------------------------------------------------------------------
@@ -250,7 +251,7 @@ PyObject* conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!check_devices("causal_conv1d", t)) return nullptr;
     REQUIRE(x.dim() == 3 && float_type(x), "x must be [B, T, D], bfloat16, float16 or float32");
     const int64_t D = x.size(2);
-    REQUIRE(D >= 1 && x.size(0) * x.size(1) <= MOST_TOKENS, "x must have at least one channel and less than 2^31 tokens");
+    REQUIRE(D >= 1 && D <= MOST_CHANNELS && x.size(0) * x.size(1) <= MOST_TOKENS, "x must have 1 to 2^24 channels and less than 2^31 tokens");
     CONV_PARAMS(w, D);
     REQUIRE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == D && float_type(bias)), "bias must be [D]");
     Sequences q;
@@ -312,7 +313,7 @@ PyObject* conv_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!parse_tensors("causal_conv1d_step", a, 4, 3, t)) return nullptr;
     const Tensor &x = t[0], &state = t[1], &w = t[2], &bias = t[3];
     if (!check_devices("causal_conv1d_step", t)) return nullptr;
-    REQUIRE(x.dim() == 2 && float_type(x) && x.size(1) >= 1, "x must be [N, D], bfloat16, float16 or float32");
+    REQUIRE(x.dim() == 2 && float_type(x) && x.size(1) >= 1 && x.size(1) <= MOST_CHANNELS, "x must be [N, D], bfloat16, float16 or float32");
     const int64_t N = x.size(0), D = x.size(1);
     REQUIRE(N <= 65535, "at most 65535 sequences");
     CONV_PARAMS(w, D);
@@ -423,6 +424,7 @@ PyObject* check_scan(const variable_list& t, int lead) {
     const Tensor &x = t[SX], &A = t[SA], &B = t[SB], &C = t[SC];
     REQUIRE(x.dim() == lead + 1 && float_type(x) && x.size(lead) >= 1, lead == 2 ? "x must be [B, T, D], bfloat16, float16 or float32" : "x must be [N, D], bfloat16, float16 or float32");
     const int64_t D = x.size(lead);
+    REQUIRE(D <= MOST_CHANNELS, "at most 2^24 channels");
     for (int i : {SDT, SB, SC, SZ}) REQUIRE(!t[i].defined() || t[i].scalar_type() == x.scalar_type(), "x, dt, B, C and z must share a dtype");
     for (int i : {SDT, SZ}) REQUIRE(!t[i].defined() || t[i].sizes() == x.sizes(), "dt and z must have the shape of x");
     REQUIRE(A.dim() == 2 && A.size(0) == D && float_type(A), "A must be [D, N]");

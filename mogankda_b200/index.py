@@ -186,11 +186,13 @@ def bounds_table(T, cu, step):
 
 def get_bounds(T, cu_seqlens, device):
     """Cached like ``get_layout``; a miss reads ``cu_seqlens`` back to the host."""
-    key, ver = ("bounds", T, device), cu_seqlens._version
-    b = _cached(key, cu_seqlens, ver)
+    key, ver = ("bounds", T, device), None if cu_seqlens.is_inference() else cu_seqlens._version
+    b = None if ver is None else _cached(key, cu_seqlens, ver)      # changes of a tensor without a version counter would not be seen
     if b is None:
         table, dims = bounds_table(T, [int(x) for x in cu_seqlens.tolist()], ENUMS["MKDA_SCAN_CHECKPOINT"])
         b = Bounds(torch.tensor(table, dtype=torch.int32, device=device), dims)
+        if ver is None:
+            return b
         with _cache_lock:
             if len(_cache) >= _CACHE_MAX:
                 _cache.pop(0)

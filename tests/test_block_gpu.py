@@ -67,7 +67,7 @@ def conv_reference(x, w, bias, act, state, cu, last):
 CONV = [  # B, T, D, W, cu
     (1, 1, 8, 4, None), (2, 3, 16, 4, None), (3, 37, 64, 3, None), (1, 130, 1001, 2, None), (2, 200, 520, 4, None), (1, 77, 1, 4, None),
     (1, 100, 40, 4, (0, 1, 3, 3, 20, 100)), (1, 70, 24, 3, (0, 0, 2, 64, 66)), (1, 9, 36, 4, (0, 2, 4, 5, 9)), (1, 300, 136, 4, (0, 0, 0, 299, 300, 300)),
-    (1, 5, 16, 2, (0,)),
+    (1, 5, 16, 2, (0,)), (2, 1500, 2056, 4, None), (1, 4099, 1032, 3, (0, 1000, 1003, 1004, 4000)),
 ]
 
 
@@ -173,6 +173,8 @@ SCAN = [  # B, T, D, states, groups, cu
     (1, 40, 200, 8, 1, None), (1, 35, 24, 1, 1, None), (1, 35, 24, 5, 3, None), (2, 20, 48, 32, 2, None), (1, 37, 17, 64, 1, None), (1, 18, 20, 50, 1, None),
     (1, 1, 1, 16, 1, None), (1, 100, 48, 16, 1, (0, 1, 17, 17, 33, 100)), (1, 60, 40, 16, 2, (0, 0, 16, 48, 50)), (1, 90, 16, 12, 1, (0, 32, 64, 90, 90)),
     (1, 5, 16, 16, 1, (0,)), (1, 70, 300, 16, 1, (0, 3, 70)),
+    (1, 257, 40, 16, 1, None), (2, 700, 33, 16, 1, None), (1, 300, 16, 8, 1, None), (1, 900, 24, 30, 1, (0, 290, 300, 899)), (1, 270, 9, 64, 1, None),
+    (1, 200, 4100, 16, 2, tuple(range(0, 196, 5)) + (197, 200)),
 ]
 
 
@@ -240,6 +242,29 @@ def test_scan_steps_continue_a_prompt(dtype, N, G, W):
     near("state", state, end.double())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [3, 8, 16, 30, 64])
+def test_scan_steps_of_many_sequences(dtype, N):
+    """Four sequences a thread give each what it gets in a call of its own."""
+    gen = torch.Generator().manual_seed(N)
+    rows, W, G = 203, {3: 3002, 8: 3002, 16: 1502, 30: 752, 64: 402}[N], 2
+    lv = {n: t.cuda() for n, t in scan_leaves(gen, rows, 1, W, N, G, None, dtype, True).items()}
+    tok = {n: lv[n][:, 0] for n in ("x", "dt", "B", "C", "z")}
+
+    def step(a, b, state):
+        return mk.selective_scan_step(tok["x"][a:b], tok["dt"][a:b], lv["A"], tok["B"][a:b], tok["C"][a:b], state, lv["D"], tok["z"][a:b], lv["bias"], dt_softplus=True)
+
+    with torch.no_grad():
+        state, parts = lv["h0"].clone(), [lv["h0"][i:i + 2].clone() for i in range(0, rows, 2)]
+        y = step(0, rows, state)
+        ys = [step(2 * i, min(2 * i + 2, rows), s) for i, s in enumerate(parts)]
+        whole, end = call_scan(lv, None, True)
+    near("y", torch.cat(ys), y.double())
+    near("state", torch.cat(parts), state.double())
+    near("y of a prompt", whole[:, 0], y.double())
+    near("state of a prompt", end, state.double())
+
+
 def test_scan_of_any_decay():
     """No decay at all, decays that leave nothing (the exponential underflows), and softplus at both ends of its range."""
     gen = torch.Generator().manual_seed(9)
@@ -298,7 +323,7 @@ def test_norm(rows, H, dtype, residual):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,H,group", [(1, 128, 128), (5, 384, 128), (3, 4096, 128), (2, 8192, 128), (4, 100, None), (3, 2048, None), (1, 32768, None), (6, 1001, None)])
+@pytest.mark.parametrize("rows,H,group", [(1, 128, 128), (5, 384, 128), (3, 4096, 128), (2, 8192, 128), (4, 100, None), (3, 2048, None), (700, 640, 128), (1300, 264, None), (1, 32768, None), (6, 1001, None)])
 @pytest.mark.parametrize("residual", [False, True])
 def test_norm_in_8_bits(rows, H, group, dtype, residual):
     """e4m3 has three bits of mantissa: half a step is 2^-4 of a normal value, 2^-10 of a subnormal one; the scale brings the largest to 448."""
@@ -457,6 +482,93 @@ def test_side_streams_graphs_and_repeated_runs():
         graph.replay()
     for a, b, c in zip(first, second, captured):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_capture_while_an_eager_graph_of_the_same_leaves_lives():
+    """What torch's own operators do there: the capture fails with an error that the program can catch, or succeeds; the process goes on."""
+    code = """
+import torch, mogankda_b200 as mk
+x = torch.randn(1, 40, 32, device="cuda", requires_grad=True)
+w = torch.randn(32, 4, device="cuda", requires_grad=True)
+A, bc = -torch.rand(32, 16, device="cuda"), torch.randn(1, 40, 16, device="cuda")
+def step():
+    y, _ = mk.causal_conv1d(mk.rms_norm(x, w[:, 0]), w, activation="silu")
+    return mk.selective_scan(y, x, A, bc, bc, D=w[:, 1], dt_softplus=True)[0]
+alive = step()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        step().backward(torch.ones_like(x))
+except RuntimeError as e:
+    print("raised", type(e).__name__)
+torch.cuda.synchronize()
+torch.autograd.grad(alive, (x, w), torch.ones_like(x))
+torch.cuda.synchronize()
+print("alive")
+"""
+    import os
+    import subprocess
+    import sys
+    run = subprocess.run([sys.executable, "-W", "ignore", "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "alive" in run.stdout, run.stderr[-2000:]
+
+
+def test_two_graphs_and_two_streams_at_once():
+    """Nothing is shared between calls: two captured steps replayed side by side, and eager calls beside them, give the bits of each alone."""
+    gen = torch.Generator().manual_seed(11)
+    steps = []
+    for T in (70, 300):
+        p, h = block_params(gen, torch.bfloat16, 1, T)
+        leaves = {n: t.clone().requires_grad_(True) for n, t in p.items()}
+        up = torch.ones(1, T, 64, dtype=torch.bfloat16, device="cuda")
+
+        def step(h=h, leaves=leaves, up=up):
+            y, s, _ = block(h, leaves)
+            return [y, s, *torch.autograd.grad((y, s), list(leaves.values()), (up, up.float()))]
+
+        steps.append(step)
+    alone = [[t.detach().clone() for t in step()] for step in steps]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for step, stream in zip(steps, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            outs.append(step())
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        eager = steps[0]()
+        torch.cuda.synchronize()
+        for got, want in zip((*outs, eager), (*alone, alone[0])):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_inference_mode_and_saved_tensor_hooks():
+    gen = torch.Generator().manual_seed(12)
+    p, h = block_params(gen, torch.bfloat16, 1, 50)
+    cu = [0, 20, 50]
+    want = block(h, p, cu=torch.tensor(cu, device="cuda"))[0]
+    with torch.inference_mode():
+        t = torch.tensor(cu, device="cuda")
+        assert torch.equal(block(h, p, cu=t)[0], want)
+        t[1] = 30                                          # no version counter tells
+        assert not torch.equal(block(h, p, cu=t)[0], want)
+        state = torch.zeros(2, 3, 16, device="cuda")
+        mk.causal_conv1d_step(torch.ones(2, 16, device="cuda"), state, torch.ones(16, 4, device="cuda"))
+        assert (state[:, 2] == 1).all()
+    leaves = {n: t.clone().requires_grad_(True) for n, t in p.items()}
+    plain = torch.autograd.grad(block(h, leaves)[0].sum(), list(leaves.values()), allow_unused=True)
+    with torch.autograd.graph.save_on_cpu():
+        y = block(h, leaves)[0]
+    for a, b in zip(plain, torch.autograd.grad(y.sum(), list(leaves.values()), allow_unused=True)):
+        assert (a is None and b is None) or torch.equal(a, b)
 
 
 def test_autograd_of_the_block_operators():
