@@ -27,6 +27,7 @@ typedef struct {
     const int* cu;
     const int* order;          /* [N] the sequences in the order in which they are started on, or NULL */
     const int* ckpt_off;       /* [N] first checkpoint of each sequence (ceil(length / MKDA_SCAN_CHECKPOINT) each), or NULL with cu == NULL */
+    int seg; int segs;         /* scan: sequences are cut into parts of seg tokens (a multiple of 64), at most segs of them, that run side by side; seg = 0: not cut */
 } MkdaSeqs;
 
 /* Depthwise causal convolution: y[t] = act(bias + sum_w weight[w] x[t - W + 1 + w]), W in 2..4.  What lies in front of a sequence's first
@@ -78,17 +79,19 @@ typedef struct {
     const float* h0;           /* [N,D,NST] or NULL */
     void* y;                   /* [TT,D] */
     float* ht;                 /* [N,D,NST] or NULL */
+    float* seg_h; float* seg_d;           /* cut sequences: [segs][N][D][P] what each part makes of nothing, [segs][N][D] its sum of d (workspace) */
     float* ckpt;               /* states in front of every MKDA_SCAN_CHECKPOINT-th token of each sequence, [checkpoints][D][P], or NULL; P = NST padded to 8, 16, 32 or 64 */
 } MkdaScanFwd;
 int mkda_scan_fwd(const MkdaScanFwd* p, void* stream);
 
 typedef struct {
-    MkdaScanFwd f;             /* the forward call: y, ht and h0 are not looked at, ckpt is read */
+    MkdaScanFwd f;             /* the forward call: y, ht, h0, seg_h and seg_d are not looked at, ckpt is read; f.S.seg need not be the forward call's */
     const void* dy;            /* [TT,D] */
     const float* dht;          /* [N,D,NST] or NULL */
     void* dx; void* ddt; void* dz;        /* [TT,D]; dz only with z */
     float* dh0;                /* [N,D,NST] or NULL */
-    int slots;                 /* the sequences are dealt to so many rows of blocks */
+    float* seg_g; float* seg_d;           /* as in the forward call, of the gradient */
+    int slots;                 /* the sequences (or their parts) are dealt to so many rows of blocks */
     int channel_blocks;        /* what mkda_scan_bwd_channel_blocks says */
     float* part_B; float* part_C;         /* [channel_blocks][TT][P]: per block of channels */
     float* part_A;             /* [slots][D][P] */

@@ -136,7 +136,7 @@ struct Sequences {
     MkdaSeqs s{};
     Tensor table;
     bool covers_all = true;
-    int64_t checkpoints = 0;
+    int64_t checkpoints = 0, longest = 0;
 };
 bool get_sequences(PyObject* table, PyObject* dims, int64_t B, int64_t T, Sequences& q) {
     if (!tensor_arg(table, q.table)) return false;
@@ -146,14 +146,16 @@ bool get_sequences(PyObject* table, PyObject* dims, int64_t B, int64_t T, Sequen
         q.s.N = (int)B;
         q.s.has_empty = T == 0;
         q.checkpoints = B * ((T + MKDA_SCAN_CHECKPOINT - 1) / MKDA_SCAN_CHECKPOINT);
+        q.longest = T;
         return true;
     }
     int all, empty;
-    long long ck;
-    if (!PyArg_ParseTuple(dims, "iiiL", &q.s.N, &all, &empty, &ck)) return false;
+    long long ck, longest;
+    if (!PyArg_ParseTuple(dims, "iiiLL", &q.s.N, &all, &empty, &ck, &longest)) return false;
     q.covers_all = all;
     q.s.has_empty = empty;
     q.checkpoints = ck;
+    q.longest = longest;
     const int* p = static_cast<const int*>(q.table.data_ptr());
     q.s.cu = p;
     q.s.ckpt_off = p + q.s.N + 1;
@@ -344,6 +346,20 @@ PyObject* conv_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // ---- scan ------------------------------------------------------------------------------------------------------------------------------------
 enum { SX, SDT, SA, SB, SC, SSKIP, SZ, SBIAS, SH0, SCAN_INPUTS };
 
+// Cuts long sequences into parts that run side by side where there are fewer blocks than places for them (`places` per SM).  The pass over the parts that comes first takes `pre` of
+// the time of the main pass over them, and both start anew, about 128 tokens' time.  Whole / cut in us, 8192 tokens, first pass included: forward
+// x 256 channels 274 / 40, x 1024 278 / 132, x 2048 280 / 254; backward x 256 970 / 77, x 1024 1059 / 254, x 2048 1064 / 520, x 4096 1066 / 911.
+void cut(MkdaSeqs& s, const Sequences& q, int blocks, int64_t P, int64_t D, int places, double pre) {
+    if (q.longest < 512 || s.N == 0) return;
+    const double side_by_side = blocks * std::max(1.0, (double)s.TT / q.longest);      // blocks that are busy as long as the longest sequence runs
+    const int64_t want = (int64_t)(places * sms() / side_by_side);
+    if (want < 2) return;
+    const int64_t seg = std::max<int64_t>(256, ((q.longest + want - 1) / want + 63) / 64 * 64), segs = (q.longest + seg - 1) / seg;
+    if ((1 + pre) * seg + 128 >= q.longest || s.N * segs * D * P * 4 > (int64_t)256 << 20) return;
+    s.seg = (int)seg;
+    s.segs = (int)segs;
+}
+
 // What a scan call hands to the library; the tensors behind the pointers are kept in `hold`.
 struct ScanCall {
     MkdaScanFwd p{};
@@ -391,8 +407,16 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
         if (in[i].defined()) out[i] = new_cuda(in[i].sizes(), in[i].scalar_type(), dev);
     p.dx = out[SX].data_ptr(); p.ddt = out[SDT].data_ptr(); p.dz = mptr(out[SZ]); p.dh0 = fmptr(out[SH0]);
     p.channel_blocks = mkda_scan_bwd_channel_blocks((int)D, (int)G, (int)N);
+    cut(p.f.S, q, p.channel_blocks, P, D, 2, 0.4);
+    const int64_t rows = p.f.S.seg ? (int64_t)q.s.N * p.f.S.segs : q.s.N;
+    Tensor seg_g, seg_d;
+    if (p.f.S.seg) {
+        seg_g = new_cuda({rows, D, P}, at::kFloat, dev);
+        seg_d = new_cuda({rows, D}, at::kFloat, dev);
+        p.seg_g = fmptr(seg_g); p.seg_d = fmptr(seg_d);
+    }
     // sequences are dealt to rows of blocks: enough of them for 16 blocks per SM; each leaves a row of sums for A, D and dt_bias
-    p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(q.s.N, (16 * sms() + p.channel_blocks - 1) / p.channel_blocks));
+    p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (16 * sms() + p.channel_blocks - 1) / p.channel_blocks));
     const std::vector<int64_t> part_size{p.channel_blocks, TT * P};
     const Tensor pB = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
     const Tensor pC = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
@@ -470,6 +494,15 @@ PyObject* scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (want) last = new_cuda({q.s.N, D, NST}, at::kFloat, x.device());
             if (grad) ckpt = new_cuda({std::max<int64_t>(q.checkpoints, 1), D, mkda_scan_padded_states((int)NST)}, at::kFloat, x.device());
             call.p.y = y.data_ptr(); call.p.ht = fmptr(last); call.p.ckpt = fmptr(ckpt);
+            const int64_t P = mkda_scan_padded_states((int)NST);
+            cut(call.p.S, q, mkda_scan_bwd_channel_blocks((int)D, call.p.G, (int)NST), P, D, 1, 0.75);      // the forward kernel has the same blocks
+            Tensor seg_h, seg_d;
+            if (call.p.S.seg) {
+                const int64_t rows = (int64_t)q.s.N * call.p.S.segs;
+                seg_h = new_cuda({rows, D, P}, at::kFloat, x.device());
+                seg_d = new_cuda({rows, D}, at::kFloat, x.device());
+                call.p.seg_h = fmptr(seg_h); call.p.seg_d = fmptr(seg_d);
+            }
             library_call([&] { check_rc(mkda_scan_fwd(&call.p, stream()), "mkda_scan_fwd"); });
         }
         if (grad) {

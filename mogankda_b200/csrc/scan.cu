@@ -105,6 +105,18 @@ __device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB)
     return Channels{g, g * per + b * CB, min(CB, per - b * CB)};
 }
 
+// A sequence, or the k-th part of one where sequences are cut: slots go over the sequences first.  `there`: a part that the sequence has.
+struct Part { int n, k, start, end; bool there, last; };
+__device__ __forceinline__ Part part_of(const MkdaSeqs& s, int slot) {
+    const int k = slot / s.N, i = slot - k * s.N, n = s.order ? s.order[i] : i;
+    const Span q = sequence(s, n);
+    if (!s.seg) return Part{n, 0, q.start, q.end, true, true};
+    const long long a = q.start + (long long)k * s.seg;
+    const int end = (int)min(a + s.seg, (long long)q.end);
+    return Part{n, k, (int)min(a, (long long)q.end), end, k == 0 || a < q.end, a + s.seg >= q.end};
+}
+__device__ __forceinline__ int parts(const MkdaSeqs& s) { return s.seg ? s.N * s.segs : s.N; }
+
 // Forward.  Four warps walk the recurrence and four beside them do the elementwise part, a tile ahead (loads, softplus) and a tile behind (skip, gate, stores); the block's
 // barrier joins them once a tile.  A channel's chain is short and there are few warps of it (4096 channels are 512), so what counts is how many cycles a token takes a warp that
 // has a scheduler to itself: with the elementwise part in the same warps 168, of which 32 are the exponentials of the special function unit.
@@ -130,6 +142,17 @@ __device__ __forceinline__ float4 flat(const Four& s) {
     return f;
 }
 
+// What enters a part: the state (or its gradient) that enters the sequence, carried over the parts in front (behind).  A (scaled by log2 e): of this lane.
+__device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S, int n, int from, int to, int step, const float* seg_h, const float* seg_d, int D, size_t ch, int NP, int n0) {
+    for (int j = from; j != to; j += step) {
+        const size_t i = ((size_t)j * S.N + n) * D + ch;
+        const Four h = four(*reinterpret_cast<const float4*>(seg_h + i * NP + n0));
+        const f32x2 d = both(seg_d[i]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s.v[e] = fma2(ex2f2_(mul2(A.v[e], d)), s.v[e], h.v[e]);
+    }
+}
+
 // (Two states a lane and twice the warps on the chain: 302 us where this takes 275.)
 template <int DT, int LPC, int TILE>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
@@ -148,13 +171,14 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
         Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero);
 #pragma unroll
         for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
-        for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-            const int n = p.S.order ? p.S.order[slot] : slot;
-            const Span sq = sequence(p.S, n);
-            const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+        for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+            const Part sq = part_of(p.S, slot);
+            if (!sq.there) continue;
+            const int n = sq.n, len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
             Four h = four(p.h0 && there ? ld_states(p.h0, (size_t)n * D + ch, n0, NST) : zero);
+            if (there) carry(h, A, p.S, n, 0, sq.k, 1, p.seg_h, p.seg_d, D, ch, NP, n0);
             const size_t ck0 = p.ckpt ? (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) : 0;
-            float* ck = p.ckpt ? p.ckpt + (ck0 * D + ch) * NP + n0 : nullptr;
+            float* ck = p.ckpt ? p.ckpt + ((ck0 + (size_t)sq.k * (p.S.seg / CKPT)) * D + ch) * NP + n0 : nullptr;
             __syncthreads();                               // the first tile is there
             for (int k = 0; k < tiles; ++k) {
                 const int buf = k & 1, t0 = k * TILE;
@@ -213,7 +237,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 put_sums<LPC, YROW>(sy, TILE - 4, c0, ys, q);
                 __syncthreads();
             }
-            if (p.ht && there) st_states(p.ht, (size_t)n * D + ch, n0, NST, flat(h));
+            if (p.ht && there && sq.last) st_states(p.ht, (size_t)n * D + ch, n0, NST, flat(h));
             __syncthreads();                               // the last tile has been stored
         }
         return;
@@ -235,8 +259,9 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
     }
     const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}, skip[2] = {pack2(fs[0], fs[1]), pack2(fs[2], fs[3])};
     const bool whole = STEP * PIECES == TILE && BSTEP * BC == TILE;      // every piece of every thread lies in the tile
-    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-        const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
+    for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+        const Part sq = part_of(p.S, slot);
+        if (!sq.there) continue;
         const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
         struct Rows { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], b[BC]; };
         Rows even, odd;                                    // rows on their way, of every other tile: requested two steps before they are used
@@ -336,6 +361,167 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
     }
 }
 
+// Where there are fewer blocks than SMs and the sequences are long, these are cut into parts that run side by side.  This kernel finds what each part makes of nothing,
+//   forward   h over the part from h = 0 (all parts but a sequence's last)     REV   g in front of the part from g = 0 behind it (all but the first)
+// and the sum of its d, from which the part's decay follows; the main kernels carry the state over the parts in front of theirs.  It is the forward kernel without
+// results per token; REV walks from the last token to the first.
+template <int DT, int LPC, int TILE>
+struct ScanPreShared {
+    using Sh = ScanShape<LPC, 1, TILE>;
+    static constexpr int AHEAD = 8;
+    float2 d[2][TILE + AHEAD][Sh::CB];     // d, and d x or the gradient of y
+    float B[2][TILE + AHEAD][Sh::NP];      // B or C
+};
+template <int DT, int LPC, int TILE, bool REV>
+__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kernel(const MkdaScanFwd p, const void* up, float* out_h, float* out_d, const bool vec, const bool bvec) {
+    follow_stream();
+    using Sh = ScanShape<LPC, 1, TILE>;
+    constexpr int NP = Sh::NP, CB = Sh::CB;
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    auto& sh = *reinterpret_cast<ScanPreShared<DT, LPC, TILE>*>(raw_shared);
+    const int D = p.D, NST = p.NST;
+    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
+    auto wanted = [](const Part& q) { return q.there && (REV ? q.k > 0 : !q.last); };
+    if (threadIdx.x < SCAN_THREADS) {
+        const int tid = threadIdx.x, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q;
+        const bool there = c0 < cs.count;
+        const size_t ch = cs.first + c0;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
+        for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+            const Part sq = part_of(p.S, slot);
+            if (!wanted(sq)) continue;
+            const int tiles = (sq.end - sq.start + TILE - 1) / TILE;
+            Four h = four(zero);
+            float sum = 0.f;
+            __syncthreads();                               // the first tile is there
+            for (int k = 0; k < tiles; ++k) {
+                const float2* sd = &sh.d[k & 1][0][c0];
+                const float* sB = &sh.B[k & 1][0][n0];
+                struct Token { float2 d; Four B; };
+                auto fetch = [&](int t) { return Token{sd[t * CB], four(*reinterpret_cast<const float4*>(sB + t * NP))}; };
+                Token now[4], next[4];
+                Four e[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) now[u] = fetch(u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) next[u] = fetch(4 + u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) e[u].v[i] = ex2f2_(mul2(A.v[i], both(now[u].d.x)));
+#pragma unroll
+                for (int t4 = 0; t4 < TILE; t4 += 4) {
+                    float part[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        part[u] = now[u].d.x;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x2 a = e[u].v[i], v = both(now[u].d.y);
+                            e[u].v[i] = ex2f2_(mul2(A.v[i], both(next[u].d.x)));
+                            h.v[i] = REV ? mul2(a, fma2(v, now[u].B.v[i], h.v[i])) : fma2(a, h.v[i], mul2(v, now[u].B.v[i]));
+                        }
+                        now[u] = next[u];
+                        next[u] = fetch(t4 + 8 + u);
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                }
+                __syncthreads();
+            }
+            if (there) {
+                const size_t i = ((size_t)sq.k * p.S.N + sq.n) * D + ch;
+                *reinterpret_cast<float4*>(out_h + i * NP + n0) = flat(h);
+                if (q == 0) out_d[i] = sum;
+            }
+        }
+        return;
+    }
+    constexpr int HELPERS = SCAN_HELPERS, ROW = CB / 4, STEP = HELPERS / ROW, PIECES = (TILE * ROW + HELPERS - 1) / HELPERS;
+    constexpr int BROW = NP / 4, BSTEP = HELPERS / BROW, BC = (TILE * BROW + HELPERS - 1) / HELPERS;
+    const int tid = threadIdx.x - SCAN_THREADS, ec = tid % ROW * 4, et = tid / ROW, valid = cs.count - ec;
+    const int bn = tid % BROW * 4, bt = tid / BROW, bvalid = NST - bn;
+    float fb[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) fb[e] = p.dt_bias && ec + e < cs.count ? p.dt_bias[cs.first + ec + e] : 0.f;
+    const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])};
+    for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+        const Part sq = part_of(p.S, slot);
+        if (!wanted(sq)) continue;
+        const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+        struct Rows { Raw4<DT> d[PIECES], x[PIECES], z[PIECES], b[BC]; };      // x: x or the gradient of the output
+        Rows even, odd;
+        auto request = [&](Rows& r, int k) {               // row i of tile k is token TILE k + i, REV: from the end
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int row = et + i * STEP, t = k * TILE + row, ok = row < TILE && t < len ? valid : 0;
+                const size_t tok = (size_t)(REV ? sq.end - 1 - t : sq.start + t), col = cs.first + ec;
+                r.d[i] = load4<DT>(p.dt, tok * p.dt_stride + col, ok, vec);
+                r.x[i] = REV ? load4<DT>(up, tok * D + col, ok, vec) : load4<DT>(p.x, tok * p.x_stride + col, ok, vec);
+                if (REV && p.z) r.z[i] = load4<DT>(p.z, tok * p.z_stride + col, ok, vec);
+            }
+#pragma unroll
+            for (int i = 0; i < BC; ++i) {
+                const int row = bt + i * BSTEP, t = k * TILE + row, ok = row < TILE && t < len ? bvalid : 0;
+                const size_t tok = (size_t)(REV ? sq.end - 1 - t : sq.start + t), col = cs.group * NST + bn;
+                r.b[i] = REV ? load4<DT>(p.C, tok * p.C_stride + col, ok, bvec) : load4<DT>(p.B, tok * p.B_stride + col, ok, bvec);
+            }
+        };
+        auto step = [&](Rows& r, int k) {                  // forms tile k + 1
+            if (k + 1 < tiles) {
+                const int buf = (k + 1) & 1, left = len - (k + 1) * TILE;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = et + i * STEP;
+                    if (t >= TILE) continue;
+                    f32x2 d[2], x[2];
+                    unpack4_2<DT>(r.d[i], d);
+                    unpack4_2<DT>(r.x[i], x);
+                    if (REV && p.z) {
+                        f32x2 z[2];
+                        unpack4_2<DT>(r.z[i], z);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) x[e] = mul2(x[e], mul2(z[e], sigmoidf2_(z[e])));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        d[e] = add2(d[e], bias[e]);
+                        if (p.softplus) d[e] = scan_softplus2(d[e]);
+                        if (!REV) x[e] = mul2(d[e], x[e]);
+                    }
+                    float4 w0, w1;
+                    unpack2(d[0], w0.x, w0.z);
+                    unpack2(x[0], w0.y, w0.w);
+                    unpack2(d[1], w1.x, w1.z);
+                    unpack2(x[1], w1.y, w1.w);
+                    if (t >= left) w0 = w1 = make_float4(0.f, 0.f, 0.f, 0.f);
+                    const int o = (tid >> 2) & 1;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 * o]) = o ? w1 : w0;
+                    *reinterpret_cast<float4*>(&sh.d[buf][t][ec + 2 - 2 * o]) = o ? w0 : w1;
+                }
+#pragma unroll
+                for (int i = 0; i < BC; ++i) {
+                    const int t = bt + i * BSTEP;
+                    if (t >= TILE) continue;
+                    float v[4];
+                    unpack4<DT>(r.b[i], v);
+                    *reinterpret_cast<float4*>(&sh.B[buf][t][bn]) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+            if (k + 3 < tiles) request(r, k + 3);
+            __syncthreads();
+        };
+        request(even, 0);
+        if (tiles > 1) request(odd, 1);
+        for (int k = -1; k < tiles; k += 2) {
+            step(even, k);
+            if (k + 1 < tiles) step(odd, k + 1);
+        }
+    }
+}
+
 // Backward: tiles of one checkpoint, from the last to the first, with the same two roles.  A tile is run forward from its checkpoint, then backward:
 // a_n h_n[t - 1], from which h_n follows with one operation, stays in the registers of the lane in between (the decays beside it, not formed twice, left the rest too few:
 // 406 us where this takes 400).  dB and dC are summed over the lanes of a warp by a butterfly
@@ -373,13 +559,17 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
         Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero), dA = four(zero);
 #pragma unroll
         for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
-        for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-            const int n = p.S.order ? p.S.order[slot] : slot;
-            const Span sq = sequence(p.S, n);
-            const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
-            const size_t ck0 = p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT);
+        for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+            const Part sq = part_of(p.S, slot);
+            if (!sq.there) continue;
+            const int n = sq.n, len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
+            const size_t ck0 = (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) + (size_t)sq.k * (p.S.seg / CKPT);
             auto checkpoint = [&](int k) { return there ? *reinterpret_cast<const float4*>(p.ckpt + ((ck0 + k) * D + ch) * NP + n0) : zero; };
             Four G = four(a.dht && there ? ld_states(a.dht, (size_t)n * D + ch, n0, NST) : zero);      // a[t + 1] g[t + 1]
+            if (there && p.S.seg) {
+                const Span all = sequence(p.S, n);
+                carry(G, A, p.S, n, max((all.end - all.start + p.S.seg - 1) / p.S.seg - 1, 0), sq.k, -1, a.seg_g, a.seg_d, D, ch, NP, n0);
+            }
             float4 rh = tiles ? checkpoint(tiles - 1) : zero;
             __syncthreads();                               // the first tile is there
             for (int j = 0; j < tiles; ++j) {
@@ -499,7 +689,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                 for (int i = 0; i < 2; ++i) dA.v[i] = add2(dA.v[i], dAt.v[i]);      // tile by tile: the sum over thousands of tokens loses less
                 __syncthreads();
             }
-            if (a.dh0 && there) st_states(a.dh0, (size_t)n * D + ch, n0, NST, flat(G));
+            if (a.dh0 && there && sq.k == 0) st_states(a.dh0, (size_t)n * D + ch, n0, NST, flat(G));
             __syncthreads();                               // the last tile has been stored
         }
         if (there) *reinterpret_cast<float4*>(a.part_A + ((size_t)blockIdx.y * D + ch) * NP + n0) = flat(dA);
@@ -525,8 +715,9 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
     }
     const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}, skip[2] = {pack2(fs[0], fs[1]), pack2(fs[2], fs[3])};
     f32x2 acc_skip[2] = {both(0.f), both(0.f)}, acc_bias[2] = {both(0.f), both(0.f)};
-    for (int slot = blockIdx.y; slot < p.S.N; slot += gridDim.y) {
-        const Span sq = sequence(p.S, p.S.order ? p.S.order[slot] : slot);
+    for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
+        const Part sq = part_of(p.S, slot);
+        if (!sq.there) continue;
         const int len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
         struct Rows { Raw4<DT> x[PIECES], d[PIECES], z[PIECES], y[PIECES], b[BC]; };
         Rows even, odd;                                    // rows on their way, of every other tile: requested two steps before they are used
@@ -788,6 +979,19 @@ static bool wide_rows(const MkdaScanFwd& f, int w) {
 }
 static bool wide_states(const MkdaScanFwd& f, int w) { return f.NST % w == 0 && f.B_stride % w == 0 && f.C_stride % w == 0 && aligned16(f.B) && aligned16(f.C); }
 static int blocks_of_channels(int D, int G, int CB) { return G * ((D / G + CB - 1) / CB); }
+static bool good_parts(const MkdaSeqs& s) { return s.seg == 0 || (s.seg > 0 && s.seg % 64 == 0 && s.segs >= 1 && (long long)s.N * s.segs <= 0x7fffffff); }
+static int rows_of_blocks(const MkdaSeqs& s) {
+    const long long n = s.seg ? (long long)s.N * s.segs : s.N;
+    return (int)(n < 65535 ? n : 65535);
+}
+template <int DT, int LPC, bool REV>
+static int launch_scan_pre(const MkdaScanFwd& p, const void* up, float* out_h, float* out_d, bool vec, cudaStream_t stream) {
+    constexpr int TILE = LPC == 2 ? 32 : 64, smem = (int)sizeof(ScanPreShared<DT, LPC, TILE>);
+    auto* kern = scan_pre_kernel<DT, LPC, TILE, REV>;
+    if (int e = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan: parts")) return e;
+    launch(kern, dim3(blocks_of_channels(p.D, p.G, ScanShape<LPC, 1, TILE>::CB), rows_of_blocks(p.S)), SCAN_THREADS + SCAN_HELPERS, smem, stream, p, up, out_h, out_d, vec, wide_states(p, 4));
+    return check_launch("scan: parts");
+}
 
 }  // namespace mkda
 
@@ -799,6 +1003,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
     if (!p || !p->A || (p->S.TT && (!p->x || !p->dt || !p->B || !p->C || !p->y))) return set_error(MKDA_ERR_ARG, "scan_fwd: null argument");
     if (int e = bad_scan(p->D, p->NST, p->G, p->dtype)) return e;
     if (!good_sequences(p->S) || (p->ckpt && p->S.cu && !p->S.ckpt_off)) return set_error(MKDA_ERR_ARG, "scan_fwd: bad sequences");
+    if (!good_parts(p->S) || (p->S.seg && (!p->seg_h || !p->seg_d || !aligned16(p->seg_h)))) return set_error(MKDA_ERR_ARG, "scan_fwd: parts of a multiple of 64 tokens, with their workspace");
     if (!aligned16(p->A) || !aligned16(p->h0) || !aligned16(p->ht) || !aligned16(p->ckpt)) return set_error(MKDA_ERR_ARG, "scan_fwd: A and states must be 16-byte aligned");
     if (p->S.N == 0) return MKDA_OK;
     int rc = MKDA_OK;
@@ -807,12 +1012,14 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const bool vec = wide_rows(*p, 4) && aligned16(p->y);
             const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC, 1, 32>::CB);
+            if (p->S.seg) rc = launch_scan_pre<DT, LPC, false>(*p, nullptr, p->seg_h, p->seg_d, vec, (cudaStream_t)stream);
+            if (rc != MKDA_OK) return;
             auto run = [&](auto tile) {
                 constexpr int TILE = decltype(tile)::value, smem = (int)sizeof(ScanFwdShared<LPC, TILE>);
                 auto* kern = scan_fwd_kernel<DT, LPC, TILE>;
                 rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_fwd");
                 if (rc == MKDA_OK)
-                    launch(kern, dim3(blocks, p->S.N < 65535 ? p->S.N : 65535), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
+                    launch(kern, dim3(blocks, rows_of_blocks(p->S)), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
             };
             // 64 tokens a tile from 256 tokens per sequence on; with two lanes per channel the rows of 64 would not fit into the registers
             if (LPC == 2 || (long long)p->S.TT < SCAN_LONG * (long long)p->S.N) run(std::integral_constant<int, 32>());
@@ -836,6 +1043,7 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
         return set_error(MKDA_ERR_ARG, "scan_bwd: null argument");
     if (int e = bad_scan(p->f.D, p->f.NST, p->f.G, p->f.dtype)) return e;
     if (!good_sequences(p->f.S) || (p->f.S.cu && !p->f.S.ckpt_off)) return set_error(MKDA_ERR_ARG, "scan_bwd: bad sequences");
+    if (!good_parts(p->f.S) || (p->f.S.seg && (!p->seg_g || !p->seg_d || !aligned16(p->seg_g)))) return set_error(MKDA_ERR_ARG, "scan_bwd: parts of a multiple of 64 tokens, with their workspace");
     if (!aligned16(p->f.A) || !aligned16(p->f.ckpt) || !aligned16(p->dht) || !aligned16(p->dh0) || !aligned16(p->part_A) || !aligned16(p->part_B) || !aligned16(p->part_C))
         return set_error(MKDA_ERR_ARG, "scan_bwd: A, states and partial sums must be 16-byte aligned");
     if (p->slots < 1 || p->slots > 65535 || p->channel_blocks != mkda_scan_bwd_channel_blocks(p->f.D, p->f.G, p->f.NST))
@@ -847,6 +1055,8 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
             const MkdaScanFwd& f = p->f;
             const bool vec = wide_rows(f, 4) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
             constexpr int smem = (int)sizeof(ScanBwdShared<DT, LPC>);
+            if (f.S.seg) rc = launch_scan_pre<DT, LPC, true>(f, p->dy, p->seg_g, p->seg_d, vec, (cudaStream_t)stream);
+            if (rc != MKDA_OK) return;
             auto* kern = scan_bwd_kernel<DT, LPC>;
             static const int regs = kernel_registers(reinterpret_cast<const void*>(kern));
             if (regs != SCAN_BWD_LAUNCH_REGS) { rc = set_error(MKDA_ERR_LAUNCH, "scan_bwd: built with other registers than its roles share"); return; }

@@ -171,7 +171,7 @@ def get_layout(B, T, cu_seqlens, device, seg_chunks=0, auto_heads=0, cost_ratio=
 class Bounds:
     """Packed sequences as the operators around the layer take them: boundaries, first checkpoint of a scan and order, longest first."""
     table: torch.Tensor         # int32: cu [N+1], first checkpoints [N], order [N]
-    dims: tuple                 # (N, covers_all, some sequence is empty, checkpoints)
+    dims: tuple                 # (N, covers_all, some sequence is empty, checkpoints, tokens of the longest sequence)
 
 
 def bounds_table(T, cu, step):
@@ -181,7 +181,7 @@ def bounds_table(T, cu, step):
     lens = np.diff(np.array(cu, dtype=np.int64))
     first = np.concatenate([[0], np.cumsum(-(-lens // step))])
     table = cu + first[:-1].tolist() + np.argsort(-lens, kind="stable").tolist()
-    return table, (len(lens), int(cu[-1] == T), int(bool((lens == 0).any())), int(first[-1]))
+    return table, (len(lens), int(cu[-1] == T), int(bool((lens == 0).any())), int(first[-1]), int(lens.max(initial=0)))
 
 
 def get_bounds(T, cu_seqlens, device):

@@ -39,8 +39,8 @@ def test_cpu_tensors_are_refused(lib):
 
 def test_tables_of_packed_sequences():
     table, dims = bounds_table(40, [0, 5, 5, 37], 16)
-    assert table == [0, 5, 5, 37, 0, 1, 1, 2, 0, 1] and dims == (3, 0, 1, 3)
-    assert bounds_table(7, [0], 16) == ([0], (0, 0, 0, 0))
+    assert table == [0, 5, 5, 37, 0, 1, 1, 2, 0, 1] and dims == (3, 0, 1, 3, 32)
+    assert bounds_table(7, [0], 16) == ([0], (0, 0, 0, 0, 0))
     for bad in ([], [1, 7], [0, 5, 4], [0, 8]):
         with pytest.raises(ValueError):
             bounds_table(7, bad, 16)
@@ -88,11 +88,11 @@ def test_entry_points_refuse_without_launching(lib):
     numbers = dict(D=8, NST=16, G=2, dtype=1, x_stride=8, dt_stride=8, B_stride=32, C_stride=32)
     f = _filled(S["MkdaScanFwd"](), ("x", "dt", "B", "C", "A", "y", "ckpt"), **numbers)
     f.S.TT, f.S.N, f.S.T = 4, 2, 2
-    _refused(lib, "mkda_scan_fwd", f, scan + seqs + [("y", 0), ("h0", 0x30008), ("ht", 0x30008), ("ckpt", 0x30008), ("S.cu", 0x30000)])
+    _refused(lib, "mkda_scan_fwd", f, scan + seqs + [("y", 0), ("h0", 0x30008), ("ht", 0x30008), ("ckpt", 0x30008), ("S.cu", 0x30000), ("S.seg", 32), ("S.seg", -64), ("S.seg", 64)])
     b = _filled(S["MkdaScanBwd"](), ("dy", "dx", "ddt", "part_A", "part_B", "part_C"), slots=1, channel_blocks=lib.mkda_scan_bwd_channel_blocks(8, 2, 16))
     b.f = f
     _refused(lib, "mkda_scan_bwd", b, [("f." + n, v) for n, v in scan + seqs] + [("f.ckpt", 0), ("f.z", 0x30000), ("dy", 0), ("part_A", 0), ("part_B", 0), ("slots", 0),
-                                      ("slots", 65536), ("channel_blocks", 1), ("dht", 0x30004), ("dh0", 0x30004)])
+                                      ("slots", 65536), ("channel_blocks", 1), ("dht", 0x30004), ("dh0", 0x30004), ("f.S.seg", 64)])
     p = _filled(S["MkdaScanStep"](), ("x", "dt", "B", "C", "A", "state", "y"), N=2, **numbers)
     _refused(lib, "mkda_scan_step", p, scan + [("state", 0), ("state", 0x30008), ("N", 65536)])
     p = _filled(S["MkdaNormFwd"](), ("x", "y"), rows=2, width=64, dtype=1, x_stride=64)

@@ -175,6 +175,8 @@ SCAN = [  # B, T, D, states, groups, cu
     (1, 5, 16, 16, 1, (0,)), (1, 70, 300, 16, 1, (0, 3, 70)),
     (1, 257, 40, 16, 1, None), (2, 700, 33, 16, 1, None), (1, 300, 16, 8, 1, None), (1, 900, 24, 30, 1, (0, 290, 300, 899)), (1, 270, 9, 64, 1, None),
     (1, 200, 4100, 16, 2, tuple(range(0, 196, 5)) + (197, 200)),
+    # few channels and long sequences: cut into parts that run side by side, in both directions or (600 tokens) only backward
+    (1, 1300, 17, 16, 1, None), (2, 600, 40, 16, 2, None), (1, 1025, 70, 5, 1, None), (1, 900, 10, 64, 2, None), (1, 1500, 20, 16, 1, (0, 3, 3, 1400, 1410, 1450)),
 ]
 
 
