@@ -348,13 +348,14 @@ enum { SX, SDT, SA, SB, SC, SSKIP, SZ, SBIAS, SH0, SCAN_INPUTS };
 
 // Cuts long sequences into parts that run side by side where there are fewer blocks than places for them (`places` per SM).  The pass over the parts that comes first takes `pre` of
 // the time of the main pass over them, and both start anew, about 128 tokens' time.  Whole / cut in us, 8192 tokens, first pass included: forward
-// x 256 channels 274 / 40, x 1024 278 / 132, x 2048 280 / 254; backward x 256 970 / 77, x 1024 1059 / 254, x 2048 1064 / 520, x 4096 1066 / 911.
+// x 256 channels 274 / 40, x 1024 278 / 132, x 2048 280 / 254; backward x 256 970 / 77, x 1024 1059 / 254, x 2048 1064 / 520, x 4096 1066 / 911;
+// 600 tokens x 512 25 / 14 and 75 / 27.
 void cut(MkdaSeqs& s, const Sequences& q, int blocks, int64_t P, int64_t D, int places, double pre) {
-    if (q.longest < 512 || s.N == 0) return;
+    if (q.longest < 400 || s.N == 0) return;
     const double side_by_side = blocks * std::max(1.0, (double)s.TT / q.longest);      // blocks that are busy as long as the longest sequence runs
     const int64_t want = (int64_t)(places * sms() / side_by_side);
     if (want < 2) return;
-    const int64_t seg = std::max<int64_t>(256, ((q.longest + want - 1) / want + 63) / 64 * 64), segs = (q.longest + seg - 1) / seg;
+    const int64_t seg = std::max<int64_t>(128, ((q.longest + want - 1) / want + 63) / 64 * 64), segs = (q.longest + seg - 1) / seg;
     if ((1 + pre) * seg + 128 >= q.longest || s.N * segs * D * P * 4 > (int64_t)256 << 20) return;
     s.seg = (int)seg;
     s.segs = (int)segs;

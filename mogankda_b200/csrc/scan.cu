@@ -1022,7 +1022,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
                     launch(kern, dim3(blocks, rows_of_blocks(p->S)), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));
             };
             // 64 tokens a tile from 256 tokens per sequence on; with two lanes per channel the rows of 64 would not fit into the registers
-            if (LPC == 2 || (long long)p->S.TT < SCAN_LONG * (long long)p->S.N) run(std::integral_constant<int, 32>());
+            if (LPC == 2 || (p->S.seg ? p->S.seg < SCAN_LONG : (long long)p->S.TT < SCAN_LONG * (long long)p->S.N)) run(std::integral_constant<int, 32>());
             else run(std::integral_constant<int, LPC == 2 ? 32 : 64>());
         });
     });
