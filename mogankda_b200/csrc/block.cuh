@@ -117,14 +117,25 @@ __device__ __forceinline__ Span sequence(const MkdaSeqs& s, int n) {
     if (!s.cu) return Span{n * s.T, (n + 1) * s.T};
     return Span{s.cu[n], s.cu[n + 1]};
 }
-// The sequence that holds token t; N if none does (t behind the last one).
+// The sequence that holds token t; N if none does (t behind the last one).  Called by whole warps: 32 boundaries are looked at together, one round trip to memory for up to 32
+// sequences where halving takes five.
 __device__ __forceinline__ int sequence_of(const MkdaSeqs& s, int t) {
     if (!s.cu) return t / s.T;
-    int lo = 0, hi = s.N;                                  // the first n with cu[n + 1] > t
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = s.N;                                  // the first n in [lo, hi] with cu[n + 1] > t, hi standing for itself
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s.cu[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
+        const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;      // the last of the lane's candidates
+        const unsigned above = __ballot_sync(0xffffffffu, at < hi && s.cu[at + 1] > t);
+        const int first = above ? __ffs(above) - 1 : 32;   // every candidate of the lanes in front is too small
+        const int full = (hi - lo) / step;                 // lanes whose last candidate was looked at
+        if (first < 32) {
+            hi = lo + (first + 1) * step - 1;
+            lo = lo + first * step;
+            if (step == 1) return hi;
+        } else {
+            lo += full * step;
+            if (step == 1) return hi;
+        }
     }
     return lo;
 }

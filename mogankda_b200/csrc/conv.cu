@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(128, vec ? CONV_FWD_BLOCKS : 3) conv_fwd_kerne
     constexpr int P = V / 2;
     constexpr int STAGES = 4;
     __shared__ __align__(16) char shared_rows[ConvFeed<DT, V, STAGES>::SHARED];
-    const int D = p.D, d0 = conv_channel<V>(vec);
+    const int D = p.D, d0 = conv_channel<V>(vec), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
+    int n = t0 < t1 ? sequence_of(p.S, t0) : p.S.N;
     if (d0 >= D) return;
     f32x2 wt[W][P], bias[P];
     conv_params<W, V>(p.weight, p.bias, d0, D, vec, wt, bias);
@@ -189,9 +190,6 @@ __global__ void __launch_bounds__(128, vec ? CONV_FWD_BLOCKS : 3) conv_fwd_kerne
             }
         }
     }
-    const int t0 = (int)blockIdx.y * run, t1 = min(t0 + run, p.S.TT);
-    if (t0 >= t1) return;
-    int n = sequence_of(p.S, t0);
     for (int a = t0; a < t1 && n < p.S.N; ++n) {
         const Span q = sequence(p.S, n);
         const int b = min(t1, q.end);
@@ -252,7 +250,8 @@ __global__ void __launch_bounds__(128, vec ? CONV_BWD_BLOCKS : 3) conv_bwd_kerne
     constexpr int P = V / 2;
     constexpr int STAGES = DT == MKDA_F32 ? 3 : 4;
     __shared__ __align__(16) char shared_rows[2][ConvFeed<DT, V, STAGES>::SHARED];
-    const int D = p.D, d0 = conv_channel<V>(vec);
+    const int D = p.D, d0 = conv_channel<V>(vec), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
+    int n = t0 < t1 ? sequence_of(p.S, t0) : p.S.N;
     if (d0 >= D) return;
     ConvFeed<DT, V, STAGES> feed_x(shared_rows[0], p.x, p.x_stride, d0, D, vec);
     ConvFeed<DT, V, STAGES> feed_y(shared_rows[1], p.dy, D, d0, D, vec);
@@ -276,8 +275,6 @@ __global__ void __launch_bounds__(128, vec ? CONV_BWD_BLOCKS : 3) conv_bwd_kerne
             }
         }
     }
-    const int t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
-    int n = t0 < t1 ? sequence_of(p.S, t0) : p.S.N;
     for (int a = t0; a < t1 && n < p.S.N; ++n) {
         const Span q = sequence(p.S, n);
         const int b = min(t1, q.end);
