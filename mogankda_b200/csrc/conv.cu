@@ -4,6 +4,8 @@
 // Bound by HBM: forward x in, y out; backward x and dy in, dx out (pre is formed again from x, cheaper than 4 bytes of it saved per element).
 // A thread owns a few neighbouring channels and walks down a run of tokens, so that every row of x is read once, with 16-byte accesses, and the
 // window of W - 1 rows stays in registers; only the rows around the ends of a run are read twice (they come from L2).
+// bf16, four taps: forward 32749 x 8192 176 us (6.1 TB/s), 8192 x 4096 30 us (4.5 TB/s, one wave of blocks and its start-up); backward 8192 x 4096 48 us (4.2 TB/s; half of the issue
+// slots, waits for the packed products of 13 warps per SM), of which the check of every token against the ends of its run and sequence was 12.
 #include <type_traits>
 
 #include "block.cuh"

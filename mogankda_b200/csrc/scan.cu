@@ -4,11 +4,13 @@
 //   g_n[t] = dy C_n + exp(d A_n)[t + 1] g_n[t + 1]     e_n = g_n exp(d A_n) h_n[t - 1]
 //   dC_n = sum_channels dy h_n     dB_n = sum_channels g_n d x     dA_n = sum_t e_n d     d(d) = x sum_n g_n B_n + sum_n e_n A_n     dx = d sum_n g_n B_n + D dy
 //
-// Layout.  A thread holds four states of CPT channels; LPC lanes share a channel (4 LPC states, NST padded with states whose B and C are zero).  A block of four
-// warps walks a sequence tile by tile: the elementwise part of a tile (loads of eight channels, softplus, gate, stores) is done by all threads with
-// one layout, the recurrence with the other, and the tile passes between the two through shared memory.  The rows of the next tile are requested
-// before the recurrence of this one and wait in registers.  Sums over the states of a channel are butterflies in which each lane ends with the
-// sum of a token of its own.  All in fp32.
+// Layout.  A thread holds four states of a channel; LPC lanes share a channel (4 LPC states, NST padded with states whose B and C are zero), 128 / LPC channels are a block.
+// Four warps of a block walk the recurrence, others do the elementwise part (loads of four channels, softplus, gate, stores), tile by tile, with a layout of their own; tiles pass
+// between the two through shared memory.  Sums over the states of a channel are butterflies in which each lane ends with the sum of a token of its own.  All in fp32: a decay
+// is off by 2^-23 or so of itself (special function unit), a state by the accumulated rounding of its memory.
+// What bounds it: 16 exponentials per token and channel (16 states) are 118 us of the special function units for 8192 x 4096, HBM 41 us; the walk reads d, d x, B and C of every
+// token from shared memory, 10 of its cycles a token and warp, which is 70 to 75 % of what an SM's shared memory gives.  bf16, 16 states, with gate: forward 8192 x 4096
+// 280 us, 4 x 2048 x 4096 285 us; backward 2 x 2048 x 4096 400 us.
 #include <type_traits>
 
 #include "block.cuh"
@@ -17,13 +19,10 @@ namespace mkda {
 
 constexpr int SCAN_THREADS = 128, SCAN_WARPS = SCAN_THREADS / 32, CKPT = MKDA_SCAN_CHECKPOINT;
 
-template <int LPC, int CPT, int TILE>
+template <int LPC>
 struct ScanShape {
     static constexpr int NP = 4 * LPC;                     // padded states
-    static constexpr int CB = SCAN_THREADS / LPC * CPT;    // channels per block
-    static constexpr int ROW = CB / 8;                     // pieces of eight channels in a row
-    static constexpr int PIECES = (TILE * ROW + SCAN_THREADS - 1) / SCAN_THREADS;      // per thread
-    static constexpr int BC = (TILE * NP / 8 + SCAN_THREADS - 1) / SCAN_THREADS;       // pieces of B (and of C) per thread
+    static constexpr int CB = SCAN_THREADS / LPC;          // channels per block
     static constexpr int YROW = CB + 8;                    // floats of a row of sums: the four tokens of a butterfly lie in different banks
 };
 
@@ -118,8 +117,8 @@ __device__ __forceinline__ Part part_of(const MkdaSeqs& s, int slot) {
 __device__ __forceinline__ int parts(const MkdaSeqs& s) { return s.seg ? s.N * s.segs : s.N; }
 
 // Forward.  Four warps walk the recurrence and four beside them do the elementwise part, a tile ahead (loads, softplus) and a tile behind (skip, gate, stores); the block's
-// barrier joins them once a tile.  A channel's chain is short and there are few warps of it (4096 channels are 512), so what counts is how many cycles a token takes a warp that
-// has a scheduler to itself: with the elementwise part in the same warps 168, of which 32 are the exponentials of the special function unit.
+// barrier joins them once a tile.  There are few warps on the chain (4096 channels are 512), so what counts is how many cycles a token takes a warp that
+// has a scheduler to itself: 168 with the elementwise part in the same warps, 65 now, of which 32 are the exponentials of the special function unit.
 constexpr int SCAN_HELPERS = 256, SCAN_LONG = 256;
 // The backward kernel: threads beside those on the chain, blocks per SM, and the registers of the two roles out of those of the launch
 constexpr int SCAN_BWD_HELPERS = 128, SCAN_BWD_THREADS = SCAN_THREADS + SCAN_BWD_HELPERS, SCAN_BWD_BLOCKS = 2, SCAN_BWD_WALK_REGS = 152, SCAN_BWD_HELP_REGS = 104, SCAN_BWD_LAUNCH_REGS = 128;
@@ -127,7 +126,7 @@ static_assert(SCAN_THREADS * SCAN_BWD_WALK_REGS + SCAN_BWD_HELPERS * SCAN_BWD_HE
               SCAN_BWD_THREADS * SCAN_BWD_LAUNCH_REGS * SCAN_BWD_BLOCKS <= 65536, "register split");
 template <int LPC, int TILE>
 struct ScanFwdShared {
-    using Sh = ScanShape<LPC, 1, TILE>;
+    using Sh = ScanShape<LPC>;
     static constexpr int AHEAD = 8;        // rows behind the last one that are read and not used
     float2 d[2][TILE + AHEAD][Sh::CB];     // d, d x
     float B[2][TILE + AHEAD][Sh::NP], C[2][TILE + AHEAD][Sh::NP], y[2][TILE][Sh::YROW];
@@ -153,11 +152,11 @@ __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S,
     }
 }
 
-// (Two states a lane and twice the warps on the chain: 302 us where this takes 275.)
+// (8192 x 4096: 280 us.  Two states a lane and twice the warps on the chain 10 % more; B and C in 16 bits side by side, or d and d x doubled for packed products, 20 %.)
 template <int DT, int LPC, int TILE>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
     follow_stream();
-    using Sh = ScanShape<LPC, 1, TILE>;
+    using Sh = ScanShape<LPC>;
     constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     auto& sh = *reinterpret_cast<ScanFwdShared<LPC, TILE>*>(raw_shared);
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) e[u].v[i] = ex2f2_(mul2(A.v[i], both(now[u].d.x)));
-#pragma unroll                                             // unrolled by 2, 4 or 8 groups 413, 341 and 315 us where wholly 275
+#pragma unroll                                             // by 2, 4 or 8 groups 413, 341 and 315 us
                 for (int t4 = 0; t4 < TILE; t4 += 4) {
                     if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = flat(h);
                     float yn[4];
@@ -367,7 +366,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
 // results per token; REV walks from the last token to the first.
 template <int DT, int LPC, int TILE>
 struct ScanPreShared {
-    using Sh = ScanShape<LPC, 1, TILE>;
+    using Sh = ScanShape<LPC>;
     static constexpr int AHEAD = 8;
     float2 d[2][TILE + AHEAD][Sh::CB];     // d, and d x or the gradient of y
     float B[2][TILE + AHEAD][Sh::NP];      // B or C
@@ -375,7 +374,7 @@ struct ScanPreShared {
 template <int DT, int LPC, int TILE, bool REV>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kernel(const MkdaScanFwd p, const void* up, float* out_h, float* out_d, const bool vec, const bool bvec) {
     follow_stream();
-    using Sh = ScanShape<LPC, 1, TILE>;
+    using Sh = ScanShape<LPC>;
     constexpr int NP = Sh::NP, CB = Sh::CB;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     auto& sh = *reinterpret_cast<ScanPreShared<DT, LPC, TILE>*>(raw_shared);
@@ -531,7 +530,7 @@ template <int DT, int LPC>
 struct ScanBwdShared {
     static constexpr int PIECES = (CKPT * SCAN_THREADS / LPC / 4 + SCAN_BWD_HELPERS - 1) / SCAN_BWD_HELPERS;
     Raw4<DT> kept[4][4][PIECES][SCAN_BWD_HELPERS];         // x, dt, z and dy of the last tiles, each thread's own: registers are what the second block needs
-    using Sh = ScanShape<LPC, 1, CKPT>;
+    using Sh = ScanShape<LPC>;
     float2 d[2][CKPT][Sh::CB];                             // d, d x
     float dy[2][CKPT][Sh::CB];
     float B[2][CKPT][Sh::NP], C[2][CKPT][Sh::NP];
@@ -543,7 +542,7 @@ template <int DT, int LPC>
 __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_kernel(const MkdaScanBwd a, const bool vec, const bool bvec) {
     follow_stream();
     constexpr int TILE = CKPT;
-    using Sh = ScanShape<LPC, 1, TILE>;
+    using Sh = ScanShape<LPC>;
     constexpr int NP = Sh::NP, CB = Sh::CB, YROW = Sh::YROW;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     auto& sh = *reinterpret_cast<ScanBwdShared<DT, LPC>*>(raw_shared);
@@ -989,7 +988,7 @@ static int launch_scan_pre(const MkdaScanFwd& p, const void* up, float* out_h, f
     constexpr int TILE = LPC == 2 ? 32 : 64, smem = (int)sizeof(ScanPreShared<DT, LPC, TILE>);
     auto* kern = scan_pre_kernel<DT, LPC, TILE, REV>;
     if (int e = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan: parts")) return e;
-    launch(kern, dim3(blocks_of_channels(p.D, p.G, ScanShape<LPC, 1, TILE>::CB), rows_of_blocks(p.S)), SCAN_THREADS + SCAN_HELPERS, smem, stream, p, up, out_h, out_d, vec, wide_states(p, 4));
+    launch(kern, dim3(blocks_of_channels(p.D, p.G, ScanShape<LPC>::CB), rows_of_blocks(p.S)), SCAN_THREADS + SCAN_HELPERS, smem, stream, p, up, out_h, out_d, vec, wide_states(p, 4));
     return check_launch("scan: parts");
 }
 
@@ -1011,7 +1010,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
         with_lanes(p->NST, [&](auto l) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const bool vec = wide_rows(*p, 4) && aligned16(p->y);
-            const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC, 1, 32>::CB);
+            const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC>::CB);
             if (p->S.seg) rc = launch_scan_pre<DT, LPC, false>(*p, nullptr, p->seg_h, p->seg_d, vec, (cudaStream_t)stream);
             if (rc != MKDA_OK) return;
             auto run = [&](auto tile) {
@@ -1033,7 +1032,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
 extern "C" int mkda_scan_bwd_channel_blocks(int D, int G, int NST) {
     int r = 0;
     if (D > 0 && G > 0 && NST > 0 && NST <= MKDA_SCAN_MAX_STATES)
-        with_lanes(NST, [&](auto l) { r = blocks_of_channels(D, G, ScanShape<decltype(l)::value, 1, CKPT>::CB); });
+        with_lanes(NST, [&](auto l) { r = blocks_of_channels(D, G, ScanShape<decltype(l)::value>::CB); });
     return r;
 }
 
