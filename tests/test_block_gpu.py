@@ -486,6 +486,66 @@ def test_side_streams_graphs_and_repeated_runs():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("how", ["stride", "size"])
+def test_offsets_past_32_bits(how):
+    """Rows whose offsets do not fit into 32 bits, by the stride of a wide projection or by the size of the tensors themselves: the last tokens are those of a short call
+    that continues from the states in front of them, bit for bit."""
+    T, W, tail = 70001, 40 if how == "stride" else 32768, 70
+    store = torch.empty(1, T, 65536 if how == "stride" else W, dtype=torch.bfloat16, device="cuda")
+    x = store[..., -W:]
+    x[:, :tail].normal_()
+    for a in range(tail, T, 10000):          # cheap to fill: the same rows again and again
+        x[:, a:a + 10000] = x[:, :tail].repeat(1, 143, 1)[:, :min(10000, T - a)]
+    assert x[0, -1, 0].data_ptr() - x.data_ptr() > 2 ** 32
+    w, A = torch.randn(W, 4, device="cuda"), -torch.rand(W, 4, device="cuda")
+    bc = torch.randn(1, T, 4, dtype=torch.bfloat16, device="cuda")
+    with torch.no_grad():
+        y, last = mk.causal_conv1d(x, w, output_final_state=True)
+        short, end = mk.causal_conv1d(x[:, -tail:].contiguous(), w, initial_state=x[:, -tail - 3:-tail].contiguous(), output_final_state=True)
+        assert torch.equal(y[:, -tail:], short) and torch.equal(last, end)
+        del y
+        n, s = mk.rms_norm(x, residual=x)
+        a, b = mk.rms_norm(x[:, -tail:].contiguous(), residual=x[:, -tail:].contiguous())
+        assert torch.equal(n[:, -tail:], a) and torch.equal(s[:, -tail:], b)
+        del n, s
+        if how == "size":                                  # many channels: not cut, so that the state in front of the tail is the long call's own
+            cut = T - 64 * 2
+            _, state = mk.selective_scan(x[:, :cut], x[:, :cut], A, bc[:, :cut], bc[:, :cut], dt_softplus=True, output_final_state=True)
+            y, last = mk.selective_scan(x, x, A, bc, bc, dt_softplus=True, output_final_state=True)
+            short, end = mk.selective_scan(x[:, cut:].contiguous(), x[:, cut:].contiguous(), A, bc[:, cut:], bc[:, cut:], dt_softplus=True, initial_state=state, output_final_state=True)
+            assert torch.equal(y[:, cut:], short) and torch.equal(last, end)
+        else:
+            y, last = mk.selective_scan(x, x, A, bc, bc, dt_softplus=True, output_final_state=True)
+            near("y", y[:, -tail:], mk.selective_scan(x.contiguous(), x.contiguous(), A, bc, bc, dt_softplus=True)[0][:, -tail:].double())
+    if how == "stride":
+        leaf = x.detach().requires_grad_(True)
+        up = torch.ones(1, T, W, dtype=torch.bfloat16, device="cuda")
+        dense = x.detach().contiguous().requires_grad_(True)
+        for call in (lambda v: mk.causal_conv1d(v, w, activation="silu")[0], lambda v: mk.rms_norm(v), lambda v: mk.selective_scan(v, v, A, bc, bc, dt_softplus=True)[0]):
+            g, = torch.autograd.grad(call(leaf), leaf, up)
+            h, = torch.autograd.grad(call(dense), dense, up)
+            assert torch.equal(g, h)
+
+
+def test_more_sequences_than_a_grid_has_rows():
+    gen = torch.Generator().manual_seed(21)
+    B, W, N = 70000, 8, 4
+    x, bc, A = rand(gen, B, 1, W).cuda().requires_grad_(True), rand(gen, B, 1, N).cuda(), -torch.rand(W, N, generator=gen).cuda()
+    h0, w, s0 = rand(gen, B, W, N).cuda().requires_grad_(True), rand(gen, W, 3).cuda(), rand(gen, B, 2, W).cuda()
+
+    def run(a, b, cu=None):
+        shape = (lambda t: t[a:b]) if cu is None else (lambda t: t[a:b].reshape(1, b - a, *t.shape[2:]))
+        y, h = mk.selective_scan(shape(x), shape(x), A, shape(bc), shape(bc), initial_state=h0[a:b], output_final_state=True, dt_softplus=True, cu_seqlens=cu)
+        c, s = mk.causal_conv1d(shape(x), w, initial_state=s0[a:b], output_final_state=True, cu_seqlens=cu)
+        g = torch.autograd.grad((y, h, c), (x, h0), (torch.ones_like(y), torch.ones_like(h), torch.ones_like(c)))
+        return y.reshape(-1, W), h, c.reshape(-1, W), s, g[0][a:b], g[1][a:b]
+
+    whole, packed = run(0, B), run(0, B, torch.arange(B + 1, device="cuda"))
+    for a, b in ((0, 3), (65534, 65537), (B - 2, B)):
+        for t, p, r in zip(whole, packed, run(a, b)):
+            assert torch.equal(t[a:b], r) and torch.equal(p[a:b], r)
+
+
 def test_capture_while_an_eager_graph_of_the_same_leaves_lives():
     """What torch's own operators do there: the capture fails with an error that the program can catch, or succeeds; the process goes on."""
     code = """
