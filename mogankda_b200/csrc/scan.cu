@@ -7,7 +7,7 @@
 // Layout.  A thread holds four states of a channel; LPC lanes share a channel (4 LPC states, NST padded with states whose B and C are zero), 128 / LPC channels are a block.
 // Four warps of a block walk the recurrence, others do the elementwise part (loads of four channels, softplus, gate, stores), tile by tile, with a layout of their own; tiles pass
 // between the two through shared memory.  Sums over the states of a channel are butterflies in which each lane ends with the sum of a token of its own.  All in fp32: a decay
-// is off by 2^-23 or so of itself (special function unit), a state by the accumulated rounding of its memory.
+// is off by 2^-24 or so of itself, a state by the accumulated rounding of its memory.
 // What bounds it: 16 exponentials per token and channel (16 states) are 118 us of the special function units for 8192 x 4096, HBM 41 us; the walk reads d, d x, B and C of every
 // token from shared memory, 10 of its cycles a token and warp, which is 70 to 75 % of what an SM's shared memory gives.  bf16, 16 states, with gate: forward 8192 x 4096
 // 280 us, 4 x 2048 x 4096 285 us; backward 2 x 2048 x 4096 400 us.
@@ -46,6 +46,11 @@ __device__ __forceinline__ float scan_softplus(float s) {
     unpack2(scan_softplus2(both(s)), a, b);
     return a;
 }
+
+// exp(d A) for two states, A scaled by log2 e.  2^x of the special function unit is low in the mean: by 0.5e-8 to 1e-8 of itself for x in (-2^-8, 0), 2e-8 to 3e-8 down to -1, 5e-8
+// below (measured over 2^18 arguments per octave).  A chain adds that up over its memory: states that keep a thousand tokens were off by 1e-6 to 3e-6 for it, twice what their
+// roundings make.  So the argument is raised by 2.2e-8, in the product's own rounding.  An argument up to 8e-8 still gives 1 exactly: d = 0 leaves the state as it is.
+__device__ __forceinline__ f32x2 scan_decay(f32x2 A, float d) { return ex2f2_(fma2(A, both(d), both(2.2e-8f))); }
 
 // Sums over the LPC lanes of a channel of four values each: v[0..3] of lane q become one (LPC >= 4: of token q & 3, in v[0]; LPC = 2: of
 // tokens q and q + 2, in v[0] and v[1]).
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) e[u].v[i] = ex2f2_(mul2(A.v[i], both(now[u].d.x)));
+                    for (int i = 0; i < 2; ++i) e[u].v[i] = scan_decay(A.v[i], now[u].d.x);
 #pragma unroll                                             // by 2, 4 or 8 groups 413, 341 and 315 us
                 for (int t4 = 0; t4 < TILE; t4 += 4) {
                     if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = flat(h);
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const f32x2 d = e[u].v[i];
-                            e[u].v[i] = ex2f2_(mul2(A.v[i], both(next[u].d.x)));
+                            e[u].v[i] = scan_decay(A.v[i], next[u].d.x);
                             h.v[i] = fma2(d, h.v[i], mul2(dx, now[u].B.v[i]));
                             y = i ? fma2(h.v[i], now[u].C.v[i], y) : mul2(h.v[i], now[u].C.v[i]);
                         }
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kerne
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) e[u].v[i] = ex2f2_(mul2(A.v[i], both(now[u].d.x)));
+                    for (int i = 0; i < 2; ++i) e[u].v[i] = scan_decay(A.v[i], now[u].d.x);
 #pragma unroll
                 for (int t4 = 0; t4 < TILE; t4 += 4) {
                     float part[4];
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kerne
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const f32x2 a = e[u].v[i], v = both(now[u].d.y);
-                            e[u].v[i] = ex2f2_(mul2(A.v[i], both(next[u].d.x)));
+                            e[u].v[i] = scan_decay(A.v[i], next[u].d.x);
                             h.v[i] = REV ? mul2(a, fma2(v, now[u].B.v[i], h.v[i])) : fma2(a, h.v[i], mul2(v, now[u].B.v[i]));
                         }
                         now[u] = next[u];
@@ -590,7 +595,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                         f32x2 y;
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const f32x2 v = mul2(ex2f2_(mul2(A.v[i], both(d.x))), h.v[i]);
+                            const f32x2 v = mul2(scan_decay(A.v[i], d.x), h.v[i]);
                             P[t4 + u].v[i] = v;
                             h.v[i] = fma2(both(d.y), B.v[i], v);
                             y = i ? fma2(h.v[i], C.v[i], y) : mul2(h.v[i], C.v[i]);
@@ -627,7 +632,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                             gb = i ? fma2(g, B.v[i], gb) : mul2(g, B.v[i]);
                             ea = i ? fma2(e, A.v[i], ea) : mul2(e, A.v[i]);
                             dAt.v[i] = fma2(e, both(d.x), dAt.v[i]);
-                            G.v[i] = mul2(ex2f2_(mul2(A.v[i], both(d.x))), g);
+                            G.v[i] = mul2(scan_decay(A.v[i], d.x), g);
                         }
                         gBs[u] = sum2(gb);
                         eAs[u] = sum2(ea);
@@ -936,7 +941,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, co
         Four o = four(h[r]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            o.v[i] = fma2(ex2f2_(mul2(A.v[i], both(dr))), o.v[i], mul2(both(dx), B[i]));
+            o.v[i] = fma2(scan_decay(A.v[i], dr), o.v[i], mul2(both(dx), B[i]));
             s = i ? fma2(C[i], o.v[i], s) : mul2(C[i], o.v[i]);
         }
         if (r < rows) st_states(p.state, row + (size_t)r * D, n0, NST, flat(o));

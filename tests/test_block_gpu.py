@@ -285,6 +285,19 @@ def test_scan_of_any_decay():
         near(n, a.cpu(), b)
 
 
+def test_scan_without_time_passing_keeps_its_state():
+    """dt = 0: exp(0) is 1 exactly, whatever A and x are; also what the tokens behind a sequence's last one inside a tile rely on."""
+    gen = torch.Generator().manual_seed(31)
+    for T, W in ((1, 40), (33, 40), (500, 8)):
+        lv = {n: t.cuda() for n, t in scan_leaves(gen, 2, T, W, 16, 1, None, torch.bfloat16, True).items()}
+        zero = torch.zeros_like(lv["x"])
+        _, h = mk.selective_scan(lv["x"], zero, 100 * lv["A"], lv["B"], lv["C"], initial_state=lv["h0"], output_final_state=True)
+        assert torch.equal(h, lv["h0"])
+        state = lv["h0"].clone()
+        mk.selective_scan_step(lv["x"][:, 0], zero[:, 0], lv["A"], lv["B"][:, 0], lv["C"][:, 0], state)
+        assert torch.equal(state, lv["h0"])
+
+
 # ---- norm ------------------------------------------------------------------------------------------------------------------------------------
 def norm_reference(x, w, res, eps, res_dtype):
     s = x
