@@ -7,6 +7,79 @@
 
 namespace mkda {
 
+// BYTES = 8 or 16 bytes from any address that is a multiple of two on, of which the first `bytes` are wanted (the others read as zero).  Rows of odd widths start anywhere: the one or two aligned
+// words of that size that hold a wanted byte are read whole, as neighbouring lanes read theirs, and shifted into place (an aligned word never leaves the allocation that one
+// of its bytes lies in).  Element by element a convolution of 8192 x 4097 in bf16 took six times as long as one of 4096 channels.
+template <int BYTES>
+struct alignas(BYTES) Words { uint32_t w[BYTES / 4]; };
+template <int BYTES>
+__device__ __forceinline__ Words<BYTES> load_shifted(const void* from, int bytes) {
+    constexpr int N = BYTES / 4;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+    const int off = (int)(at & (BYTES - 1));
+    const Words<BYTES>* p = reinterpret_cast<const Words<BYTES>*>(at - off);
+    uint32_t q[2 * N + 1];
+#pragma unroll
+    for (uint32_t& v : q) v = 0u;
+    if constexpr (BYTES == 16) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        q[0] = a.x; q[1] = a.y; q[2] = a.z; q[3] = a.w;
+        if (off + bytes > BYTES) {
+            const uint4 b = *reinterpret_cast<const uint4*>(p + 1);
+            q[4] = b.x; q[5] = b.y; q[6] = b.z; q[7] = b.w;
+        }
+    } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(p);
+        q[0] = a.x; q[1] = a.y;
+        if (off + bytes > BYTES) {
+            const uint2 b = *reinterpret_cast<const uint2*>(p + 1);
+            q[2] = b.x; q[3] = b.y;
+        }
+    }
+    // by whole words, then by half of one
+    if (BYTES == 16 && (off & 8)) {
+#pragma unroll
+        for (int i = 0; i < 2 * N - 2; ++i) q[i] = q[i + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+        for (int i = 0; i < N + 1; ++i) q[i] = q[i + 1];
+    }
+    Words<BYTES> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        r.w[i] = off & 2 ? __funnelshift_r(q[i], q[i + 1], 16) : q[i];
+        const int left = bytes - 4 * i;
+        if (left < 4) r.w[i] = left < 2 ? 0u : r.w[i] & 0xffffu;
+    }
+    return r;
+}
+// The reverse: the first `bytes` bytes of `v`, in the widest stores that the address allows.
+template <int BYTES>
+__device__ __forceinline__ void store_shifted(void* to, int bytes, const Words<BYTES>& v) {
+    constexpr int N = BYTES / 4;
+    char* const p = static_cast<char*>(to);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(to);
+    if (at & 2) {                                          // half a word, whole ones across the borders of v's, half a word
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)v.w[0];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t next = i + 1 < N ? v.w[i + 1 < N ? i + 1 : 0] : 0u;
+            if (bytes >= 4 * i + 6) *reinterpret_cast<uint32_t*>(p + 4 * i + 2) = __funnelshift_r(v.w[i], next, 16);
+            else if (bytes >= 4 * i + 4) *reinterpret_cast<uint16_t*>(p + 4 * i + 2) = (uint16_t)(v.w[i] >> 16);
+        }
+    } else if ((at & 7) == 0 && bytes == BYTES) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint2*>(p + 4 * i) = make_uint2(v.w[i], v.w[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (bytes >= 4 * i + 4) *reinterpret_cast<uint32_t*>(p + 4 * i) = v.w[i];
+            else if (bytes >= 4 * i + 2) *reinterpret_cast<uint16_t*>(p + 4 * i) = (uint16_t)v.w[i];
+        }
+    }
+}
+
 // Eight consecutive elements from `idx` on, of which the first `valid` exist (the others are zero); `vec`: idx, the address and the row
 // allow 16-byte accesses, and valid is 8 or at most 0.
 template <int DT>
@@ -17,17 +90,16 @@ __device__ __forceinline__ Raw8 load8(const void* base, size_t idx, int valid, b
     if (valid <= 0) return r;
     if (vec) {
         ldraw8<DT>(base, idx, r);
-    } else if (DT == MKDA_F32) {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = e < valid ? __float_as_uint(static_cast<const float*>(base)[idx + e]) : 0u;
-        r.a = make_uint4(w[0], w[1], w[2], w[3]);
-        r.b = make_uint4(w[4], w[5], w[6], w[7]);
     } else {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = e < valid ? static_cast<const uint16_t*>(base)[idx + e] : 0u;
-        r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        constexpr int SIZE = DT == MKDA_F32 ? 4 : 2;
+        const char* p = static_cast<const char*>(base) + idx * SIZE;
+        const int bytes = min(valid, 8) * SIZE;
+        const Words<16> a = load_shifted<16>(p, min(bytes, 16));
+        r.a = make_uint4(a.w[0], a.w[1], a.w[2], a.w[3]);
+        if (DT == MKDA_F32 && bytes > 16) {
+            const Words<16> b = load_shifted<16>(p + 16, bytes - 16);
+            r.b = make_uint4(b.w[0], b.w[1], b.w[2], b.w[3]);
+        }
     }
     return r;
 }
@@ -36,14 +108,17 @@ __device__ __forceinline__ void store8(void* base, size_t idx, int valid, bool v
     if (valid <= 0) return;
     if (vec) {
         st8<DT>(base, idx, v);
+    } else if constexpr (DT == MKDA_F32) {
+        char* p = static_cast<char*>(base) + idx * 4;
+        const int bytes = min(valid, 8) * 4;
+        store_shifted<16>(p, min(bytes, 16), Words<16>{{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}});
+        if (bytes > 16) store_shifted<16>(p + 16, bytes - 16, Words<16>{{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])}});
     } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < valid) st1(base, DT, idx + e, v[e]);
+        store_shifted<16>(static_cast<char*>(base) + idx * 2, min(valid, 8) * 2, Words<16>{{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3]), pack16<DT>(v[4], v[5]), pack16<DT>(v[6], v[7])}});
     }
 }
 
-// The same for four elements, 8-byte (fp32: 16-byte) accesses
+// The same for four elements, 8-byte (fp32: 16-byte) accesses; else element by element (shifting took registers from the scan kernels' other path: backward 400 -> 450 us)
 template <int DT>
 struct alignas(DT == MKDA_F32 ? 16 : 8) Raw4 { uint32_t w[DT == MKDA_F32 ? 4 : 2]; };
 template <int DT>

@@ -14,36 +14,33 @@ namespace mkda {
 
 constexpr int CONV_BATCH = 4;            // rows requested together, and places of the ring that holds the window (a power of two, at least W)
 
-// The V channels of a thread: neighbours from d0 on where rows allow 16-byte (8-byte) accesses, else one in 128 from d0 on, so that the single
-// elements that a warp reads are neighbours.
-template <int V>
-__device__ __forceinline__ int conv_channel(bool vec) { return vec ? (blockIdx.x * 128 + threadIdx.x) * V : blockIdx.x * 128 * V + threadIdx.x; }
-
-// Their elements in a row, as they lie in memory; those past the last channel are zero
+// The V channels of a thread from d0 on: neighbours, but one in 128 in fp32 rows that do not allow 16-byte accesses, whose single elements are then neighbours in a warp (8192 x 4097 forward
+// 61 us; shifted from aligned words, as 16-bit rows are, 114).  `vec`: rows allow 16-byte (8-byte) accesses.
+template <int DT, bool vec>
+__device__ __forceinline__ constexpr int conv_step() { return DT == MKDA_F32 && !vec ? 128 : 1; }
+template <int DT, int V, bool vec>
+__device__ __forceinline__ int conv_channel() { return conv_step<DT, vec>() == 1 ? (blockIdx.x * 128 + threadIdx.x) * V : blockIdx.x * 128 * V + threadIdx.x; }
+// Their elements in a row, as they lie in memory, those past the last channel zero
 template <int DT, int V>
 struct alignas(DT == MKDA_F32 ? V * 4 : V * 2) ConvRaw { uint32_t w[DT == MKDA_F32 ? V : V / 2]; };
 template <int DT, int V>
 __device__ __forceinline__ ConvRaw<DT, V> conv_raw(const void* base, size_t row, int d0, int D, bool vec) {
     ConvRaw<DT, V> r;
-    constexpr int WORDS = DT == MKDA_F32 ? V : V / 2;
-    if (vec) {
-        if constexpr (WORDS == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(base) + (row + d0) * (DT == MKDA_F32 ? 4 : 2));
-            r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
-        } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const char*>(base) + (row + d0) * 2);
-            r.w[0] = v.x; r.w[1] = v.y;
-        }
-    } else if constexpr (DT == MKDA_F32) {
+    constexpr int WORDS = DT == MKDA_F32 ? V : V / 2, SIZE = DT == MKDA_F32 ? 4 : 2;
+    const char* p = static_cast<const char*>(base) + (row + d0) * SIZE;
+    if (!vec && DT == MKDA_F32) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) r.w[e] = d0 + 128 * e < D ? static_cast<const uint32_t*>(base)[row + d0 + 128 * e] : 0u;
+        for (int e = 0; e < V; ++e) r.w[e] = d0 + 128 * e < D ? *reinterpret_cast<const uint32_t*>(p + 512 * e) : 0u;
+    } else if (!vec) {
+        const Words<4 * WORDS> v = load_shifted<4 * WORDS>(p, min(V, D - d0) * SIZE);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) r.w[i] = v.w[i];
+    } else if constexpr (WORDS == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
     } else {
-        const uint16_t* p = static_cast<const uint16_t*>(base) + row + d0;
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-            const uint32_t lo = d0 + 256 * e < D ? p[256 * e] : 0u, hi = d0 + 256 * e + 128 < D ? p[256 * e + 128] : 0u;
-            r.w[e] = lo | hi << 16;
-        }
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = v.x; r.w[1] = v.y;
     }
     return r;
 }
@@ -68,7 +65,7 @@ __device__ __forceinline__ void conv_unpack(const ConvRaw<DT, V>& r, f32x2 (&v)[
         }
     }
 }
-template <int DT, int V>
+template <int DT, int V, int STEP = 128>
 __device__ __forceinline__ void conv_store(void* base, size_t row, int d0, int D, bool vec, const f32x2 (&p)[V / 2]) {
     float v[V];
 #pragma unroll
@@ -76,17 +73,22 @@ __device__ __forceinline__ void conv_store(void* base, size_t row, int d0, int D
     if (vec) {
         if constexpr (V == 8) st8<DT>(base, row + d0, v);
         else st4(base, DT, row + d0, make_float4(v[0], v[1], v[2], v[3]));
-    } else {
+    } else if constexpr (DT == MKDA_F32) {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (d0 + 128 * e < D) st1(base, DT, row + d0 + 128 * e, v[e]);
+            if (d0 + e * STEP < D) static_cast<float*>(base)[row + d0 + e * STEP] = v[e];
+    } else {
+        Words<2 * V> w;
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) w.w[e] = pack16<DT>(v[2 * e], v[2 * e + 1]);
+        store_shifted<2 * V>(static_cast<uint16_t*>(base) + row + d0, min(V, D - d0) * 2, w);
     }
 }
 // weights [D][W] and biases of the thread's channels; those past the last channel are zero
 template <int W, int V>
-__device__ __forceinline__ void conv_params(const float* weight, const float* bias, int d0, int D, bool vec, f32x2 (&wt)[W][V / 2], f32x2 (&b)[V / 2]) {
+__device__ __forceinline__ void conv_params(const float* weight, const float* bias, int d0, int D, int step, f32x2 (&wt)[W][V / 2], f32x2 (&b)[V / 2]) {
     float f[V * W], g[V];
-    if (vec) {                // V W numbers in a row
+    if (step == 1 && d0 + V <= D && aligned16(weight)) {   // V W numbers in a row
 #pragma unroll
         for (int i = 0; i < V * W; i += 4) {
             const float4 v = *reinterpret_cast<const float4*>(weight + (size_t)d0 * W + i);
@@ -94,10 +96,10 @@ __device__ __forceinline__ void conv_params(const float* weight, const float* bi
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V * W; ++i) f[i] = d0 + 128 * (i / W) < D ? weight[(size_t)(d0 + 128 * (i / W)) * W + i % W] : 0.f;
+        for (int i = 0; i < V * W; ++i) f[i] = d0 + i / W * step < D ? weight[(size_t)(d0 + i / W * step) * W + i % W] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) g[e] = bias && d0 + (vec ? e : 128 * e) < D ? bias[d0 + (vec ? e : 128 * e)] : 0.f;
+    for (int e = 0; e < V; ++e) g[e] = bias && d0 + e * step < D ? bias[d0 + e * step] : 0.f;
 #pragma unroll
     for (int e = 0; e < V / 2; ++e) {
         b[e] = pack2(g[2 * e], g[2 * e + 1]);
@@ -114,8 +116,8 @@ __device__ __forceinline__ ConvRaw<DT, V> conv_row(const void* x, long long stri
     return conv_zero<DT, V>();
 }
 // Rows on their way.  A thread copies its own channels of the next STAGES - 1 batches into shared memory asynchronously and reads them back itself, so that no
-// barrier is needed and more bytes are in flight than its registers could hold (two batches in registers: 212 us for 32749 x 8192 bf16).  Single
-// elements, which the asynchronous copy does not know in 16 bits, pass through registers, a batch at a time.
+// barrier is needed and more bytes are in flight than its registers could hold (two batches in registers: 212 us for 32749 x 8192 bf16).  Rows that
+// start anywhere, which the asynchronous copy cannot shift, pass through registers, a batch at a time.
 template <int DT, int V, int STAGES>
 struct ConvFeed {
     static constexpr int BYTES = sizeof(ConvRaw<DT, V>), SHARED = STAGES * CONV_BATCH * 128 * BYTES;
@@ -174,11 +176,11 @@ __global__ void __launch_bounds__(128, vec ? CONV_FWD_BLOCKS : 3) conv_fwd_kerne
     constexpr int P = V / 2;
     constexpr int STAGES = 4;
     __shared__ __align__(16) char shared_rows[ConvFeed<DT, V, STAGES>::SHARED];
-    const int D = p.D, d0 = conv_channel<V>(vec), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
+    const int D = p.D, d0 = conv_channel<DT, V, vec>(), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
     int n = t0 < t1 ? sequence_of(p.S, t0) : p.S.N;
     if (d0 >= D) return;
     f32x2 wt[W][P], bias[P];
-    conv_params<W, V>(p.weight, p.bias, d0, D, vec, wt, bias);
+    conv_params<W, V>(p.weight, p.bias, d0, D, conv_step<DT, vec>(), wt, bias);
     ConvFeed<DT, V, STAGES> feed(shared_rows, p.x, p.x_stride, d0, D, vec);
     if (blockIdx.y == 0 && p.S.has_empty && p.last) {      // an empty sequence hands its state through
         for (int n = 0; n < p.S.N; ++n) {
@@ -252,13 +254,13 @@ __global__ void __launch_bounds__(128, vec ? CONV_BWD_BLOCKS : 3) conv_bwd_kerne
     constexpr int P = V / 2;
     constexpr int STAGES = DT == MKDA_F32 ? 3 : 4;
     __shared__ __align__(16) char shared_rows[2][ConvFeed<DT, V, STAGES>::SHARED];
-    const int D = p.D, d0 = conv_channel<V>(vec), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
+    const int D = p.D, d0 = conv_channel<DT, V, vec>(), t0 = (int)min((long long)blockIdx.y * run, (long long)p.S.TT), t1 = min(t0 + run, p.S.TT);
     int n = t0 < t1 ? sequence_of(p.S, t0) : p.S.N;
     if (d0 >= D) return;
     ConvFeed<DT, V, STAGES> feed_x(shared_rows[0], p.x, p.x_stride, d0, D, vec);
     ConvFeed<DT, V, STAGES> feed_y(shared_rows[1], p.dy, D, d0, D, vec);
     f32x2 wt[W][P], bias[P], dw[W][P], db[P];
-    conv_params<W, V>(p.weight, p.bias, d0, D, vec, wt, bias);
+    conv_params<W, V>(p.weight, p.bias, d0, D, conv_step<DT, vec>(), wt, bias);
 #pragma unroll
     for (int e = 0; e < P; ++e) {
         db[e] = both(0.f);
@@ -357,21 +359,21 @@ __global__ void __launch_bounds__(128, vec ? CONV_BWD_BLOCKS : 3) conv_bwd_kerne
     }
     float* part = p.part + (size_t)blockIdx.y * (W + 1) * D;
 #pragma unroll
-    for (int w = 0; w < W; ++w) conv_store<MKDA_F32, V>(part, (size_t)w * D, d0, D, vec, dw[w]);
-    conv_store<MKDA_F32, V>(part, (size_t)W * D, d0, D, vec, db);
+    for (int w = 0; w < W; ++w) conv_store<MKDA_F32, V, conv_step<DT, vec>()>(part, (size_t)w * D, d0, D, vec, dw[w]);
+    conv_store<MKDA_F32, V, conv_step<DT, vec>()>(part, (size_t)W * D, d0, D, vec, db);
 }
 
 template <int DT, int W, int V, bool vec>
 __global__ void __launch_bounds__(128) conv_step_kernel(const MkdaConvStep p) {
     follow_stream();
     constexpr int P = V / 2;
-    const int D = p.D, d0 = conv_channel<V>(vec), n = blockIdx.y;
+    const int D = p.D, d0 = conv_channel<DT, V, vec>(), n = blockIdx.y;
     if (d0 >= D) return;
     f32x2 rows[W][P], wt[W][P], y[P];
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) conv_unpack<DT, V>(conv_raw<DT, V>(p.state, ((size_t)n * (W - 1) + j) * D, d0, D, vec), rows[j]);
     conv_unpack<DT, V>(conv_raw<DT, V>(p.x, (size_t)n * p.x_stride, d0, D, vec), rows[W - 1]);
-    conv_params<W, V>(p.weight, p.bias, d0, D, vec, wt, y);
+    conv_params<W, V>(p.weight, p.bias, d0, D, conv_step<DT, vec>(), wt, y);
 #pragma unroll
     for (int e = 0; e < P; ++e) {
 #pragma unroll
@@ -412,14 +414,29 @@ extern "C" int mkda_conv_fwd(const MkdaConvFwd* p, void* stream) {
     if (p->W < 2 || p->W > 4 || p->D <= 0 || !good_sequences(p->S)) return set_error(MKDA_ERR_ARG, "conv_fwd: 2 to 4 taps, at least one channel");
     if (p->dtype < MKDA_F32 || p->dtype > MKDA_F16) return set_error(MKDA_ERR_ARG, "conv_fwd: unsupported dtype");
     if (p->S.N == 0 || (p->S.TT == 0 && !(p->last && p->S.has_empty))) return MKDA_OK;
+    const bool vec4 = p->D % 4 == 0 && p->x_stride % 4 == 0 && aligned16(p->x) && aligned16(p->weight) && aligned16(p->y) && aligned16(p->state) && aligned16(p->last);
+    const bool vec8 = vec4 && p->D % 8 == 0 && p->x_stride % 8 == 0;
     with_dtype(p->dtype, [&](auto dt) {
         with_taps(p->W, [&](auto w) {
-            constexpr int DT = decltype(dt)::value, W = decltype(w)::value, V = DT == MKDA_F32 ? 4 : 8;
-            const int blocks = (p->D + 128 * V - 1) / (128 * V);
-            const bool vec = p->D % V == 0 && p->x_stride % V == 0 && aligned16(p->x) && aligned16(p->weight) && aligned16(p->y) && aligned16(p->state) && aligned16(p->last);
-            const long long run = conv_run(p->S.TT, blocks, CONV_FWD_BLOCKS, 8);
-            const int rows = (int)((p->S.TT + run - 1) / run);
-            launch(vec ? conv_fwd_kernel<DT, W, V, true> : conv_fwd_kernel<DT, W, V, false>, dim3(blocks, rows ? rows : 1), 128, 0, (cudaStream_t)stream, *p, (int)run);
+            constexpr int DT = decltype(dt)::value, W = decltype(w)::value;
+            auto run = [&](auto v, auto wide) {
+                constexpr int V = decltype(v)::value;
+                constexpr bool vec = decltype(wide)::value;
+                const int blocks = (p->D + 128 * V - 1) / (128 * V);
+                const long long run = conv_run(p->S.TT, blocks, CONV_FWD_BLOCKS, 8);
+                const int rows = (int)((p->S.TT + run - 1) / run);
+                launch(conv_fwd_kernel<DT, W, V, vec>, dim3(blocks, rows ? rows : 1), 128, 0, (cudaStream_t)stream, *p, (int)run);
+            };
+            // eight channels of 16 bits a thread, four where rows are only multiples of 8 bytes (8192 x 4096 30 and 31 us)
+            using std::integral_constant;
+            if constexpr (DT == MKDA_F32) {
+                if (vec4) run(integral_constant<int, 4>(), std::true_type());
+                else run(integral_constant<int, 4>(), std::false_type());
+            } else {
+                if (vec8) run(integral_constant<int, 8>(), std::true_type());
+                else if (vec4) run(integral_constant<int, 4>(), std::true_type());
+                else run(integral_constant<int, 8>(), std::false_type());
+            }
         });
     });
     return check_launch("conv_fwd");
