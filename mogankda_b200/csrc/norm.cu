@@ -248,12 +248,26 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
             if (p.dres) store8<RT>(p.dres, (size_t)row * H + c, min(H - c, 8), vec, o);
         }
     }
-    if (p.part) {
+    if (!p.part) return;
+    if constexpr (RPB > 1) {                               // the warps of a block, in order: a row of partial sums per block
+        float* all = norm_w + TPR * NV * 8;                // [RPB][TPR * NV * 8]
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (tid + i * TPR) * 8;
-            store8<MKDA_F32>(p.part, (size_t)first * H + c, min(H - c, 8), (H & 7) == 0, dw[i]);
-        }
+        for (int i = 0; i < NV; ++i) st8<MKDA_F32>(all, (threadIdx.x / TPR) * TPR * NV * 8 + (tid + i * TPR) * 8, dw[i]);
+        __syncthreads();
+        if (threadIdx.x >= TPR) return;
+        for (int w = 1; w < RPB; ++w)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float v[8];
+                ld8(all, MKDA_F32, w * TPR * NV * 8 + (tid + i * TPR) * 8, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dw[i][e] += v[e];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (tid + i * TPR) * 8;
+        store8<MKDA_F32>(p.part, (size_t)blockIdx.x * H + c, min(H - c, 8), (H & 7) == 0, dw[i]);
     }
 }
 
@@ -321,7 +335,8 @@ static bool with_width_bwd(int H, F f) {
 template <typename F>
 static bool with_width(int H, F f) {
     using std::integral_constant;
-    if (H <= 512) f(integral_constant<int, 32>(), integral_constant<int, 2>());
+    if (H <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
+    else if (H <= 512) f(integral_constant<int, 32>(), integral_constant<int, 2>());
     else if (H <= 1024) f(integral_constant<int, 128>(), integral_constant<int, 1>());
     else if (H <= 2048) f(integral_constant<int, 128>(), integral_constant<int, 2>());
     else if (H <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
@@ -365,8 +380,7 @@ extern "C" int mkda_norm_fwd(const MkdaNormFwd* p, void* stream) {
 extern "C" int mkda_norm_bwd_part_rows(int rows, int width) {
     int r = 0;
     with_width_bwd(width, [&](auto t, auto) {
-        constexpr int TPR = decltype(t)::value, RPB = TPR < 128 ? 128 / TPR : 1;
-        r = norm_blocks<TPR, NORM_BWD_THREADS>(rows) * RPB;
+        r = norm_blocks<decltype(t)::value, NORM_BWD_THREADS>(rows);
     });
     return r;
 }
@@ -387,7 +401,7 @@ extern "C" int mkda_norm_bwd(const MkdaNormBwd* p, void* stream) {
             constexpr int DT = decltype(dt)::value, TPR = decltype(t)::value, NV = decltype(n)::value;
             auto* kern = p->s_dtype == DT ? vec ? norm_bwd_kernel<DT, DT, TPR, NV, true> : norm_bwd_kernel<DT, DT, TPR, NV, false>
                                           : vec ? norm_bwd_kernel<DT, MKDA_F32, TPR, NV, true> : norm_bwd_kernel<DT, MKDA_F32, TPR, NV, false>;
-            constexpr int smem = TPR * NV * 8 * 4;
+            constexpr int smem = TPR * NV * 8 * 4 * (TPR < 128 ? 1 + 128 / TPR : 1);
             if (smem > 40000) rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "norm_bwd");
             if (rc == MKDA_OK) launch(kern, norm_blocks<TPR, NORM_BWD_THREADS>(p->rows), TPR < 128 ? 128 : TPR, smem, (cudaStream_t)stream, *p, wvec);
         });
