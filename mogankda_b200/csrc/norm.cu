@@ -5,6 +5,7 @@
 // Bound by HBM: a row stays in the registers of the threads that share it (a warp for narrow rows, up to 1024 threads for wide ones),
 // in pieces of eight channels, so that everything is read once.  8192 x 4096 bf16 with a residual: forward 46 us (5.8 TB/s), backward 50 us (5.4 TB/s) and 5 us for the sum of the
 // weight's gradient; 65536 x 2048 with an output in e4m3 169 us (5.6 TB/s).
+#include <algorithm>
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -271,35 +272,38 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
     }
 }
 
-// A block adds the rows of 32 columns: eight threads of four columns each, 32 rows at a time, then the 32 in order.
+// A block adds the rows of 1024 / LANES columns: four columns a thread, LANES rows at a time, then the LANES in order.  Many rows of few columns by 32 lanes, few rows of many
+// columns by four (128 rows of 2 x 65536 columns 22 us by 32 lanes, 17 by four).
+template <int LANES>
 __global__ void __launch_bounds__(256) sum_rows_kernel(const MkdaSumRows p) {
     follow_stream();
-    __shared__ float4 part[32][8];
+    constexpr int QUADS = 256 / LANES, COLS = 4 * QUADS;
+    __shared__ float4 part[LANES][QUADS];
     long long blk = blockIdx.x;
     int j = 0;
     for (; j < 5; ++j) {
-        const long long n = p.job[j].out ? (p.job[j].cols + 31) / 32 * p.job[j].groups : 0;
+        const long long n = p.job[j].out ? (p.job[j].cols + COLS - 1) / COLS * p.job[j].groups : 0;
         if (blk < n) break;
         blk -= n;
     }
     if (j == 5) return;
     const MkdaSumJob& q = p.job[j];
-    const long long per = (q.cols + 31) / 32, g = blk / per, first = (blk - g * per) * 32;
-    const int l = threadIdx.x >> 3, k = threadIdx.x & 7;
+    const long long per = (q.cols + COLS - 1) / COLS, g = blk / per, first = (blk - g * per) * COLS;
+    const int l = threadIdx.x / QUADS, k = threadIdx.x % QUADS;
     const long long c = first + 4 * k;
     const float* in = q.in + (size_t)g * q.rows * q.pitch + c;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (((q.cols | q.pitch) & 3) == 0 && (reinterpret_cast<uintptr_t>(q.in) & 15) == 0) {
         if (c < q.cols) {
-#pragma unroll 4
-            for (int r = l; r < q.rows; r += 32) {
+#pragma unroll 8
+            for (int r = l; r < q.rows; r += LANES) {
                 const float4 v = *reinterpret_cast<const float4*>(in + (size_t)r * q.pitch);
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
         }
     } else {
 #pragma unroll 4
-        for (int r = l; r < q.rows; r += 32) {
+        for (int r = l; r < q.rows; r += LANES) {
             const float* v = in + (size_t)r * q.pitch;
             if (c < q.cols) s.x += v[0];
             if (c + 1 < q.cols) s.y += v[1];
@@ -309,11 +313,11 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const MkdaSumRows p) {
     }
     part[l][k] = s;
     __syncthreads();
-    if (threadIdx.x >= 32) return;
+    if (threadIdx.x >= COLS) return;
     const float* all = reinterpret_cast<const float*>(part) + threadIdx.x;      // one column per thread
     float o = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) o += all[32 * i];
+    for (int i = 0; i < LANES; ++i) o += all[COLS * i];
     const long long at = first + threadIdx.x, outer = at / q.inner, inner = at - outer * q.inner;
     if (at < q.cols && inner < q.valid) st1(q.out, q.out_dtype, (size_t)(g * q.out_group + outer * q.out_outer + inner * q.out_inner), o);
 }
@@ -412,15 +416,20 @@ extern "C" int mkda_norm_bwd(const MkdaNormBwd* p, void* stream) {
 
 extern "C" int mkda_sum_rows(const MkdaSumRows* p, void* stream) {
     if (!p) return set_error(MKDA_ERR_ARG, "sum_rows: null argument");
-    long long blocks = 0;
+    long long blocks = 0, wide = 0;
+    int most = 0;
     for (const MkdaSumJob& q : p->job) {
         if (!q.out) continue;
         if ((!q.in && q.rows > 0) || q.rows < 0 || q.groups < 0 || q.cols < 0 || q.pitch < q.cols || q.inner < 1 || !good_dtype(q.out_dtype)) return set_error(MKDA_ERR_ARG, "sum_rows: bad argument");
         blocks += (q.cols + 31) / 32 * q.groups;
+        wide += (q.cols + 255) / 256 * q.groups;
+        most = std::max(most, q.rows);
     }
     if (blocks > 0x7fffffffll) return set_error(MKDA_ERR_ARG, "sum_rows: too many columns");
     if (blocks == 0) return MKDA_OK;
-    launch(sum_rows_kernel, (unsigned)blocks, 256, 0, (cudaStream_t)stream, *p);
+    // four lanes where that leaves two blocks per SM and no job has a long way down its rows
+    if (wide >= 2 * sm_count() && most <= 512) launch(sum_rows_kernel<4>, (unsigned)wide, 256, 0, (cudaStream_t)stream, *p);
+    else launch(sum_rows_kernel<32>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, *p);
     return check_launch("sum_rows");
 }
 
