@@ -146,14 +146,23 @@ __device__ __forceinline__ float4 flat(const Four& s) {
     return f;
 }
 
-// What enters a part: the state (or its gradient) that enters the sequence, carried over the parts in front (behind).  A (scaled by log2 e): of this lane.
+// What enters a part: the state (or its gradient) that enters the sequence, carried over the parts in front (behind).  A (scaled by log2 e): of this lane.  A part's decay
+// goes in by two halves, since the whole may leave the range where decay times state does not, and nothing stays nothing under any growth.
 __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S, int n, int from, int to, int step, const float* seg_h, const float* seg_d, int D, size_t ch, int NP, int n0) {
     for (int j = from; j != to; j += step) {
         const size_t i = ((size_t)j * S.N + n) * D + ch;
         const Four h = four(*reinterpret_cast<const float4*>(seg_h + i * NP + n0));
-        const f32x2 d = both(seg_d[i]);
+        const f32x2 d = both(0.5f * seg_d[i]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s.v[e] = fma2(ex2f2_(mul2(A.v[e], d)), s.v[e], h.v[e]);
+        for (int e = 0; e < 2; ++e) {
+            const f32x2 half = ex2f2_(mul2(A.v[e], d)), first = mul2(half, s.v[e]);
+            float a, b, a1, b1;
+            unpack2(s.v[e], a, b);
+            unpack2(fma2(half, first, h.v[e]), a1, b1);
+            float ha, hb;
+            unpack2(h.v[e], ha, hb);
+            s.v[e] = pack2(a == 0.f ? ha : a1, b == 0.f ? hb : b1);
+        }
     }
 }
 

@@ -298,6 +298,36 @@ def test_scan_without_time_passing_keeps_its_state():
         assert torch.equal(state, lv["h0"])
 
 
+def test_scan_of_growing_states_behind_zeros():
+    """A > 0 and a long stretch of zeros: nothing grows into nothing, also where the growth of a part of the sequence is past the largest number."""
+    gen = torch.Generator().manual_seed(21)
+    T, D, N, few = 1500, 8, 16, 10
+    x, up = torch.zeros(1, T, D), torch.zeros(1, T, D)
+    x[:, -few:], up[:, :few] = rand(gen, 1, few, D), rand(gen, 1, few, D)
+    lv = {"x": x, "dt": torch.ones(1, T, D), "A": torch.full((D, N), 2.0), "B": rand(gen, 1, T, N), "C": rand(gen, 1, T, N)}
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+    outs, grads = differentiate(lambda: mk.selective_scan(*mine.values()), mine, [up.cuda()], list(lv))
+    routs, rgrads = differentiate(lambda: scan_reference(*wide.values()), wide, [up.double()], list(lv))
+    for n, a, b in zip(["y"] + ["d" + n for n in lv], outs + grads, routs + rgrads):
+        near(n, a.cpu(), b)
+
+
+def test_scan_of_states_that_leave_the_range_of_a_decay():
+    """What a part of a sequence lets through may be below the smallest number where what comes out of it is not: 2^90 by 2^-185 (a part of 128 tokens)."""
+    T, D, N = 512, 8, 16
+    gen = torch.Generator().manual_seed(22)
+    lv = {"x": torch.zeros(1, T, D), "dt": torch.ones(1, T, D), "A": torch.full((D, N), -1.0), "B": rand(gen, 1, T, N), "C": rand(gen, 1, T, N)}
+    h0 = (1 + rand(gen, 1, D, N).abs()) * 2.0 ** 90
+    with torch.no_grad():
+        y, _ = mk.selective_scan(*(t.cuda() for t in lv.values()), initial_state=h0.cuda())
+        ref, _ = scan_reference(*(t.double() for t in lv.values()), h0=h0.double())
+    # 140 tokens are 140 factors off by 2^-22 each and as many roundings of 2^-24: 140 (2^-22 + 2^-24) = 4.2e-5 of the value, of each term of the sum over the states
+    got, ref = y[0, :140].double().cpu(), ref[0, :140]
+    size = torch.einsum("tn,dn->td", lv["C"][0, :140].double().abs(), h0[0].double()) * torch.exp(-torch.arange(1, 141).double())[:, None]
+    assert ((got - ref).abs() <= 4.2e-5 * size).all()
+
+
 # ---- norm ------------------------------------------------------------------------------------------------------------------------------------
 def norm_reference(x, w, res, eps, res_dtype):
     s = x
