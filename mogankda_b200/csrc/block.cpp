@@ -3,6 +3,8 @@
 #include "binding.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/edge.h>
@@ -15,6 +17,8 @@
 #include <functional>
 #include <limits>
 #include <memory>
+#include <mutex>
+#include <unordered_map>
 
 using namespace mkda_host;
 using torch::autograd::SavedVariable;
@@ -162,6 +166,20 @@ bool get_sequences(PyObject* table, PyObject* dims, int64_t B, int64_t T, Sequen
     q.s.order = p + 2 * q.s.N + 1;
     return true;
 }
+// The kernels of the current stream read the table: the allocator hears of it if it is another stream than the table's own, and a table that a stream capture records is
+// kept for good, since the cache that holds it (index.py) may let go of it before the last replay.
+void reads_table(const Sequences& q) {
+    if (!q.table.defined()) return;
+    const auto on = c10::cuda::getCurrentCUDAStream();
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
+        c10::cuda::CUDACachingAllocator::recordStream(q.table.storage().data_ptr(), on);
+        return;
+    }
+    static std::mutex lock;
+    static auto* const kept = new std::unordered_map<const void*, Tensor>();      // never destroyed: CUDA may be gone by then
+    std::lock_guard<std::mutex> hold(lock);
+    kept->emplace(q.table.unsafeGetTensorImpl(), q.table);
+}
 Tensor out_like(const Tensor& x, bool covers_all) {          // contiguous; tokens outside every sequence are zero
     Tensor t = new_cuda(x.sizes(), x.scalar_type(), x.device());
     if (!covers_all) t.zero_();
@@ -215,6 +233,7 @@ MkdaConvFwd conv_call(const Sequences& q, const Rows& x, const Tensor& w, const 
 }
 
 variable_list conv_backward(const Sequences& q, int silu, const variable_list& s, const variable_list& grads) {
+    reads_table(q);
     const Tensor &x0 = s[0], w = param(s[1]), bias = param(s[2]), state = aligned(s[3]);
     const Rows x = rows_of(x0);
     const int64_t D = w.size(0), W = w.size(1), TT = q.s.TT;
@@ -269,6 +288,7 @@ PyObject* conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         pybind11::gil_scoped_release nogil;
         c10::cuda::CUDAGuard guard(x.device());
+        reads_table(q);
         const bool grad = any_requires_grad(t);
         {
             at::AutoGradMode off(false);
@@ -389,6 +409,7 @@ struct ScanCall {
 };
 
 variable_list scan_backward(const Sequences& q, int softplus, const variable_list& s, const variable_list& grads) {
+    reads_table(q);
     const variable_list in(s.begin(), s.begin() + SCAN_INPUTS);
     const Tensor ckpt = aligned(s[SCAN_INPUTS]);
     const ScanCall call(q, in, softplus);
@@ -487,6 +508,7 @@ PyObject* scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
         pybind11::gil_scoped_release nogil;
         c10::cuda::CUDAGuard guard(x.device());
+        reads_table(q);
         const bool grad = any_requires_grad(t);
         {
             at::AutoGradMode off(false);

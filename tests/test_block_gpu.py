@@ -529,6 +529,35 @@ def test_side_streams_graphs_and_repeated_runs():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_a_captured_call_keeps_the_boundaries_of_its_sequences():
+    """The table of the boundaries is the framework's own: a replay reads it however many other calls came in between."""
+    from mogankda_b200 import index
+    gen = torch.Generator().manual_seed(23)
+    x = rand(gen, 1, 90, 64).to(torch.bfloat16).cuda().requires_grad_(True)
+    bc, A, w, up = rand(gen, 1, 90, 16).to(torch.bfloat16).cuda(), -torch.ones(64, 16, device="cuda"), rand(gen, 64, 4).cuda(), torch.ones(1, 90, 64, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 20, 21, 90], device="cuda")
+
+    def step():
+        y, _ = mk.causal_conv1d(x, w, cu_seqlens=cu)
+        z, _ = mk.selective_scan(y, y, A, bc, bc, dt_softplus=True, cu_seqlens=cu)
+        return z.detach(), *torch.autograd.grad(z, x, up)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.detach().clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    index._cache.clear()
+    torch.cuda.synchronize()
+    others = [torch.zeros(10, dtype=torch.int32, device="cuda") for _ in range(512)]      # boundaries of nothing, in the memory that a lost table would have left
+    graph.replay()
+    torch.cuda.synchronize()
+    assert len(others) == 512 and all(torch.equal(a, b) for a, b in zip(want, out))
+
+
 @pytest.mark.parametrize("how", ["stride", "size"])
 def test_offsets_past_32_bits(how):
     """Rows whose offsets do not fit into 32 bits, by the stride of a wide projection or by the size of the tensors themselves: the last tokens are those of a short call
