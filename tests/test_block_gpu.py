@@ -558,6 +558,45 @@ def test_a_captured_call_keeps_the_boundaries_of_its_sequences():
     assert len(others) == 512 and all(torch.equal(a, b) for a, b in zip(want, out))
 
 
+@pytest.mark.parametrize("T", [200, 1700])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_what_is_not_finite_stays_in_its_sequence(T, what):
+    """Sequences next to one that is not finite, and in front of a tail that no sequence covers, have the bits that they have beside finite ones (1700: cut into parts)."""
+    gen = torch.Generator().manual_seed(24)
+    D, N = 40, 16
+    cu, bad = [0, 5, 37, 38, T - 90, T - 20], [1, 3]                # sequences that are spoiled
+    lv = {n: rand(gen, 1, T, m).to(torch.bfloat16) for n, m in (("x", D), ("dt", D), ("z", D), ("B", N), ("C", N))}
+    h0, w, A = rand(gen, 5, D, N), rand(gen, D, 4), -torch.rand(D, N, generator=gen)
+    up = rand(gen, 1, T, D).to(torch.bfloat16)
+    keep = torch.zeros(T, dtype=torch.bool)
+    for i, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        keep[a:b] = i not in bad
+    table = torch.tensor(cu, device="cuda")
+
+    def run(spoil):
+        def at(t):
+            t = t.clone()
+            if spoil:
+                t[:, ~keep] = what
+            return t.cuda()
+        m = {n: at(t).requires_grad_(True) for n, t in lv.items()}
+        s = h0.clone()
+        if spoil:
+            s[bad] = what
+        s, u = s.cuda().requires_grad_(True), at(up)
+        c, last = mk.causal_conv1d(m["x"], w.cuda(), cu_seqlens=table, activation="silu", output_final_state=True)
+        y, end = mk.selective_scan(m["x"], m["dt"], A.cuda(), m["B"], m["C"], z=m["z"], dt_softplus=True, initial_state=s, output_final_state=True, cu_seqlens=table)
+        g = torch.autograd.grad((c, y), [*m.values(), s], (u, u))
+        good = [i for i in range(5) if i not in bad]
+        return [t[:, keep.cuda()] for t in (c, y, *g[:-1])] + [t[good] for t in (last, end, g[-1])], [t[:, cu[-1]:] for t in (c, y, *g[:-1])]
+
+    (want, tails), (got, spoiled) = run(False), run(True)
+    for a, b in zip(want, got):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    for t in tails + spoiled:
+        assert (t == 0).all()
+
+
 @pytest.mark.parametrize("how", ["stride", "size"])
 def test_offsets_past_32_bits(how):
     """Rows whose offsets do not fit into 32 bits, by the stride of a wide projection or by the size of the tensors themselves: the last tokens are those of a short call
