@@ -5,7 +5,8 @@ Conventions of the layer hold: CUDA tensors only, bfloat16, float16 or float32, 
 ``torch.cuda.current_stream()`` of the tensors' device, packed sequences addressed by ``cu_seqlens`` (B == 1; tokens behind the last boundary give zeros,
 and have zero gradients), ``initial_state`` / final state with one row per sequence.  Activations may be slices of a wider projection: rows with any stride
 are read where they lie as long as one stride leads from token to token, other layouts are copied.  Gradients exist for every floating
-argument of the functions without ``_step``; a second differentiation is refused.  Results do not depend on the order of execution.
+argument of the functions without ``_step``; a gradient that is differentiated again (``create_graph``) raises, unless it is a constant.  Results do not depend on
+the order of execution.
 """
 import torch
 

@@ -9,12 +9,6 @@
 #include "binding.h"
 
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/edge.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/grad_mode.h>
-#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <memory>
@@ -51,6 +45,16 @@ struct DeltaRuleBackward : public torch::autograd::Node {
         }
         saved->arena.keep.clear();
     }
+    // what each gradient is a function of: without an output norm the result is linear in v and the entering state together, and in q where that is not normalised
+    std::vector<uint32_t> depends() const {
+        constexpr uint32_t Q = 1 << 0, V = 1 << 2, H0 = 1 << 7, ALL = (1 << NUM_INPUTS) - 1;
+        std::vector<uint32_t> d(NUM_INPUTS, ALL);
+        if (!call.has_ep) {
+            d[2] = d[7] = ALL & ~(V | H0);
+            if (!call.l2) d[0] = ALL & ~Q;
+        }
+        return d;
+    }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         Inputs in;
@@ -68,7 +72,6 @@ struct DeltaRuleBackward : public torch::autograd::Node {
         }
         saved->arena.point();
         const Tensor dy = grads[0], dht = grads.size() > 1 ? grads[1] : Tensor();
-        const bool twice = c10::GradMode::is_enabled() && ((dy.defined() && dy.requires_grad()) || (dht.defined() && dht.requires_grad()));
         Grads g;
         {
             at::AutoGradMode off(false);
@@ -80,11 +83,7 @@ struct DeltaRuleBackward : public torch::autograd::Node {
         variable_list out = {g.q, g.k, g.v, g.x, g.beta, g.A_log, g.dt_bias, g.h0, g.ep_w, g.ep_gate};
         for (int i = 0; i < NUM_INPUTS; ++i)
             if (!task_should_compute_output(i)) out[i] = Tensor();
-        if (twice) {      // gradients of these gradients are not provided: using them has to fail, not to give zeros
-            auto err = std::make_shared<torch::autograd::Error>("chunk_delta_rule: double backward is not supported", torch::autograd::edge_list());
-            for (auto& t : out)
-                if (t.defined()) torch::autograd::set_history(t, err);
-        }
+        refuse_second(*this, "chunk_delta_rule", grads, depends(), out);
         return out;
     }
 };

@@ -7,11 +7,6 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/edge.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <functional>
@@ -38,6 +33,7 @@ struct BlockBackward : public torch::autograd::Node {
     std::vector<bool> output;
     std::vector<std::vector<int64_t>> sizes;
     std::vector<at::ScalarType> types;
+    std::vector<uint32_t> depends;             // per gradient: the inputs that it is a function of, besides the incoming gradients
     Backward run;
     bool released = false;
 
@@ -64,9 +60,6 @@ struct BlockBackward : public torch::autograd::Node {
                         ": a saved-tensor hook returned another tensor than was saved");
         }
         c10::cuda::CUDAGuard guard(dev);
-        bool twice = false;
-        if (c10::GradMode::is_enabled())
-            for (const Tensor& g : grads) twice = twice || (g.defined() && g.requires_grad());
         variable_list out;
         {
             at::AutoGradMode off(false);
@@ -74,19 +67,16 @@ struct BlockBackward : public torch::autograd::Node {
         }
         for (size_t i = 0; i < out.size(); ++i)
             if (!task_should_compute_output(i)) out[i] = Tensor();
-        if (twice) {      // gradients of these gradients are not provided: using them has to fail, not to give zeros
-            auto err = std::make_shared<torch::autograd::Error>(what + ": double backward is not supported", torch::autograd::edge_list());
-            for (auto& t : out)
-                if (t.defined()) torch::autograd::set_history(t, err);
-        }
+        refuse_second(*this, what, grads, depends, out);
         return out;
     }
 };
 
-std::shared_ptr<BlockBackward> new_node(const char* what, const at::Device& dev, const variable_list& inputs, Backward run) {
+std::shared_ptr<BlockBackward> new_node(const char* what, const at::Device& dev, const variable_list& inputs, std::vector<uint32_t> depends, Backward run) {
     auto node = std::shared_ptr<BlockBackward>(new BlockBackward(), torch::autograd::deleteNode);
     node->what = what;
     node->dev = dev;
+    node->depends = std::move(depends);
     node->run = std::move(run);
     node->set_next_edges(torch::autograd::collect_next_edges(inputs));
     return node;
@@ -301,7 +291,9 @@ PyObject* conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
             library_call([&] { check_rc(mkda_conv_fwd(&p, stream()), "mkda_conv_fwd"); });
         }
         if (grad) {
-            auto node = new_node("causal_conv1d", x.device(), t, [q, silu](const variable_list& s, const variable_list& g, const Need&) { return conv_backward(q, silu, s, g); });
+            constexpr uint32_t X = 1, WT = 2, BIAS = 4, ST = 8, ALL = X | WT | BIAS | ST;
+            const std::vector<uint32_t> depends = silu ? std::vector<uint32_t>(4, ALL) : std::vector<uint32_t>{WT, X | ST, 0, WT};      // linear but for the product of weight and tokens
+            auto node = new_node("causal_conv1d", x.device(), t, depends, [q, silu](const variable_list& s, const variable_list& g, const Need&) { return conv_backward(q, silu, s, g); });
             for (const Tensor& v : t) node->save(v);
             torch::autograd::set_history(y, node);
             if (last.defined()) torch::autograd::set_history(last, node);
@@ -465,6 +457,24 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
     return out;
 }
 
+// what each input's gradient is a function of: the result is linear in x and the entering state together, in B, in C and in D
+std::vector<uint32_t> scan_depends() {
+    auto but = [](std::initializer_list<int> none) {
+        uint32_t m = (1u << SCAN_INPUTS) - 1;
+        for (int i : none) m &= ~(1u << i);
+        return m;
+    };
+    std::vector<uint32_t> d(SCAN_INPUTS);
+    d[SX] = but({SX, SH0});
+    d[SDT] = d[SA] = d[SBIAS] = but({SSKIP});
+    d[SB] = but({SB, SSKIP, SH0});
+    d[SC] = but({SC, SSKIP});
+    d[SSKIP] = 1u << SX | 1u << SZ;
+    d[SZ] = but({});
+    d[SH0] = but({SX, SB, SSKIP, SH0});
+    return d;
+}
+
 // the checks that prompts and single tokens share; `lead` axes in front of the channels
 PyObject* check_scan(const variable_list& t, int lead) {
     const Tensor &x = t[SX], &A = t[SA], &B = t[SB], &C = t[SC];
@@ -529,7 +539,7 @@ PyObject* scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
             library_call([&] { check_rc(mkda_scan_fwd(&call.p, stream()), "mkda_scan_fwd"); });
         }
         if (grad) {
-            auto node = new_node("selective_scan", x.device(), t, [q, softplus](const variable_list& s, const variable_list& g, const Need&) { return scan_backward(q, softplus, s, g); });
+            auto node = new_node("selective_scan", x.device(), t, scan_depends(), [q, softplus](const variable_list& s, const variable_list& g, const Need&) { return scan_backward(q, softplus, s, g); });
             for (const Tensor& v : t) node->save(v);
             node->save(ckpt);
             torch::autograd::set_history(y, node);
@@ -661,7 +671,8 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (grad) {
             const bool has = res.defined();
             const at::ScalarType dt = x.scalar_type(), rdt = has ? res.scalar_type() : dt;
-            auto node = new_node("rms_norm", x.device(), t, [eps, dt, has, rdt](const variable_list& s, const variable_list& g, const Need& need) {
+            constexpr uint32_t X = 1, WT = 2, RES = 4;
+            auto node = new_node("rms_norm", x.device(), t, {X | WT | RES, X | RES, X | WT | RES}, [eps, dt, has, rdt](const variable_list& s, const variable_list& g, const Need& need) {
                 return norm_backward(eps, dt, has, rdt, s, g, need);
             });
             torch::autograd::set_history(y, node);
