@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {      // silu' = sg (1 + z (1 - sg))
                             const f32x2 sg = sigmoidf2_(z[e]);
-                            oz[e] = mul2(mul2(dy[e], fma2(skip[e], x[e], y[e])), mul2(sg, fma2(z[e], fma2(sg, both(-1.f), both(1.f)), both(1.f))));
+                            oz[e] = mul2(mul2(dy[e], p.skip ? fma2(skip[e], x[e], y[e]) : y[e]), mul2(sg, fma2(z[e], fma2(sg, both(-1.f), both(1.f)), both(1.f))));
                             dy[e] = mul2(dy[e], mul2(z[e], sg));
                         }
                     }
@@ -834,7 +834,8 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                     for (int e = 0; e < 2; ++e) {
                         s[e] = add2(s[e], bias[e]);
                         const f32x2 d = p.softplus ? scan_softplus2(s[e]) : s[e];
-                        ox[e] = fma2(skip[e], dy[e], mul2(d, gB[e]));
+                        ox[e] = mul2(d, gB[e]);
+                        if (p.skip) ox[e] = fma2(skip[e], dy[e], ox[e]);      // 0 times infinity is no 0
                         od[e] = fma2(x[e], gB[e], mul2(eA[e], both(LN2)));
                         if (p.softplus) od[e] = mul2(od[e], sigmoidf2_(s[e]));
                         acc_skip[e] = fma2(dy[e], x[e], acc_skip[e]);
@@ -966,7 +967,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, co
 #pragma unroll
     for (int i = 0; i < MINE; ++i)
         if (mine + 2 * i < rows) {
-            float v = fmaf(skip, x[i], y[i]);
+            float v = p.skip ? fmaf(skip, x[i], y[i]) : y[i];      // 0 times infinity is no 0
             if (p.z) v *= z[i] * sigmoidf_(z[i]);
             st1(p.y, DT, row + (size_t)(mine + 2 * i) * D, v);
         }

@@ -1,0 +1,74 @@
+"""GPU: the selective scan at the far ends of its arguments' values, against its definition in 64 bits: what is finite there is near it (tolerances of test_block_gpu.py),
+what is infinite there is infinite with the same sign, and nothing else is NaN."""
+import pytest
+import torch
+
+import mogankda_b200 as mk
+from tests.test_block_gpu import near, rand, scan_leaves, scan_reference
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def alike(name, got, want):
+    got, want = got.cpu(), want.float()
+    assert torch.equal(got.isnan(), want.isnan()), f"{name}: NaN in other places"
+    assert torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()]), f"{name}: infinities"
+    ok = torch.isfinite(want)
+    near(name, got[ok], want[ok].double())
+
+
+def both(lv, ups=None, softplus=False):
+    """(results and gradients of the operator, of the definition), as dicts; gradients of all leaves where ``ups`` holds incoming ones of y and of the final state."""
+    sides = []
+    for cast, run in ((lambda t: t.cuda(), lambda m: mk.selective_scan(*(m.get(n) for n in ("x", "dt", "A", "B", "C", "D", "z", "bias")), dt_softplus=softplus,
+                                                                      initial_state=m.get("h0"), output_final_state=True)),
+                      (lambda t: t.double(), lambda m: scan_reference(*(m.get(n) for n in ("x", "dt", "A", "B", "C", "D", "z", "bias")), softplus, m.get("h0"), None, True))):
+        m = {n: cast(t).requires_grad_(ups is not None) for n, t in lv.items()}
+        y, end = run(m)
+        got = dict(y=y, end=end)
+        if ups is not None:
+            got.update(zip(("d" + n for n in m), torch.autograd.grad((y, end), list(m.values()), [cast(u) for u in ups])))
+        sides.append({n: t.detach() for n, t in got.items()})
+    return sides
+
+
+def positive(gen, T, D, N, more=()):
+    """Leaves without a sum of terms of both signs."""
+    lv = scan_leaves(gen, 1, T, D, N, 1, None, torch.float32, False)
+    lv.update((n, scan_leaves(gen, 1, T, D, N, 1, None, torch.float32, True)[n]) for n in more)
+    return {n: t if n in ("A", "dt") else t.abs() + 0.1 for n, t in lv.items()}
+
+
+def step_like(lv, rows, before, copies):
+    """One token of each of as many sequences as there are ``rows``, on states ``before``; ``copies`` of them in one call."""
+    tok = {n: lv[n][0, rows] for n in ("x", "dt", "B", "C")}
+    ref = scan_reference(*(tok[n][:, None].double() if n in tok else lv[n].double() for n in ("x", "dt", "A", "B", "C")), h0=before.double(), last=True)
+    state = before.repeat(copies, 1, 1).cuda()
+    with torch.no_grad():
+        args = [tok[n].repeat(copies, *(1,) * (tok[n].dim() - 1)).cuda() if n in tok else lv[n].cuda() for n in ("x", "dt", "A", "B", "C")]
+        y = mk.selective_scan_step(*args, state)
+    n = before.shape[0]
+    alike("y of a step", y[-n:], ref[0][:, 0])
+    alike("state of a step", state[-n:], ref[1])
+
+
+def test_infinite_values_without_a_skip():
+    """Without D there is no term D x, also where x is infinite, nor one D dy in its gradient."""
+    gen = torch.Generator().manual_seed(53)
+    T, D, N = 32, 20, 16
+    lv = positive(gen, T, D, N, more=("z",))
+    ups = [rand(gen, 1, T, D).abs() + 0.1, torch.zeros(1, D, N)]
+    lv["x"][0, 20, 7] = INF
+    got, want = both(lv, ups)
+    assert want["y"].isinf().any() and want["dz"].isinf().any()
+    for n in ("y", "end", "dz", "dx"):
+        alike(n, got[n], want[n])
+    before = torch.rand(8, D, N, generator=gen)
+    for copies in (1, 2000):
+        step_like(lv, slice(14, 22), before, copies)
+    lv["x"][0, 20, 7] = 1.0
+    ups[0][0, 9, 3] = INF
+    got, want = both(lv, ups)
+    assert want["dx"].isinf().any()
+    alike("dx of an infinite gradient", got["dx"], want["dx"])
