@@ -11,6 +11,7 @@
 // What bounds it: 16 exponentials per token and channel (16 states) are 118 us of the special function units for 8192 x 4096, HBM 41 us; the walk reads d, d x, B and C of every
 // token from shared memory, 10 of its cycles a token and warp, which is 70 to 75 % of what an SM's shared memory gives.  bf16, 16 states, with gate: forward 8192 x 4096
 // 280 us, 4 x 2048 x 4096 285 us; backward 2 x 2048 x 4096 400 us.
+#include <cfloat>
 #include <type_traits>
 
 #include "block.cuh"
@@ -89,6 +90,18 @@ __device__ __forceinline__ float4 ld_states(const float* base, size_t row, int n
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = n0 + i < NST ? base[row * NST + n0 + i] : 0.f;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+// ... rates A, times log2 e, and no infinity: A * 0 has to be 0 where no time passes (the tokens behind a sequence's last one), also where A is infinite or its product with log2 e
+// is.  The largest number leaves as little of a state as infinity does, for any d above 1e-36.
+__device__ __forceinline__ float4 ld_rates(const float* base, size_t row, int n0, int NST) {
+    const float4 f = ld_states(base, row, n0, NST);
+    float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (float& a : v) {
+        a *= RCP_LN2;
+        if (fabsf(a) > FLT_MAX) a = copysignf(FLT_MAX, a);      // NaN is not
+    }
     return make_float4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ void st_states(float* base, size_t row, int n0, int NST, const float4& v) {
@@ -181,9 +194,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
         const bool there = c0 < cs.count;
         const size_t ch = cs.first + c0;
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
+        const Four A = four(there ? ld_rates(p.A, ch, n0, NST) : zero);
         for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
             const Part sq = part_of(p.S, slot);
             if (!sq.there) continue;
@@ -400,9 +411,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kerne
         const bool there = c0 < cs.count;
         const size_t ch = cs.first + c0;
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
+        const Four A = four(there ? ld_rates(p.A, ch, n0, NST) : zero);
         for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
             const Part sq = part_of(p.S, slot);
             if (!wanted(sq)) continue;
@@ -569,9 +578,8 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
         const bool z = p.z, there = c0 < cs.count;
         const size_t ch = cs.first + c0;
-        Four A = four(there ? ld_states(p.A, ch, n0, NST) : zero), dA = four(zero);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
+        const Four A = four(there ? ld_rates(p.A, ch, n0, NST) : zero);
+        Four dA = four(zero);
         for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
             const Part sq = part_of(p.S, slot);
             if (!sq.there) continue;
@@ -927,10 +935,8 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, co
         d[i] = ok ? ld1(p.dt, DT, n * p.dt_stride + c) : 0.f;
         z[i] = ok && p.z ? ld1(p.z, DT, n * p.z_stride + c) : 0.f;
     }
-    Four A = four(there ? ld_states(p.A, c, n0, NST) : zero);
+    const Four A = four(there ? ld_rates(p.A, c, n0, NST) : zero);
     const float bias = there && p.dt_bias ? p.dt_bias[c] : 0.f, skip = there && p.skip ? p.skip[c] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) A.v[i] = mul2(A.v[i], both(RCP_LN2));
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
         d[i] += bias;

@@ -72,3 +72,30 @@ def test_infinite_values_without_a_skip():
     got, want = both(lv, ups)
     assert want["dx"].isinf().any()
     alike("dx of an infinite gradient", got["dx"], want["dx"])
+
+
+@pytest.mark.parametrize("T,D,N", [(33, 40, 16), (64, 24, 5), (70, 9, 64), (900, 8, 16)])
+def test_a_decay_rate_at_the_end_of_its_range(T, D, N):
+    """A = -3e38 times log2 e is no fp32 number.  It leaves nothing of a state, and the tokens behind a sequence's end, for which no time passes, leave the state alone."""
+    gen = torch.Generator().manual_seed(51)
+    lv = scan_leaves(gen, 2, T, D, N, 1, None, torch.float32, True)
+    lv["A"][3], lv["A"][5, 0] = -3e38, torch.finfo(torch.float32).min
+    got, want = both(lv, [rand(gen, 2, T, D), rand(gen, 2, D, N)], True)
+    for n in want:
+        near(n, got[n].cpu(), want[n])
+
+
+@pytest.mark.parametrize("T", [1, 33, 900])
+def test_an_infinite_decay_rate(T):
+    """exp(-inf) = 0: the state is what the last token brought."""
+    gen = torch.Generator().manual_seed(52)
+    lv = scan_leaves(gen, 2, T, 12, 16, 1, None, torch.float32, True)
+    lv["A"][2] = -INF
+    got, want = both(lv, softplus=True)
+    state = lv["h0"].cuda()
+    with torch.no_grad():
+        step = mk.selective_scan_step(lv["x"][:, 0].cuda(), lv["dt"][:, 0].cuda(), lv["A"].cuda(), lv["B"][:, 0].cuda(), lv["C"][:, 0].cuda(), state, lv["D"].cuda(),
+                                      lv["z"][:, 0].cuda(), lv["bias"].cuda(), dt_softplus=True)
+    for n in want:
+        near(n, got[n].cpu(), want[n])
+    near("step", step.cpu(), want["y"][:, 0])
