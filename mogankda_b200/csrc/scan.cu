@@ -115,6 +115,9 @@ __device__ __forceinline__ void st_states(float* base, size_t row, int n0, int N
         if (n0 + i < NST) base[row * NST + n0 + i] = w[i];
 }
 
+// all bits of those of the states n and n + 1 that are among the NST
+__device__ __forceinline__ f32x2 real_states(int n, int NST) { return (n < NST ? 0xffffffffull : 0ull) | (n + 1 < NST ? 0xffffffffull << 32 : 0ull); }
+
 // Channels of a block: `first` of the whole, `count` of them exist (a block never straddles two groups)
 struct Channels { int group, first, count; };
 __device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB) {
@@ -180,7 +183,8 @@ __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S,
 }
 
 // (8192 x 4096: 280 us.  Two states a lane and twice the warps on the chain 10 % more; B and C in 16 bits side by side, or d and d x doubled for packed products, 20 %.)
-template <int DT, int LPC, int TILE>
+// FILL: there are states that fill up a channel's lanes.  Their B and C are zero, but 0 times an infinite d or x is not: they are set to zero after every token.
+template <int DT, int LPC, int TILE, bool FILL>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
     follow_stream();
     using Sh = ScanShape<LPC>;
@@ -195,6 +199,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
         const size_t ch = cs.first + c0;
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
         const Four A = four(there ? ld_rates(p.A, ch, n0, NST) : zero);
+        const f32x2 real[2] = {real_states(n0, NST), real_states(n0 + 2, NST)};
         for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
             const Part sq = part_of(p.S, slot);
             if (!sq.there) continue;
@@ -244,6 +249,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                             const f32x2 d = e[u].v[i];
                             e[u].v[i] = scan_decay(A.v[i], next[u].d.x);
                             h.v[i] = fma2(d, h.v[i], mul2(dx, now[u].B.v[i]));
+                            if constexpr (FILL) h.v[i] &= real[i];
                             y = i ? fma2(h.v[i], now[u].C.v[i], y) : mul2(h.v[i], now[u].C.v[i]);
                         }
                         yn[u] = sum2(y);
@@ -936,6 +942,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, co
         z[i] = ok && p.z ? ld1(p.z, DT, n * p.z_stride + c) : 0.f;
     }
     const Four A = four(there ? ld_rates(p.A, c, n0, NST) : zero);
+    const f32x2 real[2] = {real_states(n0, NST), real_states(n0 + 2, NST)};      // states that fill up the lanes stay zero beside infinite values
     const float bias = there && p.dt_bias ? p.dt_bias[c] : 0.f, skip = there && p.skip ? p.skip[c] : 0.f;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
@@ -957,7 +964,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const MkdaScanStep p, co
         Four o = four(h[r]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            o.v[i] = fma2(scan_decay(A.v[i], dr), o.v[i], mul2(both(dx), B[i]));
+            o.v[i] = fma2(scan_decay(A.v[i], dr), o.v[i], mul2(both(dx), B[i])) & real[i];
             s = i ? fma2(C[i], o.v[i], s) : mul2(C[i], o.v[i]);
         }
         if (r < rows) st_states(p.state, row + (size_t)r * D, n0, NST, flat(o));
@@ -1036,7 +1043,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
             if (rc != MKDA_OK) return;
             auto run = [&](auto tile) {
                 constexpr int TILE = decltype(tile)::value, smem = (int)sizeof(ScanFwdShared<LPC, TILE>);
-                auto* kern = scan_fwd_kernel<DT, LPC, TILE>;
+                auto* kern = p->NST == 4 * LPC ? scan_fwd_kernel<DT, LPC, TILE, false> : scan_fwd_kernel<DT, LPC, TILE, true>;
                 rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_fwd");
                 if (rc == MKDA_OK)
                     launch(kern, dim3(blocks, rows_of_blocks(p->S)), SCAN_THREADS + SCAN_HELPERS, smem, (cudaStream_t)stream, *p, vec, wide_states(*p, 4));

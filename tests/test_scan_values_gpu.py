@@ -99,3 +99,21 @@ def test_an_infinite_decay_rate(T):
     for n in want:
         near(n, got[n].cpu(), want[n])
     near("step", step.cpu(), want["y"][:, 0])
+
+
+@pytest.mark.parametrize("N", [1, 5, 12, 16, 20, 50])
+@pytest.mark.parametrize("what", ["x", "dt"])
+@pytest.mark.parametrize("T", [37, 700])
+def test_infinite_values_beside_any_number_of_states(N, what, T):
+    """An infinite x (or dt) makes y infinite, not NaN: the states that fill up a channel's lanes have no part in it.  700: cut into parts."""
+    gen = torch.Generator().manual_seed(53)
+    D = 20
+    lv = positive(gen, T, D, N)
+    lv[what][0, T - 17, 7] = INF
+    got, want = both(lv)
+    assert want["y"].isinf().any() and not want["y"].isnan().any()
+    for n in want:
+        alike(n, got[n], want[n])
+    before = torch.rand(8, D, N, generator=gen)
+    for copies in (1, 2000):
+        step_like(lv, slice(T - 20, T - 12), before, copies)
