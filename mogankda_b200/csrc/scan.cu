@@ -631,6 +631,11 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                         if constexpr (LPC == 2) ysum[TILE / 4 + t4 / 4] = ys[1];
                     }
                 }
+                if (j == 0 && len % TILE) {                // what is behind the sequence's last token has no part in dA, also beside states that are infinite
+#pragma unroll
+                    for (int t = 1; t < TILE; ++t)
+                        if (t >= len % TILE) P[t] = four(zero);
+                }
                 if (tiles - 2 - j >= 0) rh = checkpoint(tiles - 2 - j);
                 asm volatile("" ::: "memory");             // what the first pass has read is read again: kept for sixteen tokens it would not fit into the registers
                 constexpr int KEEP = LPC >= 4 ? LPC / 4 : 1;      // sums of dB and dC per lane: 1, 1, 2 or 4

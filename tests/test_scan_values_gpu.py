@@ -117,3 +117,16 @@ def test_infinite_values_beside_any_number_of_states(N, what, T):
     before = torch.rand(8, D, N, generator=gen)
     for copies in (1, 2000):
         step_like(lv, slice(T - 20, T - 12), before, copies)
+
+
+@pytest.mark.parametrize("N", [5, 16, 50])
+@pytest.mark.parametrize("T", [37, 700])
+def test_gradients_where_only_the_last_state_is_infinite(N, T):
+    """The rates' gradient has no term of the state behind the last token, nor of the tokens that fill up its tile."""
+    gen = torch.Generator().manual_seed(54)
+    D = 12
+    lv = scan_leaves(gen, 1, T, D, N, 1, None, torch.float32, False)
+    lv["x"][0, -1, 4] = INF
+    got, want = both(lv, [rand(gen, 1, T, D), rand(gen, 1, D, N)])
+    for n in ("dx", "dA"):
+        near(n, got[n].cpu(), want[n])
