@@ -13,6 +13,7 @@
 #include <limits>
 #include <memory>
 #include <mutex>
+#include <numeric>
 #include <unordered_map>
 
 using namespace mkda_host;
@@ -362,13 +363,17 @@ enum { SX, SDT, SA, SB, SC, SSKIP, SZ, SBIAS, SH0, SCAN_INPUTS };
 // the time of the main pass over them, and both start anew, about 128 tokens' time.  Whole / cut in us, 8192 tokens, first pass included: forward
 // x 256 channels 274 / 40, x 1024 278 / 132, x 2048 280 / 254; backward x 256 970 / 77, x 1024 1059 / 254, x 2048 1064 / 520, x 4096 1066 / 911;
 // 600 tokens x 512 25 / 14 and 75 / 27.
-void cut(MkdaSeqs& s, const Sequences& q, int blocks, int64_t P, int64_t D, int places, double pre) {
+// Every sequence has a row of blocks for each part that the longest one has, and a block without tokens takes its SM 0.9 us in each of the two kernels, in the backward pass (whose
+// main kernel has fewer rows) half of that: the time of `nothing` tokens.  One document of 4096 tokens beside 512 of 8, x 256 channels: forward 140 / 534, backward 540 / 614; beside
+// 296 of 8 backward 534 / 474; 8192 beside 64 of 64 forward 276 / 150.
+void cut(MkdaSeqs& s, const Sequences& q, int blocks, int64_t P, int64_t D, int places, double pre, double nothing) {
     if (q.longest < 400 || s.N == 0) return;
     const double side_by_side = blocks * std::max(1.0, (double)s.TT / q.longest);      // blocks that are busy as long as the longest sequence runs
     const int64_t want = (int64_t)(places * sms() / side_by_side);
     if (want < 2) return;
     const int64_t seg = std::max<int64_t>(128, ((q.longest + want - 1) / want + 63) / 64 * 64), segs = (q.longest + seg - 1) / seg;
-    if ((1 + pre) * seg + 128 >= q.longest || s.N * segs * D * P * 4 > (int64_t)256 << 20) return;
+    const int64_t empty = std::max<int64_t>(0, s.N * (segs - 1) - s.TT / seg);      // parts without tokens, at least
+    if ((1 + pre) * seg + 128 + nothing * empty * blocks / sms() >= q.longest || s.N * segs * D * P * 4 > (int64_t)256 << 20) return;
     s.seg = (int)seg;
     s.segs = (int)segs;
 }
@@ -421,7 +426,7 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
         if (in[i].defined()) out[i] = new_cuda(in[i].sizes(), in[i].scalar_type(), dev);
     p.dx = out[SX].data_ptr(); p.ddt = out[SDT].data_ptr(); p.dz = mptr(out[SZ]); p.dh0 = fmptr(out[SH0]);
     p.channel_blocks = mkda_scan_bwd_channel_blocks((int)D, (int)G, (int)N);
-    cut(p.f.S, q, p.channel_blocks, P, D, 2, 0.4);
+    cut(p.f.S, q, p.channel_blocks, P, D, 2, 0.4, 9);
     const int64_t rows = p.f.S.seg ? (int64_t)q.s.N * p.f.S.segs : q.s.N;
     Tensor seg_g, seg_d;
     if (p.f.S.seg) {
@@ -431,6 +436,7 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
     }
     // sequences are dealt to rows of blocks: enough of them for 16 blocks per SM; each leaves a row of sums for A, D and dt_bias
     p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (16 * sms() + p.channel_blocks - 1) / p.channel_blocks));
+    while (p.f.S.seg && std::gcd(p.slots, q.s.N) > 1) --p.slots;      // part k of sequence i is number k N + i: the parts of a sequence go to different rows
     const std::vector<int64_t> part_size{p.channel_blocks, TT * P};
     const Tensor pB = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
     const Tensor pC = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
@@ -528,7 +534,7 @@ PyObject* scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (grad) ckpt = new_cuda({std::max<int64_t>(q.checkpoints, 1), D, mkda_scan_padded_states((int)NST)}, at::kFloat, x.device());
             call.p.y = y.data_ptr(); call.p.ht = fmptr(last); call.p.ckpt = fmptr(ckpt);
             const int64_t P = mkda_scan_padded_states((int)NST);
-            cut(call.p.S, q, mkda_scan_bwd_channel_blocks((int)D, call.p.G, (int)NST), P, D, 1, 0.75);      // the forward kernel has the same blocks
+            cut(call.p.S, q, mkda_scan_bwd_channel_blocks((int)D, call.p.G, (int)NST), P, D, 1, 0.75, 54);      // the forward kernel has the same blocks
             Tensor seg_h, seg_d;
             if (call.p.S.seg) {
                 const int64_t rows = (int64_t)q.s.N * call.p.S.segs;
