@@ -82,6 +82,7 @@ __device__ __forceinline__ void put_sums(float* sums, int t, int ch, const float
 
 __device__ __forceinline__ f32x2 lo2(const float4& v) { return pack2(v.x, v.y); }
 __device__ __forceinline__ f32x2 hi2(const float4& v) { return pack2(v.z, v.w); }
+__device__ __forceinline__ bool finite2(f32x2 v) { float a, b; unpack2(v, a, b); return fabsf(a) <= FLT_MAX && fabsf(b) <= FLT_MAX; }
 __device__ __forceinline__ float sum2(f32x2 v) { float a, b; unpack2(v, a, b); return a + b; }
 
 // four states of a channel: NST may be anything up to the padded number
@@ -631,11 +632,6 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                         if constexpr (LPC == 2) ysum[TILE / 4 + t4 / 4] = ys[1];
                     }
                 }
-                if (j == 0 && len % TILE) {                // what is behind the sequence's last token has no part in dA, also beside states that are infinite
-#pragma unroll
-                    for (int t = 1; t < TILE; ++t)
-                        if (t >= len % TILE) P[t] = four(zero);
-                }
                 if (tiles - 2 - j >= 0) rh = checkpoint(tiles - 2 - j);
                 asm volatile("" ::: "memory");             // what the first pass has read is read again: kept for sixteen tokens it would not fit into the registers
                 constexpr int KEEP = LPC >= 4 ? LPC / 4 : 1;      // sums of dB and dC per lane: 1, 1, 2 or 4
@@ -717,6 +713,37 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
 #pragma unroll
                         for (int i = 0; i < KEEP; ++i) sh.red[buf][warp][t][(first + i >= 4 ? NP : 0) + n0 + ((first + i) & 3)] = red[t][i];
                 }
+                if (j == 0 && len % TILE) {                // the same for all lanes
+                    if (!(finite2(dAt.v[0]) && finite2(dAt.v[1]))) {
+                        // The tokens that fill up the last tile add e * 0, which an infinite state behind the last token makes NaN and the definition does not have.  Formed anew without
+                        // them, each token's state from the checkpoint: seldom enough, and the loop above stays as it is (with P set to zero there 2 x 2048 x 4096 took 409 us for 401).
+                        Four g1 = four(a.dht && there ? ld_states(a.dht, (size_t)n * D + ch, n0, NST) : zero);
+                        dAt = four(zero);
+#pragma unroll 1
+                        for (int t = len % TILE - 1; t >= 0; --t) {
+                            Four hs = four(checkpoint(tiles - 1)), v;
+                            float2 d;
+#pragma unroll 1
+                            for (int s = 0; s <= t; ++s) {
+                                d = sd[s * CB];
+                                const Four B = four(*reinterpret_cast<const float4*>(sB + s * NP));
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    v.v[i] = mul2(scan_decay(A.v[i], d.x), hs.v[i]);
+                                    hs.v[i] = fma2(both(d.y), B.v[i], v.v[i]);
+                                }
+                            }
+                            const Four C = four(*reinterpret_cast<const float4*>(sC + t * NP));
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const f32x2 g = fma2(both(sdy[t * CB]), C.v[i], g1.v[i]);
+                                dAt.v[i] = fma2(mul2(g, v.v[i]), both(d.x), dAt.v[i]);
+                                g1.v[i] = mul2(scan_decay(A.v[i], d.x), g);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) dA.v[i] = add2(dA.v[i], dAt.v[i]);      // tile by tile: the sum over thousands of tokens loses less
                 __syncthreads();
@@ -746,6 +773,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
         fs[e] = p.skip && ec + e < cs.count ? p.skip[cs.first + ec + e] : 0.f;
     }
     const f32x2 bias[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}, skip[2] = {pack2(fs[0], fs[1]), pack2(fs[2], fs[3])};
+    const f32x2 skips = p.skip ? ~0ull : 0ull;             // without D there is no term of it, also beside values that are infinite (0 times infinity is no 0)
     f32x2 acc_skip[2] = {both(0.f), both(0.f)}, acc_bias[2] = {both(0.f), both(0.f)};
     for (int slot = blockIdx.y; slot < parts(p.S); slot += gridDim.y) {
         const Part sq = part_of(p.S, slot);
@@ -845,7 +873,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {      // silu' = sg (1 + z (1 - sg))
                             const f32x2 sg = sigmoidf2_(z[e]);
-                            oz[e] = mul2(mul2(dy[e], p.skip ? fma2(skip[e], x[e], y[e]) : y[e]), mul2(sg, fma2(z[e], fma2(sg, both(-1.f), both(1.f)), both(1.f))));
+                            oz[e] = mul2(mul2(dy[e], fma2(skip[e], x[e] & skips, y[e])), mul2(sg, fma2(z[e], fma2(sg, both(-1.f), both(1.f)), both(1.f))));
                             dy[e] = mul2(dy[e], mul2(z[e], sg));
                         }
                     }
@@ -853,8 +881,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
                     for (int e = 0; e < 2; ++e) {
                         s[e] = add2(s[e], bias[e]);
                         const f32x2 d = p.softplus ? scan_softplus2(s[e]) : s[e];
-                        ox[e] = mul2(d, gB[e]);
-                        if (p.skip) ox[e] = fma2(skip[e], dy[e], ox[e]);      // 0 times infinity is no 0
+                        ox[e] = fma2(skip[e], dy[e] & skips, mul2(d, gB[e]));
                         od[e] = fma2(x[e], gB[e], mul2(eA[e], both(LN2)));
                         if (p.softplus) od[e] = mul2(od[e], sigmoidf2_(s[e]));
                         acc_skip[e] = fma2(dy[e], x[e], acc_skip[e]);
