@@ -93,10 +93,11 @@ typedef struct {
     float* seg_g; float* seg_d;           /* as in the forward call, of the gradient */
     int slots;                 /* the sequences (or their parts) are dealt to so many rows of blocks */
     int channel_blocks;        /* what mkda_scan_bwd_channel_blocks says */
-    float* part_B; float* part_C;         /* [channel_blocks][TT][P]: per block of channels */
+    float* part_B; float* part_C;         /* [G][blocks][TT][P]: per block of channels; only rows of tokens of sequences are written */
     float* part_A;             /* [slots][D][P] */
     float* part_skip;          /* [slots][D] or NULL */
     float* part_bias;          /* [slots][D] or NULL */
+    int first_block; int blocks;          /* of each group's channel_blocks / G blocks of channels, the call is for `blocks` from the first_block-th on; blocks = 0: for all */
 } MkdaScanBwd;
 int mkda_scan_bwd(const MkdaScanBwd* p, void* stream);
 /* Blocks of channels of the backward kernel for D channels in G groups (each group has as many) and NST states; the padded number of states P. */

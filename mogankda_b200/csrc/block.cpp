@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <cmath>
 #include <functional>
 #include <limits>
 #include <memory>
@@ -131,7 +132,7 @@ struct Sequences {
     MkdaSeqs s{};
     Tensor table;
     bool covers_all = true;
-    int64_t checkpoints = 0, longest = 0;
+    int64_t checkpoints = 0, longest = 0, end = 0;         // end: behind the last sequence
 };
 bool get_sequences(PyObject* table, PyObject* dims, int64_t B, int64_t T, Sequences& q) {
     if (!tensor_arg(table, q.table)) return false;
@@ -142,15 +143,17 @@ bool get_sequences(PyObject* table, PyObject* dims, int64_t B, int64_t T, Sequen
         q.s.has_empty = T == 0;
         q.checkpoints = B * ((T + MKDA_SCAN_CHECKPOINT - 1) / MKDA_SCAN_CHECKPOINT);
         q.longest = T;
+        q.end = B * T;
         return true;
     }
     int all, empty;
-    long long ck, longest;
-    if (!PyArg_ParseTuple(dims, "iiiLL", &q.s.N, &all, &empty, &ck, &longest)) return false;
+    long long ck, longest, end;
+    if (!PyArg_ParseTuple(dims, "iiiLLL", &q.s.N, &all, &empty, &ck, &longest, &end)) return false;
     q.covers_all = all;
     q.s.has_empty = empty;
     q.checkpoints = ck;
     q.longest = longest;
+    q.end = end;
     const int* p = static_cast<const int*>(q.table.data_ptr());
     q.s.cu = p;
     q.s.ckpt_off = p + q.s.N + 1;
@@ -405,6 +408,17 @@ struct ScanCall {
     }
 };
 
+// The backward pass leaves dB and dC per block of channels, 8 P bytes per token and block.  Where that is more than 1 GiB, it runs over ranges of blocks whose sums are added up in
+// between.  A range has the blocks that are resident at once, two per SM, so that ranges take as many waves as one launch would.
+struct Ranges { int count, blocks; };      // blocks of each group
+Ranges ranges_of_blocks(const Sequences& q, int per, int G, int64_t P) {
+    if (q.longest == 0 || (double)per * G * q.s.TT * P * 8 <= (double)(1 << 30)) return {1, per};
+    const double side_by_side = G * std::max(1.0, (double)q.s.TT / q.longest);
+    const int most = std::max(1, (int)std::ceil(2 * sms() / side_by_side)), count = (per + most - 1) / most;
+    const int blocks = (per + count - 1) / count, ranges = (per + blocks - 1) / blocks;      // of equal size
+    return blocks + ranges < per ? Ranges{ranges, blocks} : Ranges{1, per};
+}
+
 variable_list scan_backward(const Sequences& q, int softplus, const variable_list& s, const variable_list& grads) {
     reads_table(q);
     const variable_list in(s.begin(), s.begin() + SCAN_INPUTS);
@@ -422,11 +436,14 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
     variable_list out(SCAN_INPUTS);
     for (int i : {SX, SDT, SZ})
         if (in[i].defined()) out[i] = out_like(in[i], q.covers_all);
-    for (int i : {SA, SB, SC, SSKIP, SBIAS, SH0})
+    for (int i : {SB, SC}) out[i] = out_like(in[i], q.covers_all);
+    for (int i : {SA, SSKIP, SBIAS, SH0})
         if (in[i].defined()) out[i] = new_cuda(in[i].sizes(), in[i].scalar_type(), dev);
     p.dx = out[SX].data_ptr(); p.ddt = out[SDT].data_ptr(); p.dz = mptr(out[SZ]); p.dh0 = fmptr(out[SH0]);
     p.channel_blocks = mkda_scan_bwd_channel_blocks((int)D, (int)G, (int)N);
-    cut(p.f.S, q, p.channel_blocks, P, D, 2, 0.4, 9);
+    const int per = p.channel_blocks / (int)G;
+    const Ranges ranges = ranges_of_blocks(q, per, (int)G, P);
+    cut(p.f.S, q, ranges.blocks * (int)G, P, D, 2, 0.4, 9);
     const int64_t rows = p.f.S.seg ? (int64_t)q.s.N * p.f.S.segs : q.s.N;
     Tensor seg_g, seg_d;
     if (p.f.S.seg) {
@@ -435,27 +452,42 @@ variable_list scan_backward(const Sequences& q, int softplus, const variable_lis
         p.seg_g = fmptr(seg_g); p.seg_d = fmptr(seg_d);
     }
     // sequences are dealt to rows of blocks: enough of them for 16 blocks per SM; each leaves a row of sums for A, D and dt_bias
-    p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (16 * sms() + p.channel_blocks - 1) / p.channel_blocks));
+    p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(rows, (16 * sms() + ranges.blocks * G - 1) / (ranges.blocks * G)));
     while (p.f.S.seg && std::gcd(p.slots, q.s.N) > 1) --p.slots;      // part k of sequence i is number k N + i: the parts of a sequence go to different rows
-    const std::vector<int64_t> part_size{p.channel_blocks, TT * P};
-    const Tensor pB = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
-    const Tensor pC = q.covers_all ? new_cuda(part_size, at::kFloat, dev) : at::zeros(part_size, x.options().dtype(at::kFloat));
+    const Tensor pB = new_cuda({G * ranges.blocks, TT * P}, at::kFloat, dev), pC = new_cuda({G * ranges.blocks, TT * P}, at::kFloat, dev);
+    Tensor sB, sC;                                         // of each range, [G][ranges][TT P]
+    if (ranges.count > 1) {
+        sB = new_cuda({G * ranges.count, TT * P}, at::kFloat, dev);
+        sC = new_cuda({G * ranges.count, TT * P}, at::kFloat, dev);
+    }
     const Tensor pA = new_cuda({p.slots, D * P}, at::kFloat, dev);
     Tensor pskip, pbias;
     if (out[SSKIP].defined()) pskip = new_cuda({p.slots, D}, at::kFloat, dev);
     if (out[SBIAS].defined()) pbias = new_cuda({p.slots, D}, at::kFloat, dev);
     p.part_B = fmptr(pB); p.part_C = fmptr(pC); p.part_A = fmptr(pA); p.part_skip = fmptr(pskip); p.part_bias = fmptr(pbias);
-    check_rc(mkda_scan_bwd(&p, stream()), "mkda_scan_bwd");
-    MkdaSumRows r{};
-    const int per = p.channel_blocks / (int)G;
-    auto tokens = [&](const Tensor& part, const Tensor& o) {
-        return MkdaSumJob{fptr(part), per, (int)G, TT * P, TT * P, (int)P, (int)N, N, G * N, 1, o.data_ptr(), dtype_code(o)};
+    // sums over `rows` rows of each group, of the tokens that lie in sequences
+    auto tokens = [&](const Tensor& part, int rows, const Tensor& o) {
+        return MkdaSumJob{fptr(part), rows, (int)G, TT * P, q.end * P, (int)P, (int)N, N, G * N, 1, o.data_ptr(), dtype_code(o)};
+    };
+    auto range = [&](const Tensor& part, int rows, const Tensor& o, int r) {
+        return MkdaSumJob{fptr(part), rows, (int)G, TT * P, q.end * P, (int)P, (int)P, ranges.count * TT * P, P, 1, fmptr(o) + r * TT * P, MKDA_F32};
     };
     auto channels = [&](const Tensor& part, const Tensor& o, int64_t pad, int64_t width) {
         return MkdaSumJob{fptr(part), p.slots, 1, D * pad, D * pad, (int)pad, (int)width, 0, width, 1, o.data_ptr(), dtype_code(o)};
     };
-    r.job[0] = tokens(pB, out[SB]);
-    r.job[1] = tokens(pC, out[SC]);
+    for (int r = 0; r < ranges.count; ++r) {
+        p.first_block = r * ranges.blocks;
+        p.blocks = std::min(ranges.blocks, per - p.first_block);
+        check_rc(mkda_scan_bwd(&p, stream()), "mkda_scan_bwd");
+        if (ranges.count == 1 || q.end == 0) continue;
+        MkdaSumRows part{};
+        part.job[0] = range(pB, p.blocks, sB, r);
+        part.job[1] = range(pC, p.blocks, sC, r);
+        check_rc(mkda_sum_rows(&part, stream()), "mkda_sum_rows");
+    }
+    MkdaSumRows r{};
+    r.job[0] = tokens(ranges.count > 1 ? sB : pB, ranges.count > 1 ? ranges.count : per, out[SB]);
+    r.job[1] = tokens(ranges.count > 1 ? sC : pC, ranges.count > 1 ? ranges.count : per, out[SC]);
     r.job[2] = channels(pA, out[SA], P, N);
     if (pskip.defined()) r.job[3] = channels(pskip, out[SSKIP], 1, 1);
     if (pbias.defined()) r.job[4] = channels(pbias, out[SBIAS], 1, 1);

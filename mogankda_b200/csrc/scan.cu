@@ -119,10 +119,10 @@ __device__ __forceinline__ void st_states(float* base, size_t row, int n0, int N
 // all bits of those of the states n and n + 1 that are among the NST
 __device__ __forceinline__ f32x2 real_states(int n, int NST) { return (n < NST ? 0xffffffffull : 0ull) | (n + 1 < NST ? 0xffffffffull << 32 : 0ull); }
 
-// Channels of a block: `first` of the whole, `count` of them exist (a block never straddles two groups)
+// Channels of a block: `first` of the whole, `count` of them exist (a block never straddles two groups).  A launch has `blocks` blocks of each group, from the from-th on.
 struct Channels { int group, first, count; };
-__device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB) {
-    const int per = D / G, blocks = (per + CB - 1) / CB, g = block / blocks, b = block - g * blocks;
+__device__ __forceinline__ Channels channels_of(int block, int D, int G, int CB, int from, int blocks) {
+    const int per = D / G, g = block / blocks, b = from + block - g * blocks;
     return Channels{g, g * per + b * CB, min(CB, per - b * CB)};
 }
 
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
     extern __shared__ __align__(16) unsigned char raw_shared[];
     auto& sh = *reinterpret_cast<ScanFwdShared<LPC, TILE>*>(raw_shared);
     const int D = p.D, NST = p.NST;
-    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
+    const Channels cs = channels_of(blockIdx.x, D, p.G, CB, 0, (D / p.G + CB - 1) / CB);
     if (threadIdx.x < SCAN_THREADS) {
         const int tid = threadIdx.x, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q;
         const bool there = c0 < cs.count;
@@ -404,14 +404,14 @@ struct ScanPreShared {
     float B[2][TILE + AHEAD][Sh::NP];      // B or C
 };
 template <int DT, int LPC, int TILE, bool REV>
-__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kernel(const MkdaScanFwd p, const void* up, float* out_h, float* out_d, const bool vec, const bool bvec) {
+__global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kernel(const MkdaScanFwd p, const void* up, float* out_h, float* out_d, const int from, const int blocks, const bool vec, const bool bvec) {
     follow_stream();
     using Sh = ScanShape<LPC>;
     constexpr int NP = Sh::NP, CB = Sh::CB;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     auto& sh = *reinterpret_cast<ScanPreShared<DT, LPC, TILE>*>(raw_shared);
     const int D = p.D, NST = p.NST;
-    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
+    const Channels cs = channels_of(blockIdx.x, D, p.G, CB, from, blocks);
     auto wanted = [](const Part& q) { return q.there && (REV ? q.k > 0 : !q.last); };
     if (threadIdx.x < SCAN_THREADS) {
         const int tid = threadIdx.x, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q;
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
     auto& sh = *reinterpret_cast<ScanBwdShared<DT, LPC>*>(raw_shared);
     const MkdaScanFwd& p = a.f;
     const int D = p.D, NST = p.NST;
-    const Channels cs = channels_of(blockIdx.x, D, p.G, CB);
+    const Channels cs = channels_of(blockIdx.x, D, p.G, CB, a.first_block, a.blocks);
     if (threadIdx.x < SCAN_THREADS) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(SCAN_BWD_WALK_REGS));
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = tid % LPC, c0 = tid / LPC, n0 = 4 * q, cl = lane / LPC;
@@ -1044,11 +1044,11 @@ static int rows_of_blocks(const MkdaSeqs& s) {
     return (int)(n < 65535 ? n : 65535);
 }
 template <int DT, int LPC, bool REV>
-static int launch_scan_pre(const MkdaScanFwd& p, const void* up, float* out_h, float* out_d, bool vec, cudaStream_t stream) {
+static int launch_scan_pre(const MkdaScanFwd& p, const void* up, float* out_h, float* out_d, int from, int blocks, bool vec, cudaStream_t stream) {
     constexpr int TILE = LPC == 2 ? 32 : 64, smem = (int)sizeof(ScanPreShared<DT, LPC, TILE>);
     auto* kern = scan_pre_kernel<DT, LPC, TILE, REV>;
     if (int e = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan: parts")) return e;
-    launch(kern, dim3(blocks_of_channels(p.D, p.G, ScanShape<LPC>::CB), rows_of_blocks(p.S)), SCAN_THREADS + SCAN_HELPERS, smem, stream, p, up, out_h, out_d, vec, wide_states(p, 4));
+    launch(kern, dim3(p.G * blocks, rows_of_blocks(p.S)), SCAN_THREADS + SCAN_HELPERS, smem, stream, p, up, out_h, out_d, from, blocks, vec, wide_states(p, 4));
     return check_launch("scan: parts");
 }
 
@@ -1071,7 +1071,7 @@ extern "C" int mkda_scan_fwd(const MkdaScanFwd* p, void* stream) {
             constexpr int DT = decltype(dt)::value, LPC = decltype(l)::value;
             const bool vec = wide_rows(*p, 4) && aligned16(p->y);
             const int blocks = blocks_of_channels(p->D, p->G, ScanShape<LPC>::CB);
-            if (p->S.seg) rc = launch_scan_pre<DT, LPC, false>(*p, nullptr, p->seg_h, p->seg_d, vec, (cudaStream_t)stream);
+            if (p->S.seg) rc = launch_scan_pre<DT, LPC, false>(*p, nullptr, p->seg_h, p->seg_d, 0, blocks / p->G, vec, (cudaStream_t)stream);
             if (rc != MKDA_OK) return;
             auto run = [&](auto tile) {
                 constexpr int TILE = decltype(tile)::value, smem = (int)sizeof(ScanFwdShared<LPC, TILE>);
@@ -1107,6 +1107,11 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
         return set_error(MKDA_ERR_ARG, "scan_bwd: A, states and partial sums must be 16-byte aligned");
     if (p->slots < 1 || p->slots > 65535 || p->channel_blocks != mkda_scan_bwd_channel_blocks(p->f.D, p->f.G, p->f.NST))
         return set_error(MKDA_ERR_ARG, "scan_bwd: 1 to 65535 slots, and as many blocks of channels as mkda_scan_bwd_channel_blocks says");
+    const int per_group = p->channel_blocks / p->f.G;
+    if (p->first_block < 0 || p->blocks < 0 || p->blocks > per_group || p->first_block > per_group - (p->blocks ? p->blocks : per_group))
+        return set_error(MKDA_ERR_ARG, "scan_bwd: blocks of channels that the groups do not have");
+    MkdaScanBwd q = *p;
+    if (!q.blocks) q.blocks = per_group;
     int rc = MKDA_OK;
     with_dtype(p->f.dtype, [&](auto dt) {
         with_lanes(p->f.NST, [&](auto l) {
@@ -1114,13 +1119,13 @@ extern "C" int mkda_scan_bwd(const MkdaScanBwd* p, void* stream) {
             const MkdaScanFwd& f = p->f;
             const bool vec = wide_rows(f, 4) && aligned16(p->dy) && aligned16(p->dx) && aligned16(p->ddt) && aligned16(p->dz);
             constexpr int smem = (int)sizeof(ScanBwdShared<DT, LPC>);
-            if (f.S.seg) rc = launch_scan_pre<DT, LPC, true>(f, p->dy, p->seg_g, p->seg_d, vec, (cudaStream_t)stream);
+            if (f.S.seg) rc = launch_scan_pre<DT, LPC, true>(f, p->dy, p->seg_g, p->seg_d, q.first_block, q.blocks, vec, (cudaStream_t)stream);
             if (rc != MKDA_OK) return;
             auto* kern = scan_bwd_kernel<DT, LPC>;
             static const int regs = kernel_registers(reinterpret_cast<const void*>(kern));
             if (regs != SCAN_BWD_LAUNCH_REGS) { rc = set_error(MKDA_ERR_LAUNCH, "scan_bwd: built with other registers than its roles share"); return; }
             rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "scan_bwd");
-            if (rc == MKDA_OK) launch(kern, dim3(p->channel_blocks, p->slots), SCAN_BWD_THREADS, smem, (cudaStream_t)stream, *p, vec, wide_states(f, 4));
+            if (rc == MKDA_OK) launch(kern, dim3(f.G * q.blocks, p->slots), SCAN_BWD_THREADS, smem, (cudaStream_t)stream, q, vec, wide_states(f, 4));
         });
     });
     return rc != MKDA_OK ? rc : check_launch("scan_bwd");

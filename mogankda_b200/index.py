@@ -171,7 +171,7 @@ def get_layout(B, T, cu_seqlens, device, seg_chunks=0, auto_heads=0, cost_ratio=
 class Bounds:
     """Packed sequences as the operators around the layer take them: boundaries, first checkpoint of a scan and order, longest first."""
     table: torch.Tensor         # int32: cu [N+1], first checkpoints [N], order [N]
-    dims: tuple                 # (N, covers_all, some sequence is empty, checkpoints, tokens of the longest sequence)
+    dims: tuple                 # (N, covers_all, some sequence is empty, checkpoints, tokens of the longest sequence, end of the last one)
 
 
 def bounds_table(T, cu, step):
@@ -189,8 +189,9 @@ def get_bounds(T, cu_seqlens, device):
     key, ver = ("bounds", T, device), None if cu_seqlens.is_inference() else cu_seqlens._version
     b = None if ver is None else _cached(key, cu_seqlens, ver)      # changes of a tensor without a version counter would not be seen
     if b is None:
-        table, dims = bounds_table(T, [int(x) for x in cu_seqlens.tolist()], ENUMS["MKDA_SCAN_CHECKPOINT"])
-        b = Bounds(torch.tensor(table, dtype=torch.int32, device=device), dims)
+        cu = [int(x) for x in cu_seqlens.tolist()]
+        table, dims = bounds_table(T, cu, ENUMS["MKDA_SCAN_CHECKPOINT"])
+        b = Bounds(torch.tensor(table, dtype=torch.int32, device=device), (*dims, cu[-1]))
         if ver is None:
             return b
         with _cache_lock:

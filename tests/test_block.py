@@ -113,3 +113,16 @@ def test_entry_points_refuse_without_launching(lib):
         assert lib.mkda_sum_rows(ctypes.byref(p), None) == _lib.MKDA_ERR_ARG, f
         setattr(j, f, good)
         j.pitch = 8
+
+
+def test_scan_bwd_refuses_blocks_that_the_groups_do_not_have(lib):
+    """Fake addresses: 8 channels in two groups are a block each."""
+    from mogankda_b200 import _lib
+    S = _lib.STRUCTS
+    f = _filled(S["MkdaScanFwd"](), ("x", "dt", "B", "C", "A", "y", "ckpt"), D=8, NST=16, G=2, dtype=1, x_stride=8, dt_stride=8, B_stride=32, C_stride=32)
+    f.S.TT, f.S.N, f.S.T = 4, 2, 2
+    b = _filled(S["MkdaScanBwd"](), ("dy", "dx", "ddt", "part_A", "part_B", "part_C"), slots=1, channel_blocks=lib.mkda_scan_bwd_channel_blocks(8, 2, 16))
+    b.f = f
+    for first, blocks in ((1, 0), (-1, 1), (1, 1), (0, 2), (0, -1), (2 ** 31 - 1, 1)):
+        b.first_block, b.blocks = first, blocks
+        assert lib.mkda_scan_bwd(ctypes.byref(b), None) == _lib.MKDA_ERR_ARG and b"groups do not have" in lib.mkda_last_error()

@@ -56,3 +56,35 @@ def test_scan_of_a_long_document_beside_short_ones(short, dtype):
     routs, rgrads = differentiate(lambda: scan_reference(*(wide[n] for n in args), True, wide["h0"], cu, True), wide, [u.double() for u in ups], list(lv))
     for n, a, b in zip(["y", "last"] + ["d" + n for n in lv], outs + grads, routs + rgrads):
         near(n, a.cpu(), b)
+
+
+@pytest.mark.parametrize("G", [1, 2])
+def test_workspace_of_many_blocks_of_channels(G):
+    """dB and dC are left per block of channels, 8 bytes per token, state and block: 512 blocks of 8 channels here.  More than 1 GiB of them are formed by ranges of blocks, whose
+    sums are added up in between; all else has the bits of calls on fewer channels."""
+    T, D, N, end = 6000, 4096, 64, 5990
+    g = torch.Generator(device="cuda").manual_seed(61)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, dt, up = r(1, T, D), 0.1 * torch.rand(1, T, D, generator=g, device="cuda"), r(1, T, D)
+    A, B, C, skip, h0, uph = -N * torch.rand(D, N, generator=g, device="cuda"), r(1, T, G, N), r(1, T, G, N), r(D), r(2, D, N), r(2, D, N)
+    cu = torch.tensor([0, 5000, end], device="cuda")
+
+    def gradients(ch, gr):
+        leaves = [t.contiguous().requires_grad_(True) for t in (x[..., ch], dt[..., ch], A[ch], B[:, :, gr], C[:, :, gr], skip[ch], h0[:, ch])]
+        y, end = mk.selective_scan(*leaves[:6], initial_state=leaves[6], output_final_state=True, cu_seqlens=cu)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad((y, end), leaves, (up[..., ch].contiguous(), uph[:, ch].contiguous()))
+        return torch.cuda.max_memory_allocated() - before, got
+
+    halves = [(slice(0, D // 2), slice(0, G // 2 or 1)), (slice(D // 2, D), slice(G // 2, G))]
+    (_, a), (_, b) = (gradients(*h) for h in halves)
+    peak, got = gradients(slice(0, D), slice(0, G))
+    blocks = 512
+    assert peak < 0.8 * 8 * blocks * T * N + 4 * 4 * T * D
+    for i, dim in ((0, 2), (1, 2), (2, 0), (5, 0), (6, 1)):
+        assert torch.equal(got[i], torch.cat([a[i], b[i]], dim))
+    for i in (3, 4):
+        assert (got[i][:, end:] == 0).all()
+        near("dB, dC", got[i], torch.cat([a[i], b[i]], 2).double() if G > 1 else a[i].double() + b[i].double())
