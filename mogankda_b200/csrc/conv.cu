@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(128, vec ? CONV_FWD_BLOCKS : 3) conv_fwd_kerne
     f32x2 wt[W][P], bias[P];
     conv_params<W, V>(p.weight, p.bias, d0, D, conv_step<DT, vec>(), wt, bias);
     ConvFeed<DT, V, STAGES> feed(shared_rows, p.x, p.x_stride, d0, D, vec);
-    if (blockIdx.y == 0 && p.S.has_empty && p.last) {      // an empty sequence hands its state through
-        for (int n = 0; n < p.S.N; ++n) {
+    if (p.S.has_empty && p.last) {                         // an empty sequence hands its state through: the rows of blocks share the sequences
+        for (int n = blockIdx.y; n < p.S.N; n += gridDim.y) {
             const Span q = sequence(p.S, n);
             if (q.start != q.end) continue;
 #pragma unroll
@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(128, vec ? CONV_BWD_BLOCKS : 3) conv_bwd_kerne
 #pragma unroll
         for (int w = 0; w < W; ++w) dw[w][e] = both(0.f);
     }
-    if (blockIdx.y == 0 && p.S.has_empty && p.dstate) {
-        for (int n = 0; n < p.S.N; ++n) {
+    if (p.S.has_empty && p.dstate) {
+        for (int n = blockIdx.y; n < p.S.N; n += gridDim.y) {
             const Span q = sequence(p.S, n);
             if (q.start != q.end) continue;
             for (int j = 0; j < W - 1; ++j) {
