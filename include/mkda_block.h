@@ -19,10 +19,11 @@ extern "C" {
 #define MKDA_SCAN_CHECKPOINT 16
 #define MKDA_SCAN_MAX_STATES 64
 #define MKDA_NORM_MAX_WIDTH 32768
+#define MKDA_SEQS_MAX_TOKENS 2147418111
 
 /* The sequences of a call: N rows of T tokens (cu == NULL), or packed with boundaries cu[0..N] (int32 on the device, 0 <= cu[n] <= cu[n+1] <= TT). */
 typedef struct {
-    int TT; int N; int T;
+    int TT; int N; int T;      /* TT up to MKDA_SEQS_MAX_TOKENS */
     int has_empty;             /* some sequence may have no token */
     const int* cu;
     const int* order;          /* [N] the sequences in the order in which they are started on, or NULL */

@@ -11,7 +11,6 @@
 
 #include <cmath>
 #include <functional>
-#include <limits>
 #include <memory>
 #include <mutex>
 #include <numeric>
@@ -216,7 +215,7 @@ std::string count_error(int64_t want, int64_t got) {
            std::to_string(got) + ".";
 }
 constexpr int64_t MOST_CHANNELS = 1 << 24;
-constexpr int64_t MOST_TOKENS = std::numeric_limits<int>::max() - 65536;      // tokens are counted in 32 bits, a run past the end included
+constexpr int64_t MOST_TOKENS = MKDA_SEQS_MAX_TOKENS;
 
 // ---- convolution ---------------------------------------------------------------------------------------------------------------------------
 MkdaConvFwd conv_call(const Sequences& q, const Rows& x, const Tensor& w, const Tensor& bias, const Tensor& state, int silu) {

@@ -226,6 +226,7 @@ inline bool with_dtype(int dtype, F f) {
         default: return false;
     }
 }
-inline bool good_sequences(const MkdaSeqs& s) { return s.N >= 0 && s.T >= 0 && s.TT >= 0 && (s.cu || (long long)s.N * s.T == s.TT); }
+// tokens are counted in 32 bits, a run or a tile past the last one included
+inline bool good_sequences(const MkdaSeqs& s) { return s.N >= 0 && s.T >= 0 && s.TT >= 0 && s.TT <= MKDA_SEQS_MAX_TOKENS && (s.cu || (long long)s.N * s.T == s.TT); }
 
 }  // namespace mkda

@@ -126,3 +126,17 @@ def test_scan_bwd_refuses_blocks_that_the_groups_do_not_have(lib):
     for first, blocks in ((1, 0), (-1, 1), (1, 1), (0, 2), (0, -1), (2 ** 31 - 1, 1)):
         b.first_block, b.blocks = first, blocks
         assert lib.mkda_scan_bwd(ctypes.byref(b), None) == _lib.MKDA_ERR_ARG and b"groups do not have" in lib.mkda_last_error()
+
+
+def test_more_tokens_than_are_counted_in_32_bits_are_refused(lib):
+    """The last run of tokens would end past 2^31 - 1.  Fake addresses."""
+    from mogankda_b200 import _lib
+    S, most = _lib.STRUCTS, 2 ** 31 - 1 - 65536
+    calls = [("mkda_conv_fwd", _filled(S["MkdaConvFwd"](), ("x", "weight", "y"), D=8, W=4, dtype=1, x_stride=8)),
+             ("mkda_scan_fwd", _filled(S["MkdaScanFwd"](), ("x", "dt", "B", "C", "A", "y"), D=8, NST=16, G=1, dtype=1, x_stride=8, dt_stride=8, B_stride=16, C_stride=16))]
+    b = _filled(S["MkdaConvBwd"](), ("x", "weight", "dy", "dx", "part"), D=8, W=4, dtype=1, x_stride=8)
+    b.part_rows = lib.mkda_conv_bwd_part_rows(most + 1, 8)
+    calls.append(("mkda_conv_bwd", b))
+    for name, p in calls:
+        p.S.TT, p.S.N, p.S.T = most + 1, 1, most + 1
+        assert getattr(lib, name)(ctypes.byref(p), None) == _lib.MKDA_ERR_ARG, name
