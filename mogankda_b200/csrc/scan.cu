@@ -184,7 +184,8 @@ __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S,
 }
 
 // (8192 x 4096: 280 us.  Two states a lane and twice the warps on the chain 10 % more; B and C in 16 bits side by side, or d and d x doubled for packed products, 20 %.)
-// FILL: there are states that fill up a channel's lanes.  Their B and C are zero, but 0 times an infinite d or x is not: they are set to zero after every token.
+// FILL: there are states that fill up a channel's lanes.  Their B and C are zero, but 0 times an infinite d or x is not: a tile after which they are not zero is walked once more
+// (clearing them after every token of every tile lengthens the chain: 12 states, 8192 x 4096, 314 us for 272).
 template <int DT, int LPC, int TILE, bool FILL>
 __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kernel(const MkdaScanFwd p, const bool vec, const bool bvec) {
     follow_stream();
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
             const int n = sq.n, len = sq.end - sq.start, tiles = (len + TILE - 1) / TILE;
             Four h = four(p.h0 && there ? ld_states(p.h0, (size_t)n * D + ch, n0, NST) : zero);
             if (there) carry(h, A, p.S, n, 0, sq.k, 1, p.seg_h, p.seg_d, D, ch, NP, n0);
+            if constexpr (FILL) { h.v[0] &= real[0]; h.v[1] &= real[1]; }
             const size_t ck0 = p.ckpt ? (p.S.ckpt_off ? (size_t)p.S.ckpt_off[n] : (size_t)n * ((p.S.T + CKPT - 1) / CKPT)) : 0;
             float* ck = p.ckpt ? p.ckpt + ((ck0 + (size_t)sq.k * (p.S.seg / CKPT)) * D + ch) * NP + n0 : nullptr;
             __syncthreads();                               // the first tile is there
@@ -216,6 +218,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 const float* sB = &sh.B[buf][0][n0];
                 const float* sC = &sh.C[buf][0][n0];
                 float* sy = &sh.y[buf][0][0];
+                const Four entered = h;
                 // Four tokens at a time, three groups in flight: what a token reads is requested two groups ahead, its decays are formed one group ahead, between the
                 // steps of the chain (the special function unit takes one of them every eight cycles), and the sums of a group are finished in the next one.
                 struct Token { float2 d; Four B, C; };
@@ -250,7 +253,6 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                             const f32x2 d = e[u].v[i];
                             e[u].v[i] = scan_decay(A.v[i], next[u].d.x);
                             h.v[i] = fma2(d, h.v[i], mul2(dx, now[u].B.v[i]));
-                            if constexpr (FILL) h.v[i] &= real[i];
                             y = i ? fma2(h.v[i], now[u].C.v[i], y) : mul2(h.v[i], now[u].C.v[i]);
                         }
                         yn[u] = sum2(y);
@@ -266,6 +268,28 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 }
                 lanes_sum4<LPC>(ys, q);
                 put_sums<LPC, YROW>(sy, TILE - 4, c0, ys, q);
+                if constexpr (FILL) {
+                    if (__any_sync(0xffffffffu, (h.v[0] & ~real[0]) | (h.v[1] & ~real[1]))) {      // once more, the whole warp, clearing them after every token
+                        h = entered;
+#pragma unroll 1
+                        for (int t4 = 0; t4 < TILE; t4 += 4) {
+                            if (t4 % CKPT == 0 && ck && there && t0 + t4 < len) *reinterpret_cast<float4*>(ck + (size_t)((t0 + t4) / CKPT) * D * NP) = flat(h);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const Token x = fetch(t4 + u);
+                                f32x2 y;
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    h.v[i] = fma2(scan_decay(A.v[i], x.d.x), h.v[i], mul2(both(x.d.y), x.B.v[i])) & real[i];
+                                    y = i ? fma2(h.v[i], x.C.v[i], y) : mul2(h.v[i], x.C.v[i]);
+                                }
+                                ys[u] = sum2(y);
+                            }
+                            lanes_sum4<LPC>(ys, q);
+                            put_sums<LPC, YROW>(sy, t4, c0, ys, q);
+                        }
+                    }
+                }
                 __syncthreads();
             }
             if (p.ht && there && sq.last) st_states(p.ht, (size_t)n * D + ch, n0, NST, flat(h));
