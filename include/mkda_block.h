@@ -4,7 +4,10 @@
  *
  *  - Tokens are addressed in the flattened [TT = B*T] space.  Activations are rows of D channels with a stride in elements between tokens
  *    (the last axis contiguous), outputs and gradients contiguous [TT, D].
- *  - A row stride, an address or a width that is not a multiple of 16 bytes is served element by element, not refused.
+ *  - Activations, their gradients and the convolution's states may have any address that their type allows, any row stride and any width.  Where 16-byte accesses do not fit, the
+ *    16-bit rows of a convolution and the rows of a norm are read by the aligned words of 8 or 16 bytes that hold them and shifted into place: up to 14 bytes in front of and
+ *    behind a row are read too (and not used), so those words must be readable; nothing outside a row is written.  Other rows go element by element.
+ *  - Must be 16-byte aligned, or the call is refused: A, h0, ht, ckpt, state, dht, dh0, seg_h, seg_g, part_A, part_B and part_C of the scan, and `part` of the norm.
  *  - Parameters (weight, bias, A, D, dt_bias) and states of the scan are fp32; a state of the convolution has the type of x.
  */
 #ifndef MKDA_BLOCK_H_
@@ -28,7 +31,8 @@ typedef struct {
     const int* cu;
     const int* order;          /* [N] the sequences in the order in which they are started on, or NULL */
     const int* ckpt_off;       /* [N] first checkpoint of each sequence (ceil(length / MKDA_SCAN_CHECKPOINT) each), or NULL with cu == NULL */
-    int seg; int segs;         /* scan: sequences are cut into parts of seg tokens (a multiple of 64), at most segs of them, that run side by side; seg = 0: not cut */
+    int seg; int segs;         /* scan: sequences are cut into parts of seg tokens (a multiple of 64) that run side by side, segs of them in the longest; seg = 0: not cut.
+                                  Every sequence has a row of blocks for each of the segs parts, also for those without tokens */
 } MkdaSeqs;
 
 /* Depthwise causal convolution: y[t] = act(bias + sum_w weight[w] x[t - W + 1 + w]), W in 2..4.  What lies in front of a sequence's first

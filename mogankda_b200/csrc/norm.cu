@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) norm_fwd_kernel(cons
 }
 
 // RT: the type of what was normalised and of the stream beside it.  Pieces stay as they lie in memory and are widened when they are used, and the weights are in
-// shared memory: registers are what keeps more blocks from being resident (64 for 1024 threads per SM; 128 with sixteen channels a thread 90 us where this takes 50).
+// shared memory: registers are what keeps more blocks from being resident (64 for 1024 threads per SM; 128 with sixteen channels a thread 90 us where this takes 50).  64 do hold
+// one piece a thread, up to 8192 channels (with an fp32 stream 44 to 80 bytes go to local memory); wider rows have two or four, of which 0.2 or 1 to 1.4 KB a thread do.
 template <int DT, int RT, int TPR, int NV, bool vec>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 128 ? 8 : 1024 / TPR) norm_bwd_kernel(const MkdaNormBwd p, const bool wvec) {
     follow_stream();

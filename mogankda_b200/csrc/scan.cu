@@ -10,7 +10,7 @@
 // is off by 2^-24 or so of itself, a state by the accumulated rounding of its memory.
 // What bounds it: 16 exponentials per token and channel (16 states) are 118 us of the special function units for 8192 x 4096, HBM 41 us; the walk reads d, d x, B and C of every
 // token from shared memory, 10 of its cycles a token and warp, which is 70 to 75 % of what an SM's shared memory gives.  bf16, 16 states, with gate: forward 8192 x 4096
-// 280 us, 4 x 2048 x 4096 285 us; backward 2 x 2048 x 4096 400 us.
+// 280 us, 4 x 2048 x 4096 285 us; backward 2 x 2048 x 4096 406 us.
 #include <cfloat>
 #include <type_traits>
 
@@ -577,8 +577,9 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_pre_kerne
 
 // Backward: tiles of one checkpoint, from the last to the first, with the same two roles.  A tile is run forward from its checkpoint, then backward:
 // a_n h_n[t - 1], from which h_n follows with one operation, stays in the registers of the lane in between (the decays beside it, not formed twice, left the rest too few:
-// 406 us where this takes 400).  dB and dC are summed over the lanes of a warp by a butterfly
-// that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by mkda_sum_rows: in a fixed order.  Two blocks per SM: the
+// 1.5 % more).  dB and dC are summed over the lanes of a warp by a butterfly
+// that leaves each lane one of the sums, over the warps through shared memory, and over the blocks of channels by mkda_sum_rows: in a fixed order.  bf16 with 16 states fits the
+// registers; fp32 with 8 states keeps 456 bytes a thread in local memory (and one block per SM, for its shared memory), with 64 states 192, and scan_pre_kernel with tiles of 64 76.  Two blocks per SM: the
 // chain and the butterflies are latency, and two channels per thread, which halve the butterflies but take the registers of the second block, were slower (525 us).
 template <int DT, int LPC>
 struct ScanBwdShared {
