@@ -163,8 +163,10 @@ __device__ __forceinline__ float4 flat(const Four& s) {
     return f;
 }
 
+// `old` behind a part that makes `own` of nothing, in general `both`: nothing stays nothing, and infinity infinite, which no token's decay by itself ends
+__device__ __forceinline__ float carried(float old, float both, float own) { return old == 0.f ? own : fabsf(old) > FLT_MAX ? old + own : both; }
 // What enters a part: the state (or its gradient) that enters the sequence, carried over the parts in front (behind).  A (scaled by log2 e): of this lane.  A part's decay
-// goes in by two halves, since the whole may leave the range where decay times state does not, and nothing stays nothing under any growth.
+// goes in by two halves, since the whole may leave the range where decay times state does not.
 __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S, int n, int from, int to, int step, const float* seg_h, const float* seg_d, int D, size_t ch, int NP, int n0) {
     for (int j = from; j != to; j += step) {
         const size_t i = ((size_t)j * S.N + n) * D + ch;
@@ -178,7 +180,7 @@ __device__ __forceinline__ void carry(Four& s, const Four& A, const MkdaSeqs& S,
             unpack2(fma2(half, first, h.v[e]), a1, b1);
             float ha, hb;
             unpack2(h.v[e], ha, hb);
-            s.v[e] = pack2(a == 0.f ? ha : a1, b == 0.f ? hb : b1);
+            s.v[e] = pack2(carried(a, a1, ha), carried(b, b1, hb));
         }
     }
 }

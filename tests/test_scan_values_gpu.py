@@ -130,3 +130,17 @@ def test_gradients_where_only_the_last_state_is_infinite(N, T):
     got, want = both(lv, [rand(gen, 1, T, D), rand(gen, 1, D, N)])
     for n in ("dx", "dA"):
         near(n, got[n].cpu(), want[n])
+
+
+@pytest.mark.parametrize("N", [16, 47])
+def test_infinite_states_cross_parts(N):
+    """An infinite state stays infinite over every token, also where the decay over a whole part of the sequence is 0 in fp32."""
+    gen = torch.Generator().manual_seed(56)
+    T, D = 1500, 9
+    lv = positive(gen, T, D, N)
+    lv["A"][:], lv["dt"] = -50.0, lv["dt"] + 0.05
+    lv["x"][0, 300, 4] = INF
+    got, want = both(lv)
+    assert want["end"].isinf().any()
+    for n in want:
+        alike(n, got[n], want[n])
