@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(SCAN_THREADS + SCAN_HELPERS, 1) scan_fwd_kerne
                 lanes_sum4<LPC>(ys, q);
                 put_sums<LPC, YROW>(sy, TILE - 4, c0, ys, q);
                 if constexpr (FILL) {
-                    if (__any_sync(0xffffffffu, (h.v[0] & ~real[0]) | (h.v[1] & ~real[1]))) {      // once more, the whole warp, clearing them after every token
+                    if (__any_sync(0xffffffffu, ((h.v[0] & ~real[0]) | (h.v[1] & ~real[1])) != 0)) {      // once more, the whole warp, clearing them after every token
                         h = entered;
 #pragma unroll 1
                         for (int t4 = 0; t4 < TILE; t4 += 4) {

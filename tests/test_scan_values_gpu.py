@@ -132,6 +132,18 @@ def test_gradients_where_only_the_last_state_is_infinite(N, T):
         near(n, got[n].cpu(), want[n])
 
 
+@pytest.mark.parametrize("N", [3, 7, 11, 15, 31, 47])
+@pytest.mark.parametrize("T", [37, 700])
+def test_infinite_values_beside_all_states_of_a_lane_but_one(N, T):
+    """One state fills up the last lane that has any, or none of the others of its lanes: the upper half of a pair of numbers."""
+    gen = torch.Generator().manual_seed(55)
+    lv = positive(gen, T, 9, N)
+    lv["x"][0, T // 2, 4] = INF
+    got, want = both(lv)
+    for n in want:
+        alike(n, got[n], want[n])
+
+
 @pytest.mark.parametrize("N", [16, 47])
 def test_infinite_states_cross_parts(N):
     """An infinite state stays infinite over every token, also where the decay over a whole part of the sequence is 0 in fp32."""
