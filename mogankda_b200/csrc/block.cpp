@@ -35,6 +35,7 @@ struct BlockBackward : public torch::autograd::Node {
     std::vector<std::vector<int64_t>> sizes;
     std::vector<at::ScalarType> types;
     std::vector<uint32_t> depends;             // per gradient: the inputs that it is a function of, besides the incoming gradients
+    bool state_linear = false;                 // of the second output alone it is a function of none of them
     Backward run;
     bool released = false;
 
@@ -68,7 +69,7 @@ struct BlockBackward : public torch::autograd::Node {
         }
         for (size_t i = 0; i < out.size(); ++i)
             if (!task_should_compute_output(i)) out[i] = Tensor();
-        refuse_second(*this, what, grads, depends, out);
+        refuse_second(*this, what, grads, state_linear && !grads[0].defined() ? std::vector<uint32_t>(out.size(), 0u) : depends, out);
         return out;
     }
 };
@@ -297,6 +298,7 @@ PyObject* conv(PyObject*, PyObject* const* a, Py_ssize_t n) {
             constexpr uint32_t X = 1, WT = 2, BIAS = 4, ST = 8, ALL = X | WT | BIAS | ST;
             const std::vector<uint32_t> depends = silu ? std::vector<uint32_t>(4, ALL) : std::vector<uint32_t>{WT, X | ST, 0, WT};      // linear but for the product of weight and tokens
             auto node = new_node("causal_conv1d", x.device(), t, depends, [q, silu](const variable_list& s, const variable_list& g, const Need&) { return conv_backward(q, silu, s, g); });
+            node->state_linear = true;                     // tokens and states as they are
             for (const Tensor& v : t) node->save(v);
             torch::autograd::set_history(y, node);
             if (last.defined()) torch::autograd::set_history(last, node);
@@ -712,6 +714,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             auto node = new_node("rms_norm", x.device(), t, {X | WT | RES, X | RES, X | WT | RES}, [eps, dt, has, rdt](const variable_list& s, const variable_list& g, const Need& need) {
                 return norm_backward(eps, dt, has, rdt, s, g, need);
             });
+            node->state_linear = true;                     // a sum
             torch::autograd::set_history(y, node);
             if (has) torch::autograd::set_history(sum, node);
             node->save(has ? sum : x, has);

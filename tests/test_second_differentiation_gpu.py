@@ -89,3 +89,18 @@ def test_gradients_that_depend_on_nothing_stay_usable():
         got = torch.autograd.grad(y.sum(), lv, create_graph=True)
         total = torch.autograd.grad(y.sum() + sum(g.square().sum() for g in got), lv)
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, total))
+
+
+def test_gradients_of_a_stream_or_a_state_alone_stay_usable():
+    """The sum in front of a norm and the tokens that a convolution keeps are linear in what they come from, whatever the other output is."""
+    x, res, w, s = leaves((1, 2, 32), (1, 2, 32), (32, 4), (1, 3, 32))
+    for fn, lv in ((lambda x, res: mk.rms_norm(x, w[:, 0], residual=res)[1], (x, res)),
+                   (lambda x, s: mk.causal_conv1d(x, w, activation="silu", initial_state=s, output_final_state=True)[1], (x, s))):
+        y = fn(*lv)
+        want = torch.autograd.grad(y.sum(), lv, retain_graph=True)
+        got = torch.autograd.grad(y.sum(), lv, create_graph=True)
+        for a, b, c in zip(want, got, torch.autograd.grad(y.sum() + sum(g.square().sum() for g in got), lv)):
+            assert torch.equal(a, b) and torch.equal(a, c)
+        with pytest.raises(RuntimeError, match="double backward"):
+            up = torch.ones_like(y).requires_grad_(True)
+            torch.autograd.grad(torch.autograd.grad(fn(*lv), lv, up, create_graph=True)[0].sum(), up)
