@@ -58,7 +58,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, *, dt_softplus=
     of any of the three types.  ``initial_state`` [sequences,D,N] float32.  Returns ``(y, final_state)``: y like x; the state float32 or None.
     A call that wants gradients keeps the state in front of every 16th token (P / 4 bytes per token and channel; P: N padded to 8, 16, 32 or 64).  Its backward pass leaves dB and
     dC per block of 512 / P channels, 8 P bytes per token and block, before it adds them up (4 bytes per token and channel at 16 states, 64 at 64); more than 1 GiB of it is
-    worked off by ranges of blocks that fill the GPU.  An infinite A is taken as the largest number of its sign: -inf keeps nothing of a state wherever d > 0."""
+    worked off by ranges of blocks that fill the GPU.  An infinite A is taken as the largest number of its sign: -inf keeps nothing of a state wherever d > 0.  Gradients around an
+    infinite x or dt may be NaN."""
     table, dims = _sequences(x, cu_seqlens)
     return _lib.host().scan(x, dt, A, B, C, D, z, dt_bias, initial_state, table, dims, dt_softplus, output_final_state)
 
