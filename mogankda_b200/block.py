@@ -66,7 +66,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, *, dt_softplus=
 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, *, dt_softplus=False):
     """One more token of each of N running sequences: x, dt, z [N,D], B, C [N,states] or [N,G,states], state [N,D,states] float32 (contiguous), which is
-    updated IN PLACE.  Returns y [N,D].  No backward pass."""
+    updated IN PLACE.  Returns y [N,D].  No backward pass.  Where d is 0, A has to be above -2.3e38 (A log2 e a finite number)."""
     return _lib.host().scan_step(x, dt, A, B, C, D, z, dt_bias, state, dt_softplus)
 
 
