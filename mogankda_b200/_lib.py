@@ -21,7 +21,8 @@ ENTRY_POINTS = (
 LONGER_ENTRY_POINTS = {"mkda_recur_fwd_ordered": 3, "mkda_chain_fwd_ordered": 3, "mkda_bwd_dh_ordered": 3, "mkda_gate_intra_fwd": 3, "mkda_bwd_dh_rows": 3,
                        "mkda_bwd_chunk_rows": 5}
 BLOCK_ENTRY_POINTS = ("mkda_conv_fwd", "mkda_conv_bwd", "mkda_conv_step", "mkda_scan_fwd", "mkda_scan_bwd", "mkda_scan_step", "mkda_norm_fwd",
-                      "mkda_norm_bwd", "mkda_sum_rows")
+                      "mkda_norm_bwd", "mkda_sum_rows", "mkda_linear_fwd", "mkda_linear_bwd", "mkda_linear_step", "mkda_rotary", "mkda_layer_norm_fwd",
+                      "mkda_layer_norm_bwd")
 ENUMS = {}
 STRUCTS = {}
 

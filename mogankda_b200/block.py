@@ -1,5 +1,6 @@
 """The operators that stand around the delta-rule layer in a block of a model: the short causal convolution in front of q, k and v (or of a
-scan), the selective scan, and the RMS norm with the residual's addition.
+scan), the selective scan, the RMS norm and the layer norm with the residual's addition; and its sibling without the delta rule, the linear attention with a decay
+for each head, with rotary positions of several axes in front of it.
 
 Conventions of the layer hold: CUDA tensors only, bfloat16, float16 or float32, arithmetic in 32 bits, launches on
 ``torch.cuda.current_stream()`` of the tensors' device, packed sequences addressed by ``cu_seqlens`` (B == 1; tokens behind the last boundary give zeros,
@@ -14,12 +15,12 @@ from . import _lib
 from .index import get_bounds
 
 
-def _sequences(x, cu_seqlens):
+def _sequences(x, cu_seqlens, dim=3):
     if cu_seqlens is None:
         return None, None
     if not x.is_cuda:
         raise RuntimeError("mogankda_b200 kernels need CUDA tensors (there is no CPU fallback)")
-    if x.dim() != 3 or x.shape[0] != 1:
+    if x.dim() != dim or x.shape[0] != 1:
         raise ValueError(f"The batch size is expected to be 1 rather than {x.shape[0]} when using `cu_seqlens`.")
     if cu_seqlens.dim() != 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise ValueError("cu_seqlens must be a vector of int32 or int64")
@@ -85,3 +86,44 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, out_dtype=None, scale_g
     if got[-1] is None:
         got = got[:-1]
     return got if len(got) > 1 else got[0]
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, output_final_state=False, cu_seqlens=None):
+    """Linear attention with a decay for each head, the delta-rule layer's sibling without the delta rule:
+
+        S[t] = exp(log_decay) S[t - 1] + k[t] v[t]^T;  o[t] = scale S[t]^T q[t]
+
+    q, k [B,T,HK,K] and v [B,T,HV,V] share a type, K and V up to 128; HV is a multiple of HK: v-head h reads head h // (HV // HK) of q and k.  ``log_decay`` [HV] (any of the
+    three types, natural logarithm, at most 0) has no gradient: a call that wants one is refused.  ``scale`` is K ** -0.5 by default; ``initial_state`` [N,HV,K,V] float32.
+    Returns ``(o, final_state)``: o [B,T,HV,V] in the type of q; the state float32 or None.
+
+    Pairs of tokens up to 128 apart are computed as products of q and k, earlier ones through the state, which is fp32 throughout.  Long sequences of few heads are cut into parts that run
+    side by side, by a rule on sizes: results on both sides of it agree to rounding.  What is not finite stays in its sequence, but reaches tokens in front of it that
+    share its 128 tokens."""
+    table, dims = _sequences(q, cu_seqlens, 4)
+    return _lib.host().linear(q, k, v, log_decay, initial_state, table, dims, scale, output_final_state)
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
+    """One more token of each of N running sequences: q, k [N,HK,K], v [N,HV,V], state [N,HV,K,V] float32 (contiguous), which is updated IN PLACE.  Returns o
+    [N,HV,V].  No backward pass."""
+    return _lib.host().linear_step(q, k, v, log_decay, state, scale)
+
+
+def rotary(q, k, positions, inv_freq, *, axes=None, interleaved=False):
+    """Rotary positions: pair f of the channels of each head is turned by ``positions * inv_freq[f]``.
+
+    q [..,HQ,D] and k [..,HK,D] (or None) share a type, D up to 512; ``inv_freq`` [F] float32, 2 F <= D: the pairs are channels (f, f + F), with ``interleaved``
+    (2 f, 2 f + 1), and channels behind the first 2 F stay as they are.  ``positions`` int32 or int64 with the leading axes of q; with ``axes``, F whole numbers, ``positions`` is
+    [A,..] and frequency f goes by ``positions[axes[f]]`` (time, height and width of a video's tokens: ``axes=[0] * 16 + [1] * 24 + [2] * 24``, or any other order).
+    Angles are formed in 64 bits, so that far positions keep theirs.  Returns q, or ``(q, k)``, as new tensors; gradients for q and k, none for ``inv_freq``."""
+    got = _lib.host().rotary(q, k, positions, inv_freq, axes, interleaved)
+    return got if k is not None else got[0]
+
+
+def layer_norm(x, weight=None, bias=None, *, residual=None, groups=1, eps=1e-5):
+    """Layer norm of the rows of x [..,H]: ``y = (s - mean s) / sqrt(var s + eps) * weight + bias`` with s = x, or with ``residual`` s = x + residual as the residual's type holds it
+    (that of x, or float32).  ``groups`` > 1: each of so many equal parts of a row, up to 32768 channels, by itself, as for the heads of a token's outputs; ``weight`` and ``bias`` are
+    [H] all the same.  Statistics in 32 bits, y rounded once.  Returns y; with ``residual`` ``(y, s)``."""
+    got = _lib.host().layer_norm(x, weight, bias, residual, groups, eps)
+    return got if residual is not None else got[0]

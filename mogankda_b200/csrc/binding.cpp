@@ -261,7 +261,7 @@ PyMODINIT_FUNC PyInit__host() {
         return nullptr;
     }
     PyObject* m = PyModule_Create(&module);
-    if (m && PyModule_AddFunctions(m, block_methods) != 0) {
+    if (m && (PyModule_AddFunctions(m, block_methods) != 0 || PyModule_AddFunctions(m, mixer_methods) != 0)) {
         Py_DECREF(m);
         return nullptr;
     }

@@ -78,5 +78,6 @@ inline void refuse_second(const torch::autograd::Node& node, const std::string& 
 }
 
 extern PyMethodDef block_methods[];        // block.cpp
+extern PyMethodDef mixer_methods[];        // mixer.cpp
 
 }  // namespace mkda_host

@@ -1,0 +1,426 @@
+// Linear attention with a decay for each head (linear.cuh): the kernel for any type and size of heads, the states of cut sequences, sums over the v-heads of a group, and the
+// single-token form.
+#include <algorithm>
+
+#include "linear.cuh"
+
+namespace mkda {
+
+// ---- any type, 1 to 128 channels: fp32 throughout ------------------------------------------------------------------------------------------------
+// A block carries one part of a sequence and v-head, 32 tokens at a time: their rows and the state in shared memory, every product by fused multiply-adds on tiles of registers.
+namespace ls {
+constexpr int THREADS = 256, C = 32, PP = C + 4;
+__host__ __device__ constexpr int pitch(int n) { return (n + 3) / 4 * 4 + 4; }
+inline int smem(int M, int V) { return 4 * (2 * C * pitch(M) + C * pitch(V) + C * PP + ((M + 3) / 4 * 4) * pitch(V) + PP); }
+
+// rows [0, len) of `n` channels from global memory, the rest of the C rows and of the pitch zero
+template <int DT>
+__device__ __forceinline__ void load_rows(float* to, int pit, const void* from, size_t at, long long stride, int n, int len, bool vec) {
+    const int quads = pit / 4;
+    for (int e = threadIdx.x; e < C * quads; e += THREADS) {
+        const int r = e / quads, c = 4 * (e - r * quads);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < len && c < n) {
+            const size_t i = at + (size_t)r * stride + c;
+            if (vec) {
+                v = ld4(from, DT, i);
+            } else {
+                v.x = ld1(from, DT, i);
+                if (c + 1 < n) v.y = ld1(from, DT, i + 1);
+                if (c + 2 < n) v.z = ld1(from, DT, i + 2);
+                if (c + 3 < n) v.w = ld1(from, DT, i + 3);
+            }
+        }
+        *reinterpret_cast<float4*>(to + r * pit + c) = v;
+    }
+}
+__device__ __forceinline__ void fma4(float (&d)[4], float a, const float4& b) {
+    d[0] = fmaf(a, b.x, d[0]); d[1] = fmaf(a, b.y, d[1]); d[2] = fmaf(a, b.z, d[2]); d[3] = fmaf(a, b.w, d[3]);
+}
+}  // namespace ls
+
+template <int DT>
+__global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const LinearCall call, const bool vec) {
+    using namespace ls;
+    follow_stream();
+    extern __shared__ __align__(16) float smem_f[];
+    const LinearKind& k = call.kind[blockIdx.z];
+    const int h = blockIdx.x % call.HV, part = blockIdx.x / call.HV, n = call.S.order && !call.S.seg ? call.S.order[blockIdx.y] : blockIdx.y;
+    const LinearPart w = linear_part(call.S, n, part, k.back);
+    if (w.nothing || (!k.a && w.leaves_last)) return;      // what the last part leaves is the main kernel's to find
+    const int M = k.M, V = k.V, pm = pitch(M), pv = pitch(V), M4 = (M + 3) / 4 * 4;
+    float* sa = smem_f;
+    float* sb = sa + C * pm;
+    float* sc = sb + C * pm;
+    float* sp = sc + C * pv;
+    float* st = sp + C * PP;                               // [M4][pv]
+    float* pw = st + M4 * pv;                              // lam^0 .. lam^32
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const float gamma = call.log_decay[h];
+    if (tid <= C) pw[tid] = decay_power(gamma, tid);
+    const size_t size = (size_t)M * V;
+    const float* in = call.S.seg && k.a ? k.parts + ((size_t)(n * call.S.segs + part) * call.HV + h) * size : k.a && k.first ? k.first + ((size_t)n * call.HV + h) * size : nullptr;
+    for (int e = tid; e < M4 * pv; e += THREADS) {
+        const int m = e / pv, v = e - m * pv;
+        st[e] = in && m < M && v < V ? in[k.transposed ? (size_t)v * M + m : (size_t)m * V + v] : 0.f;
+    }
+    const int chunks = (w.len + C - 1) / C;
+    for (int t = 0; t < chunks; ++t) {
+        const int c0 = (k.back ? chunks - 1 - t : t) * C, len = min(C, w.len - c0);
+        const size_t tok = w.start + c0;
+        __syncthreads();
+        if (k.a) load_rows<DT>(sa, pm, k.a, tok * k.a_stride + (size_t)(h / k.a_per) * M, k.a_stride, M, len, vec);
+        load_rows<DT>(sb, pm, k.b, tok * k.b_stride + (size_t)(h / k.b_per) * M, k.b_stride, M, len, vec);
+        load_rows<DT>(sc, pv, k.c, tok * k.c_stride + (size_t)(h / k.c_per) * V, k.c_stride, V, len, vec);
+        __syncthreads();
+        if (k.a) {
+            {                                              // pairs: row i, columns j = tid % 8 + 8 jj
+                const int i = tid >> 3;
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int m = 0; m < M4; m += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(sa + i * pm + m);
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj) {
+                        const float4 y = *reinterpret_cast<const float4*>(sb + ((tid & 7) + 8 * jj) * pm + m);
+                        d[jj] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, d[jj]))));
+                    }
+                }
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const int j = (tid & 7) + 8 * jj, away = k.back ? j - i : i - j;
+                    sp[i * PP + j] = away >= 0 && j < len ? d[jj] * pw[away] * k.pair_scale : 0.f;
+                }
+            }
+            __syncthreads();
+            const int v = 4 * lane;
+            if (v < V) {                                   // four rows, four columns
+                float o[4][4], s[4][4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[r][e] = s[r][e] = 0.f;
+#pragma unroll 2
+                for (int j = 0; j < C; j += 4) {
+                    float4 y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const float4*>(sc + (j + e) * pv + v);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float4 x = *reinterpret_cast<const float4*>(sp + (4 * warp + r) * PP + j);
+                        fma4(o[r], x.x, y[0]); fma4(o[r], x.y, y[1]); fma4(o[r], x.z, y[2]); fma4(o[r], x.w, y[3]);
+                    }
+                }
+#pragma unroll 2
+                for (int m = 0; m < M4; m += 4) {
+                    float4 y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const float4*>(st + (m + e) * pv + v);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float4 x = *reinterpret_cast<const float4*>(sa + (4 * warp + r) * pm + m);
+                        fma4(s[r], x.x, y[0]); fma4(s[r], x.y, y[1]); fma4(s[r], x.z, y[2]); fma4(s[r], x.w, y[3]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 4 * warp + r;
+                    if (i >= len) continue;
+                    const float f = pw[k.back ? len - 1 - i : i + 1] * k.state_scale;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = fmaf(f, s[r][e], o[r][e]);
+                    const size_t at = ((tok + i) * call.HV + h) * V + v;
+                    if (V % 4 == 0) {
+                        st4(k.out, k.out_dtype, at, make_float4(x[0], x[1], x[2], x[3]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (v + e < V) st1(k.out, k.out_dtype, at + e, x[e]);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        {                                                  // the state: sixteen rows, four columns
+            const int m0 = 16 * warp, v = 4 * lane;
+            if (m0 < M && v < V) {
+                float acc[16][4];
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
+                for (int j = 0; j < len; ++j) {
+                    const float f = pw[k.back ? j + 1 : len - 1 - j] * k.in_scale;
+                    float4 y = *reinterpret_cast<const float4*>(sc + j * pv + v);
+                    y.x *= f; y.y *= f; y.z *= f; y.w *= f;
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        if (m0 + r >= M4) break;
+                        const float4 x = *reinterpret_cast<const float4*>(sb + j * pm + m0 + r);
+                        fma4(acc[r], x.x, y); fma4(acc[r + 1], x.y, y); fma4(acc[r + 2], x.z, y); fma4(acc[r + 3], x.w, y);
+                    }
+                }
+                const float f = pw[len];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if (m0 + r >= M) break;
+                    float4* s = reinterpret_cast<float4*>(st + (m0 + r) * pv + v);
+                    float4 x = *s;
+                    x.x = fmaf(f, x.x, acc[r][0]); x.y = fmaf(f, x.y, acc[r][1]); x.z = fmaf(f, x.z, acc[r][2]); x.w = fmaf(f, x.w, acc[r][3]);
+                    *s = x;
+                }
+            }
+        }
+    }
+    float* out = !k.a ? k.parts + ((size_t)(n * call.S.segs + part + (k.back ? -1 : 1)) * call.HV + h) * size : k.last && w.leaves_last ? k.last + ((size_t)n * call.HV + h) * size : nullptr;
+    if (!out) return;
+    __syncthreads();
+    for (size_t e = tid; e < size; e += THREADS) {
+        const int slow = (int)(e / (k.transposed ? M : V)), fast = (int)(e - (size_t)slow * (k.transposed ? M : V));
+        out[e] = k.transposed ? st[fast * pv + slow] : st[slow * pv + fast];
+    }
+}
+
+// ---- cut sequences -------------------------------------------------------------------------------------------------------------------------------
+// A part finds what it makes of nothing and leaves it where the next part's entering state belongs; this adds what comes through from further away:
+//   parts[p] = (what part p - 1 makes of nothing) + lam^(tokens of part p - 1) parts[p - 1], parts[0] the sequence's initial state; backwards likewise.
+__global__ void __launch_bounds__(256) linear_parts_kernel(const LinearCall call) {
+    follow_stream();
+    const LinearKind& k = call.kind[blockIdx.z];
+    const int h = blockIdx.x % call.HV, n = blockIdx.y;
+    const size_t size = (size_t)k.M * k.V, e = (size_t)(blockIdx.x / call.HV) * 256 + threadIdx.x, pitch = (size_t)call.HV * size;
+    const Span w = sequence(call.S, n);
+    const int len = w.end - w.start, seg = call.S.seg, parts = len > 0 ? (len + seg - 1) / seg : 1;
+    if (e >= size) return;
+    float* at = k.parts + ((size_t)n * call.S.segs * call.HV + h) * size + e;
+    float s = k.first ? k.first[((size_t)n * call.HV + h) * size + e] : 0.f;
+    const float whole = decay_power(call.log_decay[h], seg), rest = decay_power(call.log_decay[h], len - (parts - 1) * seg);
+    if (k.back) {
+        at[(parts - 1) * pitch] = s;
+        for (int p = parts - 2; p >= 0; --p) at[p * pitch] = s = fmaf(p == parts - 2 ? rest : whole, s, at[p * pitch]);
+    } else {
+        at[0] = s;
+        for (int p = 1; p < parts; ++p) at[p * pitch] = s = fmaf(whole, s, at[p * pitch]);
+    }
+}
+
+// ---- shared heads --------------------------------------------------------------------------------------------------------------------------------
+// out[t][g] = sum over the `per` v-heads of group g, in order
+__global__ void __launch_bounds__(256) linear_group_kernel(const float* part, void* out, int dtype, long long rows, int per, int K) {
+    follow_stream();
+    const bool vec = K % 4 == 0;
+    const int step = vec ? 4 : 1;
+    const long long all = rows * (K / step);
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
+        const long long row = e / (K / step);
+        const int c = (int)(e - row * (K / step)) * step;
+        const float* p = part + (size_t)row * per * K + c;
+        if (vec) {
+            float4 s = *reinterpret_cast<const float4*>(p);
+            for (int r = 1; r < per; ++r) {
+                const float4 x = *reinterpret_cast<const float4*>(p + (size_t)r * K);
+                s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+            }
+            st4(out, dtype, (size_t)row * K + c, s);
+        } else {
+            float s = p[0];
+            for (int r = 1; r < per; ++r) s += p[(size_t)r * K];
+            st1(out, dtype, (size_t)row * K + c, s);
+        }
+    }
+}
+
+// ---- single tokens -------------------------------------------------------------------------------------------------------------------------------
+// A block per v-head and sequence: S <- lam S + k v^T where it lies, o = scale S^T q.  Eight warps share the rows of the state, a lane has four columns of each of them; all of
+// a thread's rows are requested before the first is used.  Bound by HBM: the state is read and written.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) linear_step_kernel(const MkdaLinearStep p) {
+    follow_stream();
+    __shared__ float sq[MKDA_LINEAR_MAX_DIM], sk[MKDA_LINEAR_MAX_DIM], part[8][MKDA_LINEAR_MAX_DIM];
+    const int h = blockIdx.x, n = blockIdx.y, K = p.K, V = p.V, g = h / (p.HV / p.HK), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = 4 * lane;
+    float* state = p.state + ((size_t)n * p.HV + h) * K * V;
+    float4 s[16];
+    auto row = [&](int i) { return warp + 8 * i; };
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* at = state + (size_t)row(i) * V + v;
+        if (row(i) >= K || v >= V) continue;
+        if (VEC) {
+            s[i] = *reinterpret_cast<const float4*>(at);
+        } else {
+            s[i].x = at[0];
+            if (v + 1 < V) s[i].y = at[1];
+            if (v + 2 < V) s[i].z = at[2];
+            if (v + 3 < V) s[i].w = at[3];
+        }
+    }
+    if (tid < K) sq[tid] = ld1(p.q, DT, (size_t)n * p.q_stride + (size_t)g * K + tid);
+    else if (tid >= 128 && tid - 128 < K) sk[tid - 128] = ld1(p.k, DT, (size_t)n * p.k_stride + (size_t)g * K + tid - 128);
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (v + e < V) x[e] = ld1(p.v, DT, (size_t)n * p.v_stride + (size_t)h * V + v + e);
+    const float lam = expf(p.log_decay[h]);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (row(i) >= K || v >= V) continue;
+        const float kk = sk[row(i)], qq = sq[row(i)];
+        s[i].x = fmaf(lam, s[i].x, kk * x[0]); s[i].y = fmaf(lam, s[i].y, kk * x[1]); s[i].z = fmaf(lam, s[i].z, kk * x[2]); s[i].w = fmaf(lam, s[i].w, kk * x[3]);
+        o[0] = fmaf(qq, s[i].x, o[0]); o[1] = fmaf(qq, s[i].y, o[1]); o[2] = fmaf(qq, s[i].z, o[2]); o[3] = fmaf(qq, s[i].w, o[3]);
+        float* at = state + (size_t)row(i) * V + v;
+        if (VEC) {
+            *reinterpret_cast<float4*>(at) = s[i];
+        } else {
+            at[0] = s[i].x;
+            if (v + 1 < V) at[1] = s[i].y;
+            if (v + 2 < V) at[2] = s[i].z;
+            if (v + 3 < V) at[3] = s[i].w;
+        }
+    }
+    *reinterpret_cast<float4*>(&part[warp][v]) = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (tid < V) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += part[w][tid];
+        st1(p.o, DT, ((size_t)n * p.HV + h) * V + tid, p.scale * t);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------------------------
+// The kernels that find the states of cut sequences (`before`) run first.
+static int run_linear(const LinearCall& call, const LinearCall& before, cudaStream_t stream) {
+    const MkdaSeqs& S = call.S;
+    if (S.N == 0) return MKDA_OK;
+    auto simt = [&](const LinearCall& c) {
+        int bytes = 0, rc = MKDA_OK;
+        bool vec = true;
+        for (int i = 0; i < c.kinds; ++i) {
+            const LinearKind& k = c.kind[i];
+            bytes = std::max(bytes, ls::smem(k.M, k.V));
+            vec = vec && k.M % 4 == 0 && k.V % 4 == 0 && k.a_stride % 4 == 0 && k.b_stride % 4 == 0 && k.c_stride % 4 == 0 && aligned16(k.a) && aligned16(k.b) && aligned16(k.c);
+        }
+        with_dtype(c.dtype, [&](auto dt) {
+            constexpr int DT = decltype(dt)::value;
+            rc = ensure_smem(reinterpret_cast<const void*>(linear_simt_kernel<DT>), 227 * 1024 - 1024, "linear");
+            if (rc == MKDA_OK) launch(linear_simt_kernel<DT>, dim3(c.HV * (S.seg ? S.segs : 1), S.N, c.kinds), ls::THREADS, bytes, stream, c, vec);
+        });
+        return rc != MKDA_OK ? rc : check_launch("linear");
+    };
+    if (S.seg && S.segs > 1) {
+        int rc = simt(before);
+        if (rc != MKDA_OK) return rc;
+    }
+    if (S.seg) {
+        size_t size = 0;
+        for (int i = 0; i < before.kinds; ++i) size = std::max(size, (size_t)before.kind[i].M * before.kind[i].V);
+        launch(linear_parts_kernel, dim3(before.HV * (unsigned)((size + 255) / 256), S.N, before.kinds), 256, 0, stream, before);
+        int rc = check_launch("linear parts");
+        if (rc != MKDA_OK) return rc;
+    }
+    return simt(call);
+}
+
+static const char* bad_linear(const MkdaLinearFwd& p) {
+    if (!good_sequences(p.S)) return "linear: bad sequences";
+    if (p.HK < 1 || p.HV < 1 || p.HV > 65535 || p.HV % p.HK) return "linear: the v-heads, at most 65535, must be a multiple of the q/k-heads";
+    if (p.K < 1 || p.K > MKDA_LINEAR_MAX_DIM || p.V < 1 || p.V > MKDA_LINEAR_MAX_DIM) return "linear: heads of 1 to 128 channels";
+    if (p.dtype < MKDA_F32 || p.dtype > MKDA_F16) return "linear: unsupported dtype";
+    if (p.S.N > 65535) return "linear: at most 65535 sequences";
+    if (p.S.seg < 0 || p.S.seg % 128 || (p.S.seg && (p.S.segs < 1 || !p.seg_h))) return "linear: parts of a multiple of 128 tokens, and a state for each";
+    if (p.S.seg && (long long)p.HV * p.S.segs * 64 > 0x7fffffff) return "linear: too many parts";
+    if (!p.log_decay) return "linear: null argument";
+    if (any_misaligned(p.h0, p.ht, p.seg_h, p.o)) return "linear: states and outputs must be 16-byte aligned";
+    return nullptr;
+}
+
+}  // namespace mkda
+
+using namespace mkda;
+
+// q and k of a v-head, v
+static LinearKind kind_of(const MkdaLinearFwd& p, const void* a, long long sa, bool a_v, const void* b, long long sb, bool b_v, const void* c, long long sc, bool c_v) {
+    const int per = p.HV / p.HK;
+    LinearKind k{};
+    k.a = a; k.b = b; k.c = c; k.a_stride = sa; k.b_stride = sb; k.c_stride = sc;
+    k.a_per = a_v ? 1 : per; k.b_per = b_v ? 1 : per; k.c_per = c_v ? 1 : per;
+    k.M = b_v ? p.V : p.K; k.V = c_v ? p.V : p.K;
+    k.pair_scale = p.scale; k.in_scale = 1.f; k.state_scale = p.scale;
+    k.out_dtype = p.dtype;
+    return k;
+}
+static LinearCall call_of(const MkdaLinearFwd& p) {
+    LinearCall c{};
+    c.S = p.S; c.HV = p.HV; c.dtype = p.dtype; c.log_decay = p.log_decay;
+    return c;
+}
+
+extern "C" int mkda_linear_fwd(const MkdaLinearFwd* p, void* stream) {
+    if (!p) return set_error(MKDA_ERR_ARG, "linear_fwd: null argument");
+    if (const char* bad = bad_linear(*p)) return set_error(MKDA_ERR_ARG, bad);
+    if (p->S.TT && (!p->q || !p->k || !p->v || !p->o)) return set_error(MKDA_ERR_ARG, "linear_fwd: null argument");
+    LinearCall call = call_of(*p), before = call;
+    LinearKind k = kind_of(*p, p->q, p->q_stride, false, p->k, p->k_stride, false, p->v, p->v_stride, true);
+    k.out = p->o; k.first = p->h0; k.last = p->ht; k.parts = p->seg_h;
+    call.kind[0] = k; call.kinds = 1;
+    k.a = nullptr;
+    before.kind[0] = k; before.kinds = 1;
+    return run_linear(call, before, (cudaStream_t)stream);
+}
+
+extern "C" int mkda_linear_bwd(const MkdaLinearBwd* q, void* stream) {
+    if (!q) return set_error(MKDA_ERR_ARG, "linear_bwd: null argument");
+    const MkdaLinearFwd& p = q->f;
+    if (const char* bad = bad_linear(p)) return set_error(MKDA_ERR_ARG, bad);
+    const bool shared = p.HV > p.HK;
+    if (p.S.TT && (!p.q || !p.k || !p.v || !q->d_o || !q->dq || !q->dk || !q->dv || (shared && (!q->part_q || !q->part_k)))) return set_error(MKDA_ERR_ARG, "linear_bwd: null argument");
+    if ((p.S.seg && !q->seg_g) || any_misaligned(q->d_o, q->dht, q->dq, q->dk, q->dv, q->dh0, q->seg_g, q->part_q, q->part_k))
+        return set_error(MKDA_ERR_ARG, "linear_bwd: states, gradients and workspaces must be 16-byte aligned");
+    if (q->end < 0 || q->end > p.S.TT) return set_error(MKDA_ERR_ARG, "linear_bwd: the last boundary is behind the tokens");
+    const long long so = (long long)p.HV * p.V;
+    LinearCall call = call_of(p), before = call;
+    LinearKind dq = kind_of(p, q->d_o, so, true, p.v, p.v_stride, true, p.k, p.k_stride, false);
+    LinearKind dk = kind_of(p, p.v, p.v_stride, true, q->d_o, so, true, p.q, p.q_stride, false);
+    LinearKind dv = kind_of(p, p.k, p.k_stride, false, p.q, p.q_stride, false, q->d_o, so, true);
+    dq.transposed = dk.transposed = 1;
+    dk.back = dv.back = 1;
+    dk.in_scale = dv.in_scale = p.scale;                   // the state's gradient has the scale in it
+    dk.state_scale = dv.state_scale = 1.f;
+    dq.first = p.h0; dk.first = dv.first = q->dht;
+    dv.last = q->dh0;
+    dq.parts = p.seg_h; dk.parts = dv.parts = q->seg_g;
+    dq.out = shared ? static_cast<void*>(q->part_q) : q->dq; dk.out = shared ? static_cast<void*>(q->part_k) : q->dk; dv.out = q->dv;
+    if (shared) dq.out_dtype = dk.out_dtype = MKDA_F32;
+    call.kind[0] = dq; call.kind[1] = dk; call.kind[2] = dv; call.kinds = 3;
+    LinearKind fs = kind_of(p, nullptr, 0, false, p.k, p.k_stride, false, p.v, p.v_stride, true), bs = dv;
+    fs.first = p.h0; fs.parts = p.seg_h;
+    bs.a = nullptr;
+    before.kind[0] = fs; before.kind[1] = bs; before.kinds = 2;
+    int rc = run_linear(call, before, (cudaStream_t)stream);
+    if (rc != MKDA_OK || !shared || q->end == 0) return rc;
+    const long long rows = (long long)q->end * p.HK;
+    const unsigned blocks = (unsigned)std::min<long long>((rows * p.K + 1023) / 1024, 16ll * sm_count());
+    for (int i = 0; i < 2; ++i) {
+        launch(linear_group_kernel, dim3(std::max(1u, blocks)), 256, 0, (cudaStream_t)stream, static_cast<const float*>(i ? q->part_k : q->part_q), i ? q->dk : q->dq, p.dtype, rows, p.HV / p.HK, p.K);
+        rc = check_launch("linear groups");
+        if (rc != MKDA_OK) return rc;
+    }
+    return MKDA_OK;
+}
+
+extern "C" int mkda_linear_step(const MkdaLinearStep* p, void* stream) {
+    if (!p || !p->log_decay || (p->N && (!p->q || !p->k || !p->v || !p->state || !p->o))) return set_error(MKDA_ERR_ARG, "linear_step: null argument");
+    if (p->N < 0 || p->N > 65535) return set_error(MKDA_ERR_ARG, "linear_step: at most 65535 sequences");
+    if (p->HK < 1 || p->HV < 1 || p->HV % p->HK) return set_error(MKDA_ERR_ARG, "linear_step: the v-heads must be a multiple of the q/k-heads");
+    if (p->K < 1 || p->K > MKDA_LINEAR_MAX_DIM || p->V < 1 || p->V > MKDA_LINEAR_MAX_DIM) return set_error(MKDA_ERR_ARG, "linear_step: heads of 1 to 128 channels");
+    if (p->dtype < MKDA_F32 || p->dtype > MKDA_F16) return set_error(MKDA_ERR_ARG, "linear_step: unsupported dtype");
+    if (!aligned16(p->state)) return set_error(MKDA_ERR_ARG, "linear_step: the state must be 16-byte aligned");
+    if (p->N == 0) return MKDA_OK;
+    with_dtype(p->dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        launch(p->V % 4 == 0 ? linear_step_kernel<DT, true> : linear_step_kernel<DT, false>, dim3(p->HV, p->N), 256, 0, (cudaStream_t)stream, *p);
+    });
+    return check_launch("linear_step");
+}

@@ -1,0 +1,49 @@
+// Linear attention with a decay for each head: what its kernels (linear.cu) share.
+//
+// With lam = exp(log_decay) of a head, the forward pass and the three gradients are one operator of three row tensors,
+//   out[i] = sum_j lam^|i - j| (a[i] . b[j]) c[j],   over j <= i, or backwards in time over j >= i:
+//   o: (q, k, v)     dq: (do, v, k)     dk: (v, do, q) backwards     dv: (k, q, do) backwards
+// Over a stretch of L tokens (i, j counted from its first one) it is, with the state M = sum lam^.. b c^T in front of the stretch (behind it)
+//   forwards   out[i] = sum_{j <= i} lam^(i - j) (a[i] . b[j]) c[j] + lam^(i + 1) M^T a[i]        M <- lam^L M + sum_j lam^(L - 1 - j) b[j] c[j]^T
+//   backwards  out[i] = sum_{j >= i} lam^(j - i) (a[i] . b[j]) c[j] + lam^(L - 1 - i) M^T a[i]    M <- lam^L M + sum_j lam^(j + 1) b[j] c[j]^T
+// M is the state S of the caller for o, its transpose for dq, the state's gradient for dv and its transpose for dk.
+#pragma once
+#include "block.cuh"
+
+namespace mkda {
+
+struct LinearKind {
+    const void* a; const void* b; const void* c;           // a NULL: nothing but the states that the parts of the sequences leave
+    long long a_stride, b_stride, c_stride;
+    int a_per, b_per, c_per;                               // v-heads to a head
+    int M, V;                                              // channels of a and b, of c and out
+    void* out; int out_dtype;                              // [TT, HV, V]
+    float pair_scale, in_scale, state_scale;               // of a pair's product, of what goes into the state, of what comes out of it
+    int back;
+    int transposed;                                        // states lie as [V][M] in memory
+    const float* first; float* last;                       // [N, HV, ..]
+    float* parts;                                          // [N, segs, HV, ..] cut sequences: the state that each part enters with
+};
+struct LinearCall {
+    MkdaSeqs S;
+    int HV, dtype, kinds;
+    const float* log_decay;
+    LinearKind kind[3];
+};
+
+// lam^n, rounded once
+__device__ __forceinline__ float decay_power(float log_decay, long long n) { return n == 0 ? 1.f : (float)exp((double)log_decay * (double)n); }
+
+// What a block has to do: tokens [start, start + len) of sequence n, which are part `part` of it
+struct LinearPart { int start, len; bool nothing, enters_first, leaves_last; };
+__device__ __forceinline__ LinearPart linear_part(const MkdaSeqs& s, int n, int part, bool back) {
+    const Span w = sequence(s, n);
+    const int len = w.end - w.start;
+    if (!s.seg) return {w.start, len, false, true, true};
+    const int parts = len > 0 ? (len + s.seg - 1) / s.seg : 1;
+    if (part >= parts) return {0, 0, true, false, false};
+    const int at = part * s.seg;
+    return {w.start + at, min(s.seg, len - at), false, false, back ? part == 0 : part == parts - 1};
+}
+
+}  // namespace mkda

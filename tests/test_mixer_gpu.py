@@ -1,0 +1,564 @@
+"""GPU: the linear attention with a decay for each head, the rotary positions and the layer norm against their definitions in 64 bits.
+
+Tolerances are those of test_block_gpu.py (``near``): results in 16 bits are rounded once, half a step relative to the value; the arithmetic in front of that, and results in 32
+bits, stay below 2^-17 of the 2-norm.  For the linear attention that is: products of 16-bit inputs are exact, and sums of up to 128 of them in 32 bits; pair weights and states
+that meet another product as two 16-bit halves are off by at most 2^-16 each of the value, 2^-17.2 in the root mean square of one (uniformly distributed) and less in a sum's 2-norm
+relative to its own; what goes into the state has three parts, 2^-24.  Rotary: an angle is off by 2 pi 2^-26 = 2^-23.3 at most, a sine by 2^-22."""
+import math
+
+import pytest
+import torch
+
+import mogankda_b200 as mk
+from tests.test_block_gpu import ARITHMETIC, DTYPES, differentiate, near, rand, spans
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- linear attention ------------------------------------------------------------------------------------------------------------------------
+def linear_reference(q, k, v, d, scale, h0=None, cu=None, last=False):
+    """Token by token."""
+    B, T, HK, K = q.shape
+    H, V = v.shape[2:]
+    lam = torch.exp(d)[:, None, None]
+    rows, ends = {}, []
+    q, k = q.repeat_interleave(H // HK, 2), k.repeat_interleave(H // HK, 2)
+    for i, (b, p, e) in enumerate(spans(B, T, cu)):
+        s = h0[i] if h0 is not None else v.new_zeros(H, K, V)
+        for t in range(p, e):
+            s = lam * s + k[b, t][:, :, None] * v[b, t][:, None]
+            rows[b, t] = scale * (q[b, t][:, :, None] * s).sum(1)
+        ends.append(s)
+    zero = v.new_zeros(H, V)
+    o = torch.stack([torch.stack([rows.get((b, t), zero) for t in range(T)]) if T else v.new_zeros(0, H, V) for b in range(B)])
+    return o, (torch.stack(ends) if ends else v.new_zeros(0, H, K, V)) if last else None
+
+
+LINEAR = [  # B, T, HK, HV, K, V, cu
+    (1, 1, 1, 1, 8, 8, None), (2, 3, 1, 2, 16, 16, None), (1, 33, 2, 2, 128, 128, None), (1, 130, 2, 4, 64, 128, None), (2, 257, 1, 1, 128, 64, None), (1, 100, 3, 3, 40, 24, None),
+    (1, 50, 1, 3, 1, 5, None), (1, 77, 2, 2, 17, 33, None), (1, 128, 1, 1, 128, 128, None), (1, 129, 1, 2, 128, 128, None), (3, 64, 2, 2, 32, 128, None),
+    (1, 100, 1, 2, 64, 64, (0, 1, 3, 3, 20, 100)), (1, 60, 2, 2, 128, 128, (0, 0, 16, 48, 50)), (1, 300, 1, 1, 128, 128, (0, 128, 256, 257, 299)), (1, 5, 1, 2, 16, 16, (0,)),
+    (1, 9, 2, 2, 128, 72, (0, 0, 0, 9, 9)),
+    # long sequences of few heads: cut into parts that run side by side
+    (1, 1300, 1, 1, 64, 64, None), (2, 700, 1, 2, 32, 64, None), (1, 1024, 1, 1, 128, 128, None), (1, 1500, 1, 1, 40, 128, (0, 3, 3, 1400, 1410, 1450)), (1, 900, 1, 1, 24, 24, (0, 257, 899)),
+]
+
+
+def linear_leaves(gen, shape, dtype, full):
+    B, T, HK, H, K, V, cu = shape
+    n = B if cu is None else len(cu) - 1
+    lv = dict(q=rand(gen, B, T, HK, K).to(dtype), k=rand(gen, B, T, HK, K).to(dtype), v=rand(gen, B, T, H, V).to(dtype))
+    if full:
+        lv["h0"] = rand(gen, n, H, K, V)
+    d = -torch.exp(-6 * torch.rand(H, generator=gen))      # memories of 1 to 400 tokens
+    return lv, d, [rand(gen, B, T, H, V).to(dtype), rand(gen, n, H, K, V)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", LINEAR, ids=str)
+@pytest.mark.parametrize("full", [False, True], ids=["plain", "all"])
+def test_linear(shape, dtype, full):
+    cu = shape[-1]
+    gen = torch.Generator().manual_seed(sum(shape[:-1]))
+    lv, d, ups = linear_leaves(gen, shape, dtype, full)
+    scale = 0.3 if full else None
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+    cu_t = None if cu is None else torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+    def call():
+        return mk.linear_attention(mine["q"], mine["k"], mine["v"], d.cuda(), scale=scale, initial_state=mine.get("h0"), output_final_state=full, cu_seqlens=cu_t)
+
+    outs, grads = differentiate(call, mine, [u.cuda() for u in ups], list(lv))
+    routs, rgrads = differentiate(lambda: linear_reference(wide["q"], wide["k"], wide["v"], d.double(), scale or shape[4] ** -0.5, wide.get("h0"), cu, full), wide,
+                                  [u.double() for u in ups], list(lv))
+    for n, a, b in zip((["o", "last"] if full else ["o"]) + ["d" + n for n in lv], outs + grads, routs + rgrads):
+        near(n, a.cpu(), b)
+    with torch.no_grad():          # the same without a backward pass, and twice the same
+        again = call()
+    assert torch.equal(again[0], outs[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_gradients_against_differences(dtype):
+    """The results are linear in each of q, k, v and the state: a difference of two calls is the derivative, to the rounding of the results (half a step each, and the inputs' own where
+    they are moved: steps of the size of the values, by powers of two of a random sign, are exact)."""
+    gen = torch.Generator().manual_seed(3)
+    lv, d, ups = linear_leaves(gen, (1, 200, 1, 2, 64, 64, None), dtype, True)
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    ups = [u.cuda() for u in ups]
+
+    def call(x):
+        return mk.linear_attention(x["q"], x["k"], x["v"], d.cuda(), initial_state=x["h0"], output_final_state=True)
+
+    grads = dict(zip(lv, torch.autograd.grad(call(mine), list(mine.values()), ups)))
+    for n in lv:
+        way = torch.where(torch.rand(lv[n].shape, generator=gen) < 0.5, -1.0, 1.0).cuda().to(lv[n].dtype)
+        with torch.no_grad():
+            moved = [call(dict(mine, **{n: w})) for w in (way, torch.zeros_like(way))]
+        diff = sum(((a.double() - b.double()) * u.double()).sum() for a, b, u in zip(*moved, ups)).item()
+        told = (grads[n].double() * way.double()).sum().item()
+        eps = ARITHMETIC + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+        size = sum((torch.cat([a.double().flatten(), b.double().flatten()]).norm() * u.double().abs().max()).item() for a, b, u in zip(*moved, ups)) + grads[n].double().norm().item()
+        # errors of random signs add up as their squares do: three (a sum's root mean square, four times over) times the rounding of all that is summed
+        assert abs(diff - told) <= 4 * eps * size, (n, diff, told)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 40, 2, 2, 128, 128), (2, 24, 1, 3, 17, 33), (5, 30, 2, 4, 64, 128)], ids=str)
+def test_linear_steps_continue_a_prompt(dtype, shape):
+    gen = torch.Generator().manual_seed(4)
+    lv, d, _ = linear_leaves(gen, (*shape, None), dtype, True)
+    lv, d, T = {n: t.cuda() for n, t in lv.items()}, d.cuda(), shape[1]
+    with torch.no_grad():
+        whole, end = mk.linear_attention(lv["q"], lv["k"], lv["v"], d, initial_state=lv["h0"], output_final_state=True)
+        cut = T - 7
+        o, state = mk.linear_attention(lv["q"][:, :cut], lv["k"][:, :cut], lv["v"][:, :cut], d, initial_state=lv["h0"], output_final_state=True)
+        parts = [o]
+        for t in range(cut, T):
+            before = state._version
+            parts.append(mk.linear_attention_step(lv["q"][:, t], lv["k"][:, t], lv["v"][:, t], d, state)[:, None])
+            assert state._version == before + 1
+    # both sides are rounded
+    step = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    got = torch.cat(parts, 1).double()
+    assert (got - whole.double()).norm() <= 2 * (ARITHMETIC + step) * whole.double().norm()
+    near("state", state, end.double())
+
+
+def test_linear_of_any_decay():
+    """No decay at all, hardly any, strong ones whose powers underflow, and one that leaves nothing."""
+    gen = torch.Generator().manual_seed(5)
+    for dtype in DTYPES:
+        shape = (1, 300, 3, 6, 64, 64, None)
+        lv, _, ups = linear_leaves(gen, shape, dtype, True)
+        d = torch.tensor([0.0, -1e-6, -1.0, -20.0, -1000.0, -math.inf])
+        mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+        wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+        outs, grads = differentiate(lambda: mk.linear_attention(mine["q"], mine["k"], mine["v"], d.cuda(), initial_state=mine["h0"], output_final_state=True), mine, [u.cuda() for u in ups], list(lv))
+        routs, rgrads = differentiate(lambda: linear_reference(wide["q"], wide["k"], wide["v"], d.double(), 64 ** -0.5, wide["h0"], None, True), wide, [u.double() for u in ups], list(lv))
+        for n, a, b in zip(["o", "last"] + ["d" + n for n in lv], outs + grads, routs + rgrads):
+            near(n, a.cpu(), b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_reads_slices_of_a_projection(dtype):
+    gen = torch.Generator().manual_seed(6)
+    B, T, HK, H, D = 2, 140, 2, 4, 64
+    wide = rand(gen, B, T, (2 * HK + H) * D + 8).to(dtype).cuda()
+    ups = rand(gen, B, T, H, D).to(dtype).cuda()
+    d = -torch.rand(H, generator=gen).cuda()
+
+    def call(w, copy):
+        q, k, v = w[..., :HK * D], w[..., HK * D:2 * HK * D], w[..., 2 * HK * D:(2 * HK + H) * D]
+        q, k, v = (x.unflatten(-1, (-1, D)) for x in (q, k, v))
+        if copy:
+            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        return mk.linear_attention(q, k, v, d)[0]
+
+    got = []
+    for w, copy in ((wide, False), (wide, True), (torch.cat([wide[..., :1], wide], -1)[..., 1:], False)):      # and from an odd address
+        w = w.detach().requires_grad_(True) if w.is_contiguous() else w
+        leaf = w if w.requires_grad else w.requires_grad_(True)
+        o = call(leaf, copy)
+        got.append((o, *torch.autograd.grad(o, leaf, ups)))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+def test_linear_of_broadcast_inputs():
+    """Heads and tokens that are one in memory."""
+    gen = torch.Generator().manual_seed(7)
+    q, k, v = (rand(gen, 1, 90, 1, 32).cuda().requires_grad_(True) for _ in range(3))
+    d = -torch.rand(3, generator=gen).cuda()
+    up = rand(gen, 1, 90, 3, 32).cuda()
+    a = torch.autograd.grad(mk.linear_attention(q.expand(1, 90, 3, 32), k.expand(1, 90, 3, 32), v.expand(1, 90, 3, 32), d)[0], (q, k, v), up)
+    b = torch.autograd.grad(mk.linear_attention(q, k, v.expand(1, 90, 3, 32).contiguous(), d)[0], (q, k, v), up)
+    for x, y in zip(a, b):
+        near("gradient", x, y.double())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_leaves_tokens_of_no_sequence_alone(dtype):
+    """Behind the last boundary nothing is read and results are zero; what is not finite stays in its sequence."""
+    gen = torch.Generator().manual_seed(8)
+    lv, d, ups = linear_leaves(gen, (1, 400, 1, 2, 128, 128, None), dtype, False)
+    cu = torch.tensor([0, 70, 200, 290], dtype=torch.int32).cuda()
+    got = []
+    for bad in (0.0, math.nan, math.inf):
+        x = {n: t.clone() for n, t in lv.items()}
+        up = ups[0].clone()
+        for t in (*x.values(), up):
+            t[:, 290:] = bad
+            if bad != 0:
+                t[:, 70:200] = bad                         # a sequence in the middle, too
+        x = {n: t.cuda().requires_grad_(True) for n, t in x.items()}
+        o, last = mk.linear_attention(x["q"], x["k"], x["v"], d.cuda(), cu_seqlens=cu, output_final_state=True)
+        g = torch.autograd.grad((o, last), list(x.values()), (up.cuda(), torch.ones_like(last)))
+        got.append([t[:, s] for t in (o, *g) for s in (slice(0, 70), slice(200, 400))] + [last[0], last[2]])
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    assert all(torch.isfinite(t).all() for t in got[0]) and got[0][1][:, 90:].abs().max() == 0
+
+
+def test_linear_does_not_depend_on_its_neighbours():
+    """The same sequence in a batch, packed and by itself (short sequences: none of the calls is cut)."""
+    gen = torch.Generator().manual_seed(9)
+    lv, d, _ = linear_leaves(gen, (4, 200, 2, 2, 128, 128, None), torch.bfloat16, False)
+    lv, d = {n: t.cuda() for n, t in lv.items()}, d.cuda()
+    with torch.no_grad():
+        batch, last = mk.linear_attention(*lv.values(), d, output_final_state=True)
+        packed, plast = mk.linear_attention(*(t.reshape(1, -1, *t.shape[2:]) for t in lv.values()), d, output_final_state=True, cu_seqlens=torch.arange(5, dtype=torch.int32).cuda() * 200)
+        for i in range(4):
+            one, olast = mk.linear_attention(*(t[i:i + 1] for t in lv.values()), d, output_final_state=True)
+            assert torch.equal(one[0], batch[i]) and torch.equal(olast[0], last[i]) and torch.equal(packed[0, 200 * i:200 * i + 200], batch[i]) and torch.equal(plast[i], last[i])
+
+
+def test_linear_refuses():
+    q, v, d = torch.randn(1, 5, 2, 16).cuda(), torch.randn(1, 5, 4, 16).cuda(), -torch.rand(4).cuda()
+    for bad in (lambda: mk.linear_attention(q, q, v[:, :, :3], d[:3]), lambda: mk.linear_attention(q, q.bfloat16(), v, d), lambda: mk.linear_attention(q, q[..., :8], v, d),
+                lambda: mk.linear_attention(q, q, v, d[:2]), lambda: mk.linear_attention(q, q, v[:, :4], d), lambda: mk.linear_attention(q.double(), q.double(), v.double(), d),
+                lambda: mk.linear_attention(q, q, v, d, initial_state=torch.zeros(1, 4, 16, 16).cuda().bfloat16()), lambda: mk.linear_attention(q, q, v, d, initial_state=torch.zeros(1, 4, 16, 8).cuda()),
+                lambda: mk.linear_attention(torch.randn(1, 5, 2, 129).cuda(), torch.randn(1, 5, 2, 129).cuda(), v, d), lambda: mk.linear_attention_step(q[0], q[0], v[0], d, torch.zeros(5, 4, 16, 8).cuda()),
+                lambda: mk.linear_attention_step(q[0], q[0], v[0], d, torch.zeros(5, 4, 16, 16).cuda().transpose(2, 3))):
+        with pytest.raises(AssertionError):
+            bad()
+    with pytest.raises(ValueError):
+        mk.linear_attention(q, q, v, d, initial_state=torch.zeros(2, 4, 16, 16).cuda())
+    with pytest.raises(ValueError):
+        mk.linear_attention(q.expand(2, 5, 2, 16), q.expand(2, 5, 2, 16), v.expand(2, 5, 4, 16), d, cu_seqlens=torch.tensor([0, 5]).cuda())
+    with pytest.raises(RuntimeError, match="log_decay"):
+        mk.linear_attention(q, q, v, d.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="no_grad"):
+        mk.linear_attention_step(q[0], q[0], v[0].requires_grad_(True), d, torch.zeros(5, 4, 16, 16).cuda())
+    x = torch.randn(1, 5, 2, 16).cuda().requires_grad_(True)
+    o, _ = mk.linear_attention(x, x, v.detach(), d)
+    (g,) = torch.autograd.grad(o.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="double backward"):
+        g.sum().backward()
+
+
+def test_linear_past_32_bits():
+    """More than 2^31 elements in each tensor: the last heads of the last tokens against a call of their own."""
+    T, H, D = 135000, 128, 128
+    assert T * H * D > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(1, T, H, D, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    d = torch.full((H,), -0.5, device="cuda")              # a thousand tokens are all that it remembers
+    with torch.no_grad():
+        o, last = mk.linear_attention(q, k, v, d, output_final_state=True)
+        part, plast = mk.linear_attention(*(t[:, -2000:, -2:].contiguous() for t in (q, k, v)), d[-2:], output_final_state=True)
+    near("o", o[:, -1000:, -2:].float(), part[:, -1000:].double(), terms=torch.finfo(torch.bfloat16).eps / ARITHMETIC * part[:, -1000:].double().norm().item())
+    near("last", last[:, -2:], plast.double())
+
+
+# ---- rotary positions ------------------------------------------------------------------------------------------------------------------------
+def rotary_reference(x, angle, interleaved):
+    n = angle.shape[-1]
+    z = x[..., :2 * n]
+    a, b = (z[..., 0::2], z[..., 1::2]) if interleaved else (z[..., :n], z[..., n:])
+    c, s = torch.cos(angle)[..., None, :], torch.sin(angle)[..., None, :]
+    a, b = a * c - b * s, a * s + b * c
+    return torch.cat([torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1), x[..., 2 * n:]], -1)
+
+
+ROTARY = [  # lead, HQ, HK, D, F, axes
+    ((1, 1), 1, 1, 2, 1, 0), ((3,), 4, 0, 128, 64, 0), ((2, 37), 5, 2, 64, 32, 3), ((1, 100), 3, 1, 96, 24, 2), ((2, 3, 7), 2, 2, 50, 25, 3), ((9,), 1, 1, 7, 2, 0), ((40,), 40, 8, 128, 64, 3),
+    ((5,), 2, 1, 512, 256, 4), ((4,), 3, 1, 16, 0, 0), ((0, 5), 2, 1, 16, 8, 0), ((), 2, 1, 16, 8, 0), ((1, 4000), 2, 1, 24, 8, 0), ((33,), 2, 3, 72, 35, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", ROTARY, ids=str)
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "neighbours"])
+def test_rotary(shape, dtype, interleaved):
+    lead, HQ, HK, D, F, axes = shape
+    gen = torch.Generator().manual_seed(D + F)
+    lv = dict(q=rand(gen, *lead, HQ, D).to(dtype))
+    if HK:
+        lv["k"] = rand(gen, *lead, HK, D).to(dtype)
+    freq = (10000.0 ** (-torch.arange(F) / max(F, 1))).float()
+    most = 2 ** 31 - 1 if D % 4 else 100000                # far positions: 64-bit angles of 2^31 turns are exact to 2^-21
+    pos = torch.randint(-5, most, ((axes, *lead) if axes else lead), generator=gen, dtype=torch.int64)
+    pos = pos.to(torch.int32) if D % 3 else pos
+    of = [int(i) for i in torch.randint(0, axes, (F,), generator=gen)] if axes else None
+    at = pos[of] if axes else pos[None].expand(F, *lead)
+    angle = at.double().movedim(0, -1) * freq.double()
+    ups = [rand(gen, *t.shape).to(dtype) for t in lv.values()]
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+
+    def call():
+        got = mk.rotary(mine["q"], mine.get("k"), pos.cuda(), freq.cuda(), axes=of, interleaved=interleaved)
+        return got if HK else (got,)
+
+    outs, grads = differentiate(call, mine, [u.cuda() for u in ups], list(lv))
+    routs, rgrads = differentiate(lambda: [rotary_reference(t, angle, interleaved) for t in wide.values()], wide, [u.double() for u in ups], list(lv))
+    for n, a, b in zip([n for n in lv] + ["d" + n for n in lv], outs + grads, routs + rgrads):
+        near(n, a.cpu(), b)
+        if F == 0:
+            assert torch.equal(a.cpu().double(), b)
+
+
+def test_rotary_of_slices_and_one_gradient():
+    gen = torch.Generator().manual_seed(2)
+    w = rand(gen, 2, 30, 6 * 64 + 8).cuda().bfloat16().requires_grad_(True)
+    pos, freq = torch.arange(30).expand(2, 30).cuda(), torch.rand(32, generator=gen).cuda()
+    up = rand(gen, 2, 30, 4, 64).cuda().bfloat16()
+    got = []
+    for copy in (False, True):
+        q, k = w[..., :256].unflatten(-1, (4, 64)), w[..., 256:384].unflatten(-1, (2, 64))
+        if copy:
+            q, k = q.contiguous(), k.contiguous()
+        a, b = mk.rotary(q, k, pos, freq)
+        got.append((a, b, *torch.autograd.grad(a, w, up)))           # nothing comes back through k
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and got[0][2][..., 256:].abs().max() == 0
+    with torch.no_grad():                                             # halves of a head turned in place of their order
+        odd = mk.rotary(torch.cat([w[..., :1], w], -1)[..., 1:257].unflatten(-1, (4, 64)), None, pos, freq)
+    assert torch.equal(odd, got[0][0])
+
+
+def test_rotary_refuses():
+    q, pos, freq = torch.randn(2, 5, 4, 16).cuda(), torch.zeros(2, 5, dtype=torch.long).cuda(), torch.ones(8).cuda()
+    for bad in (lambda: mk.rotary(q, q.bfloat16(), pos, freq), lambda: mk.rotary(q, None, pos.float(), freq), lambda: mk.rotary(q, None, pos[:, :4], freq), lambda: mk.rotary(q, None, pos, freq.double()),
+                lambda: mk.rotary(q, None, pos, torch.ones(9).cuda()), lambda: mk.rotary(q, None, pos, freq, axes=[0] * 8), lambda: mk.rotary(q, None, pos[None], freq),
+                lambda: mk.rotary(q, None, pos[None], freq, axes=[0] * 7), lambda: mk.rotary(q, None, pos[None], freq, axes=[0] * 7 + [1]), lambda: mk.rotary(q, None, pos[None], freq, axes=[-1] * 8),
+                lambda: mk.rotary(q, q[:1], pos, freq), lambda: mk.rotary(torch.randn(2, 5, 1, 514).cuda(), None, pos, freq)):
+        with pytest.raises(AssertionError):
+            bad()
+    with pytest.raises(TypeError):
+        mk.rotary(q, None, pos[None], freq, axes=[0.5] * 8)
+    with pytest.raises(RuntimeError, match="inv_freq"):
+        mk.rotary(q, None, pos, freq.clone().requires_grad_(True))
+
+
+def test_rotary_gradients_are_linear():
+    """A gradient of q is no function of q: a penalty on it has nothing to come back through, one on the incoming gradient raises."""
+    q, pos, freq = torch.randn(5, 4, 16).cuda().requires_grad_(True), torch.arange(5).cuda(), torch.ones(8).cuda()
+    (g,) = torch.autograd.grad(mk.rotary(q, None, pos, freq).sum(), q, create_graph=True)
+    assert not g.requires_grad
+    (g,) = torch.autograd.grad(mk.rotary(q, None, pos, freq).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="double backward"):
+        g.sum().backward()
+
+
+def test_rotary_past_32_bits():
+    T, H, D = 70000, 256, 128
+    q = torch.zeros(T, H, D, dtype=torch.bfloat16, device="cuda")
+    q[-3:] = torch.randn(3, H, D, device="cuda").bfloat16()
+    pos, freq = torch.arange(T).cuda(), torch.rand(64).cuda()
+    assert q.numel() > 2 ** 31
+    with torch.no_grad():
+        assert torch.equal(mk.rotary(q, None, pos, freq)[-3:], mk.rotary(q[-3:].clone(), None, pos[-3:], freq))
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------------------------------------------
+def layer_norm_reference(x, w, b, res, groups, held):
+    s = x
+    if res is not None:
+        s = x + res
+        s = s + (s.detach().to(held).double() - s.detach())      # rounded; its derivative is one
+    g = s.unflatten(-1, (groups, -1))
+    d = g - g.mean(-1, keepdim=True)
+    y = (d / torch.sqrt(d.square().mean(-1, keepdim=True) + 1e-5)).flatten(-2)
+    y = y * w if w is not None else y
+    return (y + b if b is not None else y), s if res is not None else None
+
+
+NORM = [  # lead, width, groups
+    ((1,), 1, 1), ((3,), 8, 1), ((2, 5), 33, 1), ((7,), 256, 1), ((4,), 257, 1), ((5,), 1000, 1), ((3,), 1025, 1), ((2,), 2048, 1), ((3,), 2056, 1), ((2,), 4096, 1), ((2,), 8192, 1),
+    ((2,), 8200, 1), ((2,), 20000, 1), ((1,), 32768, 1), ((0,), 64, 1), ((), 64, 1), ((700,), 64, 1), ((9,), 1024, 8), ((3,), 35, 5), ((5,), 4096, 4), ((2, 3), 66, 33), ((1500,), 256, 2), ((2,), 65536, 2),
+    ((2,), 2100, 2), ((600,), 520, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", NORM, ids=str)
+@pytest.mark.parametrize("option", ["plain", "all", "wide", "bias"])
+def test_layer_norm(shape, dtype, option):
+    lead, W, groups = shape
+    gen = torch.Generator().manual_seed(W + groups)
+    x = rand(gen, *lead, W) + 0.5
+    lv = dict(x=x.to(dtype))
+    held = torch.float32 if option == "wide" else dtype
+    if option in ("all", "wide"):
+        lv.update(w=1 + 0.1 * rand(gen, W).to(torch.bfloat16 if option == "wide" else torch.float32), b=rand(gen, W), res=(2 * rand(gen, *lead, W)).to(held))
+    elif option == "bias":
+        lv.update(b=rand(gen, W).to(dtype))
+    ups = [rand(gen, *lead, W).to(dtype), rand(gen, *lead, W).to(held)]
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+
+    def call():
+        got = mk.layer_norm(mine["x"], mine.get("w"), mine.get("b"), residual=mine.get("res"), groups=groups)
+        return got if "res" in lv else (got,)
+
+    outs, grads = differentiate(call, mine, [u.cuda() for u in ups], list(lv))
+    routs, rgrads = differentiate(lambda: layer_norm_reference(wide["x"], wide.get("w"), wide.get("b"), wide.get("res"), groups, held), wide, [u.double() for u in ups], list(lv))
+    ups0 = ups[0].double().norm().item()
+    for n, a, b in zip((["y", "s"] if "res" in lv else ["y"]) + ["d" + n for n in lv], outs + grads, routs + rgrads):
+        # few channels to a part: what is left of the incoming gradient may be little of it; times at most 1 / sqrt(var + eps), of the smallest of the parts
+        terms = 0.0
+        if n in ("dx", "dres") and a.numel():
+            s = (wide["x"] + (wide["res"] if "res" in lv else 0)).detach().unflatten(-1, (groups, -1))
+            terms = ups0 * (s.var(-1, correction=0).min().item() + 1e-5) ** -0.5
+        near(n, a.cpu(), b, terms)
+
+
+def test_layer_norm_of_far_means_and_outliers():
+    """A mean a thousand times the deviation, and one channel a thousand times the others: sums of differences to the mean in 32 bits.  The inputs are what 32 bits hold; the
+    difference to the mean loses 2^-24 of the mean, 2^-14 of the deviation."""
+    gen = torch.Generator().manual_seed(1)
+    x = rand(gen, 6, 4096)
+    x[:3] += 1000.0
+    x[3:, 7] = 1000.0
+    y = mk.layer_norm(x.cuda()).cpu().double()
+    ref, _ = layer_norm_reference(x.double(), None, None, None, 1, None)
+    assert (y - ref).abs().max() <= 2.0 ** -14 * (1 + ref[:3].abs().max()) and (y - ref)[3:].norm() <= ARITHMETIC * ref[3:].norm()
+
+
+def test_layer_norm_of_what_is_not_finite():
+    """Stays in its row, or its part of one."""
+    x = torch.randn(5, 64).cuda()
+    clean = mk.layer_norm(x, groups=4)
+    x[2, 20], x[3, 0] = math.inf, math.nan
+    y = mk.layer_norm(x, groups=4)
+    assert torch.isnan(y[2, 16:32]).all() and torch.isnan(y[3, :16]).all()
+    y[2, 16:32], y[3, :16] = clean[2, 16:32], clean[3, :16]
+    assert torch.equal(y, clean)
+
+
+def test_layer_norm_reads_slices():
+    gen = torch.Generator().manual_seed(3)
+    wide = rand(gen, 40, 3 * 264 + 8).cuda().bfloat16()
+    w, b = rand(gen, 264).cuda(), rand(gen, 264).cuda()
+    for start in (0, 8, 264, 3):
+        x = wide[:, start:start + 264]
+        leaf = x.detach().clone().requires_grad_(True)
+        up = rand(gen, 40, 264).cuda().bfloat16()
+        y = mk.layer_norm(leaf, w, b, groups=3)
+        (want,) = torch.autograd.grad(y, leaf, up)
+        whole = wide.clone().requires_grad_(True)
+        z = mk.layer_norm(whole[:, start:start + 264], w, b, groups=3)
+        (got,) = torch.autograd.grad(z, whole, up)
+        assert torch.equal(y, z) and torch.equal(got[:, start:start + 264], want)
+
+
+def test_layer_norm_refuses():
+    x = torch.randn(4, 64).cuda()
+    for bad in (lambda: mk.layer_norm(x, torch.ones(63).cuda()), lambda: mk.layer_norm(x, None, torch.ones(1, 64).cuda()), lambda: mk.layer_norm(x, groups=3), lambda: mk.layer_norm(x, groups=0),
+                lambda: mk.layer_norm(x, residual=x[:2]), lambda: mk.layer_norm(x, residual=x.bfloat16()), lambda: mk.layer_norm(x.double()), lambda: mk.layer_norm(torch.randn(2, 32769).cuda())):
+        with pytest.raises(AssertionError):
+            bad()
+    leaf = torch.randn(4, 64).cuda().requires_grad_(True)
+    (g,) = torch.autograd.grad(mk.layer_norm(leaf).square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="double backward"):
+        g.sum().backward()
+
+
+def test_layer_norm_past_32_bits():
+    x = torch.zeros(70000, 32768, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, 32768, device="cuda").bfloat16()
+    assert x.numel() > 2 ** 31
+    with torch.no_grad():
+        for groups in (1, 256):
+            assert torch.equal(mk.layer_norm(x, groups=groups)[-3:], mk.layer_norm(x[-3:].clone(), groups=groups))
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------------------------
+def mixer(mine, x, w, pos, freq, d, nw, cu, reference=False):
+    """A token mixer of heads with decays: projections, rotary positions, the linear attention, the norm of each head, and the residual's norm behind it."""
+    H, D = 4, 64
+    q, k, v = (x @ w).unflatten(-1, (3 * H, D)).split(H, -2)
+    if reference:
+        angle = pos[..., None].double() * freq.double()
+        q, k = (rotary_reference(t, angle, False) for t in (q, k))
+        o, _ = linear_reference(q, k, v, d.double(), D ** -0.5, None, cu)
+        y, _ = layer_norm_reference(o.flatten(-2), nw, None, None, H, None)
+        return layer_norm_reference(y, None, None, x, 1, torch.float64)
+    q, k = mine.rotary(q, k, pos, freq)
+    o, _ = mine.linear_attention(q, k, v, d, cu_seqlens=cu)
+    y = mine.layer_norm(o.flatten(-2), nw, groups=H)
+    return mine.layer_norm(y, residual=x)
+
+
+def mixer_inputs(gen):
+    x, w, nw = rand(gen, 1, 150, 256), rand(gen, 256, 3 * 256) / 16, 1 + 0.1 * rand(gen, 256)
+    pos, freq, d = torch.cat([torch.arange(60), torch.arange(90)])[None], (100.0 ** (-torch.arange(32) / 32)).float(), -torch.rand(4, generator=gen)
+    return x, w, nw, pos, freq, d, [rand(gen, 1, 150, 256) for _ in range(2)]
+
+
+def test_a_block_of_them():
+    """fp32, forward and backward; four operators in a row, each within 2^-17 of its input's error, and the products in front of them in 32 bits: within 2^-14."""
+    gen = torch.Generator().manual_seed(11)
+    x, w, nw, pos, freq, d, ups = mixer_inputs(gen)
+    cu = (0, 60, 150)
+    mine = {n: t.cuda().requires_grad_(True) for n, t in dict(x=x, w=w, nw=nw).items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in dict(x=x, w=w, nw=nw).items()}
+    outs = mixer(mk, mine["x"], mine["w"], pos.cuda(), freq.cuda(), d.cuda(), mine["nw"], torch.tensor(cu, dtype=torch.int32).cuda())
+    routs = mixer(mk, wide["x"], wide["w"], pos, freq, d, wide["nw"], cu, True)
+    grads = torch.autograd.grad(outs, list(mine.values()), [u.cuda() for u in ups])
+    rgrads = torch.autograd.grad(routs, list(wide.values()), [u.double() for u in ups])
+    for a, b in zip((*outs, *grads), (*routs, *rgrads)):
+        assert (a.cpu().double() - b).norm() <= 2.0 ** -14 * b.norm()
+
+
+def test_a_block_of_them_in_a_graph_on_another_stream():
+    """Captured and replayed on new inputs, twice over (two graphs), beside calls on another stream."""
+    gen = torch.Generator().manual_seed(12)
+    x, w, nw, pos, freq, d, ups = [t.cuda() if torch.is_tensor(t) else [u.cuda() for u in t] for t in mixer_inputs(gen)]
+    cu = torch.tensor((0, 60, 150), dtype=torch.int32).cuda()
+
+    def step(leaf):
+        outs = mixer(mk, leaf, w, pos, freq, d, nw, cu)
+        return (*outs, *torch.autograd.grad(outs, leaf, ups))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        step(x.clone().requires_grad_(True))
+        for _ in range(2):
+            static = x.clone().requires_grad_(True)
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs = step(static)
+            graphs.append((graph, static, outs))
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(3):
+        for j, (graph, static, _) in enumerate(graphs):
+            with torch.no_grad():
+                static.copy_(torch.roll(x, i + j, 1))
+            graph.replay()
+        with torch.cuda.stream(side):
+            other = step(torch.roll(x, 7, 1).requires_grad_(True))
+        for j, (_, _, outs) in enumerate(graphs):
+            want = step(torch.roll(x, i + j, 1).requires_grad_(True))
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    torch.cuda.synchronize()
+    assert all(torch.isfinite(t).all() for t in other)
+
+
+def test_single_tokens_in_a_graph():
+    gen = torch.Generator().manual_seed(13)
+    N, H, D = 3, 2, 128
+    q, k, v = (rand(gen, N, H, D).cuda().bfloat16() for _ in range(3))
+    d, pos, freq, state = -torch.rand(H, generator=gen).cuda(), torch.zeros(N, dtype=torch.int32).cuda(), torch.rand(64, generator=gen).cuda(), torch.zeros(N, H, D, D).cuda()
+    keep = state.clone()
+
+    def step(s):
+        a, b = mk.rotary(q, k, pos, freq)
+        return mk.layer_norm(mk.linear_attention_step(a, b, v, d, s).flatten(-2), groups=H)
+
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        step(keep.clone())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y = step(state)
+        for t in range(4):
+            pos.fill_(t)
+            graph.replay()
+            want = step(keep)
+            assert torch.equal(y, want) and torch.equal(state, keep)
