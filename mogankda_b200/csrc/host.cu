@@ -42,10 +42,9 @@ int sm_count() {
     return cached[dev];
 }
 
-int make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, unsigned long long rows, unsigned long long row_elems, const char* what,
-                  int box_rows, int box_cols) {
-    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                           const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static Encode encoder(const char* what) {
     static std::atomic<Encode> resolved{nullptr};      // through the runtime: the library does not link against the driver
     Encode encode = resolved.load(std::memory_order_relaxed);
     if (!encode) {
@@ -54,11 +53,36 @@ int make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, unsigned l
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) {
             (void)cudaGetLastError();
             snprintf(g_err, sizeof(g_err), "%s: the driver does not provide cuTensorMapEncodeTiled", what);
-            return MKDA_ERR_LAUNCH;
+            return nullptr;
         }
         encode = reinterpret_cast<Encode>(fn);
         resolved.store(encode, std::memory_order_relaxed);
     }
+    return encode;
+}
+
+int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what) {
+    const Encode encode = encoder(what);
+    if (!encode) return MKDA_ERR_LAUNCH;
+    if ((reinterpret_cast<uintptr_t>(base) & 15) || dim % 8 || stride % 8 || stride < 0 || tokens == 0) {
+        snprintf(g_err, sizeof(g_err), "%s: tensor not 16-byte aligned for tiled copies", what);
+        return MKDA_ERR_ARG;
+    }
+    const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, tokens}, gstride[2] = {(cuuint64_t)dim * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(g_err, sizeof(g_err), "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+        return MKDA_ERR_LAUNCH;
+    }
+    return MKDA_OK;
+}
+
+int make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, unsigned long long rows, unsigned long long row_elems, const char* what,
+                  int box_rows, int box_cols) {
+    const Encode encode = encoder(what);
+    if (!encode) return MKDA_ERR_LAUNCH;
     const unsigned long long pitch = row_elems * (unsigned long long)elem_bytes;
     if ((reinterpret_cast<uintptr_t>(base) & 15) || (pitch & 15) || row_elems < 128 || rows == 0) {
         snprintf(g_err, sizeof(g_err), "%s: tensor not 16-byte aligned for tiled copies", what);
@@ -120,6 +144,7 @@ extern "C" int mkda_device_status(void) {
     if (mkda::tc_recur_status(&f) == 0) any |= f;
     if (mkda::tc_intra_status(&f) == 0) any |= f;
     if (mkda::tc_bwd_chunk_status(&f) == 0) any |= f;
+    if (mkda::linear_tc_status(&f) == 0) any |= f;
     return (int)any;
 }
 extern "C" int mkda_device_status_clear(void) {
@@ -130,6 +155,7 @@ extern "C" int mkda_device_status_clear(void) {
     rc |= mkda::tc_recur_status_clear();
     rc |= mkda::tc_intra_status_clear();
     rc |= mkda::tc_bwd_chunk_status_clear();
+    rc |= mkda::linear_tc_status_clear();
     return rc;
 }
 extern "C" const char* mkda_last_error(void) { return mkda::g_err; }

@@ -40,7 +40,7 @@ __device__ __forceinline__ void fma4(float (&d)[4], float a, const float4& b) {
 }  // namespace ls
 
 template <int DT>
-__global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const LinearCall call, const bool vec) {
+__global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_constant__ LinearCall call, const bool vec) {
     using namespace ls;
     follow_stream();
     extern __shared__ __align__(16) float smem_f[];
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const LinearCa
 // ---- cut sequences -------------------------------------------------------------------------------------------------------------------------------
 // A part finds what it makes of nothing and leaves it where the next part's entering state belongs; this adds what comes through from further away:
 //   parts[p] = (what part p - 1 makes of nothing) + lam^(tokens of part p - 1) parts[p - 1], parts[0] the sequence's initial state; backwards likewise.
-__global__ void __launch_bounds__(256) linear_parts_kernel(const LinearCall call) {
+__global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant__ LinearCall call) {
     follow_stream();
     const LinearKind& k = call.kind[blockIdx.z];
     const int h = blockIdx.x % call.HV, n = blockIdx.y;
@@ -294,7 +294,9 @@ __global__ void __launch_bounds__(256) linear_step_kernel(const MkdaLinearStep p
 static int run_linear(const LinearCall& call, const LinearCall& before, cudaStream_t stream) {
     const MkdaSeqs& S = call.S;
     if (S.N == 0) return MKDA_OK;
-    auto simt = [&](const LinearCall& c) {
+    const bool tc = linear_tc_takes(call) && linear_tc_takes(before);
+    auto run = [&](const LinearCall& c, bool states) {
+        if (tc) return launch_linear_tc(c, states, stream);
         int bytes = 0, rc = MKDA_OK;
         bool vec = true;
         for (int i = 0; i < c.kinds; ++i) {
@@ -310,7 +312,7 @@ static int run_linear(const LinearCall& call, const LinearCall& before, cudaStre
         return rc != MKDA_OK ? rc : check_launch("linear");
     };
     if (S.seg && S.segs > 1) {
-        int rc = simt(before);
+        int rc = run(before, true);
         if (rc != MKDA_OK) return rc;
     }
     if (S.seg) {
@@ -320,7 +322,7 @@ static int run_linear(const LinearCall& call, const LinearCall& before, cudaStre
         int rc = check_launch("linear parts");
         if (rc != MKDA_OK) return rc;
     }
-    return simt(call);
+    return run(call, false);
 }
 
 static const char* bad_linear(const MkdaLinearFwd& p) {

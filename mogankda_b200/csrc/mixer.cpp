@@ -28,7 +28,9 @@ struct LinearCall {
         p.S = q.s; p.HK = (int)t[LQ].size(-2); p.HV = (int)t[LV].size(-2); p.K = (int)t[LQ].size(-1); p.V = (int)t[LV].size(-1);
         p.dtype = dtype_code(t[LQ]); p.scale = (float)scale;
         auto rows = [&](int i, const void*& ptr, long long& stride) {
-            const Rows r = rows_of(t[i], 2);
+            Rows r = rows_of(t[i], 2);
+            // tiled copies want 16-byte boundaries: rows that start elsewhere are copied, so that results do not depend on where they lie
+            if (t[i].scalar_type() == at::kBFloat16 && (r.stride % 8 || reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16)) r = {aligned(r.t), t[i].size(-1) * t[i].size(-2)};
             ptr = cptr(r.t);
             stride = r.stride;
             hold.push_back(r.t);

@@ -1,0 +1,89 @@
+"""CPU: no wait of the linear attention's tensor-core kernel rests on timing (test_barrier_order.py has the method), and its roles cannot wait for one another in a ring.
+
+Parts of several lengths, one of them without tokens, go through a block one after the other; ``states`` is the kernel that finds what parts make of nothing."""
+import os
+import re
+
+import pytest
+
+from tests.test_barrier_order import CSRC, Roles
+
+PARTS = (3, 1, 0, 2, 1)      # stretches of 128 tokens in each
+
+
+def linear_kernel(states):
+    text = open(os.path.join(CSRC, "linear_tc.cu")).read()
+    ring = int(re.search(r"SLOTS = (\d+)", text)[1])
+    members = re.search(r"struct Shared \{(.*?)\n\};", text, re.S)[1]
+    found = {n: ring if d == "SLOTS" else int(d or 1) for line in re.findall(r"uint64_t ([^;]*);", members) for n, d in re.findall(r"(\w+)(?:\[(\w+)\])?", line)}
+    r = Roles(found)
+    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free"), 2))      # of the four warps two, one of which may be late
+    per, stretches = (2 if states else 3), [(p, t, c) for p, c in enumerate(PARTS) for t in range(c)]
+    load = r.agent("load")
+    for tile in range(per * len(stretches)):
+        if tile >= ring:
+            load[0]("empty", tile - ring)
+        load[1]("full", tile)
+    wait, arrive = r.agent("products")
+    for n in range(len(stretches)):
+        a, b, c = n * per, n * per + per - 2, n * per + per - 1
+        if not states:
+            wait("full", a)
+        wait("full", b)
+        if not states:
+            arrive("p0_done", n)
+            if n:
+                wait("o_free", n - 1)
+        wait("s_ready", n)
+        if not states:
+            arrive("in_done", n)
+            arrive("empty", a)
+        for q in range(4):
+            wait("f_ready", 4 * n + q)
+            arrive("f_free", 4 * n + q)
+        arrive("x_done", n)
+        arrive("empty", b)
+        if not states:
+            wait("p_ready", n)
+            wait("o_scaled", n)
+            wait("full", c)
+            arrive("o_done", n)
+        arrive("empty", c)
+    wait("empty", len(stretches) * per - 1)
+    for w in range(2):
+        if not states:
+            wait, arrive = r.agent(f"pairs {w}")
+            for n in range(len(stretches)):
+                wait("p0_done", n)
+                arrive("p_ready", n)
+            wait, arrive = r.agent(f"output {w}")
+            for n in range(len(stretches)):
+                wait("in_done", n)
+                arrive("o_scaled", n)
+                wait("o_done", n)
+                arrive("o_free", n)
+        wait, arrive = r.agent(f"factors {w}")
+        for n, (_, t, chunks) in enumerate(stretches):
+            wait("full", n * per + per - 1)
+            if t == chunks - 1:                        # a short stretch
+                wait("full", n * per + per - 2)
+            for q in range(4):
+                if 4 * n + q >= found["f_free"]:
+                    wait("f_free", 4 * n + q - found["f_free"])
+                arrive("f_ready", 4 * n + q)
+        wait, arrive = r.agent(f"state {w}")
+        n = 0
+        for chunks in PARTS:
+            for t in range(chunks):
+                if t:
+                    wait("x_done", n - 1)
+                arrive("s_ready", n)
+                n += 1
+            if chunks:
+                wait("x_done", n - 1)
+    return r
+
+
+@pytest.mark.parametrize("states", [False, True])
+def test_waits_of_the_linear_kernel(states):
+    assert not linear_kernel(states).late_waits()
