@@ -61,6 +61,17 @@ static Encode encoder(const char* what) {
     return encode;
 }
 
+// The driver's encoder wants a current context, which a thread that has called nothing of the runtime yet does not have (torch's backward threads, a new thread of the caller's)
+template <typename F>
+static CUresult with_context(F encode) {
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        (void)cudaFree(nullptr);
+        r = encode();
+    }
+    return r;
+}
+
 int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what) {
     const Encode encode = encoder(what);
     if (!encode) return MKDA_ERR_LAUNCH;
@@ -70,8 +81,10 @@ int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens
     }
     const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, tokens}, gstride[2] = {(cuuint64_t)dim * 2, (cuuint64_t)stride * 2};
     const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
-    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = with_context([&] {
+        return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (r != CUDA_SUCCESS) {
         snprintf(g_err, sizeof(g_err), "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
         return MKDA_ERR_LAUNCH;
@@ -91,10 +104,12 @@ int make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, unsigned l
     const cuuint64_t gdim[2] = {row_elems, rows};
     const cuuint64_t gstride[1] = {pitch};
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = encode(out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), gdim,
-                              gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = with_context([&] {
+        return encode(out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), gdim,
+                      gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (r != CUDA_SUCCESS) {
         snprintf(g_err, sizeof(g_err), "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
         return MKDA_ERR_LAUNCH;

@@ -5,14 +5,15 @@
 //   P0 = a b^T                       pairs; the weights lam^|i - j| and the mask are applied to the accumulator, and P leaves as bf16 hi + lo, the left operand of P c
 //   O  = a M                         M: the state in front of the stretch as hi + lo in shared memory; lam^(i + 1) is applied to the accumulator's rows
 //   O += P c
-//   M^T = lam^L M^T + (f c)^T b      f[j] = lam^(L - 1 - j); M^T stays in its accumulator, and f c is split in three parts, so that the state is an fp32 one
+//   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts, so that the state, fp32 in registers, is exact to 32 bits
 // a, b and c are exact in bf16.  Two halves (2^-16) are enough where the result is rounded to bf16, one would show: P and M in one bf16 each are as far off as the result's own rounding.
 //
 // Roles, joined by mbarriers: a warp that fetches rows into a ring of five tiles, one that issues products, and four warps each for the pairs' weights, for f c, for the state and
-// for the output.  Every accumulator row is a lane: token i of P0 and O, channel of c of M^T.
+// for the output.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
 //
 // Bound by HBM where there are enough parts: 128 KB per stretch, 3 us of an SM's share; products take 8 x 516 cycles = 2.2 us, and each group of warps less than that.
 #include <algorithm>
+#include <type_traits>
 
 #include "host.h"
 #include "linear.cuh"
@@ -25,15 +26,18 @@ using umma::mbar_wait;
 using umma::signal_tmem;
 using umma::wait_mma;
 
-constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 576, WARP_LOAD = 16, WARP_MMA = 17;
-constexpr int P = 0, O = 128, S = 256, F = 384;            // tensor-memory columns: pairs, output, state, f c (two buffers of a quarter: 3 x 16 columns each)
+constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 640, WARP_LOAD = 16, WARP_MMA = 17;
+constexpr int P = 0, O = 128, X = 256, F = 384;            // tensor-memory columns: pairs, output, what goes into the state, f c (two buffers of a quarter: 3 x 16 columns each)
+// Registers: the state's warps have 128 values of it a thread.  Their sum is the launch's.
+constexpr int LAUNCH_REGS = 96, WORK_REGS = 88, STATE_REGS = 160, ISSUE_REGS = 56;
+static_assert(3 * WORK_REGS + STATE_REGS + ISSUE_REGS <= 5 * LAUNCH_REGS, "registers of the launch");
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
     uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free;
     uint32_t tmem;
-    float power[C + 4];                                    // lam^n of the current part's head, one copy per group of warps that reads it
-    float power_p[C + 4], power_o[C + 4];
+    // of the current part's head, a copy for each group of warps that reads it: scale lam^n and lam^(31 - e) (backwards lam^e); f; lam^n times the scale
+    __align__(16) float pair[C], column[32], factor[C], row[C + 4];
 };
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
@@ -42,6 +46,7 @@ struct Maps { CUtensorMap row[4]; };                       // rows of a head, bo
 struct Plan {
     LinearCall call;
     int map_a[3], map_b[3], map_c[3];                      // per kind
+    int wide[3];                                           // rows of the output in pieces of 32 bytes
     long long items;
 };
 
@@ -76,19 +81,22 @@ __device__ __forceinline__ const float* entering(const LinearCall& call, const L
     if (call.S.seg) return k.parts + ((size_t)(it.n * call.S.segs + it.part) * call.HV + it.h) * size;
     return k.first ? k.first + ((size_t)it.n * call.HV + it.h) * size : nullptr;
 }
-// Powers of lam for one group of 128 threads, between its own barriers
-__device__ __forceinline__ void set_powers(float* to, float log_decay, int tid, int barrier) {
-    asm volatile("bar.sync %0, 128;" :: "r"(barrier) : "memory");
-    to[tid] = decay_power(log_decay, tid);
-    if (tid == 0) to[C] = decay_power(log_decay, C);
-    asm volatile("bar.sync %0, 128;" :: "r"(barrier) : "memory");
-}
+__device__ __forceinline__ void group_sync(int barrier) { asm volatile("bar.sync %0, 128;" :: "r"(barrier) : "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&f)[32]) {
     uint32_t a[16], b[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) { a[i] = __float_as_uint(f[i]); b[i] = __float_as_uint(f[16 + i]); }
     umma::tmem_st16(taddr, a);
     umma::tmem_st16(taddr + 16, b);
+}
+// Four 8 x 8 blocks of 16-bit values, transposed: lane t gets elements (2 (t % 4), t / 4) and (2 (t % 4) + 1, t / 4) of each; lane t gives the address of row t % 8 of block t / 8
+__device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 lanes x 16 columns: lane t of the warp gives column 4 i + t % 4 of rows t / 4 (v[2 i]) and 8 + t / 4 (v[2 i + 1])
+__device__ __forceinline__ void tmem_st_16x16(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int x, int head, int token, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -126,75 +134,83 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     auto slot_of = [](uint32_t tile) { return tile % SLOTS; };
     auto parity_of = [](uint32_t tile) { return (tile / SLOTS) & 1u; };
 
-    if (warp == WARP_LOAD) {
-        if (umma::elect_one()) {
-            uint32_t tile = 0;
-            for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-                const int idx = it.kind;
-                for (int t = 0; t < chunks; ++t) {
-                    const int tok = part.start + first_of(k, chunks, t);
-                    auto fetch = [&](int map, int head) {
-                        const uint32_t s = slot_of(tile);
-                        if (tile >= SLOTS) mbar_wait(&sh.empty[s], parity_of(tile) ^ 1u);
-                        umma::mbar_expect_tx(&sh.full[s], TILE);
-                        load_box(ring + s * TILE, &maps.row[map], 0, head, tok, &sh.full[s]);
-                        load_box(ring + s * TILE + TILE / 2, &maps.row[map], 64, head, tok, &sh.full[s]);
-                        ++tile;
-                    };
-                    if (!STATES) fetch(plan.map_a[idx], it.h / k.a_per);
-                    fetch(plan.map_b[idx], it.h / k.b_per);
-                    fetch(plan.map_c[idx], it.h / k.c_per);
-                }
-            });
-        }
-        __syncwarp();
-    } else if (warp == WARP_MMA) {
-        if (umma::elect_one()) {
-            uint32_t n = 0;                                // stretches so far
-            for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
-                const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
-                const bool zero = entering(call, k, it, STATES) == nullptr;
-                const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, vn), id_pc = umma::idesc_bf16(128, vn, 0, 1), id_x = umma::idesc_bf16(128, ms * 16, 0, 1);
-                for (int t = 0; t < chunks; ++t, ++n) {
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(ISSUE_REGS));
+        if (warp == WARP_LOAD) {
+            if (umma::elect_one()) {
+                uint32_t tile = 0;
+                for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
+                    const int idx = it.kind;
+                    for (int t = 0; t < chunks; ++t) {
+                        const int tok = part.start + first_of(k, chunks, t);
+                        auto fetch = [&](int map, int head) {
+                            const uint32_t s = slot_of(tile);
+                            if (tile >= SLOTS) mbar_wait(&sh.empty[s], parity_of(tile) ^ 1u);
+                            umma::mbar_expect_tx(&sh.full[s], TILE);
+                            load_box(ring + s * TILE, &maps.row[map], 0, head, tok, &sh.full[s]);
+                            load_box(ring + s * TILE + TILE / 2, &maps.row[map], 64, head, tok, &sh.full[s]);
+                            ++tile;
+                        };
+                        if (!STATES) fetch(plan.map_a[idx], it.h / k.a_per);
+                        fetch(plan.map_b[idx], it.h / k.b_per);
+                        fetch(plan.map_c[idx], it.h / k.c_per);
+                    }
+                });
+            }
+            __syncwarp();
+        } else if (warp == WARP_MMA) {
+            if (umma::elect_one()) {
+                uint32_t n = 0;                                // stretches so far
+                // FULL: 128 channels in all heads, every loop unrolled; the address of a tile passes through an empty statement, or descriptors are kept over the loop and spilled
+                auto stretch = [&](auto full, int ms, int vn, bool from_zero) {
+                    constexpr bool FULL = decltype(full)::value;
                     const uint32_t ta = n * PER, tb = ta + (STATES ? 0 : 1), tc = tb + 1, par = n & 1;
-                    const umma::Opnd a = umma::opnd_k(ring + slot_of(ta) * TILE, nullptr, 128), bk = umma::opnd_k(ring + slot_of(tb) * TILE, nullptr, 128);
-                    const umma::Opnd bm = umma::opnd_mn(ring + slot_of(tb) * TILE, nullptr, 128), cm = umma::opnd_mn(ring + slot_of(tc) * TILE, nullptr, 128);
-                    const uint64_t ad = umma::opnd_base_desc(a, a.hi);
+                    const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, FULL ? C : vn), id_pc = umma::idesc_bf16(128, FULL ? C : vn, 0, 1),
+                                   id_x = umma::idesc_bf16(128, FULL ? C : ms * 16, 0, 1);
+                    auto k_major = [&](uint32_t addr) {
+                        asm volatile("" : "+r"(addr));
+                        return umma::make_desc(addr);
+                    };
+                    auto mn_major = [&](uint32_t addr) {
+                        asm volatile("" : "+r"(addr));
+                        return umma::make_desc(addr, TILE / 2 / 16);
+                    };
+                    auto k_step = [](int ks) { return (uint64_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
+                    auto mn_step = [](int ks) { return (uint64_t)(ks * 128); };
+                    const uint32_t ring_at = umma::smem_u32(ring), state_at = umma::smem_u32(state_hi);
                     if (!STATES) mbar_wait(&sh.full[slot_of(ta)], parity_of(ta));
                     mbar_wait(&sh.full[slot_of(tb)], parity_of(tb));
                     if (!STATES) {
-                        const uint64_t bd = umma::opnd_base_desc(bk, bk.hi);
-                        for (int ks = 0; ks < ms; ++ks) umma::mma_bf16(tmem + P, ad + umma::opnd_step16(a, ks), bd + umma::opnd_step16(bk, ks), id_p0, ks != 0);
+                        const uint64_t ad = k_major(ring_at + slot_of(ta) * TILE), bd = k_major(ring_at + slot_of(tb) * TILE);
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            if (FULL || ks < ms) umma::mma_bf16(tmem + P, ad + k_step(ks), bd + k_step(ks), id_p0, ks != 0);
                         umma::commit(&sh.p0_done);
                         if (n) wait_mma(&sh.o_free, par ^ 1u);
                     }
                     wait_mma(&sh.s_ready, par);
-                    const bool from_zero = zero && t == 0;
                     if (!STATES) {
                         if (!from_zero) {
-                            const umma::Opnd m = umma::opnd_k(state_hi, state_hi + TILE, 128);
-                            const uint64_t mh = umma::opnd_base_desc(m, m.hi), ml = umma::opnd_base_desc(m, m.lo);
-                            for (int ks = 0; ks < ms; ++ks) {
-                                const uint32_t ao = umma::opnd_step16(a, ks), mo = umma::opnd_step16(m, ks);
-                                umma::mma_bf16(tmem + O, ad + ao, ml + mo, id_in, ks != 0);
-                                umma::mma_bf16(tmem + O, ad + ao, mh + mo, id_in, 1u);
-                            }
+                            const uint64_t ad = k_major(ring_at + slot_of(ta) * TILE), mh = k_major(state_at), ml = k_major(state_at + TILE);
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                if (FULL || ks < ms) {
+                                    umma::mma_bf16_fill(tmem + O, ad + k_step(ks), ml + k_step(ks), id_in, ks != 0);
+                                    umma::mma_bf16_lastuse(tmem + O, ad + k_step(ks), mh + k_step(ks), id_in, 1u);
+                                }
                         }
                         umma::commit(&sh.in_done);
                         umma::commit(&sh.empty[slot_of(ta)]);
                     }
-                    const uint64_t bmd = umma::opnd_base_desc(bm, bm.hi);
-                    uint32_t acc = !from_zero;
+                    const uint64_t bm = mn_major(ring_at + slot_of(tb) * TILE);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {          // 32 tokens: the smallest of the three parts of f c first
                         wait_mma(&sh.f_ready[q & 1], (2 * n + (q >> 1)) & 1);
 #pragma unroll
                         for (int part = 2; part >= 0; --part)
 #pragma unroll
-                            for (int ks = 0; ks < 2; ++ks) {
-                                umma::mma_bf16_ta(tmem + S, tmem + F + 64 * (q & 1) + 16 * part + 8 * ks, bmd + umma::opnd_step16(bm, 2 * q + ks), id_x, acc);
-                                acc = 1u;
-                            }
+                            for (int ks = 0; ks < 2; ++ks)
+                                umma::mma_bf16_ta(tmem + X, tmem + F + 64 * (q & 1) + 16 * part + 8 * ks, bm + mn_step(2 * q + ks), id_x, q + ks != 0 || part != 2);
                         umma::commit(&sh.f_free[q & 1]);
                     }
                     umma::commit(&sh.x_done);
@@ -203,29 +219,42 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         wait_mma(&sh.p_ready, par);
                         wait_mma(&sh.o_scaled, par);
                         mbar_wait(&sh.full[slot_of(tc)], parity_of(tc));
-                        const uint64_t cd = umma::opnd_base_desc(cm, cm.hi);
+                        const uint64_t cd = mn_major(ring_at + slot_of(tc) * TILE);
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
                             const uint32_t at = tmem + P + 32 * (ks >> 1) + 8 * (ks & 1);
-                            umma::mma_bf16_ta(tmem + O, at + 16, cd + umma::opnd_step16(cm, ks), id_pc, ks != 0 || !from_zero);
-                            umma::mma_bf16_ta(tmem + O, at, cd + umma::opnd_step16(cm, ks), id_pc, 1u);
+                            umma::mma_bf16_ta(tmem + O, at + 16, cd + mn_step(ks), id_pc, ks != 0 || !from_zero);
+                            umma::mma_bf16_ta(tmem + O, at, cd + mn_step(ks), id_pc, 1u);
                         }
                         umma::commit(&sh.o_done);
                     }
                     umma::commit(&sh.empty[slot_of(tc)]);
-                }
-            });
-            if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1));      // the last arrival of a product
+                };
+                for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
+                    const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
+                    const bool zero = entering(call, k, it, STATES) == nullptr;
+                    if (ms == 8 && vn == C) {
+                        for (int t = 0; t < chunks; ++t, ++n) stretch(std::true_type(), ms, vn, zero && t == 0);
+                    } else {
+                        for (int t = 0; t < chunks; ++t, ++n) stretch(std::false_type(), ms, vn, zero && t == 0);
+                    }
+                });
+                if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1));      // the last arrival of a product
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else if (warp < 4) {
-        // ---- pairs: row i = this lane's token
+        // ---- pairs: row i = this lane's token.  Off the diagonal the weight is a factor of the row times one of the column, neither above 1
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         if (!STATES) {
             uint32_t n = 0;
             const int i = tid;
-            float* const power = sh.power_p;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-                set_powers(power, call.log_decay[it.h], tid, 1);
+                const float gamma = call.log_decay[it.h];
+                group_sync(1);
+                sh.pair[i] = decay_power(gamma, i) * k.pair_scale;
+                if (i < 32) sh.column[i] = decay_power(gamma, k.back ? i : 31 - i);
+                group_sync(1);
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int len = min(C, part.len - first_of(k, chunks, t));
                     wait_mma(&sh.p0_done, n & 1);
@@ -239,18 +268,28 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         } else {
                             float v[32];
                             umma::tmem_ld32(at, v);
-                            const int away = k.back ? 32 * blk - i : i - 32 * blk;      // of column 0
+                            if (blk == warp) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                float x[2];
-#pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    const int d = k.back ? away + e + u : away - e - u;
-                                    const bool good = d >= 0 && (!k.back || 32 * blk + e + u < len);
-                                    x[u] = good ? v[e + u] * (power[good ? d : 0] * k.pair_scale) : 0.f;
+                                for (int e = 0; e < 32; ++e) {
+                                    const int d = k.back ? e - lane : lane - e;
+                                    v[e] = d >= 0 ? v[e] * sh.pair[max(d, 0)] : 0.f;
                                 }
-                                umma::split2(x[0], x[1], h[e / 2], l[e / 2]);
+                            } else {
+                                const f32x2 r = both(sh.pair[k.back ? 32 * blk - i : i - 32 * blk - 31]);
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4) {
+                                    const float4 c = *reinterpret_cast<const float4*>(sh.column + e);
+                                    unpack2(mul2(pack2(v[e], v[e + 1]), mul2(r, pack2(c.x, c.y))), v[e], v[e + 1]);
+                                    unpack2(mul2(pack2(v[e + 2], v[e + 3]), mul2(r, pack2(c.z, c.w))), v[e + 2], v[e + 3]);
+                                }
                             }
+                            if (k.back && 32 * blk + 32 > len) {       // columns behind the part's end
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (32 * blk + e >= len) v[e] = 0.f;
+                            }
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) umma::split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
                         }
                         umma::tmem_st16(at, h);
                         umma::tmem_st16(at + 16, l);
@@ -261,16 +300,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             });
         }
     } else if (warp < 8) {
-        // ---- f c, transposed: row = this lane's channel of c
+        // ---- f c, transposed: row = channel of c.  Blocks of 8 tokens x 8 channels come transposed out of shared memory, in the layout that 16 rows of tensor memory take
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         uint32_t n = 0;
-        const int ch = tid - 128, k8 = ch >> 3;
-        float* const power = sh.power;
+        const int ch = tid - 128;
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-            set_powers(power, call.log_decay[it.h], ch, 2);
+            const float gamma = call.log_decay[it.h];
+            int factors_of = -1;                           // tokens that the table is for
             for (int t = 0; t < chunks; ++t, ++n) {
                 const int len = min(C, part.len - first_of(k, chunks, t));
                 const uint32_t tb = n * PER + (STATES ? 0 : 1), tc = tb + 1;
                 uint8_t* const c = ring + slot_of(tc) * TILE;
+                if (len != factors_of) {
+                    group_sync(2);
+                    sh.factor[ch] = ch < len ? decay_power(gamma, k.back ? ch + 1 : len - 1 - ch) * k.in_scale : 0.f;
+                    factors_of = len;
+                    group_sync(2);
+                }
                 mbar_wait(&sh.full[slot_of(tc)], parity_of(tc));
                 if (len < C) {                             // rows behind the part's end belong to somebody else: 0 times what is not finite is not 0
                     uint8_t* const b = ring + slot_of(tb) * TILE;
@@ -280,116 +326,133 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         *reinterpret_cast<uint4*>(b + off) = make_uint4(0, 0, 0, 0);
                         *reinterpret_cast<uint4*>(c + off) = make_uint4(0, 0, 0, 0);
                     }
-                    asm volatile("bar.sync 2, 128;" ::: "memory");
+                    group_sync(2);
                     __syncwarp();
                 }
+                const uint32_t rows = umma::smem_u32(c);
+                const int w = warp - 4;
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
-                    uint32_t w[3][16];
-                    const int j0 = 32 * q, at = k.back ? j0 + 1 : len - 1 - j0;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float x[2], r[2];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t off = umma::tile_chunk_offset(128, j0 + e + u, k8) + 2 * (ch & 7);
-                            const float v = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(c + off) << 16);
-                            const int d = k.back ? at + e + u : at - e - u;
-                            x[u] = v * (power[max(d, 0)] * k.in_scale);      // behind the part's end v is 0
-                        }
-                        w[0][e / 2] = umma::pack_bf16x2(x[0], x[1]);
-                        r[0] = x[0] - __uint_as_float(w[0][e / 2] << 16);
-                        r[1] = x[1] - __uint_as_float(w[0][e / 2] & 0xffff0000u);
-                        w[1][e / 2] = umma::pack_bf16x2(r[0], r[1]);
-                        r[0] -= __uint_as_float(w[1][e / 2] << 16);
-                        r[1] -= __uint_as_float(w[1][e / 2] & 0xffff0000u);
-                        w[2][e / 2] = umma::pack_bf16x2(r[0], r[1]);
-                    }
                     const uint32_t use = 2 * n + (q >> 1);         // of this buffer
-                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1);
+                    f32x2 f[4];                            // of this lane's two tokens in each 8
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) umma::tmem_st16(umma::tmem_addr(tmem, warp, F + 64 * (q & 1) + 16 * p), w[p]);
+                    for (int g = 0; g < 4; ++g) f[g] = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 8 * g + 2 * (lane & 3));
+                    uint32_t part_[3][8];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {       // 16 channels
+#pragma unroll
+                        for (int g2 = 0; g2 < 2; ++g2) {   // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
+                            uint32_t r[4];
+                            const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * hf) / 8 + ((lane >> 3) & 1);
+                            load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) {
+                                float a, b;
+                                f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f[2 * g2 + (m >> 1)]);
+#pragma unroll
+                                for (int p = 0; p < 3; ++p) {
+                                    unpack2(x, a, b);
+                                    const uint32_t h = umma::pack_bf16x2(a, b);
+                                    part_[p][2 * (2 * g2 + (m >> 1)) + (m & 1)] = h;
+                                    if (p < 2) x = add2(x, pack2(__uint_as_float((h << 16) ^ 0x80000000u), __uint_as_float((h & 0xffff0000u) ^ 0x80000000u)));
+                                }
+                            }
+                        }
+                        if (hf == 0 && use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1);
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) tmem_st_16x16(umma::tmem_addr(tmem, warp, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * hf) << 16), part_[p]);
+                    }
                     umma::tmem_wait_st();
                     umma::signal(&sh.f_ready[q & 1], lane);
                 }
             }
         });
     } else if (warp < 12) {
-        // ---- the state: row = this lane's channel of c, columns the channels of b
+        // ---- the state: row = this lane's channel of c, columns the channels of b, in registers.  What a stretch adds comes from an accumulator of its own: the tensor cores cut off what
+        // does not fit into 32 bits, and over a long sequence's products that is an error of one sign (2.5e-6 of the state behind 32 k tokens, this way 0.4e-6).
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGS));
         uint32_t n = 0;
         const int ch = tid - 256;
+        f32x2 s[64];
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float* in = entering(call, k, it, STATES);
             const size_t size = (size_t)k.M * k.V;
             float* out = STATES ? k.parts + ((size_t)(it.n * call.S.segs + it.part + (k.back ? -1 : 1)) * call.HV + it.h) * size
                                 : k.last && part.leaves_last ? k.last + ((size_t)it.n * call.HV + it.h) * size : nullptr;
             const float gamma = call.log_decay[it.h], whole = decay_power(gamma, C), rest = decay_power(gamma, part.len % C);
-            auto at = [&](int m) { return k.transposed ? (size_t)ch * k.M + m : (size_t)m * k.V + ch; };
-            auto from_memory = [&](int m0, float (&v)[32]) {
+            const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = in && ch < k.V && m0 + e < k.M ? in[at(m0 + e)] : 0.f;
-            };
-            for (int t = 0; t < chunks; ++t, ++n) {
-                const bool from_zero = t == 0 && !in;
-                if (t) wait_mma(&sh.x_done, (n - 1) & 1);
-                if (!from_zero) {
-                    const bool short_one = part.len - first_of(k, chunks, t) < C;
-                    const float f = short_one ? rest : whole;
-#pragma unroll 1
-                    for (int m0 = 0; m0 < k.M; m0 += 32) {
-                        float v[32];
-                        if (t) umma::tmem_ld32(umma::tmem_addr(tmem, warp, S + m0), v);
-                        else from_memory(m0, v);
-                        if (!STATES) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                const float x[8] = {v[e], v[e + 1], v[e + 2], v[e + 3], v[e + 4], v[e + 5], v[e + 6], v[e + 7]};
-                                umma::store_split8(state_hi, state_hi + TILE, 128, ch, (m0 + e) >> 3, x);
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] *= f;
-                        __syncwarp();
-                        tmem_st32(umma::tmem_addr(tmem, warp, S + m0), v);
-                    }
-                    umma::tmem_wait_st();
+            for (int m = 0; m < 128; m += 2) {
+                float v[2] = {0.f, 0.f};
+                if (in && ch < k.V) {
+                    if (m < k.M) v[0] = in[first + m * step];
+                    if (m + 1 < k.M) v[1] = in[first + (m + 1) * step];
                 }
-                umma::signal(&sh.s_ready, lane);
+                s[m / 2] = pack2(v[0], v[1]);
             }
-            if (chunks) wait_mma(&sh.x_done, (n - 1) & 1);
-            if (!out) return;
-#pragma unroll 1
-            for (int m0 = 0; m0 < k.M; m0 += 32) {
-                float v[32];
-                __syncwarp();
-                if (chunks) umma::tmem_ld32(umma::tmem_addr(tmem, warp, S + m0), v);
-                else from_memory(m0, v);
-                if (ch < k.V)
+            __syncwarp();
+            for (int t = 0; t <= chunks; ++t) {
+                f32x2 f = both(1.f);
+                if (t) {
+                    const bool short_one = part.len - first_of(k, chunks, t - 1) < C;
+                    f = both(short_one ? rest : whole);
+                    wait_mma(&sh.x_done, (n - 1) & 1);
+                }
+                const bool store = !STATES && t < chunks && (t || in);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (m0 + e < k.M) out[at(m0 + e)] = v[e];
+                for (int g = 0; g < 8; ++g) {
+                    if (16 * g >= k.M) break;
+                    if (t) {
+                        float x[16];
+                        umma::tmem_ld16(umma::tmem_addr(tmem, warp, X + 16 * g), x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[8 * g + e] = fma2(s[8 * g + e], f, pack2(x[2 * e], x[2 * e + 1]));
+                    }
+                    if (store) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            const f32x2 v[4] = {s[8 * g + e], s[8 * g + e + 1], s[8 * g + e + 2], s[8 * g + e + 3]};
+                            umma::store_split8(state_hi, state_hi + TILE, 128, ch, 2 * g + e / 4, v);
+                        }
+                    }
+                }
+                if (t == chunks) break;
+                umma::signal(&sh.s_ready, lane);
+                ++n;
+            }
+            if (!out || ch >= k.V) return;
+#pragma unroll
+            for (int m = 0; m < 128; m += 2) {
+                float a, b;
+                unpack2(s[m / 2], a, b);
+                if (m < k.M) out[first + m * step] = a;
+                if (m + 1 < k.M) out[first + (m + 1) * step] = b;
             }
         });
-    } else if (warp < 16) {
+    } else {
         // ---- the output: row i = this lane's token
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         if (!STATES) {
             uint32_t n = 0;
             const int i = tid - 384;
-            float* const power = sh.power_o;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-                set_powers(power, call.log_decay[it.h], i, 3);
-                const bool zero = entering(call, k, it, STATES) == nullptr;
+                const float gamma = call.log_decay[it.h];
+                group_sync(3);
+                sh.row[i] = decay_power(gamma, i) * k.state_scale;
+                if (i == 0) sh.row[C] = decay_power(gamma, C) * k.state_scale;
+                group_sync(3);
+                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind];
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
                     wait_mma(&sh.in_done, n & 1);
                     if (!zero || t) {
-                        const float f = power[k.back ? max(len - 1 - i, 0) : i + 1] * k.state_scale;
+                        const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1]);
 #pragma unroll 1
                         for (int m0 = 0; m0 < k.V; m0 += 32) {
                             float v[32];
                             umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0), v);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] *= f;
+                            for (int e = 0; e < 32; e += 2) unpack2(mul2(pack2(v[e], v[e + 1]), f), v[e], v[e + 1]);
                             tmem_st32(umma::tmem_addr(tmem, warp, O + m0), v);
                         }
                         umma::tmem_wait_st();
@@ -397,19 +460,57 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1);
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
+                    if (k.out_dtype == MKDA_F32) {
 #pragma unroll 1
-                    for (int m0 = 0; m0 < k.V; m0 += 32) {
-                        float v[32];
-                        __syncwarp();
-                        umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0), v);
-                        if (m0 + 32 >= k.V) signal_tmem(&sh.o_free, lane);
-                        if (i >= len) continue;
+                        for (int m0 = 0; m0 < k.V; m0 += 32) {
+                            float v[32];
+                            __syncwarp();
+                            umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0), v);
+                            if (m0 + 32 >= k.V) signal_tmem(&sh.o_free, lane);
+                            if (i < len)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (m0 + e >= k.V) break;
-                            const float x[8] = {v[e], v[e + 1], v[e + 2], v[e + 3], v[e + 4], v[e + 5], v[e + 6], v[e + 7]};
-                            if (k.out_dtype == MKDA_F32) st8<MKDA_F32>(k.out, row + m0 + e, x);
-                            else st8<MKDA_BF16>(k.out, row + m0 + e, x);
+                                for (int e = 0; e < 32; e += 8) {
+                                    if (m0 + e >= k.V) break;
+                                    uint32_t u[8];
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(v[e + j]);
+                                    float* to = static_cast<float*>(k.out) + row + m0 + e;
+                                    if (wide) {
+                                        st32b(to, u);
+                                    } else {
+                                        *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+                                        *reinterpret_cast<uint4*>(to + 4) = make_uint4(u[4], u[5], u[6], u[7]);
+                                    }
+                                }
+                        }
+                    } else {
+                        // 64 channels at a time, read before the first is stored: the next products wait for the accumulator, not for the stores
+#pragma unroll 1
+                        for (int m0 = 0; m0 < k.V; m0 += 64) {
+                            uint32_t u[32];
+                            __syncwarp();
+#pragma unroll
+                            for (int hf = 0; hf < 2; ++hf) {
+                                float v[32];
+                                umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0 + 32 * hf), v);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) u[16 * hf + e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                            }
+                            if (m0 + 64 >= k.V) signal_tmem(&sh.o_free, lane);
+                            if (i < len) {
+                                uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t p[8] = {u[8 * e], u[8 * e + 1], u[8 * e + 2], u[8 * e + 3], u[8 * e + 4], u[8 * e + 5], u[8 * e + 6], u[8 * e + 7]};
+                                    if (m0 + 16 * e >= k.V) break;
+                                    if (wide) {
+                                        st32b(to + 16 * e, p);
+                                    } else {
+                                        *reinterpret_cast<uint4*>(to + 16 * e) = make_uint4(p[0], p[1], p[2], p[3]);
+                                        if (m0 + 16 * e + 8 < k.V) *reinterpret_cast<uint4*>(to + 16 * e + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+                                    }
+                                }
+                            }
                         }
                     }
                 }
@@ -452,12 +553,15 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
         plan.map_a[i] = k.a ? map(k.a, k.a_stride, k.a_per, k.M) : 0;
         plan.map_b[i] = map(k.b, k.b_stride, k.b_per, k.M);
         plan.map_c[i] = map(k.c, k.c_stride, k.c_per, k.V);
+        plan.wide[i] = k.V % (k.out_dtype == MKDA_F32 ? 8 : 16) == 0 && !any_misaligned32(k.out);
     }
     if (rc != MKDA_OK) return rc;
     plan.items = (long long)call.S.N * (call.S.seg ? call.S.segs : 1) * call.HV * call.kinds;
     auto* kern = states ? lt::linear_tc_kernel<true> : lt::linear_tc_kernel<false>;
     rc = ensure_smem(reinterpret_cast<const void*>(kern), lt::SMEM, "linear");
     if (rc != MKDA_OK) return rc;
+    static const int regs = std::min(kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<true>)), kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<false>)));
+    if (regs < lt::LAUNCH_REGS) return set_error(MKDA_ERR_LAUNCH, "linear: built with fewer registers than its warps redistribute");
     launch(kern, dim3((unsigned)std::min<long long>(plan.items, sm_count())), lt::THREADS, lt::SMEM, stream, plan, maps);
     return check_launch("linear");
 }

@@ -214,6 +214,22 @@ def test_linear_does_not_depend_on_its_neighbours():
             assert torch.equal(one[0], batch[i]) and torch.equal(olast[0], last[i]) and torch.equal(packed[0, 200 * i:200 * i + 200], batch[i]) and torch.equal(plast[i], last[i])
 
 
+def test_linear_from_a_new_thread():
+    """A thread that has called nothing of CUDA yet, and memory that the allocator has at hand."""
+    import threading
+    q = torch.randn(1, 200, 2, 128, device="cuda", dtype=torch.bfloat16)
+    d = -torch.rand(2, device="cuda")
+    with torch.no_grad():
+        want, _ = mk.linear_attention(q, q, q, d)
+        spare = torch.empty_like(want)
+        del spare
+        got = []
+        run = threading.Thread(target=lambda: got.append(mk.linear_attention(q, q, q, d)[0]))
+        run.start()
+        run.join()
+    assert len(got) == 1 and torch.equal(got[0], want)
+
+
 def test_linear_refuses():
     q, v, d = torch.randn(1, 5, 2, 16).cuda(), torch.randn(1, 5, 4, 16).cuda(), -torch.rand(4).cuda()
     for bad in (lambda: mk.linear_attention(q, q, v[:, :, :3], d[:3]), lambda: mk.linear_attention(q, q.bfloat16(), v, d), lambda: mk.linear_attention(q, q[..., :8], v, d),
