@@ -26,11 +26,12 @@ using umma::mbar_wait;
 using umma::signal_tmem;
 using umma::wait_mma;
 
-constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 640, WARP_LOAD = 16, WARP_MMA = 17;
+constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 1024;
+constexpr int WARP_PAIRS = 0, WARP_FACTORS = 8, WARP_STATE = 16, WARP_OUT = 20, WARP_LOAD = 28, WARP_MMA = 29;
 constexpr int P = 0, O = 128, X = 256, F = 384;            // tensor-memory columns: pairs, output, what goes into the state, f c (two buffers of a quarter: 3 x 16 columns each)
-// Registers: the state's warps have 128 values of it a thread.  Their sum is the launch's.
-constexpr int LAUNCH_REGS = 96, WORK_REGS = 88, STATE_REGS = 160, ISSUE_REGS = 56;
-static_assert(3 * WORK_REGS + STATE_REGS + ISSUE_REGS <= 5 * LAUNCH_REGS, "registers of the launch");
+// Registers: a thread of the state has 128 values of it.
+constexpr int LAUNCH_REGS = 64, WORK_REGS = 48, STATE_REGS = 160, ISSUE_REGS = 40;
+static_assert(6 * WORK_REGS + STATE_REGS + ISSUE_REGS <= 8 * LAUNCH_REGS, "registers of the launch");
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
@@ -46,7 +47,7 @@ struct Maps { CUtensorMap row[4]; };                       // rows of a head, bo
 struct Plan {
     LinearCall call;
     int map_a[3], map_b[3], map_c[3];                      // per kind
-    int wide[3];                                           // rows of the output in pieces of 32 bytes
+    int wide[3];                                           // bf16 rows of the output leave in pieces of 32 bytes
     long long items;
 };
 
@@ -81,13 +82,19 @@ __device__ __forceinline__ const float* entering(const LinearCall& call, const L
     if (call.S.seg) return k.parts + ((size_t)(it.n * call.S.segs + it.part) * call.HV + it.h) * size;
     return k.first ? k.first + ((size_t)it.n * call.HV + it.h) * size : nullptr;
 }
-__device__ __forceinline__ void group_sync(int barrier) { asm volatile("bar.sync %0, 128;" :: "r"(barrier) : "memory"); }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&f)[32]) {
-    uint32_t a[16], b[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { a[i] = __float_as_uint(f[i]); b[i] = __float_as_uint(f[16 + i]); }
-    umma::tmem_st16(taddr, a);
-    umma::tmem_st16(taddr + 16, b);
+__device__ __forceinline__ void group_sync(int barrier) { asm volatile("bar.sync %0, 256;" :: "r"(barrier) : "memory"); }
+// A pair of values as bf16 pairs: hi, and what is left of them, two rounded parts in all
+__device__ __forceinline__ uint32_t take_bf16(f32x2& v) {          // hi; v becomes the rest, exactly
+    float a, b;
+    unpack2(v, a, b);
+    const uint32_t h = umma::pack_bf16x2(a, b);
+    v = fma2(pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), both(-1.f), v);
+    return h;
+}
+__device__ __forceinline__ uint32_t as_bf16(f32x2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return umma::pack_bf16x2(a, b);
 }
 // Four 8 x 8 blocks of 16-bit values, transposed: lane t gets elements (2 (t % 4), t / 4) and (2 (t % 4) + 1, t / 4) of each; lane t gives the address of row t % 8 of block t / 8
 __device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4]) {
@@ -121,7 +128,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < SLOTS; ++i) { umma::mbar_init(&sh.full[i], 1); umma::mbar_init(&sh.empty[i], 1); }
         for (uint64_t* b : {&sh.p0_done, &sh.f_free[0], &sh.f_free[1], &sh.x_done, &sh.in_done, &sh.o_done}) umma::mbar_init(b, 1);
-        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free}) umma::mbar_init(b, 4);
+        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.o_scaled, &sh.o_free}) umma::mbar_init(b, 8);
+        umma::mbar_init(&sh.s_ready, 4);
         umma::fence_barrier_init();
     }
     follow_stream();
@@ -134,7 +142,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     auto slot_of = [](uint32_t tile) { return tile % SLOTS; };
     auto parity_of = [](uint32_t tile) { return (tile / SLOTS) & 1u; };
 
-    if (warp >= 16) {
+    if (warp >= WARP_LOAD) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(ISSUE_REGS));
         if (warp == WARP_LOAD) {
             if (umma::elect_one()) {
@@ -186,10 +194,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         for (int ks = 0; ks < 8; ++ks)
                             if (FULL || ks < ms) umma::mma_bf16(tmem + P, ad + k_step(ks), bd + k_step(ks), id_p0, ks != 0);
                         umma::commit(&sh.p0_done);
-                        if (n) wait_mma(&sh.o_free, par ^ 1u);
                     }
                     wait_mma(&sh.s_ready, par);
+                    const uint64_t bm = mn_major(ring_at + slot_of(tb) * TILE);
+                    auto into_state = [&](int q) {         // 32 tokens: the smallest of the three parts of f c first
+                        wait_mma(&sh.f_ready[q & 1], (2 * n + (q >> 1)) & 1);
+#pragma unroll
+                        for (int part = 2; part >= 0; --part)
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks)
+                                umma::mma_bf16_ta(tmem + X, tmem + F + 64 * (q & 1) + 16 * part + 8 * ks, bm + mn_step(2 * q + ks), id_x, q + ks != 0 || part != 2);
+                        umma::commit(&sh.f_free[q & 1]);
+                    };
+                    // The first half of X lies in front of the product with the state, which waits for the last stretch's output to be read; the second half's parts of f c are made beside it
+                    into_state(0);
+                    into_state(1);
                     if (!STATES) {
+                        if (n) wait_mma(&sh.o_free, par ^ 1u);
                         if (!from_zero) {
                             const uint64_t ad = k_major(ring_at + slot_of(ta) * TILE), mh = k_major(state_at), ml = k_major(state_at + TILE);
 #pragma unroll
@@ -202,17 +223,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         umma::commit(&sh.in_done);
                         umma::commit(&sh.empty[slot_of(ta)]);
                     }
-                    const uint64_t bm = mn_major(ring_at + slot_of(tb) * TILE);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {          // 32 tokens: the smallest of the three parts of f c first
-                        wait_mma(&sh.f_ready[q & 1], (2 * n + (q >> 1)) & 1);
-#pragma unroll
-                        for (int part = 2; part >= 0; --part)
-#pragma unroll
-                            for (int ks = 0; ks < 2; ++ks)
-                                umma::mma_bf16_ta(tmem + X, tmem + F + 64 * (q & 1) + 16 * part + 8 * ks, bm + mn_step(2 * q + ks), id_x, q + ks != 0 || part != 2);
-                        umma::commit(&sh.f_free[q & 1]);
-                    }
+                    into_state(2);
+                    into_state(3);
                     umma::commit(&sh.x_done);
                     umma::commit(&sh.empty[slot_of(tb)]);
                     if (!STATES) {
@@ -222,8 +234,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         const uint64_t cd = mn_major(ring_at + slot_of(tc) * TILE);
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
-                            const uint32_t at = tmem + P + 32 * (ks >> 1) + 8 * (ks & 1);
-                            umma::mma_bf16_ta(tmem + O, at + 16, cd + mn_step(ks), id_pc, ks != 0 || !from_zero);
+                            const uint32_t at = tmem + P + 16 * ks;
+                            umma::mma_bf16_ta(tmem + O, at + 8, cd + mn_step(ks), id_pc, ks != 0 || !from_zero);
                             umma::mma_bf16_ta(tmem + O, at, cd + mn_step(ks), id_pc, 1u);
                         }
                         umma::commit(&sh.o_done);
@@ -243,67 +255,74 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             }
             __syncwarp();
         }
-    } else if (warp < 4) {
-        // ---- pairs: row i = this lane's token.  Off the diagonal the weight is a factor of the row times one of the column, neither above 1
+    } else if (warp < WARP_FACTORS) {
+        // ---- pairs: row i = this lane's token, half of the columns.  Off the diagonal the weight is a factor of the row times one of the column, neither above 1
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         if (!STATES) {
             uint32_t n = 0;
-            const int i = tid;
+            const int w = warp & 3, half = warp >> 2, i = 32 * w + lane;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                 const float gamma = call.log_decay[it.h];
                 group_sync(1);
-                sh.pair[i] = decay_power(gamma, i) * k.pair_scale;
-                if (i < 32) sh.column[i] = decay_power(gamma, k.back ? i : 31 - i);
+                if (half == 0) sh.pair[i] = decay_power(gamma, i) * k.pair_scale;
+                else if (i < 32) sh.column[i] = decay_power(gamma, k.back ? i : 31 - i);
                 group_sync(1);
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int len = min(C, part.len - first_of(k, chunks, t));
                     wait_mma(&sh.p0_done, n & 1);
 #pragma unroll 1
-                    for (int blk = 0; blk < 4; ++blk) {
-                        const uint32_t at = umma::tmem_addr(tmem, warp, P + 32 * blk);
-                        uint32_t h[16], l[16];
-                        if (k.back ? blk < warp || 32 * blk >= len : blk > warp) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) h[e] = l[e] = 0u;
-                        } else {
-                            float v[32];
-                            umma::tmem_ld32(at, v);
-                            if (blk == warp) {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const int d = k.back ? e - lane : lane - e;
-                                    v[e] = d >= 0 ? v[e] * sh.pair[max(d, 0)] : 0.f;
-                                }
-                            } else {
-                                const f32x2 r = both(sh.pair[k.back ? 32 * blk - i : i - 32 * blk - 31]);
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) {
-                                    const float4 c = *reinterpret_cast<const float4*>(sh.column + e);
-                                    unpack2(mul2(pack2(v[e], v[e + 1]), mul2(r, pack2(c.x, c.y))), v[e], v[e + 1]);
-                                    unpack2(mul2(pack2(v[e + 2], v[e + 3]), mul2(r, pack2(c.z, c.w))), v[e + 2], v[e + 3]);
-                                }
-                            }
-                            if (k.back && 32 * blk + 32 > len) {       // columns behind the part's end
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (32 * blk + e >= len) v[e] = 0.f;
-                            }
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) umma::split2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+                    for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
+                        const uint32_t at = umma::tmem_addr(tmem, w, P + j0);
+                        const int blk = j0 >> 5;
+                        if (k.back ? blk < w || j0 >= len : blk > w) {
+                            const uint32_t none[16] = {};
+                            umma::tmem_st16(at, none);
+                            continue;
                         }
-                        umma::tmem_st16(at, h);
-                        umma::tmem_st16(at + 16, l);
+                        float v[16];
+                        umma::tmem_ld16(at, v);
+                        if (blk == w) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const int d = k.back ? j0 + e - i : i - j0 - e;
+                                v[e] = d >= 0 ? v[e] * sh.pair[max(d, 0)] : 0.f;
+                            }
+                        } else {
+                            const f32x2 r = both(sh.pair[k.back ? 32 * blk - i : i - 32 * blk - 31]);
+                            const float* column = sh.column + (j0 & 16);
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4) {
+                                const float4 c = *reinterpret_cast<const float4*>(column + e);
+                                unpack2(mul2(pack2(v[e], v[e + 1]), mul2(r, pack2(c.x, c.y))), v[e], v[e + 1]);
+                                unpack2(mul2(pack2(v[e + 2], v[e + 3]), mul2(r, pack2(c.z, c.w))), v[e + 2], v[e + 3]);
+                            }
+                        }
+                        if (k.back && j0 + 16 > len) {     // columns behind the part's end
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (j0 + e >= len) v[e] = 0.f;
+                        }
+                        uint32_t h[8], l[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            f32x2 x = pack2(v[2 * e], v[2 * e + 1]);
+                            h[e] = take_bf16(x);
+                            l[e] = as_bf16(x);
+                        }
+                        umma::tmem_st8(at, h);
+                        umma::tmem_st8(at + 8, l);
                     }
                     umma::tmem_wait_st();
                     signal_tmem(&sh.p_ready, lane);
                 }
             });
         }
-    } else if (warp < 8) {
-        // ---- f c, transposed: row = channel of c.  Blocks of 8 tokens x 8 channels come transposed out of shared memory, in the layout that 16 rows of tensor memory take
+    } else if (warp < WARP_STATE) {
+        // ---- f c, transposed: row = channel of c, 16 of them a warp.  Blocks of 8 tokens x 8 channels come transposed out of shared memory, in the layout that 16 rows of tensor
+        // memory take
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         uint32_t n = 0;
-        const int ch = tid - 128;
+        const int me = tid - 32 * WARP_FACTORS, w = warp & 3, half = (warp - WARP_FACTORS) >> 2;
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float gamma = call.log_decay[it.h];
             int factors_of = -1;                           // tokens that the table is for
@@ -313,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 uint8_t* const c = ring + slot_of(tc) * TILE;
                 if (len != factors_of) {
                     group_sync(2);
-                    sh.factor[ch] = ch < len ? decay_power(gamma, k.back ? ch + 1 : len - 1 - ch) * k.in_scale : 0.f;
+                    if (me < C) sh.factor[me] = me < len ? decay_power(gamma, k.back ? me + 1 : len - 1 - me) * k.in_scale : 0.f;
                     factors_of = len;
                     group_sync(2);
                 }
@@ -321,58 +340,49 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 if (len < C) {                             // rows behind the part's end belong to somebody else: 0 times what is not finite is not 0
                     uint8_t* const b = ring + slot_of(tb) * TILE;
                     mbar_wait(&sh.full[slot_of(tb)], parity_of(tb));
-                    for (int e = ch; e < (C - len) * 16; e += 128) {
+                    for (int e = me; e < (C - len) * 16; e += 256) {
                         const uint32_t off = umma::tile_chunk_offset(128, len + (e >> 4), e & 15);
                         *reinterpret_cast<uint4*>(b + off) = make_uint4(0, 0, 0, 0);
                         *reinterpret_cast<uint4*>(c + off) = make_uint4(0, 0, 0, 0);
                     }
+                    umma::fence_async_smem();
                     group_sync(2);
                     __syncwarp();
                 }
                 const uint32_t rows = umma::smem_u32(c);
-                const int w = warp - 4;
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
                     const uint32_t use = 2 * n + (q >> 1);         // of this buffer
-                    f32x2 f[4];                            // of this lane's two tokens in each 8
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) f[g] = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 8 * g + 2 * (lane & 3));
                     uint32_t part_[3][8];
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {       // 16 channels
+                    for (int g2 = 0; g2 < 2; ++g2) {       // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
+                        uint32_t r[4];
+                        const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * half) / 8 + ((lane >> 3) & 1);
+                        load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
 #pragma unroll
-                        for (int g2 = 0; g2 < 2; ++g2) {   // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
-                            uint32_t r[4];
-                            const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * hf) / 8 + ((lane >> 3) & 1);
-                            load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) {
-                                float a, b;
-                                f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f[2 * g2 + (m >> 1)]);
-#pragma unroll
-                                for (int p = 0; p < 3; ++p) {
-                                    unpack2(x, a, b);
-                                    const uint32_t h = umma::pack_bf16x2(a, b);
-                                    part_[p][2 * (2 * g2 + (m >> 1)) + (m & 1)] = h;
-                                    if (p < 2) x = add2(x, pack2(__uint_as_float((h << 16) ^ 0x80000000u), __uint_as_float((h & 0xffff0000u) ^ 0x80000000u)));
-                                }
-                            }
+                        for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
+                            const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
+                            f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f);
+                            const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
+                            part_[0][to] = take_bf16(x);
+                            part_[1][to] = take_bf16(x);
+                            part_[2][to] = as_bf16(x);
                         }
-                        if (hf == 0 && use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1);
-#pragma unroll
-                        for (int p = 0; p < 3; ++p) tmem_st_16x16(umma::tmem_addr(tmem, warp, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * hf) << 16), part_[p]);
                     }
+                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) tmem_st_16x16(umma::tmem_addr(tmem, w, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * half) << 16), part_[p]);
                     umma::tmem_wait_st();
-                    umma::signal(&sh.f_ready[q & 1], lane);
+                    signal_tmem(&sh.f_ready[q & 1], lane);
                 }
             }
         });
-    } else if (warp < 12) {
+    } else if (warp < WARP_OUT) {
         // ---- the state: row = this lane's channel of c, columns the channels of b, in registers.  What a stretch adds comes from an accumulator of its own: the tensor cores cut off what
         // does not fit into 32 bits, and over a long sequence's products that is an error of one sign (2.5e-6 of the state behind 32 k tokens, this way 0.4e-6).
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGS));
         uint32_t n = 0;
-        const int ch = tid - 256;
+        const int ch = tid - 32 * WARP_STATE;
         f32x2 s[64];
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float* in = entering(call, k, it, STATES);
@@ -411,8 +421,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     if (store) {
 #pragma unroll
                         for (int e = 0; e < 8; e += 4) {
-                            const f32x2 v[4] = {s[8 * g + e], s[8 * g + e + 1], s[8 * g + e + 2], s[8 * g + e + 3]};
-                            umma::store_split8(state_hi, state_hi + TILE, 128, ch, 2 * g + e / 4, v);
+                            uint32_t h[4], l[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                f32x2 x = s[8 * g + e + j];
+                                h[j] = take_bf16(x);
+                                l[j] = as_bf16(x);
+                            }
+                            uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 2 * g + e / 4);
+                            *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
                         }
                     }
                 }
@@ -430,89 +448,68 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             }
         });
     } else {
-        // ---- the output: row i = this lane's token
+        // ---- the output: row i = this lane's token, half of the channels
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         if (!STATES) {
             uint32_t n = 0;
-            const int i = tid - 384;
+            const int w = warp & 3, half = (warp - WARP_OUT) >> 2, i = 32 * w + lane, m_first = 64 * half;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                 const float gamma = call.log_decay[it.h];
                 group_sync(3);
-                sh.row[i] = decay_power(gamma, i) * k.state_scale;
-                if (i == 0) sh.row[C] = decay_power(gamma, C) * k.state_scale;
+                if (half == 0) sh.row[i] = decay_power(gamma, i) * k.state_scale;
+                else if (i == 0) sh.row[C] = decay_power(gamma, C) * k.state_scale;
                 group_sync(3);
-                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind];
+                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind], fp32 = k.out_dtype == MKDA_F32;
+                const int m_end = min(k.V, m_first + 64);
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
                     wait_mma(&sh.in_done, n & 1);
                     if (!zero || t) {
                         const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1]);
 #pragma unroll 1
-                        for (int m0 = 0; m0 < k.V; m0 += 32) {
-                            float v[32];
-                            umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0), v);
+                        for (int m0 = m_first; m0 < m_end; m0 += 16) {
+                            const uint32_t at = umma::tmem_addr(tmem, w, O + m0);
+                            float v[16];
+                            umma::tmem_ld16(at, v);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) unpack2(mul2(pack2(v[e], v[e + 1]), f), v[e], v[e + 1]);
-                            tmem_st32(umma::tmem_addr(tmem, warp, O + m0), v);
+                            for (int g = 0; g < 16; g += 8) {
+                                f32x2 x[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[e] = mul2(pack2(v[g + 2 * e], v[g + 2 * e + 1]), f);
+                                umma::tmem_st8(at + g, x);
+                            }
                         }
                         umma::tmem_wait_st();
                     }
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1);
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
-                    if (k.out_dtype == MKDA_F32) {
 #pragma unroll 1
-                        for (int m0 = 0; m0 < k.V; m0 += 32) {
-                            float v[32];
-                            __syncwarp();
-                            umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0), v);
-                            if (m0 + 32 >= k.V) signal_tmem(&sh.o_free, lane);
-                            if (i < len)
+                    for (int m0 = m_first; m0 < m_first + 64; m0 += 16) {
+                        float v[16];
+                        __syncwarp();
+                        if (m0 < m_end) umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
+                        if (m0 == m_first + 48) signal_tmem(&sh.o_free, lane);
+                        if (i >= len || m0 >= m_end) continue;
+                        if (fp32) {
+                            float* to = static_cast<float*>(k.out) + row + m0;
 #pragma unroll
-                                for (int e = 0; e < 32; e += 8) {
-                                    if (m0 + e >= k.V) break;
-                                    uint32_t u[8];
+                            for (int e = 0; e < 16; e += 4)
+                                if (m0 + e < m_end) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        } else {
+                            uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
+                            uint32_t u[8];
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(v[e + j]);
-                                    float* to = static_cast<float*>(k.out) + row + m0 + e;
-                                    if (wide) {
-                                        st32b(to, u);
-                                    } else {
-                                        *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
-                                        *reinterpret_cast<uint4*>(to + 4) = make_uint4(u[4], u[5], u[6], u[7]);
-                                    }
-                                }
-                        }
-                    } else {
-                        // 64 channels at a time, read before the first is stored: the next products wait for the accumulator, not for the stores
-#pragma unroll 1
-                        for (int m0 = 0; m0 < k.V; m0 += 64) {
-                            uint32_t u[32];
-                            __syncwarp();
-#pragma unroll
-                            for (int hf = 0; hf < 2; ++hf) {
-                                float v[32];
-                                umma::tmem_ld32(umma::tmem_addr(tmem, warp, O + m0 + 32 * hf), v);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) u[16 * hf + e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
-                            }
-                            if (m0 + 64 >= k.V) signal_tmem(&sh.o_free, lane);
-                            if (i < len) {
-                                uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint32_t p[8] = {u[8 * e], u[8 * e + 1], u[8 * e + 2], u[8 * e + 3], u[8 * e + 4], u[8 * e + 5], u[8 * e + 6], u[8 * e + 7]};
-                                    if (m0 + 16 * e >= k.V) break;
-                                    if (wide) {
-                                        st32b(to + 16 * e, p);
-                                    } else {
-                                        *reinterpret_cast<uint4*>(to + 16 * e) = make_uint4(p[0], p[1], p[2], p[3]);
-                                        if (m0 + 16 * e + 8 < k.V) *reinterpret_cast<uint4*>(to + 16 * e + 8) = make_uint4(p[4], p[5], p[6], p[7]);
-                                    }
-                                }
+                            for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                            if (wide) {
+                                st32b(to, u);
+                            } else {
+                                *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+                                if (m0 + 8 < m_end) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
                             }
                         }
                     }
+                    __syncwarp();
                 }
             });
         }
@@ -553,7 +550,7 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
         plan.map_a[i] = k.a ? map(k.a, k.a_stride, k.a_per, k.M) : 0;
         plan.map_b[i] = map(k.b, k.b_stride, k.b_per, k.M);
         plan.map_c[i] = map(k.c, k.c_stride, k.c_per, k.V);
-        plan.wide[i] = k.V % (k.out_dtype == MKDA_F32 ? 8 : 16) == 0 && !any_misaligned32(k.out);
+        plan.wide[i] = k.V % 16 == 0 && !any_misaligned32(k.out);
     }
     if (rc != MKDA_OK) return rc;
     plan.items = (long long)call.S.N * (call.S.seg ? call.S.segs : 1) * call.HV * call.kinds;

@@ -32,15 +32,15 @@ def linear_kernel(states):
         wait("full", b)
         if not states:
             arrive("p0_done", n)
-            if n:
-                wait("o_free", n - 1)
         wait("s_ready", n)
-        if not states:
-            arrive("in_done", n)
-            arrive("empty", a)
         for q in range(4):
             wait("f_ready", 4 * n + q)
             arrive("f_free", 4 * n + q)
+            if q == 1 and not states:
+                if n:
+                    wait("o_free", n - 1)
+                arrive("in_done", n)
+                arrive("empty", a)
         arrive("x_done", n)
         arrive("empty", b)
         if not states:
