@@ -13,7 +13,6 @@
 //
 // Bound by HBM where there are enough parts: 128 KB per stretch, 3 us of an SM's share; products take 8 x 516 cycles = 2.2 us, and each group of warps less than that.
 #include <algorithm>
-#include <type_traits>
 
 #include "host.h"
 #include "linear.cuh"
@@ -22,23 +21,21 @@
 namespace mkda {
 namespace lt {
 
-using umma::mbar_wait;
 using umma::signal_tmem;
-using umma::wait_mma;
 
 constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 1024;
-constexpr int WARP_PAIRS = 0, WARP_FACTORS = 8, WARP_STATE = 16, WARP_OUT = 20, WARP_LOAD = 28, WARP_MMA = 29;
+constexpr int WARP_FACTORS = 8, WARP_STATE = 16, WARP_OUT = 20, WARP_LOAD = 28, WARP_MMA = 29;
 constexpr int P = 0, O = 128, X = 256, F = 384;            // tensor-memory columns: pairs, output, what goes into the state, f c (two buffers of a quarter: 3 x 16 columns each)
 // Registers: a thread of the state has 128 values of it.
-constexpr int LAUNCH_REGS = 64, WORK_REGS = 48, STATE_REGS = 160, ISSUE_REGS = 40;
-static_assert(6 * WORK_REGS + STATE_REGS + ISSUE_REGS <= 8 * LAUNCH_REGS, "registers of the launch");
+constexpr int LAUNCH_REGS = 64, WORK_REGS = 48, OUT_REGS = 56, STATE_REGS = 160, ISSUE_REGS = 40;
+static_assert(4 * WORK_REGS + 2 * OUT_REGS + STATE_REGS + ISSUE_REGS <= 8 * LAUNCH_REGS, "registers of the launch");
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
     uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free;
     uint32_t tmem;
-    // of the current part's head, a copy for each group of warps that reads it: scale lam^n and lam^(31 - e) (backwards lam^e); f; lam^n times the scale
-    __align__(16) float pair[C], column[32], factor[C], row[C + 4];
+    // of the current part's head, a copy for each group of warps that reads it: weights of the pairs by j - i + 128 (0 where a pair does not count), f, lam^n times the scale
+    __align__(16) float pair[2 * C], factor[C], row[C + 4];
 };
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
@@ -48,17 +45,37 @@ struct Plan {
     LinearCall call;
     int map_a[3], map_b[3], map_c[3];                      // per kind
     int wide[3];                                           // bf16 rows of the output leave in pieces of 32 bytes
-    long long items;
+    uint32_t items;
 };
 
+// Waits for the phase of `bar` with the given parity, at most `tries` times a microsecond; on expiry the status word is set, and the waits behind it are short.  umma::mbar_wait is longer
+// by a reading of the clock and a loop: the roles' code together is about as large as the instruction cache, and each runs through its own once a stretch.
+__device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, uint32_t& tries) {
+    for (uint32_t left = tries;; --left) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(umma::smem_u32(bar)), "r"(parity), "r"(1000u) : "memory");
+        if (ok) break;
+        if (left == 0) {
+            atomicExch(&umma::g_timeout_flag, 1u);
+            tries = 32;
+            break;
+        }
+    }
+}
+__device__ __forceinline__ void wait_mma(uint64_t* bar, uint32_t parity, uint32_t& tries) {
+    mbar_wait(bar, parity, tries);
+    umma::fence_after_sync();
+}
+
 struct Item { int kind, h, n, part; };
-__device__ __forceinline__ Item item_of(const LinearCall& call, long long w) {
+__device__ __forceinline__ Item item_of(const LinearCall& call, uint32_t w) {
     Item it;
-    it.kind = (int)(w % call.kinds);
-    w /= call.kinds;
-    it.h = (int)(w % call.HV);
-    w /= call.HV;
-    const int segs = call.S.seg ? call.S.segs : 1;
+    const uint32_t kinds = call.kinds, heads = call.HV, segs = call.S.seg ? call.S.segs : 1;
+    it.kind = (int)(w % kinds);
+    w /= kinds;
+    it.h = (int)(w % heads);
+    w /= heads;
     it.part = (int)(w % segs);
     const int n = (int)(w / segs);
     it.n = call.S.order ? call.S.order[n] : n;
@@ -67,7 +84,8 @@ __device__ __forceinline__ Item item_of(const LinearCall& call, long long w) {
 // Calls f(kind, item, part) for every item of this block that has something to do, the same ones in every role
 template <bool STATES, typename Body>
 __device__ __forceinline__ void for_items(const Plan& plan, Body body) {
-    for (long long w = blockIdx.x; w < plan.items; w += gridDim.x) {
+#pragma unroll 1
+    for (uint32_t w = blockIdx.x; w < plan.items; w += gridDim.x) {      // items + blocks stay below 2^32
         const Item it = item_of(plan.call, w);
         const LinearKind& k = plan.call.kind[it.kind];
         const LinearPart part = linear_part(plan.call.S, it.n, it.part, k.back);
@@ -137,6 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = sh.tmem;
+    uint32_t tries = 1u << 17;
     const LinearCall& call = plan.call;
     constexpr int PER = STATES ? 2 : 3;                    // tiles of a stretch: (a,) b, c
     auto slot_of = [](uint32_t tile) { return tile % SLOTS; };
@@ -149,11 +168,12 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 uint32_t tile = 0;
                 for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                     const int idx = it.kind;
+#pragma unroll 1
                     for (int t = 0; t < chunks; ++t) {
                         const int tok = part.start + first_of(k, chunks, t);
                         auto fetch = [&](int map, int head) {
                             const uint32_t s = slot_of(tile);
-                            if (tile >= SLOTS) mbar_wait(&sh.empty[s], parity_of(tile) ^ 1u);
+                            if (tile >= SLOTS) mbar_wait(&sh.empty[s], parity_of(tile) ^ 1u, tries);
                             umma::mbar_expect_tx(&sh.full[s], TILE);
                             load_box(ring + s * TILE, &maps.row[map], 0, head, tok, &sh.full[s]);
                             load_box(ring + s * TILE + TILE / 2, &maps.row[map], 64, head, tok, &sh.full[s]);
@@ -169,94 +189,81 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         } else if (warp == WARP_MMA) {
             if (umma::elect_one()) {
                 uint32_t n = 0;                                // stretches so far
-                // FULL: 128 channels in all heads, every loop unrolled; the address of a tile passes through an empty statement, or descriptors are kept over the loop and spilled
-                auto stretch = [&](auto full, int ms, int vn, bool from_zero) {
-                    constexpr bool FULL = decltype(full)::value;
-                    const uint32_t ta = n * PER, tb = ta + (STATES ? 0 : 1), tc = tb + 1, par = n & 1;
-                    const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, FULL ? C : vn), id_pc = umma::idesc_bf16(128, FULL ? C : vn, 0, 1),
-                                   id_x = umma::idesc_bf16(128, FULL ? C : ms * 16, 0, 1);
-                    auto k_major = [&](uint32_t addr) {
-                        asm volatile("" : "+r"(addr));
-                        return umma::make_desc(addr);
-                    };
-                    auto mn_major = [&](uint32_t addr) {
-                        asm volatile("" : "+r"(addr));
-                        return umma::make_desc(addr, TILE / 2 / 16);
-                    };
-                    auto k_step = [](int ks) { return (uint64_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
-                    auto mn_step = [](int ks) { return (uint64_t)(ks * 128); };
-                    const uint32_t ring_at = umma::smem_u32(ring), state_at = umma::smem_u32(state_hi);
-                    if (!STATES) mbar_wait(&sh.full[slot_of(ta)], parity_of(ta));
-                    mbar_wait(&sh.full[slot_of(tb)], parity_of(tb));
-                    if (!STATES) {
-                        const uint64_t ad = k_major(ring_at + slot_of(ta) * TILE), bd = k_major(ring_at + slot_of(tb) * TILE);
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)
-                            if (FULL || ks < ms) umma::mma_bf16(tmem + P, ad + k_step(ks), bd + k_step(ks), id_p0, ks != 0);
-                        umma::commit(&sh.p0_done);
-                    }
-                    wait_mma(&sh.s_ready, par);
-                    const uint64_t bm = mn_major(ring_at + slot_of(tb) * TILE);
-                    auto into_state = [&](int q) {         // 32 tokens: the smallest of the three parts of f c first
-                        wait_mma(&sh.f_ready[q & 1], (2 * n + (q >> 1)) & 1);
-#pragma unroll
-                        for (int part = 2; part >= 0; --part)
-#pragma unroll
-                            for (int ks = 0; ks < 2; ++ks)
-                                umma::mma_bf16_ta(tmem + X, tmem + F + 64 * (q & 1) + 16 * part + 8 * ks, bm + mn_step(2 * q + ks), id_x, q + ks != 0 || part != 2);
-                        umma::commit(&sh.f_free[q & 1]);
-                    };
-                    // The first half of X lies in front of the product with the state, which waits for the last stretch's output to be read; the second half's parts of f c are made beside it
-                    into_state(0);
-                    into_state(1);
-                    if (!STATES) {
-                        if (n) wait_mma(&sh.o_free, par ^ 1u);
-                        if (!from_zero) {
-                            const uint64_t ad = k_major(ring_at + slot_of(ta) * TILE), mh = k_major(state_at), ml = k_major(state_at + TILE);
-#pragma unroll
-                            for (int ks = 0; ks < 8; ++ks)
-                                if (FULL || ks < ms) {
-                                    umma::mma_bf16_fill(tmem + O, ad + k_step(ks), ml + k_step(ks), id_in, ks != 0);
-                                    umma::mma_bf16_lastuse(tmem + O, ad + k_step(ks), mh + k_step(ks), id_in, 1u);
-                                }
-                        }
-                        umma::commit(&sh.in_done);
-                        umma::commit(&sh.empty[slot_of(ta)]);
-                    }
-                    into_state(2);
-                    into_state(3);
-                    umma::commit(&sh.x_done);
-                    umma::commit(&sh.empty[slot_of(tb)]);
-                    if (!STATES) {
-                        wait_mma(&sh.p_ready, par);
-                        wait_mma(&sh.o_scaled, par);
-                        mbar_wait(&sh.full[slot_of(tc)], parity_of(tc));
-                        const uint64_t cd = mn_major(ring_at + slot_of(tc) * TILE);
-#pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) {
-                            const uint32_t at = tmem + P + 16 * ks;
-                            umma::mma_bf16_ta(tmem + O, at + 8, cd + mn_step(ks), id_pc, ks != 0 || !from_zero);
-                            umma::mma_bf16_ta(tmem + O, at, cd + mn_step(ks), id_pc, 1u);
-                        }
-                        umma::commit(&sh.o_done);
-                    }
-                    umma::commit(&sh.empty[slot_of(tc)]);
-                };
+                // Short loops: a product takes 65 cycles and an iteration less, while unrolled code of this and the other roles pushes each other out of the instruction caches
+                const uint64_t k_desc = umma::make_desc(0), mn_desc = umma::make_desc(0, TILE / 2 / 16);
+                const uint32_t ring_at = umma::smem_u32(ring) >> 4, state_at = umma::smem_u32(state_hi) >> 4;
+                auto tile_at = [&](uint32_t tile) { return ring_at + slot_of(tile) * (TILE / 16); };
+                auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
                 for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
                     const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
                     const bool zero = entering(call, k, it, STATES) == nullptr;
-                    if (ms == 8 && vn == C) {
-                        for (int t = 0; t < chunks; ++t, ++n) stretch(std::true_type(), ms, vn, zero && t == 0);
-                    } else {
-                        for (int t = 0; t < chunks; ++t, ++n) stretch(std::false_type(), ms, vn, zero && t == 0);
+                    const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, vn), id_pc = umma::idesc_bf16(128, vn, 0, 1), id_x = umma::idesc_bf16(128, ms * 16, 0, 1);
+#pragma unroll 1
+                    for (int t = 0; t < chunks; ++t, ++n) {
+                        const uint32_t ta = n * PER, tb = ta + (STATES ? 0 : 1), tc = tb + 1, par = n & 1;
+                        const bool from_zero = zero && t == 0;
+                        if (!STATES) mbar_wait(&sh.full[slot_of(ta)], parity_of(ta), tries);
+                        mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
+                        if (!STATES) {
+                            const uint64_t ad = k_desc | tile_at(ta), bd = k_desc | tile_at(tb);
+#pragma unroll 1
+                            for (int ks = 0; ks < ms; ++ks) umma::mma_bf16(tmem + P, ad + k_step(ks), bd + k_step(ks), id_p0, ks != 0);
+                            umma::commit(&sh.p0_done);
+                        }
+                        wait_mma(&sh.s_ready, par, tries);
+                        const uint64_t bm = mn_desc | tile_at(tb);
+                        // The first half of X lies in front of the product with the state, which waits for the last stretch's output to be read; the second half's parts of f c are
+                        // made beside it
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {
+                            if (!STATES && q == 2) {
+                                if (n) wait_mma(&sh.o_free, par ^ 1u, tries);
+                                if (!from_zero) {
+                                    const uint64_t ad = k_desc | tile_at(ta), m = k_desc | state_at;
+#pragma unroll 1
+                                    for (int ks = 0; ks < ms; ++ks) {
+                                        umma::mma_bf16_fill(tmem + O, ad + k_step(ks), m + TILE / 16 + k_step(ks), id_in, ks != 0);
+                                        umma::mma_bf16_lastuse(tmem + O, ad + k_step(ks), m + k_step(ks), id_in, 1u);
+                                    }
+                                }
+                                umma::commit(&sh.in_done);
+                                umma::commit(&sh.empty[slot_of(ta)]);
+                            }
+                            wait_mma(&sh.f_ready[q & 1], (2 * n + (q >> 1)) & 1, tries);
+#pragma unroll 1
+                            for (int ks = 0; ks < 2; ++ks) {       // 16 tokens: the smallest of the three parts of f c first
+                                const uint32_t at = tmem + F + 64 * (q & 1) + 8 * ks;
+                                const uint64_t bd = bm + 128 * (2 * q + ks);
+                                umma::mma_bf16_ta(tmem + X, at + 32, bd, id_x, q + ks != 0);
+                                umma::mma_bf16_ta(tmem + X, at + 16, bd, id_x, 1u);
+                                umma::mma_bf16_ta(tmem + X, at, bd, id_x, 1u);
+                            }
+                            umma::commit(&sh.f_free[q & 1]);
+                        }
+                        umma::commit(&sh.x_done);
+                        umma::commit(&sh.empty[slot_of(tb)]);
+                        if (!STATES) {
+                            wait_mma(&sh.p_ready, par, tries);
+                            wait_mma(&sh.o_scaled, par, tries);
+                            mbar_wait(&sh.full[slot_of(tc)], parity_of(tc), tries);
+                            const uint64_t cd = mn_desc | tile_at(tc);
+#pragma unroll 1
+                            for (int ks = 0; ks < 8; ++ks) {
+                                const uint32_t at = tmem + P + 16 * ks;
+                                umma::mma_bf16_ta(tmem + O, at + 8, cd + 128 * ks, id_pc, ks != 0 || !from_zero);
+                                umma::mma_bf16_ta(tmem + O, at, cd + 128 * ks, id_pc, 1u);
+                            }
+                            umma::commit(&sh.o_done);
+                        }
+                        umma::commit(&sh.empty[slot_of(tc)]);
                     }
                 });
-                if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1));      // the last arrival of a product
+                if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1), tries);      // the last arrival of a product
             }
             __syncwarp();
         }
     } else if (warp < WARP_FACTORS) {
-        // ---- pairs: row i = this lane's token, half of the columns.  Off the diagonal the weight is a factor of the row times one of the column, neither above 1
+        // ---- pairs: row i = this lane's token, half of the columns
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
         if (!STATES) {
             uint32_t n = 0;
@@ -264,12 +271,15 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                 const float gamma = call.log_decay[it.h];
                 group_sync(1);
-                if (half == 0) sh.pair[i] = decay_power(gamma, i) * k.pair_scale;
-                else if (i < 32) sh.column[i] = decay_power(gamma, k.back ? i : 31 - i);
+                {
+                    const int away = k.back ? tid - C : C - tid;
+                    sh.pair[tid] = away >= 0 && away < C ? decay_power(gamma, away) * k.pair_scale : 0.f;
+                }
                 group_sync(1);
+#pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int len = min(C, part.len - first_of(k, chunks, t));
-                    wait_mma(&sh.p0_done, n & 1);
+                    wait_mma(&sh.p0_done, n & 1, tries);
 #pragma unroll 1
                     for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
                         const uint32_t at = umma::tmem_addr(tmem, w, P + j0);
@@ -281,22 +291,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         }
                         float v[16];
                         umma::tmem_ld16(at, v);
-                        if (blk == w) {
+                        const float* weight = sh.pair + C + j0 - i;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int d = k.back ? j0 + e - i : i - j0 - e;
-                                v[e] = d >= 0 ? v[e] * sh.pair[max(d, 0)] : 0.f;
-                            }
-                        } else {
-                            const f32x2 r = both(sh.pair[k.back ? 32 * blk - i : i - 32 * blk - 31]);
-                            const float* column = sh.column + (j0 & 16);
-#pragma unroll
-                            for (int e = 0; e < 16; e += 4) {
-                                const float4 c = *reinterpret_cast<const float4*>(column + e);
-                                unpack2(mul2(pack2(v[e], v[e + 1]), mul2(r, pack2(c.x, c.y))), v[e], v[e + 1]);
-                                unpack2(mul2(pack2(v[e + 2], v[e + 3]), mul2(r, pack2(c.z, c.w))), v[e + 2], v[e + 3]);
-                            }
-                        }
+                        for (int e = 0; e < 16; ++e) v[e] = weight[e] == 0.f ? 0.f : v[e] * weight[e];      // what does not count may not be a number
                         if (k.back && j0 + 16 > len) {     // columns behind the part's end
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
@@ -326,6 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float gamma = call.log_decay[it.h];
             int factors_of = -1;                           // tokens that the table is for
+#pragma unroll 1
             for (int t = 0; t < chunks; ++t, ++n) {
                 const int len = min(C, part.len - first_of(k, chunks, t));
                 const uint32_t tb = n * PER + (STATES ? 0 : 1), tc = tb + 1;
@@ -336,10 +334,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     factors_of = len;
                     group_sync(2);
                 }
-                mbar_wait(&sh.full[slot_of(tc)], parity_of(tc));
+                mbar_wait(&sh.full[slot_of(tc)], parity_of(tc), tries);
                 if (len < C) {                             // rows behind the part's end belong to somebody else: 0 times what is not finite is not 0
                     uint8_t* const b = ring + slot_of(tb) * TILE;
-                    mbar_wait(&sh.full[slot_of(tb)], parity_of(tb));
+                    mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
                     for (int e = me; e < (C - len) * 16; e += 256) {
                         const uint32_t off = umma::tile_chunk_offset(128, len + (e >> 4), e & 15);
                         *reinterpret_cast<uint4*>(b + off) = make_uint4(0, 0, 0, 0);
@@ -369,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             part_[2][to] = as_bf16(x);
                         }
                     }
-                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1);
+                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1, tries);
 #pragma unroll
                     for (int p = 0; p < 3; ++p) tmem_st_16x16(umma::tmem_addr(tmem, w, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * half) << 16), part_[p]);
                     umma::tmem_wait_st();
@@ -383,50 +381,60 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGS));
         uint32_t n = 0;
         const int ch = tid - 32 * WARP_STATE;
-        f32x2 s[64];
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float* in = entering(call, k, it, STATES);
             const size_t size = (size_t)k.M * k.V;
             float* out = STATES ? k.parts + ((size_t)(it.n * call.S.segs + it.part + (k.back ? -1 : 1)) * call.HV + it.h) * size
                                 : k.last && part.leaves_last ? k.last + ((size_t)it.n * call.HV + it.h) * size : nullptr;
-            const float gamma = call.log_decay[it.h], whole = decay_power(gamma, C), rest = decay_power(gamma, part.len % C);
-            const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
-#pragma unroll
-            for (int m = 0; m < 128; m += 2) {
-                float v[2] = {0.f, 0.f};
-                if (in && ch < k.V) {
-                    if (m < k.M) v[0] = in[first + m * step];
-                    if (m + 1 < k.M) v[1] = in[first + (m + 1) * step];
-                }
-                s[m / 2] = pack2(v[0], v[1]);
+            const float gamma = call.log_decay[it.h];
+            float whole = 0.f, rest = 0.f;                 // lam to the tokens of a whole stretch and of the sequence's last one
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                whole = rest;
+                rest = decay_power(gamma, u ? part.len % C : C);
             }
-            __syncwarp();
+            // the state enters and leaves through the accumulator of X, so that what touches memory is a short loop
+            const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
+            f32x2 s[64];
+#pragma unroll
+            for (int m = 0; m < 64; ++m) s[m] = 0ull;
+            if (in) {
+#pragma unroll 1
+                for (int m0 = 0; m0 < (k.M + 15) / 16 * 16; m0 += 8) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = ch < k.V && m0 + e < k.M ? __float_as_uint(in[first + (m0 + e) * step]) : 0u;
+                    __syncwarp();
+                    umma::tmem_st8(umma::tmem_addr(tmem, warp, X + m0), v);
+                }
+                umma::tmem_wait_st();
+            }
+#pragma unroll 1
             for (int t = 0; t <= chunks; ++t) {
-                f32x2 f = both(1.f);
+                const bool add = t || in, store = !STATES && t < chunks && add;
+                f32x2 f = both(0.f);
                 if (t) {
                     const bool short_one = part.len - first_of(k, chunks, t - 1) < C;
                     f = both(short_one ? rest : whole);
-                    wait_mma(&sh.x_done, (n - 1) & 1);
+                    wait_mma(&sh.x_done, (n - 1) & 1, tries);
                 }
-                const bool store = !STATES && t < chunks && (t || in);
+                if (add) {
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    if (16 * g >= k.M) break;
-                    if (t) {
+                    for (int g = 0; g < 8; ++g) {
+                        if (16 * g >= k.M) break;
                         float x[16];
                         umma::tmem_ld16(umma::tmem_addr(tmem, warp, X + 16 * g), x);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) s[8 * g + e] = fma2(s[8 * g + e], f, pack2(x[2 * e], x[2 * e + 1]));
-                    }
-                    if (store) {
+                        if (!store) continue;
 #pragma unroll
                         for (int e = 0; e < 8; e += 4) {
                             uint32_t h[4], l[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                f32x2 x = s[8 * g + e + j];
-                                h[j] = take_bf16(x);
-                                l[j] = as_bf16(x);
+                                f32x2 y = s[8 * g + e + j];
+                                h[j] = take_bf16(y);
+                                l[j] = as_bf16(y);
                             }
                             uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 2 * g + e / 4);
                             *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -438,32 +446,43 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 umma::signal(&sh.s_ready, lane);
                 ++n;
             }
-            if (!out || ch >= k.V) return;
+            if (!out) return;
 #pragma unroll
-            for (int m = 0; m < 128; m += 2) {
-                float a, b;
-                unpack2(s[m / 2], a, b);
-                if (m < k.M) out[first + m * step] = a;
-                if (m + 1 < k.M) out[first + (m + 1) * step] = b;
+            for (int g = 0; g < 16; ++g) {
+                const f32x2 v[4] = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+                umma::tmem_st8(umma::tmem_addr(tmem, warp, X + 8 * g), v);
             }
+            umma::tmem_wait_st();
+#pragma unroll 1
+            for (int m0 = 0; m0 < k.M; m0 += 8) {
+                float v[8];
+                __syncwarp();
+                umma::tmem_ld8(umma::tmem_addr(tmem, warp, X + m0), v);
+                if (ch >= k.V) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (m0 + e < k.M) out[first + (m0 + e) * step] = v[e];
+            }
+            __syncwarp();
         });
     } else {
         // ---- the output: row i = this lane's token, half of the channels
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(OUT_REGS));
         if (!STATES) {
             uint32_t n = 0;
             const int w = warp & 3, half = (warp - WARP_OUT) >> 2, i = 32 * w + lane, m_first = 64 * half;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                 const float gamma = call.log_decay[it.h];
                 group_sync(3);
-                if (half == 0) sh.row[i] = decay_power(gamma, i) * k.state_scale;
-                else if (i == 0) sh.row[C] = decay_power(gamma, C) * k.state_scale;
+                const int me = tid - 32 * WARP_OUT;
+                if (me <= C) sh.row[me] = decay_power(gamma, me) * k.state_scale;
                 group_sync(3);
                 const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind], fp32 = k.out_dtype == MKDA_F32;
                 const int m_end = min(k.V, m_first + 64);
+#pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
-                    wait_mma(&sh.in_done, n & 1);
+                    wait_mma(&sh.in_done, n & 1, tries);
                     if (!zero || t) {
                         const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1]);
 #pragma unroll 1
@@ -482,30 +501,44 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         umma::tmem_wait_st();
                     }
                     signal_tmem(&sh.o_scaled, lane);
-                    wait_mma(&sh.o_done, n & 1);
+                    wait_mma(&sh.o_done, n & 1, tries);
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
+                    if (fp32) {
 #pragma unroll 1
-                    for (int m0 = m_first; m0 < m_first + 64; m0 += 16) {
-                        float v[16];
-                        __syncwarp();
-                        if (m0 < m_end) umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
-                        if (m0 == m_first + 48) signal_tmem(&sh.o_free, lane);
-                        if (i >= len || m0 >= m_end) continue;
-                        if (fp32) {
+                        for (int m0 = m_first; m0 < m_first + 64; m0 += 16) {
+                            float v[16];
+                            __syncwarp();
+                            if (m0 < m_end) umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
+                            if (m0 == m_first + 48) signal_tmem(&sh.o_free, lane);
+                            if (i >= len) continue;
                             float* to = static_cast<float*>(k.out) + row + m0;
 #pragma unroll
                             for (int e = 0; e < 16; e += 4)
                                 if (m0 + e < m_end) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                        } else {
-                            uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
-                            uint32_t u[8];
+                        }
+                    } else {
+                        // all that this thread has is read before the first piece is stored: the next product waits for the accumulator, not for the stores
+                        uint32_t u[32];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
-                            if (wide) {
-                                st32b(to, u);
-                            } else {
-                                *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
-                                if (m0 + 8 < m_end) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+                        for (int g = 0; g < 4; ++g) {
+                            float v[16];
+                            umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m_first + 16 * g), v);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) u[8 * g + e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                        }
+                        signal_tmem(&sh.o_free, lane);
+                        if (i < len) {
+                            uint16_t* to = static_cast<uint16_t*>(k.out) + row + m_first;
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                if (m_first + 16 * g >= m_end) break;
+                                const uint32_t p[8] = {u[8 * g], u[8 * g + 1], u[8 * g + 2], u[8 * g + 3], u[8 * g + 4], u[8 * g + 5], u[8 * g + 6], u[8 * g + 7]};
+                                if (wide) {
+                                    st32b(to + 16 * g, p);
+                                } else {
+                                    *reinterpret_cast<uint4*>(to + 16 * g) = make_uint4(p[0], p[1], p[2], p[3]);
+                                    if (m_first + 16 * g + 8 < m_end) *reinterpret_cast<uint4*>(to + 16 * g + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+                                }
                             }
                         }
                     }
@@ -522,8 +555,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 
 }  // namespace lt
 
+static long long linear_items(const LinearCall& call) { return (long long)call.S.N * (call.S.seg ? call.S.segs : 1) * call.HV * call.kinds; }
 bool linear_tc_takes(const LinearCall& call) {
-    if (call.dtype != MKDA_BF16 || call.S.TT < 1) return false;
+    if (call.dtype != MKDA_BF16 || call.S.TT < 1 || linear_items(call) > 0x7fffffff) return false;
     for (int i = 0; i < call.kinds; ++i) {
         const LinearKind& k = call.kind[i];
         if (k.M % 8 || k.V % 8 || (k.a && (k.a_stride % 8 || !aligned16(k.a))) || k.b_stride % 8 || k.c_stride % 8 || !aligned16(k.b) || !aligned16(k.c)) return false;
@@ -553,13 +587,13 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
         plan.wide[i] = k.V % 16 == 0 && !any_misaligned32(k.out);
     }
     if (rc != MKDA_OK) return rc;
-    plan.items = (long long)call.S.N * (call.S.seg ? call.S.segs : 1) * call.HV * call.kinds;
+    plan.items = (uint32_t)linear_items(call);
     auto* kern = states ? lt::linear_tc_kernel<true> : lt::linear_tc_kernel<false>;
     rc = ensure_smem(reinterpret_cast<const void*>(kern), lt::SMEM, "linear");
     if (rc != MKDA_OK) return rc;
     static const int regs = std::min(kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<true>)), kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<false>)));
     if (regs < lt::LAUNCH_REGS) return set_error(MKDA_ERR_LAUNCH, "linear: built with fewer registers than its warps redistribute");
-    launch(kern, dim3((unsigned)std::min<long long>(plan.items, sm_count())), lt::THREADS, lt::SMEM, stream, plan, maps);
+    launch(kern, dim3((unsigned)std::min<uint32_t>(plan.items, sm_count())), lt::THREADS, lt::SMEM, stream, plan, maps);
     return check_launch("linear");
 }
 int linear_tc_status(unsigned int* out) { return cudaMemcpyFromSymbol(out, umma::g_timeout_flag, sizeof(unsigned int)) == cudaSuccess ? 0 : -1; }
