@@ -8,8 +8,8 @@
 //   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts, so that the state, fp32 in registers, is exact to 32 bits
 // a, b and c are exact in bf16.  Two halves (2^-16) are enough where the result is rounded to bf16, one would show: P and M in one bf16 each are as far off as the result's own rounding.
 //
-// Roles, joined by mbarriers: a warp that fetches rows into a ring of five tiles, one that issues products, and four warps each for the pairs' weights, for f c, for the state and
-// for the output.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
+// Roles, joined by mbarriers: a warp that fetches rows into a ring of five tiles, one that issues products, and eight warps each for the pairs' weights and the output, for f c and for
+// the state.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
 //
 // Bound by HBM where there are enough parts: 128 KB per stretch, 3 us of an SM's share; products take 8 x 516 cycles = 2.2 us, and each group of warps less than that.
 #include <algorithm>
@@ -23,12 +23,12 @@ namespace lt {
 
 using umma::signal_tmem;
 
-constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 1024;
-constexpr int WARP_FACTORS = 8, WARP_STATE = 16, WARP_OUT = 20, WARP_LOAD = 28, WARP_MMA = 29;
+constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 896;
+constexpr int WARP_FACTORS = 8, WARP_STATE = 16, WARP_LOAD = 24, WARP_MMA = 25;
 constexpr int P = 0, O = 128, X = 256, F = 384;            // tensor-memory columns: pairs, output, what goes into the state, f c (two buffers of a quarter: 3 x 16 columns each)
-// Registers: a thread of the state has 128 values of it.
-constexpr int LAUNCH_REGS = 64, WORK_REGS = 48, OUT_REGS = 56, STATE_REGS = 160, ISSUE_REGS = 40;
-static_assert(4 * WORK_REGS + 2 * OUT_REGS + STATE_REGS + ISSUE_REGS <= 8 * LAUNCH_REGS, "registers of the launch");
+// Registers: a thread of the state has 64 values of it.
+constexpr int LAUNCH_REGS = 72, FACTOR_REGS = 48, STATE_REGS = 104, ISSUE_REGS = 56;
+static_assert(2 * (LAUNCH_REGS + FACTOR_REGS + STATE_REGS) + ISSUE_REGS <= 7 * LAUNCH_REGS, "registers of the launch");
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
@@ -128,6 +128,10 @@ __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int 
                  :: "r"(umma::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(umma::smem_u32(bar)) : "memory");
 }
 
+// Whether a state of 32 bits leaves: f c then has three parts, else two, as the state that only meets bf16 rows needs no more
+template <bool STATES>
+__device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
+
 // STATES: nothing but what the parts of cut sequences make of a zero state
 template <bool STATES>
 __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_constant__ Plan plan, const __grid_constant__ Maps maps) {
@@ -146,8 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < SLOTS; ++i) { umma::mbar_init(&sh.full[i], 1); umma::mbar_init(&sh.empty[i], 1); }
         for (uint64_t* b : {&sh.p0_done, &sh.f_free[0], &sh.f_free[1], &sh.x_done, &sh.in_done, &sh.o_done}) umma::mbar_init(b, 1);
-        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.o_scaled, &sh.o_free}) umma::mbar_init(b, 8);
-        umma::mbar_init(&sh.s_ready, 4);
+        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free}) umma::mbar_init(b, 8);
         umma::fence_barrier_init();
     }
     follow_stream();
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
                 for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
                     const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
-                    const bool zero = entering(call, k, it, STATES) == nullptr;
+                    const bool zero = entering(call, k, it, STATES) == nullptr, exact = exact_state<STATES>(k);
                     const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, vn), id_pc = umma::idesc_bf16(128, vn, 0, 1), id_x = umma::idesc_bf16(128, ms * 16, 0, 1);
 #pragma unroll 1
                     for (int t = 0; t < chunks; ++t, ++n) {
@@ -234,8 +237,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             for (int ks = 0; ks < 2; ++ks) {       // 16 tokens: the smallest of the three parts of f c first
                                 const uint32_t at = tmem + F + 64 * (q & 1) + 8 * ks;
                                 const uint64_t bd = bm + 128 * (2 * q + ks);
-                                umma::mma_bf16_ta(tmem + X, at + 32, bd, id_x, q + ks != 0);
-                                umma::mma_bf16_ta(tmem + X, at + 16, bd, id_x, 1u);
+                                if (exact) umma::mma_bf16_ta(tmem + X, at + 32, bd, id_x, q + ks != 0);
+                                umma::mma_bf16_ta(tmem + X, at + 16, bd, id_x, exact || q + ks != 0);
                                 umma::mma_bf16_ta(tmem + X, at, bd, id_x, 1u);
                             }
                             umma::commit(&sh.f_free[q & 1]);
@@ -263,22 +266,26 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             __syncwarp();
         }
     } else if (warp < WARP_FACTORS) {
-        // ---- pairs: row i = this lane's token, half of the columns
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
+        // ---- pairs and output: row i = this lane's token, half of the columns
         if (!STATES) {
             uint32_t n = 0;
-            const int w = warp & 3, half = warp >> 2, i = 32 * w + lane;
+            const int w = warp & 3, half = warp >> 2, i = 32 * w + lane, m_first = 64 * half;
             for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
                 const float gamma = call.log_decay[it.h];
                 group_sync(1);
-                {
-                    const int away = k.back ? tid - C : C - tid;
-                    sh.pair[tid] = away >= 0 && away < C ? decay_power(gamma, away) * k.pair_scale : 0.f;
+#pragma unroll 1
+                for (int u = 0; u < 2; ++u) {
+                    const int away = u ? tid : k.back ? tid - C : C - tid;
+                    const float power = away >= 0 && away <= C ? decay_power(gamma, away) : 0.f;
+                    if (u == 0) sh.pair[tid] = away < C ? power * k.pair_scale : 0.f;
+                    else if (tid <= C) sh.row[tid] = power * k.state_scale;
                 }
                 group_sync(1);
+                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind], fp32 = k.out_dtype == MKDA_F32;
+                const int m_end = min(k.V, m_first + 64);
 #pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
-                    const int len = min(C, part.len - first_of(k, chunks, t));
+                    const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
                     wait_mma(&sh.p0_done, n & 1, tries);
 #pragma unroll 1
                     for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
@@ -311,177 +318,6 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     }
                     umma::tmem_wait_st();
                     signal_tmem(&sh.p_ready, lane);
-                }
-            });
-        }
-    } else if (warp < WARP_STATE) {
-        // ---- f c, transposed: row = channel of c, 16 of them a warp.  Blocks of 8 tokens x 8 channels come transposed out of shared memory, in the layout that 16 rows of tensor
-        // memory take
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(WORK_REGS));
-        uint32_t n = 0;
-        const int me = tid - 32 * WARP_FACTORS, w = warp & 3, half = (warp - WARP_FACTORS) >> 2;
-        for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-            const float gamma = call.log_decay[it.h];
-            int factors_of = -1;                           // tokens that the table is for
-#pragma unroll 1
-            for (int t = 0; t < chunks; ++t, ++n) {
-                const int len = min(C, part.len - first_of(k, chunks, t));
-                const uint32_t tb = n * PER + (STATES ? 0 : 1), tc = tb + 1;
-                uint8_t* const c = ring + slot_of(tc) * TILE;
-                if (len != factors_of) {
-                    group_sync(2);
-                    if (me < C) sh.factor[me] = me < len ? decay_power(gamma, k.back ? me + 1 : len - 1 - me) * k.in_scale : 0.f;
-                    factors_of = len;
-                    group_sync(2);
-                }
-                mbar_wait(&sh.full[slot_of(tc)], parity_of(tc), tries);
-                if (len < C) {                             // rows behind the part's end belong to somebody else: 0 times what is not finite is not 0
-                    uint8_t* const b = ring + slot_of(tb) * TILE;
-                    mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
-                    for (int e = me; e < (C - len) * 16; e += 256) {
-                        const uint32_t off = umma::tile_chunk_offset(128, len + (e >> 4), e & 15);
-                        *reinterpret_cast<uint4*>(b + off) = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(c + off) = make_uint4(0, 0, 0, 0);
-                    }
-                    umma::fence_async_smem();
-                    group_sync(2);
-                    __syncwarp();
-                }
-                const uint32_t rows = umma::smem_u32(c);
-#pragma unroll 1
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t use = 2 * n + (q >> 1);         // of this buffer
-                    uint32_t part_[3][8];
-#pragma unroll
-                    for (int g2 = 0; g2 < 2; ++g2) {       // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
-                        uint32_t r[4];
-                        const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * half) / 8 + ((lane >> 3) & 1);
-                        load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
-                            const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
-                            f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f);
-                            const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
-                            part_[0][to] = take_bf16(x);
-                            part_[1][to] = take_bf16(x);
-                            part_[2][to] = as_bf16(x);
-                        }
-                    }
-                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1, tries);
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) tmem_st_16x16(umma::tmem_addr(tmem, w, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * half) << 16), part_[p]);
-                    umma::tmem_wait_st();
-                    signal_tmem(&sh.f_ready[q & 1], lane);
-                }
-            }
-        });
-    } else if (warp < WARP_OUT) {
-        // ---- the state: row = this lane's channel of c, columns the channels of b, in registers.  What a stretch adds comes from an accumulator of its own: the tensor cores cut off what
-        // does not fit into 32 bits, and over a long sequence's products that is an error of one sign (2.5e-6 of the state behind 32 k tokens, this way 0.4e-6).
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGS));
-        uint32_t n = 0;
-        const int ch = tid - 32 * WARP_STATE;
-        for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-            const float* in = entering(call, k, it, STATES);
-            const size_t size = (size_t)k.M * k.V;
-            float* out = STATES ? k.parts + ((size_t)(it.n * call.S.segs + it.part + (k.back ? -1 : 1)) * call.HV + it.h) * size
-                                : k.last && part.leaves_last ? k.last + ((size_t)it.n * call.HV + it.h) * size : nullptr;
-            const float gamma = call.log_decay[it.h];
-            float whole = 0.f, rest = 0.f;                 // lam to the tokens of a whole stretch and of the sequence's last one
-#pragma unroll 1
-            for (int u = 0; u < 2; ++u) {
-                whole = rest;
-                rest = decay_power(gamma, u ? part.len % C : C);
-            }
-            // the state enters and leaves through the accumulator of X, so that what touches memory is a short loop
-            const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
-            f32x2 s[64];
-#pragma unroll
-            for (int m = 0; m < 64; ++m) s[m] = 0ull;
-            if (in) {
-#pragma unroll 1
-                for (int m0 = 0; m0 < (k.M + 15) / 16 * 16; m0 += 8) {
-                    uint32_t v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = ch < k.V && m0 + e < k.M ? __float_as_uint(in[first + (m0 + e) * step]) : 0u;
-                    __syncwarp();
-                    umma::tmem_st8(umma::tmem_addr(tmem, warp, X + m0), v);
-                }
-                umma::tmem_wait_st();
-            }
-#pragma unroll 1
-            for (int t = 0; t <= chunks; ++t) {
-                const bool add = t || in, store = !STATES && t < chunks && add;
-                f32x2 f = both(0.f);
-                if (t) {
-                    const bool short_one = part.len - first_of(k, chunks, t - 1) < C;
-                    f = both(short_one ? rest : whole);
-                    wait_mma(&sh.x_done, (n - 1) & 1, tries);
-                }
-                if (add) {
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        if (16 * g >= k.M) break;
-                        float x[16];
-                        umma::tmem_ld16(umma::tmem_addr(tmem, warp, X + 16 * g), x);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) s[8 * g + e] = fma2(s[8 * g + e], f, pack2(x[2 * e], x[2 * e + 1]));
-                        if (!store) continue;
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4) {
-                            uint32_t h[4], l[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                f32x2 y = s[8 * g + e + j];
-                                h[j] = take_bf16(y);
-                                l[j] = as_bf16(y);
-                            }
-                            uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 2 * g + e / 4);
-                            *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
-                        }
-                    }
-                }
-                if (t == chunks) break;
-                umma::signal(&sh.s_ready, lane);
-                ++n;
-            }
-            if (!out) return;
-#pragma unroll
-            for (int g = 0; g < 16; ++g) {
-                const f32x2 v[4] = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
-                umma::tmem_st8(umma::tmem_addr(tmem, warp, X + 8 * g), v);
-            }
-            umma::tmem_wait_st();
-#pragma unroll 1
-            for (int m0 = 0; m0 < k.M; m0 += 8) {
-                float v[8];
-                __syncwarp();
-                umma::tmem_ld8(umma::tmem_addr(tmem, warp, X + m0), v);
-                if (ch >= k.V) continue;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (m0 + e < k.M) out[first + (m0 + e) * step] = v[e];
-            }
-            __syncwarp();
-        });
-    } else {
-        // ---- the output: row i = this lane's token, half of the channels
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(OUT_REGS));
-        if (!STATES) {
-            uint32_t n = 0;
-            const int w = warp & 3, half = (warp - WARP_OUT) >> 2, i = 32 * w + lane, m_first = 64 * half;
-            for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
-                const float gamma = call.log_decay[it.h];
-                group_sync(3);
-                const int me = tid - 32 * WARP_OUT;
-                if (me <= C) sh.row[me] = decay_power(gamma, me) * k.state_scale;
-                group_sync(3);
-                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind], fp32 = k.out_dtype == MKDA_F32;
-                const int m_end = min(k.V, m_first + 64);
-#pragma unroll 1
-                for (int t = 0; t < chunks; ++t, ++n) {
-                    const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
                     wait_mma(&sh.in_done, n & 1, tries);
                     if (!zero || t) {
                         const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1]);
@@ -546,6 +382,164 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 }
             });
         }
+    } else if (warp < WARP_STATE) {
+        // ---- f c, transposed: row = channel of c, 16 of them a warp.  Blocks of 8 tokens x 8 channels come transposed out of shared memory, in the layout that 16 rows of tensor
+        // memory take
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(FACTOR_REGS));
+        uint32_t n = 0;
+        const int me = tid - 32 * WARP_FACTORS, w = warp & 3, half = (warp - WARP_FACTORS) >> 2;
+        for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
+            const float gamma = call.log_decay[it.h];
+            const bool exact = exact_state<STATES>(k);
+            int factors_of = -1;                           // tokens that the table is for
+#pragma unroll 1
+            for (int t = 0; t < chunks; ++t, ++n) {
+                const int len = min(C, part.len - first_of(k, chunks, t));
+                const uint32_t tb = n * PER + (STATES ? 0 : 1), tc = tb + 1;
+                uint8_t* const c = ring + slot_of(tc) * TILE;
+                if (len != factors_of) {
+                    group_sync(2);
+                    if (me < C) sh.factor[me] = me < len ? decay_power(gamma, k.back ? me + 1 : len - 1 - me) * k.in_scale : 0.f;
+                    factors_of = len;
+                    group_sync(2);
+                }
+                mbar_wait(&sh.full[slot_of(tc)], parity_of(tc), tries);
+                if (len < C) {                             // rows behind the part's end belong to somebody else: 0 times what is not finite is not 0
+                    uint8_t* const b = ring + slot_of(tb) * TILE;
+                    mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
+                    for (int e = me; e < (C - len) * 16; e += 256) {
+                        const uint32_t off = umma::tile_chunk_offset(128, len + (e >> 4), e & 15);
+                        *reinterpret_cast<uint4*>(b + off) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(c + off) = make_uint4(0, 0, 0, 0);
+                    }
+                    umma::fence_async_smem();
+                    group_sync(2);
+                    __syncwarp();
+                }
+                const uint32_t rows = umma::smem_u32(c);
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t use = 2 * n + (q >> 1);         // of this buffer
+                    uint32_t part_[3][8];
+#pragma unroll
+                    for (int g2 = 0; g2 < 2; ++g2) {       // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
+                        uint32_t r[4];
+                        const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * half) / 8 + ((lane >> 3) & 1);
+                        load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
+                            const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
+                            f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f);
+                            const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
+                            part_[0][to] = take_bf16(x);
+                            if (exact) {
+                                part_[1][to] = take_bf16(x);
+                                part_[2][to] = as_bf16(x);
+                            } else {
+                                part_[1][to] = as_bf16(x);
+                            }
+                        }
+                    }
+                    if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1, tries);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        if (p < 2 || exact) tmem_st_16x16(umma::tmem_addr(tmem, w, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * half) << 16), part_[p]);
+                    umma::tmem_wait_st();
+                    signal_tmem(&sh.f_ready[q & 1], lane);
+                }
+            }
+        });
+    } else {
+        // ---- the state: row = this lane's channel of c, half of the channels of b as columns, in registers.  What a stretch adds comes from an accumulator of its own: the tensor cores cut off what
+        // does not fit into 32 bits, and over a long sequence's products that is an error of one sign (2.5e-6 of the state behind 32 k tokens, this way 0.4e-6).
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGS));
+        uint32_t n = 0;
+        const int w = warp & 3, half = (warp - WARP_STATE) >> 2, ch = 32 * w + lane, m_first = 64 * half;
+        for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
+            const float* in = entering(call, k, it, STATES);
+            const size_t size = (size_t)k.M * k.V;
+            float* out = STATES ? k.parts + ((size_t)(it.n * call.S.segs + it.part + (k.back ? -1 : 1)) * call.HV + it.h) * size
+                                : k.last && part.leaves_last ? k.last + ((size_t)it.n * call.HV + it.h) * size : nullptr;
+            const float gamma = call.log_decay[it.h];
+            float whole = 0.f, rest = 0.f;                 // lam to the tokens of a whole stretch and of the sequence's last one
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                whole = rest;
+                rest = decay_power(gamma, u ? part.len % C : C);
+            }
+            // the state enters and leaves through the accumulator of X, so that what touches memory is a short loop
+            const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
+            f32x2 s[32];
+            const int m_end = min(k.M, m_first + 64);
+#pragma unroll
+            for (int m = 0; m < 32; ++m) s[m] = 0ull;
+            if (in) {
+#pragma unroll 1
+                for (int m0 = m_first; m0 < (m_end + 15) / 16 * 16; m0 += 8) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = ch < k.V && m0 + e < k.M ? __float_as_uint(in[first + (m0 + e) * step]) : 0u;
+                    __syncwarp();
+                    umma::tmem_st8(umma::tmem_addr(tmem, w, X + m0), v);
+                }
+                umma::tmem_wait_st();
+            }
+#pragma unroll 1
+            for (int t = 0; t <= chunks; ++t) {
+                const bool add = t || in, store = !STATES && t < chunks && add;
+                f32x2 f = both(0.f);
+                if (t) {
+                    const bool short_one = part.len - first_of(k, chunks, t - 1) < C;
+                    f = both(short_one ? rest : whole);
+                    wait_mma(&sh.x_done, (n - 1) & 1, tries);
+                }
+                if (add) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (m_first + 16 * g >= m_end) break;
+                        float x[16];
+                        umma::tmem_ld16(umma::tmem_addr(tmem, w, X + m_first + 16 * g), x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[8 * g + e] = fma2(s[8 * g + e], f, pack2(x[2 * e], x[2 * e + 1]));
+                        if (!store) continue;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            uint32_t h[4], l[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                f32x2 y = s[8 * g + e + j];
+                                h[j] = take_bf16(y);
+                                l[j] = as_bf16(y);
+                            }
+                            uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 8 * half + 2 * g + e / 4);
+                            *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                        }
+                    }
+                }
+                if (t == chunks) break;
+                umma::signal(&sh.s_ready, lane);
+                ++n;
+            }
+            if (!out) return;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                const f32x2 v[4] = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+                umma::tmem_st8(umma::tmem_addr(tmem, w, X + m_first + 8 * g), v);
+            }
+            umma::tmem_wait_st();
+#pragma unroll 1
+            for (int m0 = m_first; m0 < m_end; m0 += 8) {
+                float v[8];
+                __syncwarp();
+                umma::tmem_ld8(umma::tmem_addr(tmem, w, X + m0), v);
+                if (ch >= k.V) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (m0 + e < k.M) out[first + (m0 + e) * step] = v[e];
+            }
+            __syncwarp();
+        });
     }
     umma::fence_before_sync();
     __syncthreads();

@@ -17,7 +17,7 @@ def linear_kernel(states):
     members = re.search(r"struct Shared \{(.*?)\n\};", text, re.S)[1]
     found = {n: ring if d == "SLOTS" else int(d or 1) for line in re.findall(r"uint64_t ([^;]*);", members) for n, d in re.findall(r"(\w+)(?:\[(\w+)\])?", line)}
     r = Roles(found)
-    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free"), 2))      # of the four warps two, one of which may be late
+    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free"), 2))      # of the eight warps two, one of which may be late
     per, stretches = (2 if states else 3), [(p, t, c) for p, c in enumerate(PARTS) for t in range(c)]
     load = r.agent("load")
     for tile in range(per * len(stretches)):
@@ -52,12 +52,10 @@ def linear_kernel(states):
     wait("empty", len(stretches) * per - 1)
     for w in range(2):
         if not states:
-            wait, arrive = r.agent(f"pairs {w}")
+            wait, arrive = r.agent(f"rows {w}")
             for n in range(len(stretches)):
                 wait("p0_done", n)
                 arrive("p_ready", n)
-            wait, arrive = r.agent(f"output {w}")
-            for n in range(len(stretches)):
                 wait("in_done", n)
                 arrive("o_scaled", n)
                 wait("o_done", n)
