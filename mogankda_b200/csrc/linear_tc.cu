@@ -24,7 +24,7 @@ namespace lt {
 using umma::signal_tmem;
 
 constexpr int C = 128, TILE = 32768, SLOTS = 5, THREADS = 896;
-constexpr int WARP_FACTORS = 8, WARP_STATE = 16, WARP_LOAD = 24, WARP_MMA = 25;
+constexpr int WARP_FACTORS = 8, WARP_STATE = 16, WARP_LOAD = 24, WARP_MMA = 25, WARP_STORE = 26;
 constexpr int P = 0, O = 128, X = 256, F = 384;            // tensor-memory columns: pairs, output, what goes into the state, f c (two buffers of a quarter: 3 x 16 columns each)
 // Registers: a thread of the state has 64 values of it.
 constexpr int LAUNCH_REGS = 72, FACTOR_REGS = 48, STATE_REGS = 104, ISSUE_REGS = 56;
@@ -32,7 +32,7 @@ static_assert(2 * (LAUNCH_REGS + FACTOR_REGS + STATE_REGS) + ISSUE_REGS <= 7 * L
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
-    uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free;
+    uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free, o_staged[2];
     uint32_t tmem;
     // of the current part's head, a copy for each group of warps that reads it: weights of the pairs by j - i + 128 (0 where a pair does not count), f, lam^n times the scale
     __align__(16) float pair[2 * C], factor[C], row[C + 4];
@@ -40,11 +40,10 @@ struct Shared {
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
 
-struct Maps { CUtensorMap row[4]; };                       // rows of a head, boxes of 64 channels x 128 tokens
+struct Maps { CUtensorMap row[4], out[3]; };               // rows of a head, boxes of 64 channels x 128 tokens; out per kind
 struct Plan {
     LinearCall call;
     int map_a[3], map_b[3], map_c[3];                      // per kind
-    int wide[3];                                           // bf16 rows of the output leave in pieces of 32 bytes
     uint32_t items;
 };
 
@@ -128,6 +127,12 @@ __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int 
                  :: "r"(umma::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(umma::smem_u32(bar)) : "memory");
 }
 
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int head, int token, const void* src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 :: "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(umma::smem_u32(src)) : "memory");
+}
+// Whether rows leave as a tiled copy: of a whole stretch in bf16 (rows behind a short one's end are another sequence's)
+__device__ __forceinline__ bool staged(const LinearKind& k, int left) { return left >= C && k.out_dtype == MKDA_BF16; }
 // Whether a state of 32 bits leaves: f c then has three parts, else two, as the state that only meets bf16 rows needs no more
 template <bool STATES>
 __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
@@ -150,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < SLOTS; ++i) { umma::mbar_init(&sh.full[i], 1); umma::mbar_init(&sh.empty[i], 1); }
         for (uint64_t* b : {&sh.p0_done, &sh.f_free[0], &sh.f_free[1], &sh.x_done, &sh.in_done, &sh.o_done}) umma::mbar_init(b, 1);
-        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free}) umma::mbar_init(b, 8);
+        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free, &sh.o_staged[0], &sh.o_staged[1]}) umma::mbar_init(b, 8);
         umma::fence_barrier_init();
     }
     follow_stream();
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             umma::commit(&sh.f_free[q & 1]);
                         }
                         umma::commit(&sh.x_done);
-                        umma::commit(&sh.empty[slot_of(tb)]);
+                        if (STATES) umma::commit(&sh.empty[slot_of(tb)]);
                         if (!STATES) {
                             wait_mma(&sh.p_ready, par, tries);
                             wait_mma(&sh.o_scaled, par, tries);
@@ -264,6 +269,28 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1), tries);      // the last arrival of a product
             }
             __syncwarp();
+        } else if (!STATES && warp == WARP_STORE) {
+            // The rows of a whole stretch are put down in the place of its b, which the products are through with, and leave as a tiled copy: stored from registers, 32 rows at a time, they
+            // kept the load / store units busy for 3000 of 8000 cycles
+            if (umma::elect_one()) {
+                uint32_t n = 0;
+                for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
+#pragma unroll 1
+                    for (int t = 0; t < chunks; ++t, ++n) {
+                        const int c0 = first_of(k, chunks, t);
+                        const uint32_t slot = slot_of(n * PER + 1);
+                        mbar_wait(&sh.o_staged[n & 1], (n >> 1) & 1, tries);
+                        if (staged(k, part.len - c0)) {
+                            store_box(&maps.out[it.kind], 0, it.h, part.start + c0, ring + slot * TILE);
+                            if (k.V > 64) store_box(&maps.out[it.kind], 64, it.h, part.start + c0, ring + slot * TILE + TILE / 2);
+                            umma::bulk_store_commit();
+                            umma::bulk_store_wait_read();
+                        }
+                        umma::arrive(&sh.empty[slot]);
+                    }
+                });
+            }
+            __syncwarp();
         }
     } else if (warp < WARP_FACTORS) {
         // ---- pairs and output: row i = this lane's token, half of the columns
@@ -281,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     else if (tid <= C) sh.row[tid] = power * k.state_scale;
                 }
                 group_sync(1);
-                const bool zero = entering(call, k, it, STATES) == nullptr, wide = plan.wide[it.kind], fp32 = k.out_dtype == MKDA_F32;
+                const bool zero = entering(call, k, it, STATES) == nullptr, fp32 = k.out_dtype == MKDA_F32;
                 const int m_end = min(k.V, m_first + 64);
 #pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
@@ -339,42 +366,43 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1, tries);
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
-                    if (fp32) {
+                    if (staged(k, part.len - c0)) {
+                        uint8_t* const to = ring + slot_of(n * PER + 1) * TILE;
+#pragma unroll 1
+                        for (int m0 = m_first; m0 < m_end; m0 += 16) {
+                            float v[16];
+                            umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
+                            uint32_t u[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                            *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, m0 >> 3)) = make_uint4(u[0], u[1], u[2], u[3]);
+                            *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, (m0 >> 3) + 1)) = make_uint4(u[4], u[5], u[6], u[7]);
+                        }
+                        signal_tmem(&sh.o_free, lane);
+                        umma::signal(&sh.o_staged[n & 1], lane);
+                    } else {
 #pragma unroll 1
                         for (int m0 = m_first; m0 < m_first + 64; m0 += 16) {
                             float v[16];
                             __syncwarp();
                             if (m0 < m_end) umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
-                            if (m0 == m_first + 48) signal_tmem(&sh.o_free, lane);
-                            if (i >= len) continue;
-                            float* to = static_cast<float*>(k.out) + row + m0;
+                            if (m0 == m_first + 48) {
+                                signal_tmem(&sh.o_free, lane);
+                                signal_tmem(&sh.o_staged[n & 1], lane);
+                            }
+                            if (i >= len || m0 >= m_end) continue;
+                            if (fp32) {
+                                float* to = static_cast<float*>(k.out) + row + m0;
 #pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                if (m0 + e < m_end) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                        }
-                    } else {
-                        // all that this thread has is read before the first piece is stored: the next product waits for the accumulator, not for the stores
-                        uint32_t u[32];
+                                for (int e = 0; e < 16; e += 4)
+                                    if (m0 + e < m_end) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                            } else {
+                                uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
+                                uint32_t u[8];
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            float v[16];
-                            umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m_first + 16 * g), v);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) u[8 * g + e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
-                        }
-                        signal_tmem(&sh.o_free, lane);
-                        if (i < len) {
-                            uint16_t* to = static_cast<uint16_t*>(k.out) + row + m_first;
-#pragma unroll
-                            for (int g = 0; g < 4; ++g) {
-                                if (m_first + 16 * g >= m_end) break;
-                                const uint32_t p[8] = {u[8 * g], u[8 * g + 1], u[8 * g + 2], u[8 * g + 3], u[8 * g + 4], u[8 * g + 5], u[8 * g + 6], u[8 * g + 7]};
-                                if (wide) {
-                                    st32b(to + 16 * g, p);
-                                } else {
-                                    *reinterpret_cast<uint4*>(to + 16 * g) = make_uint4(p[0], p[1], p[2], p[3]);
-                                    if (m_first + 16 * g + 8 < m_end) *reinterpret_cast<uint4*>(to + 16 * g + 8) = make_uint4(p[4], p[5], p[6], p[7]);
-                                }
+                                for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                                *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+                                if (m0 + 8 < m_end) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
                             }
                         }
                     }
@@ -578,7 +606,7 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
         plan.map_a[i] = k.a ? map(k.a, k.a_stride, k.a_per, k.M) : 0;
         plan.map_b[i] = map(k.b, k.b_stride, k.b_per, k.M);
         plan.map_c[i] = map(k.c, k.c_stride, k.c_per, k.V);
-        plan.wide[i] = k.V % 16 == 0 && !any_misaligned32(k.out);
+        if (rc == MKDA_OK && !states && k.out_dtype == MKDA_BF16) rc = make_heads_map(&maps.out[i], k.out, call.S.TT, call.HV, k.V, (long long)call.HV * k.V, "linear");
     }
     if (rc != MKDA_OK) return rc;
     plan.items = (uint32_t)linear_items(call);

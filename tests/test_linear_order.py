@@ -17,7 +17,7 @@ def linear_kernel(states):
     members = re.search(r"struct Shared \{(.*?)\n\};", text, re.S)[1]
     found = {n: ring if d == "SLOTS" else int(d or 1) for line in re.findall(r"uint64_t ([^;]*);", members) for n, d in re.findall(r"(\w+)(?:\[(\w+)\])?", line)}
     r = Roles(found)
-    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free"), 2))      # of the eight warps two, one of which may be late
+    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free", "o_staged"), 2))      # of the eight warps two, one of which may be late
     per, stretches = (2 if states else 3), [(p, t, c) for p, c in enumerate(PARTS) for t in range(c)]
     load = r.agent("load")
     for tile in range(per * len(stretches)):
@@ -42,7 +42,8 @@ def linear_kernel(states):
                 arrive("in_done", n)
                 arrive("empty", a)
         arrive("x_done", n)
-        arrive("empty", b)
+        if states:
+            arrive("empty", b)
         if not states:
             wait("p_ready", n)
             wait("o_scaled", n)
@@ -50,6 +51,11 @@ def linear_kernel(states):
             arrive("o_done", n)
         arrive("empty", c)
     wait("empty", len(stretches) * per - 1)
+    if not states:
+        wait, arrive = r.agent("store")
+        for n in range(len(stretches)):
+            wait("o_staged", n)
+            arrive("empty", n * per + 1)
     for w in range(2):
         if not states:
             wait, arrive = r.agent(f"rows {w}")
@@ -60,6 +66,7 @@ def linear_kernel(states):
                 arrive("o_scaled", n)
                 wait("o_done", n)
                 arrive("o_free", n)
+                arrive("o_staged", n)
         wait, arrive = r.agent(f"factors {w}")
         for n, (_, t, chunks) in enumerate(stretches):
             wait("full", n * per + per - 1)
