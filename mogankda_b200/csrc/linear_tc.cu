@@ -80,11 +80,14 @@ __device__ __forceinline__ Item item_of(const LinearCall& call, uint32_t w) {
     it.n = call.S.order ? call.S.order[n] : n;
     return it;
 }
-// Calls f(kind, item, part) for every item of this block that has something to do, the same ones in every role
+// Calls body(kind, item, part, stretches) for every item of this block that has something to do, the same ones in every role.  The longest sequences come first; every other round of
+// the blocks runs the other way, so that who got the longest of one gets the shortest of the next (11 documents of 204 to 1712 tokens x 48: 28 stretches for the busiest block, 24 so).
 template <bool STATES, typename Body>
 __device__ __forceinline__ void for_items(const Plan& plan, Body body) {
 #pragma unroll 1
-    for (uint32_t w = blockIdx.x; w < plan.items; w += gridDim.x) {      // items + blocks stay below 2^32
+    for (uint32_t round = 0; round * gridDim.x < plan.items; ++round) {      // items + blocks stay below 2^32
+        const uint32_t w = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (w >= plan.items) continue;
         const Item it = item_of(plan.call, w);
         const LinearKind& k = plan.call.kind[it.kind];
         const LinearPart part = linear_part(plan.call.S, it.n, it.part, k.back);

@@ -8,16 +8,26 @@ namespace {
 // ---- linear attention ------------------------------------------------------------------------------------------------------------------------
 enum { LQ, LK, LV, LDECAY, LH0, LINEAR_INPUTS };
 
-// Cuts long sequences into parts that run side by side where there are fewer chains (sequences x v-heads x kinds of results) than SMs.
-void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t chains_per_sequence, int64_t state) {
+// Cuts long sequences into parts of `seg` tokens that run side by side, where there are too few chains (sequences x v-heads x kinds of results) for the SMs or where they fill
+// them unevenly: the cheapest of all lengths of parts by what a stretch of 128 tokens costs an SM, in us (128 channels), against no cut.  A cut costs a pass over all parts but one
+// that finds what they make of nothing (`kinds_before` of them), and the traffic of their states, 2.6 times in and out.
+//   one sequence of 32749 tokens, 32 heads: uncut 1060 us, parts of 64 stretches 373, of 29 (what the rule takes) see below
+void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t heads, int kinds, int kinds_before, int64_t state, bool tensor_cores) {
     if (q.longest < 512 || s.N == 0) return;
-    const double side_by_side = chains_per_sequence * std::max(1.0, (double)s.TT / q.longest);      // chains that are busy as long as the longest sequence runs
-    const int64_t want = (int64_t)(sms() / side_by_side);
-    if (want < 2) return;
-    const int64_t seg = std::max<int64_t>(256, ((q.longest + want - 1) / want + 127) / 128 * 128), segs = (q.longest + seg - 1) / seg;
-    if (2 * seg > q.longest || s.N * segs * state * 4 > (int64_t)256 << 20) return;
-    s.seg = (int)seg;
-    s.segs = (int)segs;
+    const double main = tensor_cores ? 4.2 : 28.0, before = tensor_cores ? 1.9 : 9.0, launch = 8.0, state_us = 4.0 * 4 * state * kinds_before / heads / 5e6;      // per part and head
+    const int64_t longest = (q.longest + 127) / 128, most = std::max<int64_t>(longest, (s.TT + 127) / 128), n_sm = sms();
+    auto rounds = [&](int64_t items) { return (items + n_sm - 1) / n_sm; };
+    double best = std::max<double>(longest, (double)most * heads * kinds / n_sm) * main;
+    for (int64_t parts = 2; parts <= longest / 2; ++parts) {
+        const int64_t seg = (longest + parts - 1) / parts, all = (most + seg - 1) / seg;      // parts with tokens, about
+        if (s.N * parts * state * 4 > (int64_t)256 << 20) break;
+        const double us = (rounds(all * heads * kinds) * main + rounds(std::max<int64_t>(0, all - 1) * heads * kinds_before) * before) * seg + launch + all * heads * state_us + 0.002 * s.N * parts * heads;
+        if (us < 0.97 * best) {
+            best = us;
+            s.seg = (int)(seg * 128);
+            s.segs = (int)((longest + seg - 1) / seg);
+        }
+    }
 }
 
 // What a call hands to the library; the tensors behind the pointers are kept in `hold`.
@@ -52,7 +62,7 @@ variable_list linear_backward(const Sequences& q, double scale, const variable_l
     LinearCall call(q, s, scale);
     MkdaLinearBwd p{};
     const at::Device dev = s[LQ].device();
-    cut_linear(call.p.S, q, 3ll * call.p.HV, (int64_t)call.p.HV * call.p.K * call.p.V);
+    cut_linear(call.p.S, q, call.p.HV, 3, 2, (int64_t)call.p.HV * call.p.K * call.p.V, s[LQ].scalar_type() == at::kBFloat16);
     p.f = call.p;
     const Tensor dy = grads[0].defined() ? aligned(grads[0]) : at::zeros_like(s[LV], at::MemoryFormat::Contiguous);
     const Tensor dht = grads.size() > 1 && grads[1].defined() ? aligned(grads[1]) : Tensor();
@@ -128,7 +138,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             o = out_like(v, q.covers_all);
             if (want) last = new_cuda({q.s.N, HV, K, V}, at::kFloat, v.device());
             call.p.o = o.data_ptr(); call.p.ht = fmptr(last);
-            cut_linear(call.p.S, q, HV, HV * K * V);
+            cut_linear(call.p.S, q, HV, 1, 1, HV * K * V, v.scalar_type() == at::kBFloat16);
             Tensor seg_h;
             if (call.p.S.seg) {
                 seg_h = call.parts(v.device());
