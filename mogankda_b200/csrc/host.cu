@@ -72,17 +72,17 @@ static CUresult with_context(F encode) {
     return r;
 }
 
-int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what) {
+int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what, int elem_bytes) {
     const Encode encode = encoder(what);
     if (!encode) return MKDA_ERR_LAUNCH;
     if ((reinterpret_cast<uintptr_t>(base) & 15) || dim % 8 || stride % 8 || stride < 0 || tokens == 0) {
         snprintf(g_err, sizeof(g_err), "%s: tensor not 16-byte aligned for tiled copies", what);
         return MKDA_ERR_ARG;
     }
-    const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, tokens}, gstride[2] = {(cuuint64_t)dim * 2, (cuuint64_t)stride * 2};
-    const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+    const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, tokens}, gstride[2] = {(cuuint64_t)dim * elem_bytes, (cuuint64_t)stride * elem_bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / elem_bytes), 1, 128}, estr[3] = {1, 1, 1};
     const CUresult r = with_context([&] {
-        return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        return encode(out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     });
     if (r != CUDA_SUCCESS) {

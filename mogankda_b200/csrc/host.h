@@ -21,9 +21,9 @@ int kernel_registers(const void* func);
 // described (base not 16-byte aligned, row pitch not a multiple of 16 bytes, or the driver lacks the encoder).
 int make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, unsigned long long rows, unsigned long long row_elems, const char* what,
                   int box_rows = 64, int box_cols = 128);
-// Tensor map over bf16 rows [tokens][heads][dim] with `stride` elements between tokens (heads one behind the other, dim and stride multiples of 8): boxes of 64 channels of one
-// head x 128 tokens with the 128-byte swizzle, a column block of an operand tile.  Channels past the head's and tokens past the last one read as zeros.
-int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what);
+// Tensor map over rows [tokens][heads][dim] with `stride` elements between tokens (heads one behind the other, dim and stride multiples of 8): boxes of 128 bytes (64 channels of 2 bytes,
+// 32 of 4) of one head x 128 tokens with the 128-byte swizzle, a column block of an operand tile.  Channels past the head's and tokens past the last one read as zeros and are not written.
+int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what, int elem_bytes = 2);
 // True if any of the (possibly null) pointers is not 16-byte aligned: the kernels read and write their tensors with
 // 16-byte vector accesses and bulk copies, and a misaligned address would fault the device instead of returning an error.
 template <typename... P>

@@ -134,8 +134,6 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int hea
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
                  :: "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(umma::smem_u32(src)) : "memory");
 }
-// Whether rows leave as a tiled copy: of a whole stretch in bf16 (rows behind a short one's end are another sequence's)
-__device__ __forceinline__ bool staged(const LinearKind& k, int left) { return left >= C && k.out_dtype == MKDA_BF16; }
 // Whether a state of 32 bits leaves: f c then has three parts, else two, as the state that only meets bf16 rows needs no more
 template <bool STATES>
 __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
@@ -171,6 +169,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     constexpr int PER = STATES ? 2 : 3;                    // tiles of a stretch: (a,) b, c
     auto slot_of = [](uint32_t tile) { return tile % SLOTS; };
     auto parity_of = [](uint32_t tile) { return (tile / SLOTS) & 1u; };
+    // where rows of the output lie before they leave, in blocks of 128 bytes of each row: bf16 in the place of b, fp32 from channel 64 on in that of c
+    auto staging = [&](uint32_t n, bool fp32, int channel) {
+        return fp32 ? ring + slot_of(n * PER + 1 + (channel >> 6)) * TILE + ((channel >> 5) & 1) * (TILE / 2) : ring + slot_of(n * PER + 1) * TILE + (channel >> 6) * (TILE / 2);
+    };
 
     if (warp >= WARP_LOAD) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(ISSUE_REGS));
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
                 for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
                     const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
-                    const bool zero = entering(call, k, it, STATES) == nullptr, exact = exact_state<STATES>(k);
+                    const bool zero = entering(call, k, it, STATES) == nullptr, exact = exact_state<STATES>(k), fp32 = k.out_dtype == MKDA_F32;
                     const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, vn), id_pc = umma::idesc_bf16(128, vn, 0, 1), id_x = umma::idesc_bf16(128, ms * 16, 0, 1);
 #pragma unroll 1
                     for (int t = 0; t < chunks; ++t, ++n) {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             }
                             umma::commit(&sh.o_done);
                         }
-                        umma::commit(&sh.empty[slot_of(tc)]);
+                        if (STATES || !fp32) umma::commit(&sh.empty[slot_of(tc)]);
                     }
                 });
                 if (n) mbar_wait(&sh.empty[slot_of(n * PER - 1)], parity_of(n * PER - 1), tries);      // the last arrival of a product
@@ -283,13 +285,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         const int c0 = first_of(k, chunks, t);
                         const uint32_t slot = slot_of(n * PER + 1);
                         mbar_wait(&sh.o_staged[n & 1], (n >> 1) & 1, tries);
-                        if (staged(k, part.len - c0)) {
-                            store_box(&maps.out[it.kind], 0, it.h, part.start + c0, ring + slot * TILE);
-                            if (k.V > 64) store_box(&maps.out[it.kind], 64, it.h, part.start + c0, ring + slot * TILE + TILE / 2);
+                        const bool fp32 = k.out_dtype == MKDA_F32;
+                        const int box = fp32 ? 32 : 64;
+                        if (part.len - c0 >= C) {          // rows behind a short stretch's end are another sequence's
+#pragma unroll 1
+                            for (int m0 = 0; m0 < k.V; m0 += box) store_box(&maps.out[it.kind], m0, it.h, part.start + c0, staging(n, fp32, m0));
                             umma::bulk_store_commit();
                             umma::bulk_store_wait_read();
                         }
                         umma::arrive(&sh.empty[slot]);
+                        if (fp32) umma::arrive(&sh.empty[slot_of(n * PER + 2)]);
                     }
                 });
             }
@@ -369,17 +374,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1, tries);
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
-                    if (staged(k, part.len - c0)) {
-                        uint8_t* const to = ring + slot_of(n * PER + 1) * TILE;
+                    if (len == C) {
 #pragma unroll 1
                         for (int m0 = m_first; m0 < m_end; m0 += 16) {
                             float v[16];
                             umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
-                            uint32_t u[8];
+                            uint8_t* const to = staging(n, fp32, m0);
+                            if (fp32) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
-                            *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, m0 >> 3)) = make_uint4(u[0], u[1], u[2], u[3]);
-                            *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, (m0 >> 3) + 1)) = make_uint4(u[4], u[5], u[6], u[7]);
+                                for (int e = 0; e < 4; ++e)
+                                    *reinterpret_cast<float4*>(to + umma::tile_chunk_offset(128, i, ((m0 & 31) >> 2) + e)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                            } else {
+                                uint32_t u[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                                *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, (m0 & 63) >> 3)) = make_uint4(u[0], u[1], u[2], u[3]);
+                                *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, ((m0 & 63) >> 3) + 1)) = make_uint4(u[4], u[5], u[6], u[7]);
+                            }
                         }
                         signal_tmem(&sh.o_free, lane);
                         umma::signal(&sh.o_staged[n & 1], lane);
@@ -609,7 +620,7 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
         plan.map_a[i] = k.a ? map(k.a, k.a_stride, k.a_per, k.M) : 0;
         plan.map_b[i] = map(k.b, k.b_stride, k.b_per, k.M);
         plan.map_c[i] = map(k.c, k.c_stride, k.c_per, k.V);
-        if (rc == MKDA_OK && !states && k.out_dtype == MKDA_BF16) rc = make_heads_map(&maps.out[i], k.out, call.S.TT, call.HV, k.V, (long long)call.HV * k.V, "linear");
+        if (rc == MKDA_OK && !states) rc = make_heads_map(&maps.out[i], k.out, call.S.TT, call.HV, k.V, (long long)call.HV * k.V, "linear", k.out_dtype == MKDA_F32 ? 4 : 2);
     }
     if (rc != MKDA_OK) return rc;
     plan.items = (uint32_t)linear_items(call);
