@@ -123,6 +123,21 @@ int kernel_registers(const void* func) {
     return a.numRegs;
 }
 
+int resident(const void* func, int threads) {
+    struct Known { const void* func; int blocks; };
+    static Known known[256];
+    static int count = 0;
+    static std::mutex mutex;
+    std::lock_guard<std::mutex> lock(mutex);
+    for (int i = 0; i < count; ++i)
+        if (known[i].func == func) return known[i].blocks;
+    int blocks = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, func, threads, 0) != cudaSuccess) (void)cudaGetLastError();
+    if (blocks < 1) blocks = 1;
+    if (count < 256) known[count++] = Known{func, blocks};
+    return blocks;
+}
+
 int ensure_smem(const void* func, int bytes, const char* what) {
     // (function, device) pairs whose limit is already raised; a launcher asks before every launch.  Launches come from several threads: callers
     // that have released the GIL, and the autograd engine's thread of each device.

@@ -10,14 +10,14 @@
 
 namespace mkda {
 
-constexpr int LN_FWD_THREADS = 1024, LN_BWD_THREADS = 1024;      // per SM
+constexpr int LN_BWD_THREADS = 768;                        // per SM
 
 template <int DT, int RDT, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) layer_norm_fwd_kernel(const MkdaLayerNormFwd p, const bool vec, const bool wvec) {
     follow_stream();
     constexpr int RPB = TPR < 128 ? 128 / TPR : 1, RT = RDT < 0 ? DT : RDT;
     constexpr bool AHEAD = TPR <= 512, KEEP = AHEAD && NV <= 2;      // a thread of 1024 has registers neither for the next row nor for the weights
-    __shared__ __align__(16) float part[2][TPR / 32][1], part2[2][TPR / 32][1];
+    __shared__ __align__(16) float part[2][TPR < 32 ? 1 : TPR / 32][1], part2[2][TPR < 32 ? 1 : TPR / 32][1];
     const int tid = threadIdx.x % TPR, W = p.width / p.groups, g0 = blockIdx.y * W;
     const long long stride = (long long)gridDim.x * RPB;
     const float over = 1.f / (float)W;
@@ -49,9 +49,12 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) layer_norm_fwd_kerne
             if constexpr (RDT >= 0) rr[i] = load8<RT>(p.residual, (size_t)row * p.res_stride + g0 + c, ok, vec);
         }
     };
-    long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    // A block's rows go together: where parts share a warp, those behind the last row are zeros that nobody stores, and take part in the sums' exchanges
+    const long long mine = threadIdx.x / TPR;
+    long long base = (long long)blockIdx.x * RPB, row = base + mine;
     if (AHEAD) request(row);
-    for (int turn = 0; row < p.rows; row += stride, turn ^= 1) {      // rows of a block end together, or a row is a warp
+    for (int turn = 0; base < p.rows; base += stride, row = base + mine, turn ^= 1) {
+        const bool real = row < p.rows;
         if (!AHEAD) request(row);
         float s[NV][8], sum[1] = {0.f};
 #pragma unroll
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) layer_norm_fwd_kerne
                 unpack8<RT>(rr[i], r);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[i][e] = as_held<RT>(s[i][e] + r[e]);
-                store8<RT>(p.sum, (size_t)row * p.width + g0 + c, min(W - c, 8), vec, s[i]);
+                store8<RT>(p.sum, (size_t)row * p.width + g0 + c, real ? min(W - c, 8) : 0, vec, s[i]);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[0] += s[i][e];           // zeros behind the part's end
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) layer_norm_fwd_kerne
         }
         row_reduce<TPR, 1, false>(sq, part2[turn]);
         const float r = rsqrtf(fmaf(sq[0], over, p.eps));
-        if (p.stats && tid == 0) *reinterpret_cast<float2*>(p.stats + 2 * ((size_t)row * p.groups + blockIdx.y)) = make_float2(m, r);
+        if (p.stats && tid == 0 && real) *reinterpret_cast<float2*>(p.stats + 2 * ((size_t)row * p.groups + blockIdx.y)) = make_float2(m, r);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8;
@@ -91,21 +94,21 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, 1) layer_norm_fwd_kerne
             if constexpr (!KEEP) params(c, v, u);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[i][e] = fmaf(s[i][e] * r, KEEP ? w[KEEP ? i : 0][e] : v[e], KEEP ? b[KEEP ? i : 0][e] : u[e]);
-            store8<DT>(p.y, (size_t)row * p.width + g0 + c, min(W - c, 8), vec, s[i]);
+            store8<DT>(p.y, (size_t)row * p.width + g0 + c, real ? min(W - c, 8) : 0, vec, s[i]);
         }
     }
 }
 
 // RT: the type of what was normalised and of the stream beside it.  As in norm.cu pieces stay as they lie in memory until they are used, and the weights are in shared memory.
 template <int DT, int RT, int TPR, int NV, bool vec>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 128 ? 6 : TPR == 1024 ? 1 : 768 / TPR) layer_norm_bwd_kernel(const MkdaLayerNormBwd p, const bool wvec) {
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR <= 128 ? 6 : TPR == 1024 ? 1 : 768 / TPR) layer_norm_bwd_kernel(const MkdaLayerNormBwd p, const bool wvec) {
     follow_stream();
     constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
     constexpr bool AHEAD = NV == 1;
-    __shared__ __align__(16) float part[2][TPR / 32][2];
+    __shared__ __align__(16) float part[2][TPR < 32 ? 1 : TPR / 32][2];
     extern __shared__ __align__(16) float norm_w[];        // [TPR * NV * 8]
     const int tid = threadIdx.x % TPR, W = p.width / p.groups, g0 = blockIdx.y * W;
-    const long long first = (long long)blockIdx.x * RPB + threadIdx.x / TPR, stride = (long long)gridDim.x * RPB;
+    const long long mine = threadIdx.x / TPR, stride = (long long)gridDim.x * RPB;
     const float over = 1.f / (float)W;
     for (int c = threadIdx.x * 8; c < TPR * NV * 8; c += blockDim.x * 8) {
         float w[8];
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
     Raw8 rs[NV], rg[NV], ru[NV];
     float2 rm = make_float2(0.f, 0.f);
     auto request = [&](long long row) {
-        if (row < p.rows) rm = *reinterpret_cast<const float2*>(p.stats + 2 * ((size_t)row * p.groups + blockIdx.y));
+        rm = row < p.rows ? *reinterpret_cast<const float2*>(p.stats + 2 * ((size_t)row * p.groups + blockIdx.y)) : make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8, ok = row < p.rows ? W - c : 0;
@@ -135,9 +138,10 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
             if (p.dsum) ru[i] = load8<RT>(p.dsum, (size_t)row * p.width + g0 + c, ok, vec);
         }
     };
-    if (AHEAD) request(first);
-    int turn = 0;
-    for (long long row = first; row < p.rows; row += stride, turn ^= 1) {
+    long long base = (long long)blockIdx.x * RPB, row = base + mine;      // a block's rows go together, as in the forward kernel
+    if (AHEAD) request(row);
+    for (int turn = 0; base < p.rows; base += stride, row = base + mine, turn ^= 1) {
+        const bool real = row < p.rows;
         if (!AHEAD) request(row);
         Raw8 qs[NV], qg[NV], qu[NV];
         const float m = rm.x, r = rm.y;
@@ -174,8 +178,9 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
                 o[e] = r * (fmaf(g[e], w[e], -m1) - h * m2);
                 if (p.dsum) o[e] += u[e];
             }
-            store8<DT>(p.dx, (size_t)row * p.width + g0 + c, min(W - c, 8), vec, o);
-            if (p.dres) store8<RT>(p.dres, (size_t)row * p.width + g0 + c, min(W - c, 8), vec, o);
+            const int keep = real ? min(W - c, 8) : 0;
+            store8<DT>(p.dx, (size_t)row * p.width + g0 + c, keep, vec, o);
+            if (p.dres) store8<RT>(p.dres, (size_t)row * p.width + g0 + c, keep, vec, o);
         }
     }
     if (!p.part) return;
@@ -209,12 +214,23 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 32 ? 5 : TPR == 
     leave(db, to + p.width);
 }
 
-// Blocks of a group that walk the rows: as many as are resident over all groups
-template <int TPR, int THREADS>
-static int group_blocks(int rows, int groups) {
-    const int all = norm_blocks<TPR, THREADS>(0x7fffffff), want = norm_blocks<TPR, THREADS>(rows);
-    return std::max(1, std::min(want, (all + groups - 1) / groups));
+// Threads of a part: narrow ones share a warp (heads of 128 channels by whole warps, half of them idle: forward 49 us, backward 83, where this takes 28 and 55)
+template <bool BWD, typename F>
+static bool with_part_width(int W, F f) {
+    using std::integral_constant;
+    if (W <= 64) f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    else if (W <= 128) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else return BWD ? with_width_bwd(W, f) : with_width(W, f);
+    return true;
 }
+// Blocks of a group that walk the rows, of `most` that are resident over all groups
+template <int TPR>
+static int group_blocks(int rows, int groups, int most) {
+    constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
+    return std::max(1, std::min((int)(((long long)rows + RPB - 1) / RPB), (most + groups - 1) / groups));
+}
+template <int TPR>
+static int bwd_blocks(int rows, int groups) { return group_blocks<TPR>(rows, groups, sm_count() * (TPR == 1024 ? 1 : LN_BWD_THREADS / (TPR < 128 ? 128 : TPR))); }
 
 }  // namespace mkda
 
@@ -237,10 +253,10 @@ extern "C" int mkda_layer_norm_fwd(const MkdaLayerNormFwd* p, void* stream) {
     const bool vec = W % 8 == 0 && p->x_stride % 8 == 0 && (!p->residual || p->res_stride % 8 == 0) && aligned16(p->x) && aligned16(p->residual) && aligned16(p->sum) && aligned16(p->y);
     const bool wvec = W % 8 == 0 && aligned16(p->weight) && aligned16(p->bias);
     with_dtype(p->dtype, [&](auto dt) {
-        with_width(W, [&](auto t, auto n) {
-            constexpr int DT = decltype(dt)::value, TPR = decltype(t)::value, NV = decltype(n)::value;
+        with_part_width<false>(W, [&](auto t, auto n) {
+            constexpr int DT = decltype(dt)::value, TPR = decltype(t)::value, NV = decltype(n)::value, THREADS = TPR < 128 ? 128 : TPR;
             auto* kern = !p->residual ? layer_norm_fwd_kernel<DT, -1, TPR, NV> : p->res_dtype == DT ? layer_norm_fwd_kernel<DT, DT, TPR, NV> : layer_norm_fwd_kernel<DT, MKDA_F32, TPR, NV>;
-            launch(kern, dim3(group_blocks<TPR, LN_FWD_THREADS>(p->rows, p->groups), p->groups), TPR < 128 ? 128 : TPR, 0, (cudaStream_t)stream, *p, vec, wvec);
+            launch(kern, dim3(group_blocks<TPR>(p->rows, p->groups, sm_count() * resident(reinterpret_cast<const void*>(kern), THREADS)), p->groups), THREADS, 0, (cudaStream_t)stream, *p, vec, wvec);
         });
     });
     return check_launch("layer_norm_fwd");
@@ -249,7 +265,7 @@ extern "C" int mkda_layer_norm_fwd(const MkdaLayerNormFwd* p, void* stream) {
 extern "C" int mkda_layer_norm_bwd_part_rows(int rows, int width, int groups) {
     int r = 0;
     if (bad_shape(rows, width, groups)) return 0;
-    with_width_bwd(width / groups, [&](auto t, auto) { r = group_blocks<decltype(t)::value, LN_BWD_THREADS>(rows, groups); });
+    with_part_width<true>(width / groups, [&](auto t, auto) { r = bwd_blocks<decltype(t)::value>(rows, groups); });
     return r;
 }
 
@@ -267,13 +283,13 @@ extern "C" int mkda_layer_norm_bwd(const MkdaLayerNormBwd* p, void* stream) {
     const bool vec = W % 8 == 0 && p->s_stride % 8 == 0 && aligned16(p->s) && aligned16(p->dy) && aligned16(p->dsum) && aligned16(p->dx) && aligned16(p->dres);
     const bool wvec = W % 8 == 0 && aligned16(p->weight);
     with_dtype(p->dtype, [&](auto dt) {
-        with_width_bwd(W, [&](auto t, auto n) {
+        with_part_width<true>(W, [&](auto t, auto n) {
             constexpr int DT = decltype(dt)::value, TPR = decltype(t)::value, NV = decltype(n)::value;
             auto* kern = p->s_dtype == DT ? vec ? layer_norm_bwd_kernel<DT, DT, TPR, NV, true> : layer_norm_bwd_kernel<DT, DT, TPR, NV, false>
                                           : vec ? layer_norm_bwd_kernel<DT, MKDA_F32, TPR, NV, true> : layer_norm_bwd_kernel<DT, MKDA_F32, TPR, NV, false>;
             constexpr int smem = TPR * NV * 8 * 4 * (TPR < 128 ? 1 + 128 / TPR : 1);
             if (smem > 40000) rc = ensure_smem(reinterpret_cast<const void*>(kern), smem, "layer_norm_bwd");
-            if (rc == MKDA_OK) launch(kern, dim3(group_blocks<TPR, LN_BWD_THREADS>(p->rows, p->groups), p->groups), TPR < 128 ? 128 : TPR, smem, (cudaStream_t)stream, *p, wvec);
+            if (rc == MKDA_OK) launch(kern, dim3(bwd_blocks<TPR>(p->rows, p->groups), p->groups), TPR < 128 ? 128 : TPR, smem, (cudaStream_t)stream, *p, wvec);
         });
     });
     if (rc != MKDA_OK) return rc;

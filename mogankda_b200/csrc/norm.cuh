@@ -12,11 +12,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Sums (or maxima) of N = 1 or 2 values over the TPR threads of a row, the same in all of them; `part` is shared memory that two calls later may be used again
+// Sums (or maxima) of N = 1 or 2 values over the TPR threads of a row (neighbouring lanes where they are fewer than 32), the same in all of them; `part` is shared memory that two calls
+// later may be used again
 template <int TPR, int N, bool MAX>
 __device__ __forceinline__ void row_reduce(float (&v)[N], float (*part)[N]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const float w = __shfl_xor_sync(0xffffffffu, v[k], o);
