@@ -23,8 +23,9 @@ __device__ __forceinline__ float2 turn(const MkdaRotary& p, long long token, int
     return make_float2(c, p.inverse ? -s : s);
 }
 
-// VEC: pairs in pieces of eight, 16-byte accesses; else pair by pair.
-template <int DT, bool VEC>
+// VEC: pairs in pieces of eight, 16-byte accesses; else pair by pair.  A thread has the same piece of every head that it takes, and goes on from head to head without a division
+// (one for the token and one for the head of each piece took as long as the bytes: 32749 tokens x 40 heads 195 us).
+template <int DT, bool VEC, bool NEIGHBOURS>
 __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const MkdaRotary p, const int per_block) {
     follow_stream();
     extern __shared__ __align__(16) float2 turns[];        // [per_block][freqs]
@@ -34,73 +35,80 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const MkdaRotary
     for (int e = threadIdx.x; e < n * F; e += ROTARY_THREADS) turns[e] = turn(p, first + e / F, e % F);
     __syncthreads();
     constexpr int P = VEC ? 8 : 1;
-    const int pairs = F / P, rest = (D - 2 * F) / P, units = pairs + rest, per_token = heads * units, all = n * per_token;
-    for (int base = threadIdx.x; base < all; base += ROTARY_BATCH * ROTARY_THREADS) {
-        Raw8 ra[ROTARY_BATCH], rb[ROTARY_BATCH];
-        float fa[ROTARY_BATCH], fb[ROTARY_BATCH];
-        int tok[ROTARY_BATCH], unit[ROTARY_BATCH];
-        size_t to[ROTARY_BATCH];
-        bool of_k[ROTARY_BATCH];
+    const int pairs = F / P, units = pairs + (D - 2 * F) / P;      // pieces of a head: of pairs, then of channels that stay
+    const int at_once = max(1, ROTARY_THREADS / units);            // heads that the block takes together
+    for (int unit = threadIdx.x % min(units, ROTARY_THREADS); unit < units; unit += ROTARY_THREADS) {
+        int tok = 0, h = threadIdx.x / min(units, ROTARY_THREADS);
+        if (h >= at_once) break;                                   // threads that are left over
+        const bool turned = unit < pairs;
+        const int a = turned ? (NEIGHBOURS ? 2 : 1) * P * unit : 2 * F + P * (unit - pairs), b = a + (NEIGHBOURS ? P : F);
+        auto settle = [&] {
+            while (h >= heads) { h -= heads; ++tok; }
+        };
+        settle();
+        while (tok < n) {
+            Raw8 ra[ROTARY_BATCH], rb[ROTARY_BATCH];
+            float fa[ROTARY_BATCH], fb[ROTARY_BATCH];
+            int toks[ROTARY_BATCH];
+            char* to[ROTARY_BATCH];
+            constexpr int SIZE = DT == MKDA_F32 ? 4 : 2;
 #pragma unroll
-        for (int i = 0; i < ROTARY_BATCH; ++i) {
-            const int u = base + i * ROTARY_THREADS;
-            tok[i] = -1;
-            if (u >= all) continue;
-            tok[i] = u / per_token;
-            const int in = u - tok[i] * per_token, h = in / units;
-            unit[i] = in - h * units;
-            of_k[i] = h >= p.heads_q;
-            const int hh = of_k[i] ? h - p.heads_q : h;
-            const void* from = of_k[i] ? p.k : p.q;
-            const size_t at = (size_t)(first + tok[i]) * (of_k[i] ? p.k_stride : p.q_stride) + (size_t)hh * D;
-            to[i] = ((size_t)(first + tok[i]) * (of_k[i] ? p.heads_k : p.heads_q) + hh) * D;
-            const bool turned = unit[i] < pairs;
-            const int a = turned ? (p.interleaved ? 2 : 1) * P * unit[i] : 2 * F + P * (unit[i] - pairs), b = a + (p.interleaved ? P : F);
-            if constexpr (VEC) {
-                ldraw8<DT>(from, at + a, ra[i]);
-                if (turned) ldraw8<DT>(from, at + b, rb[i]);
-            } else {
-                fa[i] = ld1(from, DT, at + a);
-                if (turned) fb[i] = ld1(from, DT, at + b);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < ROTARY_BATCH; ++i) {
-            if (tok[i] < 0) continue;
-            void* out = of_k[i] ? p.k_out : p.q_out;
-            const bool turned = unit[i] < pairs;
-            const int a = turned ? (p.interleaved ? 2 : 1) * P * unit[i] : 2 * F + P * (unit[i] - pairs), b = a + (p.interleaved ? P : F);
-            const float2* cs = turns + (size_t)tok[i] * F + P * unit[i];
-            if constexpr (VEC) {
-                float x[8], y[8];
-                unpack8<DT>(ra[i], x);
-                if (turned) {
-                    unpack8<DT>(rb[i], y);
-                    if (p.interleaved) {
-#pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const float2 t0 = cs[e / 2], t1 = cs[4 + e / 2];
-                            const float u = x[e], v = x[e + 1], r = y[e], s = y[e + 1];
-                            x[e] = u * t0.x - v * t0.y; x[e + 1] = u * t0.y + v * t0.x;
-                            y[e] = r * t1.x - s * t1.y; y[e + 1] = r * t1.y + s * t1.x;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float2 t = cs[e];
-                            const float u = x[e], v = y[e];
-                            x[e] = u * t.x - v * t.y; y[e] = u * t.y + v * t.x;
-                        }
-                    }
-                    st8<DT>(out, to[i] + b, y);
-                }
-                st8<DT>(out, to[i] + a, x);
-            } else {
-                if (turned) {
-                    st1(out, DT, to[i] + a, fa[i] * cs->x - fb[i] * cs->y);
-                    st1(out, DT, to[i] + b, fa[i] * cs->y + fb[i] * cs->x);
+            for (int i = 0; i < ROTARY_BATCH; ++i) {
+                toks[i] = tok;
+                if (tok >= n) continue;
+                const bool of_k = h >= p.heads_q;
+                const int hh = of_k ? h - p.heads_q : h;
+                const void* from = of_k ? p.k : p.q;
+                const size_t at = (size_t)(first + tok) * (of_k ? p.k_stride : p.q_stride) + (size_t)hh * D;
+                to[i] = static_cast<char*>(of_k ? p.k_out : p.q_out) + ((size_t)(first + tok) * (of_k ? p.heads_k : p.heads_q) + hh) * D * SIZE;
+                if constexpr (VEC) {
+                    ldraw8<DT>(from, at + a, ra[i]);
+                    if (turned) ldraw8<DT>(from, at + b, rb[i]);
                 } else {
-                    st1(out, DT, to[i] + a, fa[i]);
+                    fa[i] = ld1(from, DT, at + a);
+                    if (turned) fb[i] = ld1(from, DT, at + b);
+                }
+                h += at_once;
+                settle();
+            }
+#pragma unroll
+            for (int i = 0; i < ROTARY_BATCH; ++i) {
+                if (toks[i] >= n) continue;
+                const float2* cs = turns + (size_t)toks[i] * F + P * unit;
+                if constexpr (VEC) {
+                    float x[8], y[8];
+                    unpack8<DT>(ra[i], x);
+                    if (turned) {
+                        unpack8<DT>(rb[i], y);
+                        float4 t[4];                           // two pairs' cosine and sine each
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t[e] = *reinterpret_cast<const float4*>(cs + 2 * e);
+                        auto one = [](float& u, float& v, float c, float s) {
+                            const float w = u;
+                            u = w * c - v * s;
+                            v = w * s + v * c;
+                        };
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (NEIGHBOURS) {
+                                float (&z)[8] = e < 2 ? x : y;
+                                one(z[4 * (e & 1)], z[4 * (e & 1) + 1], t[e].x, t[e].y);
+                                one(z[4 * (e & 1) + 2], z[4 * (e & 1) + 3], t[e].z, t[e].w);
+                            } else {
+                                one(x[2 * e], y[2 * e], t[e].x, t[e].y);
+                                one(x[2 * e + 1], y[2 * e + 1], t[e].z, t[e].w);
+                            }
+                        }
+                        st8<DT>(to[i], b, y);
+                    }
+                    st8<DT>(to[i], a, x);
+                } else {
+                    if (turned) {
+                        st1(to[i], DT, a, fa[i] * cs->x - fb[i] * cs->y);
+                        st1(to[i], DT, b, fa[i] * cs->y + fb[i] * cs->x);
+                    } else {
+                        st1(to[i], DT, a, fa[i]);
+                    }
                 }
             }
         }
@@ -131,7 +139,8 @@ extern "C" int mkda_rotary(const MkdaRotary* p, void* stream) {
     const long long blocks = ((long long)p->tokens + per - 1) / per;
     with_dtype(p->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        launch(vec ? rotary_kernel<DT, true> : rotary_kernel<DT, false>, dim3((unsigned)blocks), ROTARY_THREADS, (size_t)per * p->freqs * sizeof(float2), (cudaStream_t)stream, *p, per);
+        auto* kern = vec ? p->interleaved ? rotary_kernel<DT, true, true> : rotary_kernel<DT, true, false> : p->interleaved ? rotary_kernel<DT, false, true> : rotary_kernel<DT, false, false>;
+        launch(kern, dim3((unsigned)blocks), ROTARY_THREADS, (size_t)per * p->freqs * sizeof(float2), (cudaStream_t)stream, *p, per);
     });
     return check_launch("rotary");
 }
