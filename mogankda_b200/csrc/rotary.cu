@@ -5,6 +5,7 @@
 // once, in shared memory, for all heads of q and k.
 // Bound by HBM: each channel is read and written once.
 #include <algorithm>
+#include <type_traits>
 
 #include "block.cuh"
 
@@ -23,18 +24,52 @@ __device__ __forceinline__ float2 turn(const MkdaRotary& p, long long token, int
     return make_float2(c, p.inverse ? -s : s);
 }
 
-// VEC: pairs in pieces of eight, 16-byte accesses; else pair by pair.  A thread has the same piece of every head that it takes, and goes on from head to head without a division
-// (one for the token and one for the head of each piece took as long as the bytes: 32749 tokens x 40 heads 195 us).
-template <int DT, bool VEC, bool NEIGHBOURS>
+// P neighbouring elements, in one access (two for eight of fp32)
+template <int DT, int P>
+struct Piece {
+    using T = typename std::conditional<DT == MKDA_F32, uint32_t, uint16_t>::type;
+    struct alignas(P * sizeof(T) < 16 ? P * sizeof(T) : 16) Raw { T v[P]; };
+    static __device__ __forceinline__ void load(const void* base, size_t idx, Raw& r) { r = *reinterpret_cast<const Raw*>(static_cast<const T*>(base) + idx); }
+    static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[P]) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            if constexpr (DT == MKDA_F32) v[e] = __uint_as_float(r.v[e]);
+            else if constexpr (DT == MKDA_BF16) v[e] = __uint_as_float((uint32_t)r.v[e] << 16);
+            else v[e] = __half2float(__ushort_as_half(r.v[e]));
+        }
+    }
+    static __device__ __forceinline__ void store(void* base, size_t idx, const float (&v)[P]) {
+        Raw r;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            if constexpr (DT == MKDA_F32) r.v[e] = __float_as_uint(v[e]);
+            else if constexpr (DT == MKDA_BF16) r.v[e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+            else r.v[e] = __half_as_ushort(__float2half_rn(v[e]));
+        }
+        *reinterpret_cast<Raw*>(static_cast<T*>(base) + idx) = r;
+    }
+};
+template <int DT>
+struct Piece<DT, 8> {
+    using T = typename Piece<DT, 4>::T;
+    using Raw = Raw8;
+    static __device__ __forceinline__ void load(const void* base, size_t idx, Raw& r) { ldraw8<DT>(base, idx, r); }
+    static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[8]) { unpack8<DT>(r, v); }
+    static __device__ __forceinline__ void store(void* base, size_t idx, const float (&v)[8]) { st8<DT>(base, idx, v); }
+};
+
+// Pairs in pieces of P, as many as sizes, strides and addresses allow in one access.  A thread has the same piece of every head that it takes, and goes on from head to head without a
+// division (one for the token and one for the head of each piece took as long as the bytes: 32749 tokens x 40 heads 195 us).
+template <int DT, int P, bool NEIGHBOURS>
 __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const MkdaRotary p, const int per_block) {
     follow_stream();
     extern __shared__ __align__(16) float2 turns[];        // [per_block][freqs]
+    using Q = Piece<DT, P>;
     const int F = p.freqs, D = p.dim, heads = p.heads_q + p.heads_k;
     const long long first = (long long)blockIdx.x * per_block;
     const int n = (int)min((long long)per_block, p.tokens - first);
     for (int e = threadIdx.x; e < n * F; e += ROTARY_THREADS) turns[e] = turn(p, first + e / F, e % F);
     __syncthreads();
-    constexpr int P = VEC ? 8 : 1;
     const int pairs = F / P, units = pairs + (D - 2 * F) / P;      // pieces of a head: of pairs, then of channels that stay
     const int at_once = max(1, ROTARY_THREADS / units);            // heads that the block takes together
     for (int unit = threadIdx.x % min(units, ROTARY_THREADS); unit < units; unit += ROTARY_THREADS) {
@@ -47,11 +82,9 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const MkdaRotary
         };
         settle();
         while (tok < n) {
-            Raw8 ra[ROTARY_BATCH], rb[ROTARY_BATCH];
-            float fa[ROTARY_BATCH], fb[ROTARY_BATCH];
+            typename Q::Raw ra[ROTARY_BATCH], rb[ROTARY_BATCH];
             int toks[ROTARY_BATCH];
-            char* to[ROTARY_BATCH];
-            constexpr int SIZE = DT == MKDA_F32 ? 4 : 2;
+            void* to[ROTARY_BATCH];
 #pragma unroll
             for (int i = 0; i < ROTARY_BATCH; ++i) {
                 toks[i] = tok;
@@ -60,56 +93,42 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const MkdaRotary
                 const int hh = of_k ? h - p.heads_q : h;
                 const void* from = of_k ? p.k : p.q;
                 const size_t at = (size_t)(first + tok) * (of_k ? p.k_stride : p.q_stride) + (size_t)hh * D;
-                to[i] = static_cast<char*>(of_k ? p.k_out : p.q_out) + ((size_t)(first + tok) * (of_k ? p.heads_k : p.heads_q) + hh) * D * SIZE;
-                if constexpr (VEC) {
-                    ldraw8<DT>(from, at + a, ra[i]);
-                    if (turned) ldraw8<DT>(from, at + b, rb[i]);
-                } else {
-                    fa[i] = ld1(from, DT, at + a);
-                    if (turned) fb[i] = ld1(from, DT, at + b);
-                }
+                to[i] = static_cast<typename Q::T*>(of_k ? p.k_out : p.q_out) + ((size_t)(first + tok) * (of_k ? p.heads_k : p.heads_q) + hh) * D;
+                Q::load(from, at + a, ra[i]);
+                if (turned) Q::load(from, at + b, rb[i]);
                 h += at_once;
                 settle();
             }
 #pragma unroll
             for (int i = 0; i < ROTARY_BATCH; ++i) {
                 if (toks[i] >= n) continue;
-                const float2* cs = turns + (size_t)toks[i] * F + P * unit;
-                if constexpr (VEC) {
-                    float x[8], y[8];
-                    unpack8<DT>(ra[i], x);
-                    if (turned) {
-                        unpack8<DT>(rb[i], y);
-                        float4 t[4];                           // two pairs' cosine and sine each
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) t[e] = *reinterpret_cast<const float4*>(cs + 2 * e);
-                        auto one = [](float& u, float& v, float c, float s) {
-                            const float w = u;
-                            u = w * c - v * s;
-                            v = w * s + v * c;
-                        };
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if constexpr (NEIGHBOURS) {
-                                float (&z)[8] = e < 2 ? x : y;
-                                one(z[4 * (e & 1)], z[4 * (e & 1) + 1], t[e].x, t[e].y);
-                                one(z[4 * (e & 1) + 2], z[4 * (e & 1) + 3], t[e].z, t[e].w);
-                            } else {
-                                one(x[2 * e], y[2 * e], t[e].x, t[e].y);
-                                one(x[2 * e + 1], y[2 * e + 1], t[e].z, t[e].w);
-                            }
-                        }
-                        st8<DT>(to[i], b, y);
-                    }
-                    st8<DT>(to[i], a, x);
-                } else {
-                    if (turned) {
-                        st1(to[i], DT, a, fa[i] * cs->x - fb[i] * cs->y);
-                        st1(to[i], DT, b, fa[i] * cs->y + fb[i] * cs->x);
+                float x[P], y[P];
+                Q::unpack(ra[i], x);
+                if (turned) {
+                    Q::unpack(rb[i], y);
+                    const float2* cs = turns + (size_t)toks[i] * F + P * unit;
+                    float2 t[P];
+                    if constexpr (P == 1) {
+                        t[0] = *cs;
                     } else {
-                        st1(to[i], DT, a, fa[i]);
+#pragma unroll
+                        for (int e = 0; e < P; e += 2) {
+                            const float4 two = *reinterpret_cast<const float4*>(cs + e);
+                            t[e] = make_float2(two.x, two.y);
+                            t[e + 1] = make_float2(two.z, two.w);
+                        }
                     }
+#pragma unroll
+                    for (int e = 0; e < P; ++e) {          // of neighbours, pair e is elements 2 e and 2 e + 1 of x and y one behind the other
+                        float& u = !NEIGHBOURS ? x[e] : 2 * e < P ? x[2 * e < P ? 2 * e : 0] : y[2 * e >= P ? 2 * e - P : 0];
+                        float& v = !NEIGHBOURS ? y[e] : 2 * e + 1 < P ? x[2 * e + 1 < P ? 2 * e + 1 : 0] : y[2 * e + 1 >= P ? 2 * e + 1 - P : 0];
+                        const float w = u;
+                        u = w * t[e].x - v * t[e].y;
+                        v = w * t[e].y + v * t[e].x;
+                    }
+                    Q::store(to[i], b, y);
                 }
+                Q::store(to[i], a, x);
             }
         }
     }
@@ -129,18 +148,21 @@ extern "C" int mkda_rotary(const MkdaRotary* p, void* stream) {
         if (((p->axis_of[f >> 2] >> (8 * (f & 3))) & 255) >= p->axes) return set_error(MKDA_ERR_ARG, "rotary: a frequency of an axis that there is not");
     if (p->tokens == 0 || p->heads_q + p->heads_k == 0) return MKDA_OK;
     if ((p->heads_q && (!p->q || !p->q_out)) || (p->heads_k && (!p->k || !p->k_out)) || (p->freqs && (!p->positions || !p->inv_freq))) return set_error(MKDA_ERR_ARG, "rotary: null argument");
-    const bool vec = p->dim % 8 == 0 && p->freqs % 8 == 0 && (!p->heads_q || p->q_stride % 8 == 0) && (!p->heads_k || p->k_stride % 8 == 0) && aligned16(p->q) && aligned16(p->k) &&
-                     aligned16(p->q_out) && aligned16(p->k_out);
-    const int units = (p->heads_q + p->heads_k) * (p->dim - p->freqs) / (vec ? 8 : 1);      // a token's
-    // tokens of a block: work for a few batches of its threads, at most 32 KB of sines and cosines, and a block for each place on the GPU as long as there are tokens
+    const int size = p->dtype == MKDA_F32 ? 4 : 2;
+    int piece = 8;
+    auto fits = [&](const void* at) { return reinterpret_cast<uintptr_t>(at) % std::min(16, piece * size) == 0; };
+    while (piece > 1 && (p->dim % piece || p->freqs % piece || (p->heads_q && p->q_stride % piece) || (p->heads_k && p->k_stride % piece) || !fits(p->q) || !fits(p->k) || !fits(p->q_out) || !fits(p->k_out))) piece /= 2;
+    const int units = (p->heads_q + p->heads_k) * (p->dim - p->freqs) / piece;      // a token's
+    // tokens of a block: work for a few batches of its threads, at most 32 KB of sines and cosines, and as many blocks as fill whole waves of the places on the GPU
     int per = std::max(1, 4 * ROTARY_BATCH * ROTARY_THREADS / std::max(units, 1));
     per = std::min(per, std::max(1, 4096 / std::max(p->freqs, 1)));
-    per = (int)std::min<long long>(per, std::max<long long>(1, p->tokens / (4 * sm_count())));
-    const long long blocks = ((long long)p->tokens + per - 1) / per;
     with_dtype(p->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        auto* kern = vec ? p->interleaved ? rotary_kernel<DT, true, true> : rotary_kernel<DT, true, false> : p->interleaved ? rotary_kernel<DT, false, true> : rotary_kernel<DT, false, false>;
-        launch(kern, dim3((unsigned)blocks), ROTARY_THREADS, (size_t)per * p->freqs * sizeof(float2), (cudaStream_t)stream, *p, per);
+        auto* kern = piece == 8 ? p->interleaved ? rotary_kernel<DT, 8, true> : rotary_kernel<DT, 8, false> : piece == 4 ? p->interleaved ? rotary_kernel<DT, 4, true> : rotary_kernel<DT, 4, false>
+                   : piece == 2 ? p->interleaved ? rotary_kernel<DT, 2, true> : rotary_kernel<DT, 2, false> : p->interleaved ? rotary_kernel<DT, 1, true> : rotary_kernel<DT, 1, false>;
+        const long long places = (long long)sm_count() * std::min(resident(reinterpret_cast<const void*>(kern), ROTARY_THREADS), 200 * 1024 / std::max(1, per * p->freqs * 8)), waves = (p->tokens + per * places - 1) / (per * places);
+        per = (int)((p->tokens + waves * places - 1) / (waves * places));
+        launch(kern, dim3((unsigned)(((long long)p->tokens + per - 1) / per)), ROTARY_THREADS, (size_t)per * p->freqs * sizeof(float2), (cudaStream_t)stream, *p, per);
     });
     return check_launch("rotary");
 }
