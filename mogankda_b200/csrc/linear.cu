@@ -7,18 +7,22 @@
 namespace mkda {
 
 // ---- any type, 1 to 128 channels: fp32 throughout ------------------------------------------------------------------------------------------------
-// A block carries one part of a sequence and v-head, 32 tokens at a time: their rows and the state in shared memory, every product by fused multiply-adds on tiles of registers.
+// A block carries one part of a sequence and v-head, 64 tokens at a time: their rows and the state in shared memory, every product by fused multiply-adds on tiles of registers.  Bound by
+// those, 49 thousand of them per token at 128 channels (the older tensor instructions, as compensated TF32, are no faster), and by the tiles' way out of shared memory: four rows and
+// four columns a thread.  ROWS x COLS: what the channels of b and of c are padded to for the threads' tiles, 64 or 128.
 namespace ls {
-constexpr int THREADS = 256, C = 32, PP = C + 4;
+constexpr int THREADS = 512, C = 64, PP = C + 4;
 __host__ __device__ constexpr int pitch(int n) { return (n + 3) / 4 * 4 + 4; }
 inline int smem(int M, int V) { return 4 * (2 * C * pitch(M) + C * pitch(V) + C * PP + ((M + 3) / 4 * 4) * pitch(V) + PP); }
 
 // rows [0, len) of `n` channels from global memory, the rest of the C rows and of the pitch zero
 template <int DT>
 __device__ __forceinline__ void load_rows(float* to, int pit, const void* from, size_t at, long long stride, int n, int len, bool vec) {
-    const int quads = pit / 4;
-    for (int e = threadIdx.x; e < C * quads; e += THREADS) {
-        const int r = e / quads, c = 4 * (e - r * quads);
+    const int quads = pit / 4, step = THREADS / quads;     // rows at once
+    const int r0 = threadIdx.x / quads, c = 4 * (threadIdx.x - r0 * quads);
+    if (r0 >= step) return;
+#pragma unroll 4
+    for (int r = r0; r < C; r += step) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < len && c < n) {
             const size_t i = at + (size_t)r * stride + c;
@@ -37,10 +41,25 @@ __device__ __forceinline__ void load_rows(float* to, int pit, const void* from, 
 __device__ __forceinline__ void fma4(float (&d)[4], float a, const float4& b) {
     d[0] = fmaf(a, b.x, d[0]); d[1] = fmaf(a, b.y, d[1]); d[2] = fmaf(a, b.z, d[2]); d[3] = fmaf(a, b.w, d[3]);
 }
+// d[R][4] += rows x[R] (`xp` floats apart) times the columns y: terms [from, to), multiples of four
+template <int R>
+__device__ __forceinline__ void product(float (&d)[R][4], const float* x, int xp, const float* y, int yp, int from, int to) {
+#pragma unroll 2
+    for (int t = from; t < to; t += 4) {
+        float4 q[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const float4*>(y + (t + e) * yp);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float4 f = *reinterpret_cast<const float4*>(x + r * xp + t);
+            fma4(d[r], f.x, q[0]); fma4(d[r], f.y, q[1]); fma4(d[r], f.z, q[2]); fma4(d[r], f.w, q[3]);
+        }
+    }
+}
 }  // namespace ls
 
-template <int DT>
-__global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_constant__ LinearCall call, const bool vec) {
+template <int DT, int ROWS, int COLS>
+__global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linear_simt_kernel(const __grid_constant__ LinearCall call, const bool vec) {
     using namespace ls;
     follow_stream();
     extern __shared__ __align__(16) float smem_f[];
@@ -54,8 +73,8 @@ __global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_c
     float* sc = sb + C * pm;
     float* sp = sc + C * pv;
     float* st = sp + C * PP;                               // [M4][pv]
-    float* pw = st + M4 * pv;                              // lam^0 .. lam^32
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float* pw = st + M4 * pv;                              // lam^0 .. lam^64
+    const int tid = threadIdx.x;
     const float gamma = call.log_decay[h];
     if (tid <= C) pw[tid] = decay_power(gamma, tid);
     const size_t size = (size_t)M * V;
@@ -64,6 +83,8 @@ __global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_c
         const int m = e / pv, v = e - m * pv;
         st[e] = in && m < M && v < V ? in[k.transposed ? (size_t)v * M + m : (size_t)m * V + v] : 0.f;
     }
+    constexpr int ACROSS = COLS / 4, GROUPS = THREADS / ACROSS, OUT = C / GROUPS, STATE = ROWS / GROUPS;      // threads of a row, of a column, and rows of each
+    const int v = 4 * (tid % ACROSS), group = tid / ACROSS;
     const int chunks = (w.len + C - 1) / C;
     for (int t = 0; t < chunks; ++t) {
         const int c0 = (k.back ? chunks - 1 - t : t) * C, len = min(C, w.len - c0);
@@ -74,56 +95,36 @@ __global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_c
         load_rows<DT>(sc, pv, k.c, tok * k.c_stride + (size_t)(h / k.c_per) * V, k.c_stride, V, len, vec);
         __syncthreads();
         if (k.a) {
-            {                                              // pairs: row i, columns j = tid % 8 + 8 jj
-                const int i = tid >> 3;
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+            {                                              // pairs: rows i and i + 32, columns j = tid % 16 + 16 jj
+                const int i = tid >> 4;
+                float d[2][4] = {};
                 for (int m = 0; m < M4; m += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(sa + i * pm + m);
+                    const float4 x = *reinterpret_cast<const float4*>(sa + i * pm + m), z = *reinterpret_cast<const float4*>(sa + (i + 32) * pm + m);
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
-                        const float4 y = *reinterpret_cast<const float4*>(sb + ((tid & 7) + 8 * jj) * pm + m);
-                        d[jj] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, d[jj]))));
+                        const float4 y = *reinterpret_cast<const float4*>(sb + ((tid & 15) + 16 * jj) * pm + m);
+                        d[0][jj] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, d[0][jj]))));
+                        d[1][jj] = fmaf(z.x, y.x, fmaf(z.y, y.y, fmaf(z.z, y.z, fmaf(z.w, y.w, d[1][jj]))));
                     }
                 }
 #pragma unroll
-                for (int jj = 0; jj < 4; ++jj) {
-                    const int j = (tid & 7) + 8 * jj, away = k.back ? j - i : i - j;
-                    sp[i * PP + j] = away >= 0 && j < len ? d[jj] * pw[away] * k.pair_scale : 0.f;
-                }
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj) {
+                        const int row = i + 32 * u, j = (tid & 15) + 16 * jj, away = k.back ? j - row : row - j;
+                        sp[row * PP + j] = away >= 0 && j < len ? d[u][jj] * pw[away] * k.pair_scale : 0.f;
+                    }
             }
             __syncthreads();
-            const int v = 4 * lane;
-            if (v < V) {                                   // four rows, four columns
-                float o[4][4], s[4][4];
+            if (v < V) {
+                float o[OUT][4] = {}, s[OUT][4] = {};
+                const int i0 = OUT * group;
+                // pairs of these rows: forwards up to the last one, backwards from the first one on
+                product<OUT>(o, sp + i0 * PP, PP, sc + v, pv, k.back ? i0 & ~3 : 0, k.back ? C : (i0 + OUT + 3) & ~3);
+                product<OUT>(s, sa + i0 * pm, pm, st + v, pv, 0, M4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[r][e] = s[r][e] = 0.f;
-#pragma unroll 2
-                for (int j = 0; j < C; j += 4) {
-                    float4 y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const float4*>(sc + (j + e) * pv + v);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float4 x = *reinterpret_cast<const float4*>(sp + (4 * warp + r) * PP + j);
-                        fma4(o[r], x.x, y[0]); fma4(o[r], x.y, y[1]); fma4(o[r], x.z, y[2]); fma4(o[r], x.w, y[3]);
-                    }
-                }
-#pragma unroll 2
-                for (int m = 0; m < M4; m += 4) {
-                    float4 y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const float4*>(st + (m + e) * pv + v);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float4 x = *reinterpret_cast<const float4*>(sa + (4 * warp + r) * pm + m);
-                        fma4(s[r], x.x, y[0]); fma4(s[r], x.y, y[1]); fma4(s[r], x.z, y[2]); fma4(s[r], x.w, y[3]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 4 * warp + r;
+                for (int r = 0; r < OUT; ++r) {
+                    const int i = i0 + r;
                     if (i >= len) continue;
                     const float f = pw[k.back ? len - 1 - i : i + 1] * k.state_scale;
                     float x[4];
@@ -141,34 +142,30 @@ __global__ void __launch_bounds__(ls::THREADS) linear_simt_kernel(const __grid_c
             }
             __syncthreads();
         }
-        {                                                  // the state: sixteen rows, four columns
-            const int m0 = 16 * warp, v = 4 * lane;
-            if (m0 < M && v < V) {
-                float acc[16][4];
+        const int m0 = STATE * group;
+        if (m0 < M && v < V) {                             // the state
+            float acc[STATE][4] = {};
+#pragma unroll 4
+            for (int j = 0; j < len; ++j) {
+                const float f = pw[k.back ? j + 1 : len - 1 - j] * k.in_scale;
+                float4 y = *reinterpret_cast<const float4*>(sc + j * pv + v);
+                y.x *= f; y.y *= f; y.z *= f; y.w *= f;
+                const float* x = sb + j * pm + m0;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
-                for (int j = 0; j < len; ++j) {
-                    const float f = pw[k.back ? j + 1 : len - 1 - j] * k.in_scale;
-                    float4 y = *reinterpret_cast<const float4*>(sc + j * pv + v);
-                    y.x *= f; y.y *= f; y.z *= f; y.w *= f;
-#pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        if (m0 + r >= M4) break;
-                        const float4 x = *reinterpret_cast<const float4*>(sb + j * pm + m0 + r);
-                        fma4(acc[r], x.x, y); fma4(acc[r + 1], x.y, y); fma4(acc[r + 2], x.z, y); fma4(acc[r + 3], x.w, y);
-                    }
+                for (int r = 0; r < STATE; r += 2) {
+                    const float2 q = *reinterpret_cast<const float2*>(x + r);
+                    fma4(acc[r], q.x, y);
+                    fma4(acc[r + 1], q.y, y);
                 }
-                const float f = pw[len];
+            }
+            const float f = pw[len];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    if (m0 + r >= M) break;
-                    float4* s = reinterpret_cast<float4*>(st + (m0 + r) * pv + v);
-                    float4 x = *s;
-                    x.x = fmaf(f, x.x, acc[r][0]); x.y = fmaf(f, x.y, acc[r][1]); x.z = fmaf(f, x.z, acc[r][2]); x.w = fmaf(f, x.w, acc[r][3]);
-                    *s = x;
-                }
+            for (int r = 0; r < STATE; ++r) {
+                if (m0 + r >= M) break;
+                float4* s = reinterpret_cast<float4*>(st + (m0 + r) * pv + v);
+                float4 x = *s;
+                x.x = fmaf(f, x.x, acc[r][0]); x.y = fmaf(f, x.y, acc[r][1]); x.z = fmaf(f, x.z, acc[r][2]); x.w = fmaf(f, x.w, acc[r][3]);
+                *s = x;
             }
         }
     }
@@ -297,17 +294,20 @@ static int run_linear(const LinearCall& call, const LinearCall& before, cudaStre
     const bool tc = linear_tc_takes(call) && linear_tc_takes(before);
     auto run = [&](const LinearCall& c, bool states) {
         if (tc) return launch_linear_tc(c, states, stream);
-        int bytes = 0, rc = MKDA_OK;
+        int bytes = 0, rc = MKDA_OK, rows = 0, cols = 0;
         bool vec = true;
         for (int i = 0; i < c.kinds; ++i) {
             const LinearKind& k = c.kind[i];
             bytes = std::max(bytes, ls::smem(k.M, k.V));
+            rows = std::max(rows, k.M);
+            cols = std::max(cols, k.V);
             vec = vec && k.M % 4 == 0 && k.V % 4 == 0 && k.a_stride % 4 == 0 && k.b_stride % 4 == 0 && k.c_stride % 4 == 0 && aligned16(k.a) && aligned16(k.b) && aligned16(k.c);
         }
         with_dtype(c.dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
-            rc = ensure_smem(reinterpret_cast<const void*>(linear_simt_kernel<DT>), 227 * 1024 - 1024, "linear");
-            if (rc == MKDA_OK) launch(linear_simt_kernel<DT>, dim3(c.HV * (S.seg ? S.segs : 1), S.N, c.kinds), ls::THREADS, bytes, stream, c, vec);
+            auto* kern = rows > 64 ? cols > 64 ? linear_simt_kernel<DT, 128, 128> : linear_simt_kernel<DT, 128, 64> : cols > 64 ? linear_simt_kernel<DT, 64, 128> : linear_simt_kernel<DT, 64, 64>;
+            rc = ensure_smem(reinterpret_cast<const void*>(kern), 227 * 1024 - 1024, "linear");
+            if (rc == MKDA_OK) launch(kern, dim3(c.HV * (S.seg ? S.segs : 1), S.N, c.kinds), ls::THREADS, bytes, stream, c, vec);
         });
         return rc != MKDA_OK ? rc : check_launch("linear");
     };

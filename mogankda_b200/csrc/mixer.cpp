@@ -14,7 +14,7 @@ enum { LQ, LK, LV, LDECAY, LH0, LINEAR_INPUTS };
 //   one sequence of 32749 tokens, 32 heads: uncut 1060 us, parts of 64 stretches 373, of 29 (what the rule takes) see below
 void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t heads, int kinds, int kinds_before, int64_t state, bool tensor_cores) {
     if (q.longest < 512 || s.N == 0) return;
-    const double main = tensor_cores ? 4.2 : 28.0, before = tensor_cores ? 1.9 : 9.0, launch = 8.0, state_us = 4.0 * 4 * state * kinds_before / heads / 5e6;      // per part and head
+    const double main = tensor_cores ? 4.2 : 60.0, before = tensor_cores ? 1.9 : 32.0, launch = 8.0, state_us = 4.0 * 4 * state * kinds_before / heads / 5e6;      // per part and head
     const int64_t longest = (q.longest + 127) / 128, most = std::max<int64_t>(longest, (s.TT + 127) / 128), n_sm = sms();
     auto rounds = [&](int64_t items) { return (items + n_sm - 1) / n_sm; };
     double best = std::max<double>(longest, (double)most * heads * kinds / n_sm) * main;
