@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
     const LinearKind& k = call.kind[blockIdx.z];
     const int h = blockIdx.x % call.HV, part = blockIdx.x / call.HV, n = call.S.order && !call.S.seg ? call.S.order[blockIdx.y] : blockIdx.y;
     const LinearPart w = linear_part(call.S, n, part, k.back);
-    if (w.nothing || (!k.a && w.leaves_last)) return;      // what the last part leaves is the main kernel's to find
+    if (w.nothing || (k.states && w.leaves_last)) return;      // what the last part leaves is the main kernel's to find
     const int M = k.M, V = k.V, pm = pitch(M), pv = pitch(V), M4 = (M + 3) / 4 * 4;
     float* sa = smem_f;
     float* sb = sa + C * pm;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
     const float gamma = call.log_decay[h];
     if (tid <= C) pw[tid] = decay_power(gamma, tid);
     const size_t size = (size_t)M * V;
-    const float* in = call.S.seg && k.a ? k.parts + ((size_t)(n * call.S.segs + part) * call.HV + h) * size : k.a && k.first ? k.first + ((size_t)n * call.HV + h) * size : nullptr;
+    const float* in = k.states ? nullptr : call.S.seg ? k.parts + ((size_t)(n * call.S.segs + part) * call.HV + h) * size : k.first ? k.first + ((size_t)n * call.HV + h) * size : nullptr;
     for (int e = tid; e < M4 * pv; e += THREADS) {
         const int m = e / pv, v = e - m * pv;
         st[e] = in && m < M && v < V ? in[k.transposed ? (size_t)v * M + m : (size_t)m * V + v] : 0.f;
@@ -90,11 +90,11 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
         const int c0 = (k.back ? chunks - 1 - t : t) * C, len = min(C, w.len - c0);
         const size_t tok = w.start + c0;
         __syncthreads();
-        if (k.a) load_rows<DT>(sa, pm, k.a, tok * k.a_stride + (size_t)(h / k.a_per) * M, k.a_stride, M, len, vec);
+        if (!k.states) load_rows<DT>(sa, pm, k.a, tok * k.a_stride + (size_t)(h / k.a_per) * M, k.a_stride, M, len, vec);
         load_rows<DT>(sb, pm, k.b, tok * k.b_stride + (size_t)(h / k.b_per) * M, k.b_stride, M, len, vec);
         load_rows<DT>(sc, pv, k.c, tok * k.c_stride + (size_t)(h / k.c_per) * V, k.c_stride, V, len, vec);
         __syncthreads();
-        if (k.a) {
+        if (!k.states) {
             {                                              // pairs: rows i and i + 32, columns j = tid % 16 + 16 jj
                 const int i = tid >> 4;
                 float d[2][4] = {};
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
             }
         }
     }
-    float* out = !k.a ? k.parts + ((size_t)(n * call.S.segs + part + (k.back ? -1 : 1)) * call.HV + h) * size : k.last && w.leaves_last ? k.last + ((size_t)n * call.HV + h) * size : nullptr;
+    float* out = k.states ? k.parts + ((size_t)(n * call.S.segs + part + (k.back ? -1 : 1)) * call.HV + h) * size : k.last && w.leaves_last ? k.last + ((size_t)n * call.HV + h) * size : nullptr;
     if (!out) return;
     __syncthreads();
     for (size_t e = tid; e < size; e += THREADS) {
@@ -333,6 +333,7 @@ static const char* bad_linear(const MkdaLinearFwd& p) {
     if (p.S.N > 65535) return "linear: at most 65535 sequences";
     if (p.S.seg < 0 || p.S.seg % 128 || (p.S.seg && (p.S.segs < 1 || !p.seg_h))) return "linear: parts of a multiple of 128 tokens, and a state for each";
     if (p.S.seg && (long long)p.HV * p.S.segs * 64 > 0x7fffffff) return "linear: too many parts";
+    if (p.S.seg && !p.S.cu && (long long)p.S.seg * p.S.segs < p.S.T) return "linear: more tokens than the parts have";
     if (!p.log_decay) return "linear: null argument";
     if (any_misaligned(p.h0, p.ht, p.seg_h, p.o)) return "linear: states and outputs must be 16-byte aligned";
     return nullptr;
@@ -367,7 +368,7 @@ extern "C" int mkda_linear_fwd(const MkdaLinearFwd* p, void* stream) {
     LinearKind k = kind_of(*p, p->q, p->q_stride, false, p->k, p->k_stride, false, p->v, p->v_stride, true);
     k.out = p->o; k.first = p->h0; k.last = p->ht; k.parts = p->seg_h;
     call.kind[0] = k; call.kinds = 1;
-    k.a = nullptr;
+    k.states = 1;
     before.kind[0] = k; before.kinds = 1;
     return run_linear(call, before, (cudaStream_t)stream);
 }
@@ -398,7 +399,7 @@ extern "C" int mkda_linear_bwd(const MkdaLinearBwd* q, void* stream) {
     call.kind[0] = dq; call.kind[1] = dk; call.kind[2] = dv; call.kinds = 3;
     LinearKind fs = kind_of(p, nullptr, 0, false, p.k, p.k_stride, false, p.v, p.v_stride, true), bs = dv;
     fs.first = p.h0; fs.parts = p.seg_h;
-    bs.a = nullptr;
+    fs.states = bs.states = 1;
     before.kind[0] = fs; before.kind[1] = bs; before.kinds = 2;
     int rc = run_linear(call, before, (cudaStream_t)stream);
     if (rc != MKDA_OK || !shared || q->end == 0) return rc;

@@ -13,7 +13,8 @@
 namespace mkda {
 
 struct LinearKind {
-    const void* a; const void* b; const void* c;           // a NULL: nothing but the states that the parts of the sequences leave
+    const void* a; const void* b; const void* c;
+    int states;                                            // nothing but the states that the parts of the sequences leave; a is not looked at
     long long a_stride, b_stride, c_stride;
     int a_per, b_per, c_per;                               // v-heads to a head
     int M, V;                                              // channels of a and b, of c and out

@@ -596,7 +596,7 @@ bool linear_tc_takes(const LinearCall& call) {
     if (call.dtype != MKDA_BF16 || call.S.TT < 1 || linear_items(call) > 0x7fffffff) return false;
     for (int i = 0; i < call.kinds; ++i) {
         const LinearKind& k = call.kind[i];
-        if (k.M % 8 || k.V % 8 || (k.a && (k.a_stride % 8 || !aligned16(k.a))) || k.b_stride % 8 || k.c_stride % 8 || !aligned16(k.b) || !aligned16(k.c)) return false;
+        if (k.M % 8 || k.V % 8 || (!k.states && (k.a_stride % 8 || !aligned16(k.a))) || k.b_stride % 8 || k.c_stride % 8 || !aligned16(k.b) || !aligned16(k.c)) return false;
     }
     return true;
 }
@@ -617,7 +617,7 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
     };
     for (int i = 0; i < call.kinds; ++i) {
         const LinearKind& k = call.kind[i];
-        plan.map_a[i] = k.a ? map(k.a, k.a_stride, k.a_per, k.M) : 0;
+        plan.map_a[i] = k.states ? 0 : map(k.a, k.a_stride, k.a_per, k.M);
         plan.map_b[i] = map(k.b, k.b_stride, k.b_per, k.M);
         plan.map_c[i] = map(k.c, k.c_stride, k.c_per, k.V);
         if (rc == MKDA_OK && !states) rc = make_heads_map(&maps.out[i], k.out, call.S.TT, call.HV, k.V, (long long)call.HV * k.V, "linear", k.out_dtype == MKDA_F32 ? 4 : 2);

@@ -21,7 +21,7 @@ void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t heads, int kinds, int k
     for (int64_t parts = 2; parts <= longest / 2; ++parts) {
         const int64_t seg = (longest + parts - 1) / parts, all = (most + seg - 1) / seg;      // parts with tokens, about
         if (s.N * parts * state * 4 > (int64_t)256 << 20) break;
-        const double us = (rounds(all * heads * kinds) * main + rounds(std::max<int64_t>(0, all - 1) * heads * kinds_before) * before) * seg + launch + all * heads * state_us + 0.002 * s.N * parts * heads;
+        const double us = (rounds(all * heads * kinds) * main + rounds(std::max<int64_t>(0, all - 1) * heads * kinds_before) * before) * seg + launch + (all + s.N) * heads * state_us + 0.002 * s.N * parts * heads;
         if (us < 0.97 * best) {
             best = us;
             s.seg = (int)(seg * 128);
@@ -37,10 +37,12 @@ struct LinearCall {
     LinearCall(const Sequences& q, const variable_list& t, double scale) {
         p.S = q.s; p.HK = (int)t[LQ].size(-2); p.HV = (int)t[LV].size(-2); p.K = (int)t[LQ].size(-1); p.V = (int)t[LV].size(-1);
         p.dtype = dtype_code(t[LQ]); p.scale = (float)scale;
+        const bool tiles = t[LQ].scalar_type() == at::kBFloat16 && p.K % 8 == 0 && p.V % 8 == 0;
         auto rows = [&](int i, const void*& ptr, long long& stride) {
             Rows r = rows_of(t[i], 2);
-            // tiled copies want 16-byte boundaries: rows that start elsewhere are copied, so that results do not depend on where they lie
-            if (t[i].scalar_type() == at::kBFloat16 && (r.stride % 8 || reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16)) r = {aligned(r.t), t[i].size(-1) * t[i].size(-2)};
+            // tiled copies want 16-byte boundaries and a stride that leads on: other rows are copied, so that results do not depend on where they lie
+            const int64_t width = t[i].size(-1) * t[i].size(-2);
+            if (tiles && (r.stride % 8 || r.stride < width || reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16)) r = {aligned(r.t), width};
             ptr = cptr(r.t);
             stride = r.stride;
             hold.push_back(r.t);

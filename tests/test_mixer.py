@@ -42,7 +42,7 @@ def test_entry_points_refuse_without_launching(lib):
                                         ("end", 5), ("end", -1)])
     f.S.seg, f.S.segs, f.seg_h = 128, 1, 0x30000
     b.f = f
-    _refused(lib, "mkda_linear_bwd", b, [("seg_g", 0), ("f.S.segs", 0)])
+    _refused(lib, "mkda_linear_bwd", b, [("seg_g", 0), ("f.S.segs", 0), ("f.S.T", 129)])
     p = _filled(S["MkdaLinearStep"](), ("q", "k", "v", "log_decay", "state", "o"), N=2, **numbers)
     _refused(lib, "mkda_linear_step", p, bad[:3] + bad[4:] + [("state", 0), ("state", 0x30008), ("o", 0), ("N", 65536), ("N", -1)])
     p = _filled(S["MkdaRotary"](), ("q", "k", "q_out", "k_out", "positions", "inv_freq"), tokens=3, heads_q=2, heads_k=1, dim=16, freqs=8, axes=2, dtype=1, q_stride=32, k_stride=16)

@@ -179,6 +179,62 @@ def test_linear_of_broadcast_inputs():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_one_token_over_and_over(dtype):
+    """All tokens are one in memory (a stride of 0), or half of one overlaps the next."""
+    gen = torch.Generator().manual_seed(14)
+    d = -torch.rand(2, generator=gen).cuda()
+    one = rand(gen, 1, 1, 2, 32).cuda().to(dtype)
+    flat = rand(gen, 32 * 150 + 64).cuda().to(dtype)
+    lap = flat.as_strided((1, 150, 2, 32), (0, 32, 32, 1))
+    for x in (one.expand(1, 150, 2, 32), lap):
+        with torch.no_grad():
+            a, b = mk.linear_attention(x, x, x, d), mk.linear_attention(*(x.contiguous() for _ in range(3)), d)
+        assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,cu", [(0, 7, None), (2, 0, None), (1, 0, (0, 0, 0)), (1, 40, (0, 0, 40, 40)), (1, 40, (0, 0, 0))], ids=str)
+def test_linear_of_nothing(dtype, B, T, cu):
+    """No sequence, no token, sequences without tokens: states pass through, and so do their gradients."""
+    n = B if cu is None else len(cu) - 1
+    gen = torch.Generator().manual_seed(15)
+    lv = dict(q=rand(gen, B, T, 1, 64).to(dtype), k=rand(gen, B, T, 1, 64).to(dtype), v=rand(gen, B, T, 2, 64).to(dtype), h0=rand(gen, n, 2, 64, 64))
+    mine = {m: t.cuda().requires_grad_(True) for m, t in lv.items()}
+    d = -torch.rand(2, generator=gen)
+    o, last = mk.linear_attention(mine["q"], mine["k"], mine["v"], d.cuda(), initial_state=mine["h0"], output_final_state=True, cu_seqlens=None if cu is None else torch.tensor(cu, dtype=torch.int32).cuda())
+    up = rand(gen, n, 2, 64, 64).cuda()
+    grads = torch.autograd.grad(last, list(mine.values()), up)          # nothing comes back through o
+    assert o.shape == lv["v"].shape and all(g.shape == t.shape for g, t in zip(grads, lv.values()))
+    for i in range(n):
+        if cu is None or cu[i] == cu[i + 1]:
+            assert torch.equal(last[i], mine["h0"][i]) and torch.equal(grads[3][i], up[i])
+    if cu and cu[-1] == 0:
+        assert (o == 0).all() and all((g == 0).all() for g in grads[:3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_many_sequences_beside_a_long_one(dtype):
+    """Sequences of a few tokens, more than a wave of blocks has places, and one that is cut by itself."""
+    gen = torch.Generator().manual_seed(16)
+    few, long = 500, 3000
+    lens = [int(x) for x in torch.randint(0, 9, (few,), generator=gen)]
+    cu = [0]
+    for n in lens[:250] + [long] + lens[250:]:
+        cu.append(cu[-1] + n)
+    q, k, v = (rand(gen, 1, cu[-1], 1, 64).to(dtype).cuda() for _ in range(3))
+    d = torch.tensor([-0.02]).cuda()
+    with torch.no_grad():
+        o, last = mk.linear_attention(q, k, v, d, cu_seqlens=torch.tensor(cu, dtype=torch.int32).cuda(), output_final_state=True)
+        for i in (0, 100, 249, 250, 251, 400, 500):
+            s = slice(cu[i], cu[i + 1])
+            a, b = mk.linear_attention(q[:, s], k[:, s], v[:, s], d, output_final_state=True)
+            near("state", last[i:i + 1], b.double())
+            if a.numel():          # both are rounded
+                step = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+                assert (a.double() - o[:, s].double()).norm() <= 2 * (ARITHMETIC + step) * a.double().norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_leaves_tokens_of_no_sequence_alone(dtype):
     """Behind the last boundary nothing is read and results are zero; what is not finite stays in its sequence."""
     gen = torch.Generator().manual_seed(8)
