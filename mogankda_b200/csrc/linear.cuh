@@ -47,7 +47,7 @@ __device__ __forceinline__ LinearPart linear_part(const MkdaSeqs& s, int n, int 
     return {w.start + at, min(s.seg, len - at), false, false, back ? part == 0 : part == parts - 1};
 }
 
-// linear_tc.cu: bf16 rows on the tensor cores, where tiled copies can fetch them.  `states`: nothing but what the parts of cut sequences make of a zero state.
+// linear_tc.cu: rows of 16 bits on the tensor cores, where tiled copies can fetch them.  `states`: nothing but what the parts of cut sequences make of a zero state.
 bool linear_tc_takes(const LinearCall& call);
 int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream);
 

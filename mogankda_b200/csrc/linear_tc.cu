@@ -1,17 +1,19 @@
-// Linear attention with a decay for each head (linear.cuh) in bf16 on the Blackwell tensor cores.
+// Linear attention with a decay for each head (linear.cuh) in bf16 and fp16 on the Blackwell tensor cores.
 //
 // A block (one per SM) carries parts of sequences and v-heads one after the other, 128 tokens at a time.  With the rows of a, b and c in shared memory (tiled copies, 128-byte
 // swizzle) a stretch is four products with fp32 accumulators in tensor memory:
-//   P0 = a b^T                       pairs; the weights lam^|i - j| and the mask are applied to the accumulator, and P leaves as bf16 hi + lo, the left operand of P c
+//   P0 = a b^T                       pairs; the weights lam^|i - j| and the mask are applied to the accumulator, and P leaves as hi + lo in 16 bits, the left operand of P c
 //   O  = a M                         M: the state in front of the stretch as hi + lo in shared memory; lam^(i + 1) is applied to the accumulator's rows
 //   O += P c
-//   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts, so that the state, fp32 in registers, is exact to 32 bits
-// a, b and c are exact in bf16.  Two halves (2^-16) are enough where the result is rounded to bf16, one would show: P and M in one bf16 each are as far off as the result's own rounding.
+//   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts (fp16: two), so that the state, fp32 in registers, is exact to 32 bits
+// a, b and c are exact as they are.  Two halves (2^-16) are enough where the result is rounded to bf16, one would show: P and M in one bf16 each are as far off as the result's own rounding.
 //
 // Roles, joined by mbarriers: a warp that fetches rows into a ring of five tiles, one that issues products, and eight warps each for the pairs' weights and the output, for f c and for
 // the state.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
 //
-// Bound by HBM where there are enough parts: 128 KB per stretch, 3 us of an SM's share; products take 8 x 516 cycles = 2.2 us, and each group of warps less than that.
+// Bound by the hand-overs between the products and, in runs that last, by 1000 W: a stretch takes 3.3 us where few SMs are busy, 4.2 (7 k cycles) where all are.  HBM alone would
+// take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 560 us, 0.68 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 258 us, where
+// the fp32 units (linear.cu) take 2890.
 #include <algorithm>
 
 #include "host.h"
@@ -32,10 +34,12 @@ static_assert(2 * (LAUNCH_REGS + FACTOR_REGS + STATE_REGS) + ISSUE_REGS <= 7 * L
 
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
-    uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free, o_staged[2];
+    uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free, o_staged[2], e_ready[2];
     uint32_t tmem;
     // of the current part's head, a copy for each group of warps that reads it: weights of the pairs by j - i + 128 (0 where a pair does not count), f, lam^n times the scale
     __align__(16) float pair[2 * C], factor[C], row[C + 4];
+    // fp16: powers of two that f c, the pairs and the state are scaled by, of even and odd stretches, and what warps find for them
+    float f_scale[2], p_scale[2], s_scale[2], f_top[8], a_top[8], b_top[8], s_top[8];
 };
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
@@ -103,18 +107,60 @@ __device__ __forceinline__ const float* entering(const LinearCall& call, const L
     return k.first ? k.first + ((size_t)it.n * call.HV + it.h) * size : nullptr;
 }
 __device__ __forceinline__ void group_sync(int barrier) { asm volatile("bar.sync %0, 256;" :: "r"(barrier) : "memory"); }
-// A pair of values as bf16 pairs: hi, and what is left of them, two rounded parts in all
-__device__ __forceinline__ uint32_t take_bf16(f32x2& v) {          // hi; v becomes the rest, exactly
+// A pair of values in 16 bits, and back
+template <bool HALF>
+__device__ __forceinline__ uint32_t as_part(f32x2 v) {
     float a, b;
     unpack2(v, a, b);
-    const uint32_t h = umma::pack_bf16x2(a, b);
-    v = fma2(pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), both(-1.f), v);
+    return HALF ? pack16<MKDA_F16>(a, b) : umma::pack_bf16x2(a, b);
+}
+template <bool HALF>
+__device__ __forceinline__ f32x2 of_part(uint32_t h) {
+    if constexpr (HALF) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        return pack2(f.x, f.y);
+    } else {
+        return pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+    }
+}
+// hi; v becomes the rest, exactly
+template <bool HALF>
+__device__ __forceinline__ uint32_t take_part(f32x2& v) {
+    const uint32_t h = as_part<HALF>(v);
+    v = fma2(of_part<HALF>(h), both(-1.f), v);
     return h;
 }
-__device__ __forceinline__ uint32_t as_bf16(f32x2 v) {
-    float a, b;
-    unpack2(v, a, b);
-    return umma::pack_bf16x2(a, b);
+// The power of two that brings `top` to [2^(to - 1), 2^to); 1 for 0
+__device__ __forceinline__ float scale_to(float top, int to) {
+    const int e = (int)(__float_as_uint(top) >> 23) & 255;
+    return top == 0.f ? 1.f : __uint_as_float((uint32_t)min(max(to - 1 + 254 - e, 4), 250) << 23);
+}
+__device__ __forceinline__ float warp_top(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float top_of(const float (&tops)[8]) {
+    float v = tops[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v = fmaxf(v, tops[i]);
+    return v;
+}
+// The largest magnitude of a fp16 tile's rows [0, len), of this thread's pieces (of 256 threads)
+__device__ __forceinline__ float tile_top(const uint8_t* tile, int me, int len) {
+    __half2 top = __half2half2(__ushort_as_half(0));
+#pragma unroll 2
+    for (int e = me; e < len * 16; e += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + umma::tile_chunk_offset(128, e >> 4, e & 15));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t m = w[i] & 0x7fff7fffu;
+            top = __hmax2(top, *reinterpret_cast<const __half2*>(&m));
+        }
+    }
+    const float2 f = __half22float2(top);
+    return fmaxf(f.x, f.y);
 }
 // Four 8 x 8 blocks of 16-bit values, transposed: lane t gets elements (2 (t % 4), t / 4) and (2 (t % 4) + 1, t / 4) of each; lane t gives the address of row t % 8 of block t / 8
 __device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4]) {
@@ -139,7 +185,9 @@ template <bool STATES>
 __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
 
 // STATES: nothing but what the parts of cut sequences make of a zero state
-template <bool STATES>
+// HALF: fp16 rows.  Their products are exact as those of bf16 are, but pair weights, f c and states leave fp16's range where bf16 has fp32's: each is scaled by a power of two, found from
+// the stretch's rows and the state, that keeps it below 2^15, and two parts (22 bits, or 2^-39 of the largest) are as good as fp32.
+template <bool STATES, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_constant__ Plan plan, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* base = smem_raw;                              // no static shared memory: the dynamic block starts on a 1024-byte boundary
@@ -156,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < SLOTS; ++i) { umma::mbar_init(&sh.full[i], 1); umma::mbar_init(&sh.empty[i], 1); }
         for (uint64_t* b : {&sh.p0_done, &sh.f_free[0], &sh.f_free[1], &sh.x_done, &sh.in_done, &sh.o_done}) umma::mbar_init(b, 1);
-        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free, &sh.o_staged[0], &sh.o_staged[1]}) umma::mbar_init(b, 8);
+        for (uint64_t* b : {&sh.p_ready, &sh.f_ready[0], &sh.f_ready[1], &sh.s_ready, &sh.o_scaled, &sh.o_free, &sh.o_staged[0], &sh.o_staged[1], &sh.e_ready[0], &sh.e_ready[1]}) umma::mbar_init(b, 8);
         umma::fence_barrier_init();
     }
     follow_stream();
@@ -209,8 +257,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * (TILE / 2 / 16) + (ks & 3) * 2); };
                 for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart&, int chunks) {
                     const int ms = (k.M + 15) / 16, vn = (k.V + 15) / 16 * 16;
-                    const bool zero = entering(call, k, it, STATES) == nullptr, exact = exact_state<STATES>(k), fp32 = k.out_dtype == MKDA_F32;
-                    const uint32_t id_p0 = umma::idesc_bf16(128, C), id_in = umma::idesc_bf16(128, vn), id_pc = umma::idesc_bf16(128, vn, 0, 1), id_x = umma::idesc_bf16(128, ms * 16, 0, 1);
+                    const bool zero = entering(call, k, it, STATES) == nullptr, exact = !HALF && exact_state<STATES>(k), fp32 = k.out_dtype == MKDA_F32;
+                    constexpr uint32_t F16 = HALF ? ~(1u << 7 | 1u << 10) : ~0u;         // both operands fp16
+                    const uint32_t id_p0 = umma::idesc_bf16(128, C) & F16, id_in = umma::idesc_bf16(128, vn) & F16, id_pc = umma::idesc_bf16(128, vn, 0, 1) & F16,
+                                   id_x = umma::idesc_bf16(128, ms * 16, 0, 1) & F16;
 #pragma unroll 1
                     for (int t = 0; t < chunks; ++t, ++n) {
                         const uint32_t ta = n * PER, tb = ta + (STATES ? 0 : 1), tc = tb + 1, par = n & 1;
@@ -321,6 +371,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 #pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
+                    float up = 1.f;
+                    if (HALF) {
+                        mbar_wait(&sh.e_ready[n & 1], (n >> 1) & 1, tries);
+                        up = sh.p_scale[n & 1];
+                    }
                     wait_mma(&sh.p0_done, n & 1, tries);
 #pragma unroll 1
                     for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
@@ -345,8 +400,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             f32x2 x = pack2(v[2 * e], v[2 * e + 1]);
-                            h[e] = take_bf16(x);
-                            l[e] = as_bf16(x);
+                            if (HALF) x = mul2(x, both(up));
+                            h[e] = take_part<HALF>(x);
+                            l[e] = as_part<HALF>(x);
                         }
                         umma::tmem_st8(at, h);
                         umma::tmem_st8(at + 8, l);
@@ -355,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     signal_tmem(&sh.p_ready, lane);
                     wait_mma(&sh.in_done, n & 1, tries);
                     if (!zero || t) {
-                        const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1]);
+                        const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1] * (HALF ? up / sh.s_scale[n & 1] : 1.f));
 #pragma unroll 1
                         for (int m0 = m_first; m0 < m_end; m0 += 16) {
                             const uint32_t at = umma::tmem_addr(tmem, w, O + m0);
@@ -373,12 +429,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     }
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1, tries);
+                    const float down = HALF ? 1.f / up : 1.f;
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
                     if (len == C) {
 #pragma unroll 1
                         for (int m0 = m_first; m0 < m_end; m0 += 16) {
                             float v[16];
                             umma::tmem_ld16(umma::tmem_addr(tmem, w, O + m0), v);
+                            if (HALF)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] *= down;
                             uint8_t* const to = staging(n, fp32, m0);
                             if (fp32) {
 #pragma unroll
@@ -387,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             } else {
                                 uint32_t u[8];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                                for (int e = 0; e < 8; ++e) u[e] = as_part<HALF>(pack2(v[2 * e], v[2 * e + 1]));
                                 *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, (m0 & 63) >> 3)) = make_uint4(u[0], u[1], u[2], u[3]);
                                 *reinterpret_cast<uint4*>(to + umma::tile_chunk_offset(128, i, ((m0 & 63) >> 3) + 1)) = make_uint4(u[4], u[5], u[6], u[7]);
                             }
@@ -405,6 +465,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                                 signal_tmem(&sh.o_staged[n & 1], lane);
                             }
                             if (i >= len || m0 >= m_end) continue;
+                            if (HALF)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] *= down;
                             if (fp32) {
                                 float* to = static_cast<float*>(k.out) + row + m0;
 #pragma unroll
@@ -414,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                                 uint16_t* to = static_cast<uint16_t*>(k.out) + row + m0;
                                 uint32_t u[8];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) u[e] = umma::pack_bf16x2(v[2 * e], v[2 * e + 1]);
+                                for (int e = 0; e < 8; ++e) u[e] = as_part<HALF>(pack2(v[2 * e], v[2 * e + 1]));
                                 *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
                                 if (m0 + 8 < m_end) *reinterpret_cast<uint4*>(to + 8) = make_uint4(u[4], u[5], u[6], u[7]);
                             }
@@ -432,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         const int me = tid - 32 * WARP_FACTORS, w = warp & 3, half = (warp - WARP_FACTORS) >> 2;
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float gamma = call.log_decay[it.h];
-            const bool exact = exact_state<STATES>(k);
+            const bool exact = !HALF && exact_state<STATES>(k);
             int factors_of = -1;                           // tokens that the table is for
 #pragma unroll 1
             for (int t = 0; t < chunks; ++t, ++n) {
@@ -458,6 +521,32 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     group_sync(2);
                     __syncwarp();
                 }
+                f32x2 scale = both(1.f);
+                if (HALF) {                                // nothing frees these tiles in front of this stretch's first parts of f c
+                    float b_top = 0.f, a_top = 0.f;
+                    if (!STATES) {
+                        mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
+                        mbar_wait(&sh.full[slot_of(tb - 1)], parity_of(tb - 1), tries);
+                        b_top = warp_top(tile_top(ring + slot_of(tb) * TILE, me, len));
+                        a_top = warp_top(tile_top(ring + slot_of(tb - 1) * TILE, me, len));
+                    }
+                    const float c_top = warp_top(tile_top(c, me, len));
+                    group_sync(2);                         // what was found for the last stretch has been read
+                    if (lane == 0) {
+                        sh.f_top[me >> 5] = c_top;
+                        sh.a_top[me >> 5] = a_top;
+                        sh.b_top[me >> 5] = b_top;
+                    }
+                    group_sync(2);
+                    const float up = scale_to(top_of(sh.f_top) * fmaxf(1.f, fabsf(k.in_scale)), 15);
+                    scale = both(up);
+                    if (me == 0) {
+                        sh.f_scale[n & 1] = up;
+                        sh.p_scale[n & 1] = scale_to(top_of(sh.a_top) * top_of(sh.b_top) * (float)k.M * fabsf(k.pair_scale), 15);
+                    }
+                    __syncwarp();
+                    if (!STATES && lane == 0) umma::arrive(&sh.e_ready[n & 1]);
+                }
                 const uint32_t rows = umma::smem_u32(c);
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
@@ -471,14 +560,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
                             const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
-                            f32x2 x = mul2(pack2(__uint_as_float(r[m] << 16), __uint_as_float(r[m] & 0xffff0000u)), f);
+                            f32x2 x = mul2(of_part<HALF>(r[m]), HALF ? mul2(f, scale) : f);
                             const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
-                            part_[0][to] = take_bf16(x);
+                            part_[0][to] = take_part<HALF>(x);
                             if (exact) {
-                                part_[1][to] = take_bf16(x);
-                                part_[2][to] = as_bf16(x);
+                                part_[1][to] = take_part<HALF>(x);
+                                part_[2][to] = as_part<HALF>(x);
                             } else {
-                                part_[1][to] = as_bf16(x);
+                                part_[1][to] = as_part<HALF>(x);
                             }
                         }
                     }
@@ -526,6 +615,21 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 }
                 umma::tmem_wait_st();
             }
+            auto state_pieces = [&](int g, f32x2 up) {     // 16 columns as the right operand of the next products
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f32x2 y = HALF ? mul2(s[8 * g + e + j], up) : s[8 * g + e + j];
+                        h[j] = take_part<HALF>(y);
+                        l[j] = as_part<HALF>(y);
+                    }
+                    uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 8 * half + 2 * g + e / 4);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            };
 #pragma unroll 1
             for (int t = 0; t <= chunks; ++t) {
                 const bool add = t || in, store = !STATES && t < chunks && add;
@@ -536,26 +640,38 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     wait_mma(&sh.x_done, (n - 1) & 1, tries);
                 }
                 if (add) {
+                    // what has come from memory into X is not scaled
+                    const f32x2 down = both(HALF && t ? 1.f / sh.f_scale[(n - 1) & 1] : 1.f);
+                    float top = 0.f;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         if (m_first + 16 * g >= m_end) break;
                         float x[16];
                         umma::tmem_ld16(umma::tmem_addr(tmem, w, X + m_first + 16 * g), x);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) s[8 * g + e] = fma2(s[8 * g + e], f, pack2(x[2 * e], x[2 * e + 1]));
-                        if (!store) continue;
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4) {
-                            uint32_t h[4], l[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                f32x2 y = s[8 * g + e + j];
-                                h[j] = take_bf16(y);
-                                l[j] = as_bf16(y);
+                        for (int e = 0; e < 8; ++e) {
+                            f32x2 y = pack2(x[2 * e], x[2 * e + 1]);
+                            if (HALF) y = mul2(y, down);
+                            s[8 * g + e] = fma2(s[8 * g + e], f, y);
+                            if (HALF) {
+                                float a, b;
+                                unpack2(s[8 * g + e], a, b);
+                                top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
                             }
-                            uint8_t* const to = state_hi + umma::tile_chunk_offset(128, ch, 8 * half + 2 * g + e / 4);
-                            *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4*>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                        }
+                        if (!HALF && store) state_pieces(g, both(1.f));
+                    }
+                    if (HALF && store) {
+                        top = warp_top(top);
+                        if (lane == 0) sh.s_top[warp - WARP_STATE] = top;
+                        group_sync(3);
+                        const float up = scale_to(top_of(sh.s_top), 15);
+                        group_sync(3);
+                        if (warp == WARP_STATE && lane == 0) sh.s_scale[n & 1] = up;
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            if (m_first + 16 * g >= m_end) break;
+                            state_pieces(g, both(up));
                         }
                     }
                 }
@@ -593,7 +709,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 
 static long long linear_items(const LinearCall& call) { return (long long)call.S.N * (call.S.seg ? call.S.segs : 1) * call.HV * call.kinds; }
 bool linear_tc_takes(const LinearCall& call) {
-    if (call.dtype != MKDA_BF16 || call.S.TT < 1 || linear_items(call) > 0x7fffffff) return false;
+    if (call.dtype == MKDA_F32 || call.S.TT < 1 || linear_items(call) > 0x7fffffff) return false;
     for (int i = 0; i < call.kinds; ++i) {
         const LinearKind& k = call.kind[i];
         if (k.M % 8 || k.V % 8 || (!k.states && (k.a_stride % 8 || !aligned16(k.a))) || k.b_stride % 8 || k.c_stride % 8 || !aligned16(k.b) || !aligned16(k.c)) return false;
@@ -624,10 +740,11 @@ int launch_linear_tc(const LinearCall& call, bool states, cudaStream_t stream) {
     }
     if (rc != MKDA_OK) return rc;
     plan.items = (uint32_t)linear_items(call);
-    auto* kern = states ? lt::linear_tc_kernel<true> : lt::linear_tc_kernel<false>;
+    auto* kern = call.dtype == MKDA_F16 ? states ? lt::linear_tc_kernel<true, true> : lt::linear_tc_kernel<false, true> : states ? lt::linear_tc_kernel<true, false> : lt::linear_tc_kernel<false, false>;
     rc = ensure_smem(reinterpret_cast<const void*>(kern), lt::SMEM, "linear");
     if (rc != MKDA_OK) return rc;
-    static const int regs = std::min(kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<true>)), kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<false>)));
+    static const int regs = std::min({kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<true, true>)), kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<false, true>)),
+                                      kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<true, false>)), kernel_registers(reinterpret_cast<const void*>(lt::linear_tc_kernel<false, false>))});
     if (regs < lt::LAUNCH_REGS) return set_error(MKDA_ERR_LAUNCH, "linear: built with fewer registers than its warps redistribute");
     launch(kern, dim3((unsigned)std::min<uint32_t>(plan.items, sm_count())), lt::THREADS, lt::SMEM, stream, plan, maps);
     return check_launch("linear");

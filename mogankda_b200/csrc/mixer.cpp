@@ -42,7 +42,7 @@ struct LinearCall {
     LinearCall(const Sequences& q, const variable_list& t, double scale) {
         p.S = q.s; p.HK = (int)t[LQ].size(-2); p.HV = (int)t[LV].size(-2); p.K = (int)t[LQ].size(-1); p.V = (int)t[LV].size(-1);
         p.dtype = dtype_code(t[LQ]); p.scale = (float)scale;
-        const bool tiles = t[LQ].scalar_type() == at::kBFloat16 && p.K % 8 == 0 && p.V % 8 == 0;
+        const bool tiles = t[LQ].scalar_type() != at::kFloat && p.K % 8 == 0 && p.V % 8 == 0;
         auto rows = [&](int i, const void*& ptr, long long& stride) {
             Rows r = rows_of(t[i], 2);
             // tiled copies want 16-byte boundaries and a stride that leads on: other rows are copied, so that results do not depend on where they lie
@@ -69,7 +69,7 @@ variable_list linear_backward(const Sequences& q, double scale, const variable_l
     LinearCall call(q, s, scale);
     MkdaLinearBwd p{};
     const at::Device dev = s[LQ].device();
-    cut_linear(call.p.S, q, call.p.HV, 3, 2, call.p.K, call.p.V, s[LQ].scalar_type() == at::kBFloat16);
+    cut_linear(call.p.S, q, call.p.HV, 3, 2, call.p.K, call.p.V, s[LQ].scalar_type() != at::kFloat);
     p.f = call.p;
     const Tensor dy = grads[0].defined() ? aligned(grads[0]) : at::zeros_like(s[LV], at::MemoryFormat::Contiguous);
     const Tensor dht = grads.size() > 1 && grads[1].defined() ? aligned(grads[1]) : Tensor();
@@ -145,7 +145,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             o = out_like(v, q.covers_all);
             if (want) last = new_cuda({q.s.N, HV, K, V}, at::kFloat, v.device());
             call.p.o = o.data_ptr(); call.p.ht = fmptr(last);
-            cut_linear(call.p.S, q, HV, 1, 1, K, V, v.scalar_type() == at::kBFloat16);
+            cut_linear(call.p.S, q, HV, 1, 1, K, V, v.scalar_type() != at::kFloat);
             Tensor seg_h;
             if (call.p.S.seg) {
                 seg_h = call.parts(v.device());

@@ -11,13 +11,13 @@ from tests.test_barrier_order import CSRC, Roles
 PARTS = (3, 1, 0, 2, 1)      # stretches of 128 tokens in each
 
 
-def linear_kernel(states, fp32=False):
+def linear_kernel(states, fp32=False, half=False):
     text = open(os.path.join(CSRC, "linear_tc.cu")).read()
     ring = int(re.search(r"SLOTS = (\d+)", text)[1])
     members = re.search(r"struct Shared \{(.*?)\n\};", text, re.S)[1]
     found = {n: ring if d == "SLOTS" else int(d or 1) for line in re.findall(r"uint64_t ([^;]*);", members) for n, d in re.findall(r"(\w+)(?:\[(\w+)\])?", line)}
     r = Roles(found)
-    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free", "o_staged"), 2))      # of the eight warps two, one of which may be late
+    r.count.update(dict.fromkeys(("p_ready", "f_ready", "s_ready", "o_scaled", "o_free", "o_staged", "e_ready"), 2))      # of the eight warps two, one of which may be late
     per, stretches = (2 if states else 3), [(p, t, c) for p, c in enumerate(PARTS) for t in range(c)]
     load = r.agent("load")
     for tile in range(per * len(stretches)):
@@ -63,6 +63,8 @@ def linear_kernel(states, fp32=False):
         if not states:
             wait, arrive = r.agent(f"rows {w}")
             for n in range(len(stretches)):
+                if half:
+                    wait("e_ready", n)
                 wait("p0_done", n)
                 arrive("p_ready", n)
                 wait("in_done", n)
@@ -75,6 +77,10 @@ def linear_kernel(states, fp32=False):
             wait("full", n * per + per - 1)
             if t == chunks - 1:                        # a short stretch
                 wait("full", n * per + per - 2)
+            if half and not states:                    # the largest magnitudes of all three tiles
+                wait("full", n * per + 1)
+                wait("full", n * per)
+                arrive("e_ready", n)
             for q in range(4):
                 if 4 * n + q >= found["f_free"]:
                     wait("f_free", 4 * n + q - found["f_free"])
@@ -92,6 +98,7 @@ def linear_kernel(states, fp32=False):
     return r
 
 
+@pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("states,fp32", [(False, False), (False, True), (True, False)])
-def test_waits_of_the_linear_kernel(states, fp32):
-    assert not linear_kernel(states, fp32).late_waits()
+def test_waits_of_the_linear_kernel(states, fp32, half):
+    assert not linear_kernel(states, fp32, half).late_waits()

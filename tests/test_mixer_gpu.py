@@ -3,7 +3,7 @@
 Tolerances are those of test_block_gpu.py (``near``): results in 16 bits are rounded once, half a step relative to the value; the arithmetic in front of that, and results in 32
 bits, stay below 2^-17 of the 2-norm.  For the linear attention that is: products of 16-bit inputs are exact, and sums of up to 128 of them in 32 bits; pair weights and states
 that meet another product as two 16-bit halves are off by at most 2^-16 each of the value, 2^-17.2 in the root mean square of one (uniformly distributed) and less in a sum's 2-norm
-relative to its own; what goes into the state has three parts, 2^-24.  Rotary: an angle is off by 2 pi 2^-26 = 2^-23.3 at most, a sine by 2^-22."""
+relative to its own; what goes into the state has three parts, 2^-24.  fp16 inputs: two parts of 11 bits each, of values scaled by powers of two, 2^-22.  Rotary: an angle is off by 2 pi 2^-26 = 2^-23.3 at most, a sine by 2^-22."""
 import math
 
 import pytest
@@ -139,6 +139,29 @@ def test_linear_of_any_decay():
         routs, rgrads = differentiate(lambda: linear_reference(wide["q"], wide["k"], wide["v"], d.double(), 64 ** -0.5, wide["h0"], None, True), wide, [u.double() for u in ups], list(lv))
         for n, a, b in zip(["o", "last"] + ["d" + n for n in lv], outs + grads, routs + rgrads):
             near(n, a.cpu(), b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [(-10, -10, 8), (6, 6, -6), (-4, 12, -12), (0, 0, -14), (7, -7, 4)], ids=str)
+def test_linear_of_any_size(dtype, sizes):
+    """q, k and v of very different sizes (powers of two), whose products leave fp16's range where results do not; rows of a stretch, too, differ by 2^8."""
+    gen = torch.Generator().manual_seed(17)
+    shape = (1, 300, 1, 2, 128, 128, None)
+    lv, d, ups = linear_leaves(gen, shape, torch.float32, True)
+    by = torch.exp2(torch.randint(-8, 1, (1, 300, 1, 1), generator=gen).float())
+    for n, e in zip("qkv", sizes):
+        lv[n] = (lv[n] * 2.0 ** e * (by if n != "q" else 1.0)).to(dtype)
+    lv["h0"] = lv["h0"] * 2.0 ** (sizes[1] + sizes[2])
+    ups = [ups[0].to(dtype), ups[1]]
+    mine = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+    wide = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+    scale = 2.0 ** -(sizes[0] + sizes[1] + sizes[2]) / 16 if abs(sum(sizes)) > 4 else 1 / 16
+    outs, grads = differentiate(lambda: mk.linear_attention(mine["q"], mine["k"], mine["v"], d.cuda(), scale=scale, initial_state=mine["h0"], output_final_state=True), mine, [u.cuda() for u in ups], list(lv))
+    routs, rgrads = differentiate(lambda: linear_reference(wide["q"], wide["k"], wide["v"], d.double(), scale, wide["h0"], None, True), wide, [u.double() for u in ups], list(lv))
+    for n, a, b in zip(["o", "last"] + ["d" + n for n in lv], outs + grads, routs + rgrads):
+        if dtype == torch.float16 and (b.abs().max() > 60000 or b.abs().median() < 2.0 ** -12):
+            continue                                       # not a result that fp16 holds to half a step
+        near(n, a.cpu(), b)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
