@@ -61,15 +61,26 @@ static Encode encoder(const char* what) {
     return encode;
 }
 
-// The driver's encoder wants a current context, which a thread that has called nothing of the runtime yet does not have (torch's backward threads, a new thread of the caller's)
+// The driver's encoder wants a current context, which a thread that has called nothing of the runtime yet does not have (torch's backward threads, a new thread of the caller's): it gets
+// the device's own, which the runtime holds and would make current with the first launch.
 template <typename F>
 static CUresult with_context(F encode) {
-    CUresult r = encode();
-    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
-        (void)cudaFree(nullptr);
-        r = encode();
+    const CUresult r = encode();
+    if (r != CUDA_ERROR_INVALID_CONTEXT && r != CUDA_ERROR_NOT_INITIALIZED) return r;
+    void *retain = nullptr, *make_current = nullptr, *release = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    int dev = 0;
+    CUcontext ctx = nullptr;
+    auto found = [&](const char* name, void** fn) { return cudaGetDriverEntryPoint(name, fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess && *fn; };
+    if (cudaGetDevice(&dev) != cudaSuccess || !found("cuDevicePrimaryCtxRetain", &retain) || !found("cuCtxSetCurrent", &make_current) || !found("cuDevicePrimaryCtxRelease", &release)) {
+        (void)cudaGetLastError();
+        return r;
     }
-    return r;
+    if (reinterpret_cast<CUresult (*)(CUcontext*, CUdevice)>(retain)(&ctx, dev) != CUDA_SUCCESS) return r;
+    const CUresult set = reinterpret_cast<CUresult (*)(CUcontext)>(make_current)(ctx);
+    const CUresult again = set == CUDA_SUCCESS ? encode() : r;
+    (void)reinterpret_cast<CUresult (*)(CUdevice)>(release)(dev);      // the runtime's own hold on it stays
+    return again;
 }
 
 int make_heads_map(CUtensorMap* out, const void* base, unsigned long long tokens, int heads, int dim, long long stride, const char* what, int elem_bytes) {
@@ -123,21 +134,6 @@ int kernel_registers(const void* func) {
     return a.numRegs;
 }
 
-int resident(const void* func, int threads) {
-    struct Known { const void* func; int blocks; };
-    static Known known[256];
-    static int count = 0;
-    static std::mutex mutex;
-    std::lock_guard<std::mutex> lock(mutex);
-    for (int i = 0; i < count; ++i)
-        if (known[i].func == func) return known[i].blocks;
-    int blocks = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, func, threads, 0) != cudaSuccess) (void)cudaGetLastError();
-    if (blocks < 1) blocks = 1;
-    if (count < 256) known[count++] = Known{func, blocks};
-    return blocks;
-}
-
 int ensure_smem(const void* func, int bytes, const char* what) {
     // (function, device) pairs whose limit is already raised; a launcher asks before every launch.  Launches come from several threads: callers
     // that have released the GIL, and the autograd engine's thread of each device.
@@ -174,7 +170,6 @@ extern "C" int mkda_device_status(void) {
     if (mkda::tc_recur_status(&f) == 0) any |= f;
     if (mkda::tc_intra_status(&f) == 0) any |= f;
     if (mkda::tc_bwd_chunk_status(&f) == 0) any |= f;
-    if (mkda::linear_tc_status(&f) == 0) any |= f;
     return (int)any;
 }
 extern "C" int mkda_device_status_clear(void) {
@@ -185,7 +180,6 @@ extern "C" int mkda_device_status_clear(void) {
     rc |= mkda::tc_recur_status_clear();
     rc |= mkda::tc_intra_status_clear();
     rc |= mkda::tc_bwd_chunk_status_clear();
-    rc |= mkda::linear_tc_status_clear();
     return rc;
 }
 extern "C" const char* mkda_last_error(void) { return mkda::g_err; }

@@ -14,7 +14,7 @@ int check_launch(const char* what);
 int ensure_smem(const void* func, int bytes, const char* what);
 // Registers per thread the kernel is launched with (0 if unknown): a kernel whose warps redistribute registers checks its build with it.
 int kernel_registers(const void* func);
-// Blocks of `threads` threads of a kernel without dynamic shared memory that an SM holds at once (at least 1; asked for once per kernel).
+// Blocks of `threads` threads of a kernel without dynamic shared memory that an SM holds at once (at least 1; asked for once per kernel; layer_norm.cu).
 int resident(const void* func, int threads);
 // Tensor map over a row-major [rows][row_elems] tensor of 2- or 4-byte elements whose boxes are `box_rows` (64) rows x 128 elements,
 // not swizzled: one tiled TMA copy then brings 64 strided 128-element rows (token rows of one head) into shared memory as a dense

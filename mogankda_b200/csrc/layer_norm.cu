@@ -5,6 +5,7 @@
 // mean, a second sum over what is in registers: in one pass it would lose what mean^2 is larger than it.  m and r are kept for the backward pass (8 bytes a part), which then
 // has one pair of sums to form.
 #include <algorithm>
+#include <mutex>
 
 #include "norm.cuh"
 
@@ -231,6 +232,21 @@ static int group_blocks(int rows, int groups, int most) {
 }
 template <int TPR>
 static int bwd_blocks(int rows, int groups) { return group_blocks<TPR>(rows, groups, sm_count() * (TPR == 1024 ? 1 : LN_BWD_THREADS / (TPR < 128 ? 128 : TPR))); }
+
+int resident(const void* func, int threads) {
+    struct Known { const void* func; int blocks; };
+    static Known known[256];
+    static int count = 0;
+    static std::mutex mutex;
+    std::lock_guard<std::mutex> lock(mutex);
+    for (int i = 0; i < count; ++i)
+        if (known[i].func == func) return known[i].blocks;
+    int blocks = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, func, threads, 0) != cudaSuccess) (void)cudaGetLastError();
+    if (blocks < 1) blocks = 1;
+    if (count < 256) known[count++] = Known{func, blocks};
+    return blocks;
+}
 
 }  // namespace mkda
 

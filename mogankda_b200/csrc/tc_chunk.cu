@@ -137,15 +137,15 @@ __global__ void __launch_bounds__(512, 1) out_fwd_tc_kernel(const MkdaOutFwd p) 
     tc_end(&sh, tmem, 64);
 }
 
-int tc_chunk_status(unsigned int* out) {                   // and of the step kernel
-    unsigned int step = 0;
-    if (cudaMemcpyFromSymbol(out, umma::g_timeout_flag, sizeof(unsigned int)) != cudaSuccess || step_status(&step) != 0) return -1;
-    *out |= step;
+int tc_chunk_status(unsigned int* out) {                   // and of the step kernel and the linear attention
+    unsigned int step = 0, linear = 0;
+    if (cudaMemcpyFromSymbol(out, umma::g_timeout_flag, sizeof(unsigned int)) != cudaSuccess || step_status(&step) != 0 || linear_tc_status(&linear) != 0) return -1;
+    *out |= step | linear;
     return 0;
 }
 int tc_chunk_status_clear() {
     const unsigned int z = 0;
-    return cudaMemcpyToSymbol(umma::g_timeout_flag, &z, sizeof(z)) == cudaSuccess && step_status_clear() == 0 ? 0 : -1;
+    return cudaMemcpyToSymbol(umma::g_timeout_flag, &z, sizeof(z)) == cudaSuccess && step_status_clear() == 0 && linear_tc_status_clear() == 0 ? 0 : -1;
 }
 
 template <int GDT>

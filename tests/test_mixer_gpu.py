@@ -309,6 +309,29 @@ def test_linear_from_a_new_thread():
     assert len(got) == 1 and torch.equal(got[0], want)
 
 
+def test_linear_backward_as_the_first_call_of_its_thread():
+    """In a process of its own: the thread that torch runs backward passes in has called nothing of CUDA yet."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+import mogankda_b200 as mk
+q, k, v = (torch.randn(1, 200, 2, 128, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+d, up = -torch.rand(2, device="cuda"), torch.randn_like(v)
+spare = [torch.empty_like(v) for _ in range(8)]
+del spare
+for x in (q, k, v):
+    x.requires_grad_(True)
+o, _ = mk.linear_attention(q, k, v, d)
+g = torch.autograd.grad(o, (q, k, v), up)
+assert all(torch.isfinite(x).all() for x in g) and mk.device_status() == 0
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
 def test_linear_refuses():
     q, v, d = torch.randn(1, 5, 2, 16).cuda(), torch.randn(1, 5, 4, 16).cuda(), -torch.rand(4).cuda()
     for bad in (lambda: mk.linear_attention(q, q, v[:, :, :3], d[:3]), lambda: mk.linear_attention(q, q.bfloat16(), v, d), lambda: mk.linear_attention(q, q[..., :8], v, d),
