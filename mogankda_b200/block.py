@@ -98,8 +98,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, outp
     Returns ``(o, final_state)``: o [B,T,HV,V] in the type of q; the state float32 or None.
 
     Pairs of tokens up to 128 apart are computed as products of q and k, earlier ones through the state, which is fp32 throughout.  Long sequences of few heads are cut into parts that run
-    side by side, by a rule on sizes: results on both sides of it agree to rounding.  What is not finite stays in its sequence, but reaches tokens in front of it that
-    share its 128 tokens."""
+    side by side, by a rule on sizes: results on both sides of it agree to rounding.  What is not finite stays in its sequence and reaches no
+    token in front of it (in the gradients: behind it); where the definition has an infinity, a result may be NaN."""
     table, dims = _sequences(q, cu_seqlens, 4)
     return _lib.host().linear(q, k, v, log_decay, initial_state, table, dims, scale, output_final_state)
 

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR <= 128 ? 6 : TPR ==
     leave(db, to + p.width);
 }
 
-// Threads of a part: narrow ones share a warp (heads of 128 channels by whole warps, half of them idle: forward 49 us, backward 83, where this takes 28 and 55)
+// Threads of a part: narrow ones share a warp (heads of 128 channels by whole warps, half of them idle: 262112 of 128 channels: forward 49 us, backward 83, where this takes 28 and 66)
 template <bool BWD, typename F>
 static bool with_part_width(int W, F f) {
     using std::integral_constant;

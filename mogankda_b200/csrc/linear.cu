@@ -1,6 +1,7 @@
 // Linear attention with a decay for each head (linear.cuh): the kernel for any type and size of heads, the states of cut sequences, sums over the v-heads of a group, and the
 // single-token form.
 #include <algorithm>
+#include <cfloat>
 
 #include "linear.cuh"
 
@@ -121,6 +122,17 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
                 const int i0 = OUT * group;
                 // pairs of these rows: forwards up to the last one, backwards from the first one on
                 product<OUT>(o, sp + i0 * PP, PP, sc + v, pv, k.back ? i0 & ~3 : 0, k.back ? C : (i0 + OUT + 3) & ~3);
+                float odd = 0.f;
+#pragma unroll
+                for (int r = 0; r < OUT; ++r) odd += (o[r][0] + o[r][1]) + (o[r][2] + o[r][3]);
+                if (!(fabsf(odd) <= FLT_MAX)) {            // 0 times what is not finite is not 0: once more, over the pairs that count
+#pragma unroll
+                    for (int r = 0; r < OUT; ++r) {
+                        o[r][0] = o[r][1] = o[r][2] = o[r][3] = 0.f;
+#pragma unroll 1
+                        for (int j = k.back ? i0 + r : 0; j < (k.back ? len : min(len, i0 + r + 1)); ++j) fma4(o[r], sp[(i0 + r) * PP + j], *reinterpret_cast<const float4*>(sc + j * pv + v));
+                    }
+                }
                 product<OUT>(s, sa + i0 * pm, pm, st + v, pv, 0, M4);
 #pragma unroll
                 for (int r = 0; r < OUT; ++r) {

@@ -12,7 +12,7 @@
 // the state.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
 //
 // Bound by the hand-overs between the products and, in runs that last, by 1000 W: a stretch takes 3.3 us where few SMs are busy, 4.2 (7 k cycles) where all are.  HBM alone would
-// take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 560 us, 0.68 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 258 us, where
+// take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 575 us, 0.66 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 271 us, where
 // the fp32 units (linear.cu) take 2890.
 #include <algorithm>
 
@@ -40,6 +40,9 @@ struct Shared {
     __align__(16) float pair[2 * C], factor[C], row[C + 4];
     // fp16: powers of two that f c, the pairs and the state are scaled by, of even and odd stretches, and what warps find for them
     float f_scale[2], p_scale[2], s_scale[2], f_top[8], a_top[8], b_top[8], s_top[8];
+    // of even and odd stretches: which 16 channels of c have values that are not finite (by the warp that made f c of them), and the first of them in each channel in the order of the walk
+    __align__(8) uint8_t bad[2][8];
+    __align__(16) uint8_t edge[2][C];
 };
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
@@ -146,7 +149,7 @@ __device__ __forceinline__ float top_of(const float (&tops)[8]) {
     for (int i = 1; i < 8; ++i) v = fmaxf(v, tops[i]);
     return v;
 }
-// The largest magnitude of a fp16 tile's rows [0, len), of this thread's pieces (of 256 threads)
+// The largest finite magnitude of a fp16 tile's rows [0, len), of this thread's pieces (of 256 threads)
 __device__ __forceinline__ float tile_top(const uint8_t* tile, int me, int len) {
     __half2 top = __half2half2(__ushort_as_half(0));
 #pragma unroll 2
@@ -156,7 +159,8 @@ __device__ __forceinline__ float tile_top(const uint8_t* tile, int me, int len) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t m = w[i] & 0x7fff7fffu;
-            top = __hmax2(top, *reinterpret_cast<const __half2*>(&m));
+            const __half2 v2 = *reinterpret_cast<const __half2*>(&m);
+            top = __hmax2(top, __hfma2(v2, __half2half2(__ushort_as_half(0)), v2));      // infinity becomes NaN, and NaN is no maximum
         }
     }
     const float2 f = __half22float2(top);
@@ -180,6 +184,12 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int hea
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
                  :: "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(umma::smem_u32(src)) : "memory");
 }
+// z stays 0 as long as the pairs of 16-bit values are finite
+template <bool HALF>
+__device__ __forceinline__ void note_not_finite(uint32_t& z, uint32_t v) {
+    if constexpr (HALF) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(z) : "r"(v), "r"(0u));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(z) : "r"(v), "r"(0u));
+}
 // Whether a state of 32 bits leaves: f c then has three parts, else two, as the state that only meets bf16 rows needs no more
 template <bool STATES>
 __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
@@ -201,6 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         return;
     }
     if (warp == 0) umma::tmem_alloc(&sh.tmem, 512);
+    if (tid < 2) *reinterpret_cast<unsigned long long*>(sh.bad[tid]) = 0;
     if (tid == 0) {
         for (int i = 0; i < SLOTS; ++i) { umma::mbar_init(&sh.full[i], 1); umma::mbar_init(&sh.empty[i], 1); }
         for (uint64_t* b : {&sh.p0_done, &sh.f_free[0], &sh.f_free[1], &sh.x_done, &sh.in_done, &sh.o_done}) umma::mbar_init(b, 1);
@@ -429,6 +440,21 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     }
                     signal_tmem(&sh.o_scaled, lane);
                     wait_mma(&sh.o_done, n & 1, tries);
+                    if (*reinterpret_cast<const volatile unsigned long long*>(sh.bad[n & 1])) {      // c had 0 in the place of what is not finite: the rows that it counts in are NaN
+                        const int turn = k.back ? C - 1 - i : i;
+#pragma unroll 1
+                        for (int m0 = m_first; m0 < m_end; m0 += 16) {
+                            if (!*reinterpret_cast<const volatile uint8_t*>(&sh.bad[n & 1][(m0 >> 5) + ((m0 >> 4) & 1) * 4])) continue;
+                            const uint32_t at = umma::tmem_addr(tmem, w, O + m0);
+                            float v[16];
+                            umma::tmem_ld16(at, v);
+                            uint32_t u[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) u[e] = turn >= sh.edge[n & 1][m0 + e] ? 0x7fffffffu : __float_as_uint(v[e]);
+                            umma::tmem_st16(at, u);
+                        }
+                        umma::tmem_wait_st();
+                    }
                     const float down = HALF ? 1.f / up : 1.f;
                     const size_t row = ((size_t)(part.start + c0 + i) * call.HV + it.h) * k.V;
                     if (len == C) {
@@ -493,6 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(FACTOR_REGS));
         uint32_t n = 0;
         const int me = tid - 32 * WARP_FACTORS, w = warp & 3, half = (warp - WARP_FACTORS) >> 2;
+        uint32_t marked = 0;                               // whether sh.bad has a note of this warp for even and for odd stretches
         for_items<STATES>(plan, [&](const LinearKind& k, const Item& it, const LinearPart& part, int chunks) {
             const float gamma = call.log_decay[it.h];
             const bool exact = !HALF && exact_state<STATES>(k);
@@ -548,6 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     if (!STATES && lane == 0) umma::arrive(&sh.e_ready[n & 1]);
                 }
                 const uint32_t rows = umma::smem_u32(c);
+                uint32_t odd = 0;                          // not 0: a value of this thread is not finite
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
                     const uint32_t use = 2 * n + (q >> 1);         // of this buffer
@@ -559,6 +587,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
+                            if (!STATES) note_not_finite<HALF>(odd, r[m]);
                             const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
                             f32x2 x = mul2(of_part<HALF>(r[m]), HALF ? mul2(f, scale) : f);
                             const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
@@ -572,6 +601,27 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         }
                     }
                     if (use) wait_mma(&sh.f_free[q & 1], (use - 1) & 1, tries);
+                    // The product with P would carry what is not finite to every token of the stretch: it gets 0 in its place, and the output's warps say where that counts.  They have read
+                    // the notes of two stretches ago: behind them the products freed the buffer.
+                    if (!STATES && q == 3 && __any_sync(0xffffffffu, (odd | marked) != 0)) {
+                        const bool found = __any_sync(0xffffffffu, odd != 0);
+                        uint8_t* const edge = sh.edge[n & 1] + 32 * w + 16 * half;
+                        if (lane < 16) edge[lane] = C;
+                        if (lane == 0) sh.bad[n & 1][warp - WARP_FACTORS] = found;
+                        marked = found ? marked | 1u << (n & 1) : marked & ~(1u << (n & 1));
+                        __syncwarp();
+#pragma unroll 1
+                        for (int e = lane; e < (found ? 16 * C : 0); e += 32) {      // two tokens at a time: 16 channels by half of the lanes each
+                            const int j = e >> 4, ch = 32 * w + 16 * half + (e & 15);
+                            uint16_t* const at = reinterpret_cast<uint16_t*>(c + umma::tile_chunk_offset(128, j, ch >> 3)) + (ch & 7);
+                            constexpr uint32_t TOP = HALF ? 0x7c00 : 0x7f80;
+                            int turn = (*at & TOP) == TOP ? k.back ? C - 1 - j : j : C;
+                            if (turn < C) *at = 0;
+                            turn = min(turn, __shfl_xor_sync(0xffffffffu, turn, 16));
+                            if (lane < 16 && turn < edge[lane]) edge[lane] = (uint8_t)turn;
+                        }
+                        umma::fence_async_smem();
+                    }
 #pragma unroll
                     for (int p = 0; p < 3; ++p)
                         if (p < 2 || exact) tmem_st_16x16(umma::tmem_addr(tmem, w, F + 64 * (q & 1) + 16 * p) + ((uint32_t)(16 * half) << 16), part_[p]);
@@ -656,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                             if (HALF) {
                                 float a, b;
                                 unpack2(s[8 * g + e], a, b);
-                                top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+                                top = fmaxf(top, fmaxf(fabsf(fmaf(a, 0.f, a)), fabsf(fmaf(b, 0.f, b))));      // finite ones
                             }
                         }
                         if (!HALF && store) state_pieces(g, both(1.f));

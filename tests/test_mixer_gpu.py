@@ -280,6 +280,67 @@ def test_linear_leaves_tokens_of_no_sequence_alone(dtype):
     assert all(torch.isfinite(t).all() for t in got[0]) and got[0][1][:, 90:].abs().max() == 0
 
 
+NOT_FINITE = [  # K, V, tokens, the token and the channel
+    (128, 128, 300, 200, 70), (64, 40, 128, 0, 3), (64, 64, 130, 129, 63), (17, 33, 150, 70, 16), (128, 64, 1200, 640, 5),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", NOT_FINITE, ids=str)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan], ids=str)
+def test_linear_of_what_is_not_finite(shape, dtype, bad):
+    """One element of q, k, v or the gradient from above: what it has no part in stays as it is.  Those results are compared with the ones beside a finite value; both are rounded."""
+    K, V, T, at, ch = shape
+    gen = torch.Generator().manual_seed(17)
+    lv, d, ups = linear_leaves(gen, (1, T, 2, 2, K, V, None), dtype, False)
+    up, dev = ups[0], torch.device("cuda")
+    step = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+
+    def run(name, value):
+        x = {n: t.clone() for n, t in (*lv.items(), ("up", up))}
+        x[name][0, at, 1, ch if name in ("v", "up") else ch % K] = value
+        x = {n: t.to(dev) for n, t in x.items()}
+        rows = [x[n].requires_grad_(True) for n in "qkv"]
+        o, last = mk.linear_attention(*rows, d.to(dev), output_final_state=True)
+        return dict(zip(("o", "last", "dq", "dk", "dv"), (t.detach().cpu().double() for t in (o, last, *torch.autograd.grad(o, rows, x["up"])))))
+
+    front, behind, one, other = slice(0, at), slice(at + 1, T), [t for t in range(T) if t != at], [c for c in range(V) if c != ch]
+    # result: the tokens that the element has no part in
+    clean = {"q": dict(o=one, dq=slice(0, T), dk=behind, dv=behind), "k": dict(o=front, dq=front, dk=slice(0, T), dv=one), "v": dict(o=front, dq=front, dk=one, dv=slice(0, T)),
+             "up": dict(o=slice(0, T), dq=one, dk=behind, dv=behind)}
+    hit = {"q": ("o", "dk", "dv"), "k": ("o", "dq", "dv"), "v": ("o", "dq", "dk"), "up": ("dq", "dk", "dv")}
+    for name in clean:
+        got, want = run(name, bad), run(name, 0.5)
+        for n, tokens in clean[name].items():
+            a, b = got[n][0, tokens], want[n][0, tokens]
+            assert torch.isfinite(a).all(), (name, n)
+            assert (a - b).norm() <= 2 * (ARITHMETIC + step) * b.norm(), (name, n)
+            assert torch.isfinite(got[n][0, :, 0]).all(), (name, n)          # the other head
+        for n in hit[name]:
+            assert not torch.isfinite(got[n][0, at, 1]).all(), (name, n)
+        if name == "v":          # a channel of v is one of o and of the state
+            for n in ("o", "last"):
+                assert torch.isfinite(got[n][..., other]).all() and not torch.isfinite(got[n][0, 1 if n == "last" else at, ..., ch]).all()
+                assert (got[n][..., other] - want[n][..., other]).norm() <= 2 * (ARITHMETIC + step) * want[n][..., other].norm()
+            assert not torch.isfinite(got["o"][0, at:at + 20, 1, ch]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_a_state_that_is_not_finite(dtype):
+    """A column of the state is one of the results; the others stay as they are."""
+    gen = torch.Generator().manual_seed(18)
+    lv, d, ups = linear_leaves(gen, (1, 140, 1, 1, 64, 64, None), dtype, True)
+    step = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    got, other = [], [c for c in range(64) if c != 9]
+    for value in (0.5, math.inf, math.nan):
+        lv["h0"][0, 0, 3, 9] = value
+        o, last = mk.linear_attention(*(lv[n].cuda() for n in "qkv"), d.cuda(), initial_state=lv["h0"].cuda(), output_final_state=True)
+        got.append([t.cpu().double() for t in (o, last)])
+    for case in got[1:]:
+        for a, b in zip(got[0], case):
+            assert (a[..., other] - b[..., other]).norm() <= 2 * (ARITHMETIC + step) * a[..., other].norm() and not torch.isfinite(b[..., 9]).all()
+
+
 def test_linear_does_not_depend_on_its_neighbours():
     """The same sequence in a batch, packed and by itself (short sequences: none of the calls is cut)."""
     gen = torch.Generator().manual_seed(9)
