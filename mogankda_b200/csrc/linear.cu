@@ -9,15 +9,18 @@ namespace mkda {
 
 // ---- any type, 1 to 128 channels: fp32 throughout ------------------------------------------------------------------------------------------------
 // A block carries one part of a sequence and v-head, 64 tokens at a time: their rows and the state in shared memory, every product by fused multiply-adds on tiles of registers.  Bound by
-// those, 49 thousand of them per token at 128 channels (the older tensor instructions, as compensated TF32, are no faster), and by the tiles' way out of shared memory: four rows and
-// four columns a thread.  ROWS x COLS: what the channels of b and of c are padded to for the threads' tiles, 64 or 128.
+// the tiles' way out of shared memory, four cycles for a warp's 16 bytes each, whoever shares them: with four rows and four columns a thread twice what its 49 thousand multiply-adds per
+// token at 128 channels take (the older tensor instructions, as compensated TF32, are no faster).  ROWS x COLS: what the channels of b and of c are padded to for the threads' tiles.  64 x 64
+// by 256 threads, two blocks to an SM: 4 x 1000 tokens x 8 heads forward 90 us, by 512 threads of two rows 99, 296 x 512 tokens 196 and 229.  128 channels by 512, in us 279 for 148 x 512
+// tokens; 256 threads with eight rows each have too few warps to cover the waits (319).
 namespace ls {
-constexpr int THREADS = 512, C = 64, PP = C + 4;
+constexpr int C = 64, PP = C + 4;
+__host__ __device__ constexpr int threads(int rows, int cols) { return rows + cols == 128 ? 256 : 512; }
 __host__ __device__ constexpr int pitch(int n) { return (n + 3) / 4 * 4 + 4; }
 inline int smem(int M, int V) { return 4 * (2 * C * pitch(M) + C * pitch(V) + C * PP + ((M + 3) / 4 * 4) * pitch(V) + PP); }
 
 // rows [0, len) of `n` channels from global memory, the rest of the C rows and of the pitch zero
-template <int DT>
+template <int DT, int THREADS>
 __device__ __forceinline__ void load_rows(float* to, int pit, const void* from, size_t at, long long stride, int n, int len, bool vec) {
     const int quads = pit / 4, step = THREADS / quads;     // rows at once
     const int r0 = threadIdx.x / quads, c = 4 * (threadIdx.x - r0 * quads);
@@ -60,8 +63,9 @@ __device__ __forceinline__ void product(float (&d)[R][4], const float* x, int xp
 }  // namespace ls
 
 template <int DT, int ROWS, int COLS>
-__global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linear_simt_kernel(const __grid_constant__ LinearCall call, const bool vec) {
+__global__ void __launch_bounds__(ls::threads(ROWS, COLS), ROWS + COLS == 128 ? 2 : 1) linear_simt_kernel(const __grid_constant__ LinearCall call, const bool vec) {
     using namespace ls;
+    constexpr int THREADS = threads(ROWS, COLS);
     follow_stream();
     extern __shared__ __align__(16) float smem_f[];
     const LinearKind& k = call.kind[blockIdx.z];
@@ -91,28 +95,32 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
         const int c0 = (k.back ? chunks - 1 - t : t) * C, len = min(C, w.len - c0);
         const size_t tok = w.start + c0;
         __syncthreads();
-        if (!k.states) load_rows<DT>(sa, pm, k.a, tok * k.a_stride + (size_t)(h / k.a_per) * M, k.a_stride, M, len, vec);
-        load_rows<DT>(sb, pm, k.b, tok * k.b_stride + (size_t)(h / k.b_per) * M, k.b_stride, M, len, vec);
-        load_rows<DT>(sc, pv, k.c, tok * k.c_stride + (size_t)(h / k.c_per) * V, k.c_stride, V, len, vec);
+        if (!k.states) load_rows<DT, THREADS>(sa, pm, k.a, tok * k.a_stride + (size_t)(h / k.a_per) * M, k.a_stride, M, len, vec);
+        load_rows<DT, THREADS>(sb, pm, k.b, tok * k.b_stride + (size_t)(h / k.b_per) * M, k.b_stride, M, len, vec);
+        load_rows<DT, THREADS>(sc, pv, k.c, tok * k.c_stride + (size_t)(h / k.c_per) * V, k.c_stride, V, len, vec);
         __syncthreads();
         if (!k.states) {
-            {                                              // pairs: rows i and i + 32, columns j = tid % 16 + 16 jj
+            {                                              // pairs: rows i + STEP u, columns j = tid % 16 + 16 jj
+                constexpr int STEP = THREADS / 16, PAIRS = C / STEP;
                 const int i = tid >> 4;
-                float d[2][4] = {};
+                float d[PAIRS][4] = {};
+#pragma unroll 2
                 for (int m = 0; m < M4; m += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(sa + i * pm + m), z = *reinterpret_cast<const float4*>(sa + (i + 32) * pm + m);
+                    float4 x[PAIRS];
+#pragma unroll
+                    for (int u = 0; u < PAIRS; ++u) x[u] = *reinterpret_cast<const float4*>(sa + (i + STEP * u) * pm + m);
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
                         const float4 y = *reinterpret_cast<const float4*>(sb + ((tid & 15) + 16 * jj) * pm + m);
-                        d[0][jj] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, d[0][jj]))));
-                        d[1][jj] = fmaf(z.x, y.x, fmaf(z.y, y.y, fmaf(z.z, y.z, fmaf(z.w, y.w, d[1][jj]))));
+#pragma unroll
+                        for (int u = 0; u < PAIRS; ++u) d[u][jj] = fmaf(x[u].x, y.x, fmaf(x[u].y, y.y, fmaf(x[u].z, y.z, fmaf(x[u].w, y.w, d[u][jj]))));
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < PAIRS; ++u)
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
-                        const int row = i + 32 * u, j = (tid & 15) + 16 * jj, away = k.back ? j - row : row - j;
+                        const int row = i + STEP * u, j = (tid & 15) + 16 * jj, away = k.back ? j - row : row - j;
                         sp[row * PP + j] = away >= 0 && j < len ? d[u][jj] * pw[away] * k.pair_scale : 0.f;
                     }
             }
@@ -164,10 +172,12 @@ __global__ void __launch_bounds__(ls::THREADS, ROWS + COLS == 128 ? 2 : 1) linea
                 y.x *= f; y.y *= f; y.z *= f; y.w *= f;
                 const float* x = sb + j * pm + m0;
 #pragma unroll
-                for (int r = 0; r < STATE; r += 2) {
-                    const float2 q = *reinterpret_cast<const float2*>(x + r);
+                for (int r = 0; r < STATE; r += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(x + r);
                     fma4(acc[r], q.x, y);
                     fma4(acc[r + 1], q.y, y);
+                    fma4(acc[r + 2], q.z, y);
+                    fma4(acc[r + 3], q.w, y);
                 }
             }
             const float f = pw[len];
@@ -204,12 +214,20 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
     float* at = k.parts + ((size_t)n * call.S.segs * call.HV + h) * size + e;
     float s = k.first ? k.first[((size_t)n * call.HV + h) * size + e] : 0.f;
     const float whole = decay_power(call.log_decay[h], seg), rest = decay_power(call.log_decay[h], len - (parts - 1) * seg);
-    if (k.back) {
-        at[(parts - 1) * pitch] = s;
-        for (int p = parts - 2; p >= 0; --p) at[p * pitch] = s = fmaf(p == parts - 2 ? rest : whole, s, at[p * pitch]);
-    } else {
-        at[0] = s;
-        for (int p = 1; p < parts; ++p) at[p * pitch] = s = fmaf(whole, s, at[p * pitch]);
+    // in the order of the walk; eight parts are requested before the first is written, or each would wait for memory by itself
+    const int step = k.back ? -1 : 1;
+    float* to = at + (k.back ? (parts - 1) * pitch : 0);
+    *to = s;
+    for (int p = 1; p < parts; p += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = p + i < parts ? to[(ptrdiff_t)(i + 1) * step * (ptrdiff_t)pitch] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (p + i >= parts) break;
+            to += (ptrdiff_t)step * (ptrdiff_t)pitch;
+            *to = s = fmaf(k.back && p + i == 1 ? rest : whole, s, x[i]);
+        }
     }
 }
 
@@ -319,7 +337,7 @@ static int run_linear(const LinearCall& call, const LinearCall& before, cudaStre
             constexpr int DT = decltype(dt)::value;
             auto* kern = rows > 64 ? cols > 64 ? linear_simt_kernel<DT, 128, 128> : linear_simt_kernel<DT, 128, 64> : cols > 64 ? linear_simt_kernel<DT, 64, 128> : linear_simt_kernel<DT, 64, 64>;
             rc = ensure_smem(reinterpret_cast<const void*>(kern), 227 * 1024 - 1024, "linear");
-            if (rc == MKDA_OK) launch(kern, dim3(c.HV * (S.seg ? S.segs : 1), S.N, c.kinds), ls::THREADS, bytes, stream, c, vec);
+            if (rc == MKDA_OK) launch(kern, dim3(c.HV * (S.seg ? S.segs : 1), S.N, c.kinds), ls::threads(rows > 64 ? 128 : 64, cols > 64 ? 128 : 64), bytes, stream, c, vec);
         });
         return rc != MKDA_OK ? rc : check_launch("linear");
     };
@@ -343,7 +361,7 @@ static const char* bad_linear(const MkdaLinearFwd& p) {
     if (p.K < 1 || p.K > MKDA_LINEAR_MAX_DIM || p.V < 1 || p.V > MKDA_LINEAR_MAX_DIM) return "linear: heads of 1 to 128 channels";
     if (p.dtype < MKDA_F32 || p.dtype > MKDA_F16) return "linear: unsupported dtype";
     if (p.S.N > 65535) return "linear: at most 65535 sequences";
-    if (p.S.seg < 0 || p.S.seg % 128 || (p.S.seg && (p.S.segs < 1 || !p.seg_h))) return "linear: parts of a multiple of 128 tokens, and a state for each";
+    if (p.S.seg < 0 || p.S.seg % (p.dtype == MKDA_F32 ? 64 : 128) || (p.S.seg && (p.S.segs < 1 || !p.seg_h))) return "linear: parts of a multiple of 128 tokens (fp32: 64), and a state for each";
     if (p.S.seg && (long long)p.HV * p.S.segs * 64 > 0x7fffffff) return "linear: too many parts";
     if (p.S.seg && !p.S.cu && (long long)p.S.seg * p.S.segs < p.S.T) return "linear: more tokens than the parts have";
     if (!p.log_decay) return "linear: null argument";

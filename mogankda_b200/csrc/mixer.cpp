@@ -9,27 +9,32 @@ namespace {
 enum { LQ, LK, LV, LDECAY, LH0, LINEAR_INPUTS };
 
 // Cuts long sequences into parts of `seg` tokens that run side by side, where there are too few chains (sequences x v-heads x kinds of results) for the SMs or where they fill
-// them unevenly: the cheapest of all lengths of parts, against no cut, by what a stretch of 128 tokens costs an SM in us (on the tensor cores more where all SMs draw on HBM and power than
+// them unevenly: the cheapest of all lengths of parts, against no cut, by what a stretch (128 tokens, in fp32 64) costs an SM in us (on the tensor cores more where all SMs draw on HBM and power than
 // where few do).  A cut costs two more kernels, a pass over all parts but one that finds what they make of nothing (`kinds_before` of them), and the traffic of their states.
 // In us, uncut / parts of so many stretches (what the rule takes in brackets), 128 channels: bf16 forward 32749 tokens x 32 heads 836 / 8 435 [29 378] 64 392; 8192 x 16 248 / [8 78] 16 118;
 // 4096 x 2 113 / [2 32] 8 58; 2 x 2048 x 8 57 / [2 34] 4 40; 1024 x 16 [31] / 2 30; 8 x 4096 x 32 [257] / 16 410; backward 32749 x 32 [920] / 29 1019; 8192 x 16 244 / 8 183 [22 152];
-// 4096 x 2 113 / [2 39] 8 64; 2 x 2048 x 8 [59] / 6 61; 4 x 1000 x 8 [35] / 4 82; fp32 forward 4096 x 8 1972 / [2 192] 8 668; backward 2006 / [2 543] 8 747.
-void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t heads, int kinds, int kinds_before, int64_t K, int64_t V, bool tensor_cores) {
-    if (q.longest < 512 || s.N == 0) return;
-    const int64_t longest = (q.longest + 127) / 128, most = std::max<int64_t>(longest, (s.TT + 127) / 128), n_sm = sms(), state = heads * K * V;
+// 4096 x 2 113 / [2 39] 8 64; 2 x 2048 x 8 [59] / 6 61; 4 x 1000 x 8 [35] / 4 82; fp32, parts of stretches of 64 tokens: forward 300 x 2 146 / [1 61];
+// 700 x 2 [1 62] 2 101; 4096 x 8 1972 / [4 189] 16 668; 64 channels 4 x 1000 x 8 [2 74] 4 90; 2 x 700 x 2 [1 33] 2 50; forward and backward 16384 x 4 [1331] with parts of 64 allowed, 1600 without.
+void cut_linear(MkdaSeqs& s, const Sequences& q, int64_t heads, int kinds, int kinds_before, int64_t K, int64_t V, at::ScalarType dt) {
+    const bool tensor_cores = dt != at::kFloat && K % 8 == 0 && V % 8 == 0;
+    const int64_t unit = dt == at::kFloat ? 64 : 128;      // tokens that parts are multiples of
+    if (q.longest < 4 * unit || s.N == 0) return;
+    const int64_t longest = (q.longest + unit - 1) / unit, most = std::max<int64_t>(longest, (s.TT + unit - 1) / unit), n_sm = sms(), state = heads * K * V;
     const double size = std::sqrt((double)K * V) / 128, launch = 16.0, state_us = 16.0 * K * V * kinds_before / 5e6;      // of a part and head
-    auto rounds = [&](int64_t items) { return (items + n_sm - 1) / n_sm; };
-    auto main = [&](int64_t items) { return !tensor_cores ? 60.0 * size : items > n_sm / 2 ? 4.2 : 3.4; };
-    auto before = [&](int64_t items) { return !tensor_cores ? 22.0 * size : items > n_sm / 2 ? 1.9 : 1.4; };
-    double best = std::max(longest * main(0), (double)most * heads * kinds / n_sm * main(n_sm));
-    for (int64_t parts = 2; parts <= (longest + 1) / 2; ++parts) {
+    const int64_t places = !tensor_cores && K <= 64 && V <= 64 ? 2 * n_sm : n_sm;      // narrow heads: two blocks to an SM, each half as slow again
+    auto rounds = [&](int64_t items) { return (items + places - 1) / places; };
+    auto shared = [&](int64_t items) { return places > n_sm && items > n_sm ? 1.5 : 1.0; };
+    auto main = [&](int64_t items) { return !tensor_cores ? unit / 64 * 30.0 * size * shared(items) : items > n_sm / 2 ? 4.2 : 3.4; };
+    auto before = [&](int64_t items) { return !tensor_cores ? unit / 64 * 11.0 * size * shared(items) : items > n_sm / 2 ? 1.9 : 1.4; };
+    double best = std::max(longest * main(0), (double)most * heads * kinds / places * main(places));
+    for (int64_t parts = 2; parts <= (tensor_cores ? (longest + 1) / 2 : longest); ++parts) {
         const int64_t seg = (longest + parts - 1) / parts, all = (most + seg - 1) / seg;      // parts with tokens, about
         if (s.N * parts * state * 4 > (int64_t)256 << 20) break;
         const int64_t items = all * heads * kinds, items_before = std::max<int64_t>(0, all - 1) * heads * kinds_before;
         const double us = (rounds(items) * main(items) + rounds(items_before) * before(items_before)) * seg + launch + (all + s.N) * heads * state_us + 0.002 * s.N * parts * heads;
         if (us < 0.97 * best) {
             best = us;
-            s.seg = (int)(seg * 128);
+            s.seg = (int)(seg * unit);
             s.segs = (int)((longest + seg - 1) / seg);
         }
     }
@@ -69,7 +74,7 @@ variable_list linear_backward(const Sequences& q, double scale, const variable_l
     LinearCall call(q, s, scale);
     MkdaLinearBwd p{};
     const at::Device dev = s[LQ].device();
-    cut_linear(call.p.S, q, call.p.HV, 3, 2, call.p.K, call.p.V, s[LQ].scalar_type() != at::kFloat);
+    cut_linear(call.p.S, q, call.p.HV, 3, 2, call.p.K, call.p.V, s[LQ].scalar_type());
     p.f = call.p;
     const Tensor dy = grads[0].defined() ? aligned(grads[0]) : at::zeros_like(s[LV], at::MemoryFormat::Contiguous);
     const Tensor dht = grads.size() > 1 && grads[1].defined() ? aligned(grads[1]) : Tensor();
@@ -145,7 +150,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             o = out_like(v, q.covers_all);
             if (want) last = new_cuda({q.s.N, HV, K, V}, at::kFloat, v.device());
             call.p.o = o.data_ptr(); call.p.ht = fmptr(last);
-            cut_linear(call.p.S, q, HV, 1, 1, K, V, v.scalar_type() != at::kFloat);
+            cut_linear(call.p.S, q, HV, 1, 1, K, V, v.scalar_type());
             Tensor seg_h;
             if (call.p.S.seg) {
                 seg_h = call.parts(v.device());

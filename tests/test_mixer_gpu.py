@@ -40,7 +40,7 @@ LINEAR = [  # B, T, HK, HV, K, V, cu
     (1, 100, 1, 2, 64, 64, (0, 1, 3, 3, 20, 100)), (1, 60, 2, 2, 128, 128, (0, 0, 16, 48, 50)), (1, 300, 1, 1, 128, 128, (0, 128, 256, 257, 299)), (1, 5, 1, 2, 16, 16, (0,)),
     (1, 9, 2, 2, 128, 72, (0, 0, 0, 9, 9)),
     # long sequences of few heads: cut into parts that run side by side
-    (1, 1300, 1, 1, 64, 64, None), (2, 700, 1, 2, 32, 64, None), (1, 1024, 1, 1, 128, 128, None), (1, 1500, 1, 1, 40, 128, (0, 3, 3, 1400, 1410, 1450)), (1, 900, 1, 1, 24, 24, (0, 257, 899)),
+    (1, 300, 2, 2, 128, 128, None), (1, 330, 1, 2, 17, 33, (0, 64, 64, 321, 329)), (3, 257, 1, 1, 64, 24, None), (1, 1300, 1, 1, 64, 64, None), (2, 700, 1, 2, 32, 64, None), (1, 1024, 1, 1, 128, 128, None), (1, 1500, 1, 1, 40, 128, (0, 3, 3, 1400, 1410, 1450)), (1, 900, 1, 1, 24, 24, (0, 257, 899)),
 ]
 
 
