@@ -741,3 +741,37 @@ def test_single_tokens_in_a_graph():
             graph.replay()
             want = step(keep)
             assert torch.equal(y, want) and torch.equal(state, keep)
+
+
+def test_gradients_that_arrive_broadcast_or_alone():
+    """A sum's gradient is one number for all elements; a result that nobody uses has none.  The definition's gradients are taken of the other results alone."""
+    gen = torch.Generator().manual_seed(23)
+    for dtype in (torch.float32, torch.bfloat16):
+        lv, d, ups = linear_leaves(gen, (1, 140, 1, 2, 64, 64, None), dtype, True)
+        x = {n: t.cuda().requires_grad_(True) for n, t in lv.items()}
+        for decay in (d, d.to(dtype)):
+            o, last = mk.linear_attention(x["q"], x["k"], x["v"], decay.cuda(), initial_state=x["h0"], output_final_state=True)
+            wide = torch.autograd.grad(o.float().sum() + last.sum(), list(x.values()), retain_graph=True)
+            full = torch.autograd.grad((o, last), list(x.values()), (torch.ones_like(o), torch.ones_like(last)), retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(wide, full))
+            alone = torch.autograd.grad(last, list(x.values()), ups[1].cuda())
+            r = {n: t.double().requires_grad_(True) for n, t in lv.items()}
+            _, rlast = linear_reference(r["q"], r["k"], r["v"], decay.double(), 0.125, r["h0"], None, True)
+            want = torch.autograd.grad(rlast, [r[n] for n in ("k", "v", "h0")], ups[1].double())
+            assert alone[0].abs().max() == 0
+            for n, a, b in zip(("dk", "dv", "dh0"), alone[1:], want):
+                near(n, a.cpu(), b)
+        s = rand(gen, 7, 96).to(dtype).cuda().requires_grad_(True)
+        w = rand(gen, 96).cuda().requires_grad_(True)
+        y, total = mk.layer_norm(s, w, residual=s, groups=3)
+        both = torch.autograd.grad(y.sum() + total.sum(), (s, w), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(both, torch.autograd.grad((y, total), (s, w), (torch.ones_like(y), torch.ones_like(total)), retain_graph=True)))
+        ds, dw = torch.autograd.grad(total.sum(), (s, w))          # the stream alone: 1 from each of the two that are one tensor
+        assert torch.equal(ds, torch.full_like(ds, 2)) and dw.abs().max() == 0
+        q = rand(gen, 5, 2, 16).to(dtype).cuda().requires_grad_(True)
+        args = torch.arange(5).cuda(), torch.tensor([1.0, 0.5, 0.25]).cuda()
+        a, b = mk.rotary(q, q, *args)
+        assert torch.equal(a, b)
+        both = torch.autograd.grad(a.sum() + b.sum(), q, retain_graph=True)[0]
+        one = torch.autograd.grad(a, q, torch.ones_like(a))[0]
+        assert torch.equal(both, 2 * one)
