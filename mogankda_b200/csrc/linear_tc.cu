@@ -15,6 +15,7 @@
 // take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 575 us, 0.66 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 271 us, where
 // the fp32 units (linear.cu) take 2890.
 #include <algorithm>
+#include <cfloat>
 
 #include "host.h"
 #include "linear.cuh"
@@ -38,8 +39,9 @@ struct Shared {
     uint32_t tmem;
     // of the current part's head, a copy for each group of warps that reads it: weights of the pairs by j - i + 128 (0 where a pair does not count), f, lam^n times the scale
     __align__(16) float pair[2 * C], factor[C], row[C + 4];
-    // fp16: powers of two that f c, the pairs and the state are scaled by, of even and odd stretches, and what warps find for them
-    float f_scale[2], p_scale[2], s_scale[2], f_top[8], a_top[8], b_top[8], s_top[8];
+    // fp16: powers of two that f c and the state are scaled by, of even and odd stretches, and what warps find for them and for the rows of the pairs (half of the columns each)
+    float f_scale[2], s_scale[2], f_top[8], s_top[8];
+    uint8_t p_top[2][C];                                   // as exponents
     // of even and odd stretches: which 16 channels of c have values that are not finite (by the warp that made f c of them), and the first of them in each channel in the order of the walk
     __align__(8) uint8_t bad[2][8];
     __align__(16) uint8_t edge[2][C];
@@ -133,11 +135,11 @@ __device__ __forceinline__ uint32_t take_part(f32x2& v) {
     v = fma2(of_part<HALF>(h), both(-1.f), v);
     return h;
 }
-// The power of two that brings `top` to [2^(to - 1), 2^to); 1 for 0
-__device__ __forceinline__ float scale_to(float top, int to) {
-    const int e = (int)(__float_as_uint(top) >> 23) & 255;
-    return top == 0.f ? 1.f : __uint_as_float((uint32_t)min(max(to - 1 + 254 - e, 4), 250) << 23);
-}
+// The power of two that brings a value of this exponent to [2^(to - 1), 2^to)
+__device__ __forceinline__ int exponent_of(float v) { return (int)(__float_as_uint(v) >> 23) & 255; }
+__device__ __forceinline__ float scale_of(int exponent, int to) { return __uint_as_float((uint32_t)min(max(to - 1 + 254 - exponent, 4), 250) << 23); }
+// ... `top`; 1 for 0
+__device__ __forceinline__ float scale_to(float top, int to) { return top == 0.f ? 1.f : scale_of(exponent_of(top), to); }
 __device__ __forceinline__ float warp_top(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -195,8 +197,9 @@ template <bool STATES>
 __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES || k.last; }
 
 // STATES: nothing but what the parts of cut sequences make of a zero state
-// HALF: fp16 rows.  Their products are exact as those of bf16 are, but pair weights, f c and states leave fp16's range where bf16 has fp32's: each is scaled by a power of two, found from
-// the stretch's rows and the state, that keeps it below 2^15, and two parts (22 bits, or 2^-39 of the largest) are as good as fp32.
+// HALF: fp16 rows.  Their products are exact as those of bf16 are, but pair weights, f c and states leave fp16's range where bf16 has fp32's: each is scaled by a power of two that
+// keeps it below 2^15, and its two parts are off by 2^-22 of the value or 2^-40 of the largest that shares the power of two.  That is, for pairs, of one row, found from its accumulator:
+// from the stretch's largest q and k, one large token took the bits of all others, also of those in front of it.  For f c it is the largest c of the stretch, for the state its largest value.
 template <bool STATES, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_constant__ Plan plan, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -385,47 +388,68 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 #pragma unroll 1
                 for (int t = 0; t < chunks; ++t, ++n) {
                     const int c0 = first_of(k, chunks, t), len = min(C, part.len - c0);
-                    float up = 1.f;
-                    if (HALF) {
-                        mbar_wait(&sh.e_ready[n & 1], (n >> 1) & 1, tries);
-                        up = sh.p_scale[n & 1];
-                    }
+                    float up = 1.f;                        // fp16: what this row is scaled by
                     wait_mma(&sh.p0_done, n & 1, tries);
 #pragma unroll 1
-                    for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
-                        const uint32_t at = umma::tmem_addr(tmem, w, P + j0);
-                        const int blk = j0 >> 5;
-                        if (k.back ? blk < w || j0 >= len : blk > w) {
-                            const uint32_t none[16] = {};
-                            umma::tmem_st16(at, none);
-                            continue;
-                        }
-                        float v[16];
-                        umma::tmem_ld16(at, v);
-                        const float* weight = sh.pair + C + j0 - i;
+                    for (int pass = HALF ? 0 : 1; pass < 2; ++pass) {      // the first one only looks for the largest of the row
+                        float top = 0.f;
+#pragma unroll 1
+                        for (int j0 = 64 * half; j0 < 64 * half + 64; j0 += 16) {      // 16 columns leave as 8 of hi and 8 of lo in their place
+                            const uint32_t at = umma::tmem_addr(tmem, w, P + j0);
+                            const int blk = j0 >> 5;
+                            if (k.back ? blk < w || j0 >= len : blk > w) {
+                                const uint32_t none[16] = {};
+                                if (!HALF || pass) umma::tmem_st16(at, none);
+                                continue;
+                            }
+                            float v[16];
+                            umma::tmem_ld16(at, v);
+                            const float* weight = sh.pair + C + j0 - i;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = weight[e] == 0.f ? 0.f : v[e] * weight[e];      // what does not count may not be a number
-                        if (k.back && j0 + 16 > len) {     // columns behind the part's end
+                            for (int e = 0; e < 16; ++e) v[e] = weight[e] == 0.f ? 0.f : v[e] * weight[e];      // what does not count may not be a number
+                            if (k.back && j0 + 16 > len) {     // columns behind the part's end
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (j0 + e >= len) v[e] = 0.f;
-                        }
-                        uint32_t h[8], l[8];
+                                for (int e = 0; e < 16; ++e)
+                                    if (j0 + e >= len) v[e] = 0.f;
+                            }
+                            if (HALF && !pass) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            f32x2 x = pack2(v[2 * e], v[2 * e + 1]);
-                            if (HALF) x = mul2(x, both(up));
-                            h[e] = take_part<HALF>(x);
-                            l[e] = as_part<HALF>(x);
+                                for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(fmaf(v[e], 0.f, v[e])));      // finite ones
+                                continue;
+                            }
+                            uint32_t h[8], l[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                f32x2 x = pack2(v[2 * e], v[2 * e + 1]);
+                                if (HALF) x = mul2(x, both(up));
+                                h[e] = take_part<HALF>(x);
+                                l[e] = as_part<HALF>(x);
+                            }
+                            umma::tmem_st8(at, h);
+                            umma::tmem_st8(at + 8, l);
                         }
-                        umma::tmem_st8(at, h);
-                        umma::tmem_st8(at + 8, l);
+                        if (HALF && !pass) {               // nobody writes the next stretch's in front of the products of this one, which wait for all rows
+                            const int mine = exponent_of(top);
+                            sh.p_top[half][i] = (uint8_t)mine;
+                            __syncwarp();
+                            if (lane == 0) umma::arrive(&sh.e_ready[n & 1]);
+                            mbar_wait(&sh.e_ready[n & 1], (n >> 1) & 1, tries);
+                            // 2^40 at most, which leaves the state's part of the row room in fp32: what that takes from a pair, 2^-65, is nothing beside fp16's smallest number, 2^-24
+                            up = fminf(scale_of(max(mine, (int)sh.p_top[half ^ 1][i]), 15), 0x1p40f);
+                            __syncwarp();
+                        }
                     }
                     umma::tmem_wait_st();
                     signal_tmem(&sh.p_ready, lane);
                     wait_mma(&sh.in_done, n & 1, tries);
                     if (!zero || t) {
-                        const f32x2 f = both(sh.row[k.back ? max(len - 1 - i, 0) : i + 1] * (HALF ? up / sh.s_scale[n & 1] : 1.f));
+                        float factor = sh.row[k.back ? max(len - 1 - i, 0) : i + 1];
+                        if (HALF) {
+                            factor *= 1.f / sh.s_scale[n & 1];
+                            factor *= up;
+                            if (fabsf(factor) > FLT_MAX) factor = copysignf(FLT_MAX, factor);      // 0 times infinity is not 0
+                        }
+                        const f32x2 f = both(factor);
 #pragma unroll 1
                         for (int m0 = m_first; m0 < m_end; m0 += 16) {
                             const uint32_t at = umma::tmem_addr(tmem, w, O + m0);
@@ -552,30 +576,15 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     __syncwarp();
                 }
                 f32x2 scale = both(1.f);
-                if (HALF) {                                // nothing frees these tiles in front of this stretch's first parts of f c
-                    float b_top = 0.f, a_top = 0.f;
-                    if (!STATES) {
-                        mbar_wait(&sh.full[slot_of(tb)], parity_of(tb), tries);
-                        mbar_wait(&sh.full[slot_of(tb - 1)], parity_of(tb - 1), tries);
-                        b_top = warp_top(tile_top(ring + slot_of(tb) * TILE, me, len));
-                        a_top = warp_top(tile_top(ring + slot_of(tb - 1) * TILE, me, len));
-                    }
+                if (HALF) {
                     const float c_top = warp_top(tile_top(c, me, len));
                     group_sync(2);                         // what was found for the last stretch has been read
-                    if (lane == 0) {
-                        sh.f_top[me >> 5] = c_top;
-                        sh.a_top[me >> 5] = a_top;
-                        sh.b_top[me >> 5] = b_top;
-                    }
+                    if (lane == 0) sh.f_top[me >> 5] = c_top;
                     group_sync(2);
                     const float up = scale_to(top_of(sh.f_top) * fmaxf(1.f, fabsf(k.in_scale)), 15);
                     scale = both(up);
-                    if (me == 0) {
-                        sh.f_scale[n & 1] = up;
-                        sh.p_scale[n & 1] = scale_to(top_of(sh.a_top) * top_of(sh.b_top) * (float)k.M * fabsf(k.pair_scale), 15);
-                    }
+                    if (me == 0) sh.f_scale[n & 1] = up;
                     __syncwarp();
-                    if (!STATES && lane == 0) umma::arrive(&sh.e_ready[n & 1]);
                 }
                 const uint32_t rows = umma::smem_u32(c);
                 uint32_t odd = 0;                          // not 0: a value of this thread is not finite
