@@ -226,6 +226,8 @@ inline bool with_dtype(int dtype, F f) {
         default: return false;
     }
 }
+// Parts of `seg` tokens that a sequence of `len` is cut into, one of none; len + seg may leave 32 bits
+__host__ __device__ constexpr int part_count(int len, int seg) { return len > 0 ? (len - 1) / seg + 1 : 1; }
 // tokens are counted in 32 bits, a run or a tile past the last one included
 inline bool good_sequences(const MkdaSeqs& s) { return s.N >= 0 && s.T >= 0 && s.TT >= 0 && s.TT <= MKDA_SEQS_MAX_TOKENS && (s.cu || (long long)s.N * s.T == s.TT); }
 

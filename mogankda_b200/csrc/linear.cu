@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
     const int h = blockIdx.x % call.HV, n = blockIdx.y;
     const size_t size = (size_t)k.M * k.V, e = (size_t)(blockIdx.x / call.HV) * 256 + threadIdx.x, pitch = (size_t)call.HV * size;
     const Span w = sequence(call.S, n);
-    const int len = w.end - w.start, seg = call.S.seg, parts = len > 0 ? (len + seg - 1) / seg : 1;
+    const int len = w.end - w.start, seg = call.S.seg, parts = part_count(len, seg);
     if (e >= size) return;
     float* at = k.parts + ((size_t)n * call.S.segs * call.HV + h) * size + e;
     float s = k.first ? k.first[((size_t)n * call.HV + h) * size + e] : 0.f;

@@ -41,7 +41,7 @@ __device__ __forceinline__ LinearPart linear_part(const MkdaSeqs& s, int n, int 
     const Span w = sequence(s, n);
     const int len = w.end - w.start;
     if (!s.seg) return {w.start, len, false, true, true};
-    const int parts = len > 0 ? (len + s.seg - 1) / s.seg : 1;
+    const int parts = part_count(len, s.seg);
     if (part >= parts) return {0, 0, true, false, false};
     const int at = part * s.seg;
     return {w.start + at, min(s.seg, len - at), false, false, back ? part == 0 : part == parts - 1};
