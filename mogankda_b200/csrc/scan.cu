@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(SCAN_BWD_THREADS, SCAN_BWD_BLOCKS) scan_bwd_ke
             Four G = four(a.dht && there ? ld_states(a.dht, (size_t)n * D + ch, n0, NST) : zero);      // a[t + 1] g[t + 1]
             if (there && p.S.seg) {
                 const Span all = sequence(p.S, n);
-                carry(G, A, p.S, n, max((all.end - all.start + p.S.seg - 1) / p.S.seg - 1, 0), sq.k, -1, a.seg_g, a.seg_d, D, ch, NP, n0);
+                carry(G, A, p.S, n, part_count(all.end - all.start, p.S.seg) - 1, sq.k, -1, a.seg_g, a.seg_d, D, ch, NP, n0);
             }
             float4 rh = tiles ? checkpoint(tiles - 1) : zero;
             __syncthreads();                               // the first tile is there

@@ -31,5 +31,5 @@ def test_parts_of_long_sequences(tmp_path):
 
 
 def test_no_kernel_counts_parts_by_itself():
-    for name in ("linear.cu", "linear.cuh", "linear_tc.cu"):
-        assert "seg - 1)" not in open(os.path.join(CSRC, name)).read(), name
+    for name in ("linear.cu", "linear.cuh", "linear_tc.cu", "scan.cu"):
+        assert "seg - 1) /" not in open(os.path.join(CSRC, name)).read(), name
