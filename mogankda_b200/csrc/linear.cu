@@ -2,6 +2,7 @@
 // single-token form.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "linear.cuh"
 
@@ -260,12 +261,16 @@ __global__ void __launch_bounds__(256) linear_group_kernel(const float* part, vo
 // ---- single tokens -------------------------------------------------------------------------------------------------------------------------------
 // A block per v-head and sequence: S <- lam S + k v^T where it lies, o = scale S^T q.  Eight warps share the rows of the state, a lane has four columns of each of them; all of
 // a thread's rows are requested before the first is used.  Bound by HBM: the state is read and written.
+// lam has two parts: rounded to 32 bits it is off by up to 2^-25 with one sign at every token, and a memory of a million tokens would be 5 % off.  What the second one adds is less than half
+// a step of the state: it goes in beside k v, in front of the last rounding.  An infinite state stays one: a thread that has something that is not finite leaves that part out there.
+// 64 sequences x 32 heads of 128 channels 45.3 us, 44.4 with lam in one part (with scalar arithmetic 47.2).
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) linear_step_kernel(const MkdaLinearStep p) {
     follow_stream();
-    __shared__ float sq[MKDA_LINEAR_MAX_DIM], sk[MKDA_LINEAR_MAX_DIM], part[8][MKDA_LINEAR_MAX_DIM];
+    __shared__ float sq[MKDA_LINEAR_MAX_DIM], sk[MKDA_LINEAR_MAX_DIM], part[8][MKDA_LINEAR_MAX_DIM], decay[2];
     const int h = blockIdx.x, n = blockIdx.y, K = p.K, V = p.V, g = h / (p.HV / p.HK), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, v = 4 * lane;
     float* state = p.state + ((size_t)n * p.HV + h) * K * V;
+    const float rate = p.log_decay[h];
     float4 s[16];
     auto row = [&](int i) { return warp + 8 * i; };
 #pragma unroll
@@ -288,24 +293,50 @@ __global__ void __launch_bounds__(256) linear_step_kernel(const MkdaLinearStep p
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (v + e < V) x[e] = ld1(p.v, DT, (size_t)n * p.v_stride + (size_t)h * V + v + e);
-    const float lam = expf(p.log_decay[h]);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (row(i) >= K || v >= V) continue;
-        const float kk = sk[row(i)], qq = sq[row(i)];
-        s[i].x = fmaf(lam, s[i].x, kk * x[0]); s[i].y = fmaf(lam, s[i].y, kk * x[1]); s[i].z = fmaf(lam, s[i].z, kk * x[2]); s[i].w = fmaf(lam, s[i].w, kk * x[3]);
-        o[0] = fmaf(qq, s[i].x, o[0]); o[1] = fmaf(qq, s[i].y, o[1]); o[2] = fmaf(qq, s[i].z, o[2]); o[3] = fmaf(qq, s[i].w, o[3]);
-        float* at = state + (size_t)row(i) * V + v;
-        if (VEC) {
-            *reinterpret_cast<float4*>(at) = s[i];
-        } else {
-            at[0] = s[i].x;
-            if (v + 1 < V) at[1] = s[i].y;
-            if (v + 2 < V) at[2] = s[i].z;
-            if (v + 3 < V) at[3] = s[i].w;
-        }
+    if (tid == 0) {
+        const double lam = exp((double)rate);
+        decay[0] = (float)lam;
+        decay[1] = (float)(lam - (double)decay[0]);
     }
+    f32x2 odd = both(0.f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd = fma2(pack2(s[i].z, s[i].w), both(0.f), fma2(pack2(s[i].x, s[i].y), both(0.f), odd));
+    float odd0, odd1;
+    unpack2(odd, odd0, odd1);
+    __syncthreads();
+    const float hi = decay[0], lo = decay[1];
+    auto update = [&](auto finite) {
+        const f32x2 x01 = pack2(x[0], x[1]), x23 = pack2(x[2], x[3]);
+        f32x2 o01 = both(0.f), o23 = both(0.f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (row(i) >= K || v >= V) continue;
+            const f32x2 kk = both(sk[row(i)]), qq = both(sq[row(i)]);
+            auto next = [&](float a, float b, f32x2 xs) {
+                const f32x2 ab = pack2(a, b), small = decltype(finite)::value ? ab : pack2(fabsf(a) <= FLT_MAX ? a : 0.f, fabsf(b) <= FLT_MAX ? b : 0.f);
+                return fma2(both(hi), ab, fma2(both(lo), small, mul2(kk, xs)));
+            };
+            const f32x2 s01 = next(s[i].x, s[i].y, x01), s23 = next(s[i].z, s[i].w, x23);
+            o01 = fma2(qq, s01, o01);
+            o23 = fma2(qq, s23, o23);
+            float4 r;
+            unpack2(s01, r.x, r.y);
+            unpack2(s23, r.z, r.w);
+            float* at = state + (size_t)row(i) * V + v;
+            if (VEC) {
+                *reinterpret_cast<float4*>(at) = r;
+            } else {
+                at[0] = r.x;
+                if (v + 1 < V) at[1] = r.y;
+                if (v + 2 < V) at[2] = r.z;
+                if (v + 3 < V) at[3] = r.w;
+            }
+        }
+        unpack2(o01, o[0], o[1]);
+        unpack2(o23, o[2], o[3]);
+    };
+    if (odd0 + odd1 == 0.f) update(std::true_type());
+    else update(std::false_type());
     *reinterpret_cast<float4*>(&part[warp][v]) = make_float4(o[0], o[1], o[2], o[3]);
     __syncthreads();
     if (tid < V) {

@@ -1,6 +1,7 @@
 """GPU: values of the linear attention where tokens, channels and decays differ by much, against its definition in 64 bits.
 
 Tolerances are those of test_block_gpu.py (``near``).  They hold for the tokens and channels that a large one has no part in by themselves: those are compared apart."""
+import math
 
 import pytest
 import torch
@@ -36,3 +37,58 @@ def test_one_large_token(shape, dtype, rate):
         if rate > 1:          # on its other side: exp(-3 x 30) of it, 2^-130
             far = slice(at + 31, T) if n in ("o", "dq") else slice(0, max(at - 30, 0))
             near(n, got[n][:, far].detach().cpu(), ref[n][:, far].detach())
+
+
+WEAK = [-1e-6, -3e-7, -1e-7, -1e-4, -0.03, -1.0, -20.0, 0.0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_steps_of_weak_decays(dtype):
+    """4096 single tokens of memories that reach much further.  A step rounds its state twice, half a step each: 90 of 2^-24 / sqrt(3) in the root mean square, 3.1e-6, below 2^-17;
+    a decay that is off by 2^-25 in each would be off by 1.2e-4 behind them.  That is for k v of 32 bits, whose last places make the roundings fall either way.  k v of 16-bit inputs has
+    16 bits (fp16 22) and is mostly a whole multiple of the state's last place: there is nothing but the decay's own share to round, and all 4096 roundings, 2^-24 at most each, may fall the
+    same way: 2^-12, which is 32 x 2^-17."""
+    n, K, H = 4096, 16, len(WEAK)
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (rand(gen, n, 1, H, K).to(dtype).cuda() for _ in range(3))
+    start = 64 * rand(gen, 1, H, K, K).cuda()
+    d = torch.tensor(WEAK, dtype=torch.float32).cuda()
+    state = start.clone()
+    for t in range(n):
+        o = mk.linear_attention_step(q[t], k[t], v[t], d, state)
+    left = torch.exp(d.double()[:, None] * torch.arange(n - 1, -1, -1, device="cuda"))
+    want = torch.exp(n * d.double())[:, None, None] * start[0].double() + torch.einsum("ht,thk,thv->hkv", left, k[:, 0].double(), v[:, 0].double())
+    same_way = 0 if dtype == torch.float32 else 32
+    for h in range(H):
+        near(f"state of {WEAK[h]}", state[0, h], want[h], terms=same_way * want[h].norm().item())
+    ref = K ** -0.5 * torch.einsum("hk,hkv->hv", q[-1, 0].double(), want)
+    near("o", o[0], ref, terms=same_way * (K ** -0.5 * q[-1, 0].double().norm(dim=-1) * want.flatten(1).norm(dim=-1)).norm().item())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_step_of_weak_decays(dtype):
+    """The state behind a step is lam S + k v rounded once, 2^-24 of it, but for what is rounded in front of that: k v, 2^-24 of it, and its sum with the small part of lam S, which is
+    2^-25 S at most: 2^-24 of both."""
+    gen = torch.Generator().manual_seed(6)
+    H, K = len(WEAK), 64
+    q, k, v = (rand(gen, 3, H, K).to(dtype).cuda() for _ in range(3))
+    start = 64 * rand(gen, 3, H, K, K).cuda()
+    d = torch.tensor(WEAK, dtype=torch.float32).cuda()
+    state = start.clone()
+    mk.linear_attention_step(q, k, v, d, state)
+    kv = k.double()[..., None] * v.double()[..., None, :]
+    want = torch.exp(d.double())[:, None, None] * start.double() + kv
+    assert ((state.double() - want).abs() <= 2.0 ** -24 * (want.abs() + 2 * kv.abs() + 2.0 ** -23 * start.double().abs())).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steps_of_states_that_are_not_finite(dtype):
+    """An infinity stays one where something is left of it, NaN stays NaN, and neither reaches another column."""
+    state = torch.ones(1, 3, 8, 8, device="cuda")
+    state[0, :, 2, 3], state[0, :, 4, 5] = math.inf, math.nan
+    one = torch.ones(1, 3, 8, device="cuda").to(dtype)
+    o = mk.linear_attention_step(one, one, one, torch.tensor([0.0, -1e-7, -1.0]).cuda(), state)
+    assert (state[0, :, 2, 3] == math.inf).all() and torch.isnan(state[0, :, 4, 5]).all()
+    assert (o[0, :, 3].float() == math.inf).all() and torch.isnan(o[0, :, 5]).all()
+    rest = [c for c in range(8) if c not in (3, 5)]
+    assert torch.isfinite(state[..., rest]).all() and torch.isfinite(o[..., rest]).all()
