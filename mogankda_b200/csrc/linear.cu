@@ -79,10 +79,11 @@ __global__ void __launch_bounds__(ls::threads(ROWS, COLS), ROWS + COLS == 128 ? 
     float* sc = sb + C * pm;
     float* sp = sc + C * pv;
     float* st = sp + C * PP;                               // [M4][pv]
-    float* pw = st + M4 * pv;                              // lam^0 .. lam^64
+    float* pw = st + M4 * pv;                              // lam^0 .. lam^64; what lam^64 and lam to the sequence's last tokens lack
     const int tid = threadIdx.x;
     const float gamma = call.log_decay[h];
     if (tid <= C) pw[tid] = decay_power(gamma, tid);
+    else if (tid <= C + 2) pw[tid] = decay_parts(gamma, tid == C + 1 ? C : w.len % C).lo;
     const size_t size = (size_t)M * V;
     const float* in = k.states ? nullptr : call.S.seg ? k.parts + ((size_t)(n * call.S.segs + part) * call.HV + h) * size : k.first ? k.first + ((size_t)n * call.HV + h) * size : nullptr;
     for (int e = tid; e < M4 * pv; e += THREADS) {
@@ -181,13 +182,13 @@ __global__ void __launch_bounds__(ls::threads(ROWS, COLS), ROWS + COLS == 128 ? 
                     fma4(acc[r + 3], q.w, y);
                 }
             }
-            const float f = pw[len];
+            const Decay f = {pw[len], pw[len == C ? C + 1 : C + 2]};
 #pragma unroll
             for (int r = 0; r < STATE; ++r) {
                 if (m0 + r >= M) break;
                 float4* s = reinterpret_cast<float4*>(st + (m0 + r) * pv + v);
                 float4 x = *s;
-                x.x = fmaf(f, x.x, acc[r][0]); x.y = fmaf(f, x.y, acc[r][1]); x.z = fmaf(f, x.z, acc[r][2]); x.w = fmaf(f, x.w, acc[r][3]);
+                x.x = decayed(f, x.x, acc[r][0]); x.y = decayed(f, x.y, acc[r][1]); x.z = decayed(f, x.z, acc[r][2]); x.w = decayed(f, x.w, acc[r][3]);
                 *s = x;
             }
         }
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
     if (e >= size) return;
     float* at = k.parts + ((size_t)n * call.S.segs * call.HV + h) * size + e;
     float s = k.first ? k.first[((size_t)n * call.HV + h) * size + e] : 0.f;
-    const float whole = decay_power(call.log_decay[h], seg), rest = decay_power(call.log_decay[h], len - (parts - 1) * seg);
+    const Decay whole = decay_parts(call.log_decay[h], seg), rest = decay_parts(call.log_decay[h], len - (parts - 1) * seg);
     // in the order of the walk; eight parts are requested before the first is written, or each would wait for memory by itself
     const int step = k.back ? -1 : 1;
     float* to = at + (k.back ? (parts - 1) * pitch : 0);
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
         for (int i = 0; i < 8; ++i) {
             if (p + i >= parts) break;
             to += (ptrdiff_t)step * (ptrdiff_t)pitch;
-            *to = s = fmaf(k.back && p + i == 1 ? rest : whole, s, x[i]);
+            *to = s = decayed(k.back && p + i == 1 ? rest : whole, s, x[i]);
         }
     }
 }

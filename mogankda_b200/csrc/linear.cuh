@@ -8,6 +8,8 @@
 //   backwards  out[i] = sum_{j >= i} lam^(j - i) (a[i] . b[j]) c[j] + lam^(L - 1 - i) M^T a[i]    M <- lam^L M + sum_j lam^(j + 1) b[j] c[j]^T
 // M is the state S of the caller for o, its transpose for dq, the state's gradient for dv and its transpose for dk.
 #pragma once
+#include <cfloat>
+
 #include "block.cuh"
 
 namespace mkda {
@@ -34,6 +36,15 @@ struct LinearCall {
 
 // lam^n, rounded once
 __device__ __forceinline__ float decay_power(float log_decay, long long n) { return n == 0 ? 1.f : (float)exp((double)log_decay * (double)n); }
+// ... and in two parts, for what a state is multiplied by over and over: rounded once it is off by up to 2^-25 with one sign every time (behind 131072 tokens of 128 at a time 4e-5 of the state)
+struct Decay { float hi, lo; };
+__device__ __forceinline__ Decay decay_parts(float log_decay, long long n) {
+    const double x = n == 0 ? 1.0 : exp((double)log_decay * (double)n);
+    const float hi = (float)x;
+    return {hi, (float)(x - (double)hi)};
+}
+// lam^n s + x; an infinite s stays so
+__device__ __forceinline__ float decayed(const Decay& d, float s, float x) { return fmaf(d.hi, s, fmaf(d.lo, fabsf(s) <= FLT_MAX ? s : 0.f, x)); }
 
 // What a block has to do: tokens [start, start + len) of sequence n, which are part `part` of it
 struct LinearPart { int start, len; bool nothing, enters_first, leaves_last; };

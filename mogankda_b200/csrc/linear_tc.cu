@@ -654,11 +654,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
             float* out = STATES ? k.parts + ((size_t)(it.n * call.S.segs + it.part + (k.back ? -1 : 1)) * call.HV + it.h) * size
                                 : k.last && part.leaves_last ? k.last + ((size_t)it.n * call.HV + it.h) * size : nullptr;
             const float gamma = call.log_decay[it.h];
-            float whole = 0.f, rest = 0.f;                 // lam to the tokens of a whole stretch and of the sequence's last one
+            Decay whole = {0.f, 0.f}, rest = {0.f, 0.f};   // lam to the tokens of a whole stretch and of the sequence's last one
 #pragma unroll 1
             for (int u = 0; u < 2; ++u) {
                 whole = rest;
-                rest = decay_power(gamma, u ? part.len % C : C);
+                rest = decay_parts(gamma, u ? part.len % C : C);
             }
             // the state enters and leaves through the accumulator of X, so that what touches memory is a short loop
             const size_t first = k.transposed ? (size_t)ch * k.M : ch, step = k.transposed ? 1 : k.V;
@@ -695,10 +695,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
 #pragma unroll 1
             for (int t = 0; t <= chunks; ++t) {
                 const bool add = t || in, store = !STATES && t < chunks && add;
-                f32x2 f = both(0.f);
+                f32x2 f = both(0.f), f_lo = both(0.f);
                 if (t) {
                     const bool short_one = part.len - first_of(k, chunks, t - 1) < C;
-                    f = both(short_one ? rest : whole);
+                    f = both(short_one ? rest.hi : whole.hi);
+                    f_lo = both(short_one ? rest.lo : whole.lo);
                     wait_mma(&sh.x_done, (n - 1) & 1, tries);
                 }
                 if (add) {
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                         for (int e = 0; e < 8; ++e) {
                             f32x2 y = pack2(x[2 * e], x[2 * e + 1]);
                             if (HALF) y = mul2(y, down);
-                            s[8 * g + e] = fma2(s[8 * g + e], f, y);
+                            s[8 * g + e] = fma2(s[8 * g + e], f, fma2(s[8 * g + e], f_lo, y));
                             if (HALF) {
                                 float a, b;
                                 unpack2(s[8 * g + e], a, b);

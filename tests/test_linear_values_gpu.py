@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mogankda_b200 as mk
-from tests.test_block_gpu import DTYPES, near, rand
+from tests.test_block_gpu import ARITHMETIC, DTYPES, near, rand
 from tests.test_mixer_gpu import linear_reference
 
 pytestmark = pytest.mark.gpu
@@ -79,6 +79,24 @@ def test_one_step_of_weak_decays(dtype):
     kv = k.double()[..., None] * v.double()[..., None, :]
     want = torch.exp(d.double())[:, None, None] * start.double() + kv
     assert ((state.double() - want).abs() <= 2.0 ** -24 * (want.abs() + 2 * kv.abs() + 2.0 ** -23 * start.double().abs())).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_prompts_of_weak_decays(dtype):
+    """131072 tokens of more heads than there are SMs, so that no sequence is cut, with memories that reach further than that.  A state is multiplied once for 128 tokens, 1024 times: a
+    decay rounded to 32 bits, off by up to 2^-25 with one sign for a head, would be off by 3e-5 behind them; sums of 1024 terms, rounded half a step each, are off by 32 x 2^-24."""
+    T, H, K = 131072, 160, 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn(1, T, H, K, generator=gen, device="cuda").to(dtype) for _ in range(3))
+    d = -1e-6 * torch.rand(H, generator=gen, device="cuda")
+    start = torch.randn(1, H, K, K, generator=gen, device="cuda") * 256
+    with torch.no_grad():
+        _, last = mk.linear_attention(q, k, v, d, initial_state=start, output_final_state=True)
+    at = torch.arange(T - 1, -1, -1, device="cuda")
+    for h in range(0, H, 5):
+        r = d[h].double()
+        want = torch.exp(T * r) * start[0, h].double() + (k[0, :, h].double() * torch.exp(r * at)[:, None]).t() @ v[0, :, h].double()
+        near(f"state of {d[h].item()}", last[0, h], want)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
