@@ -234,13 +234,13 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
 }
 
 // ---- shared heads --------------------------------------------------------------------------------------------------------------------------------
-// out[t][g] = sum over the `per` v-heads of group g, in order
-__global__ void __launch_bounds__(256) linear_group_kernel(const float* part, void* out, int dtype, long long rows, int per, int K) {
+// out[t][g] = sum over the `per` v-heads of group g, in order, for the tokens from the first sequence's first one (`first`, or 0 without it) on: nobody has written those in front of it
+__global__ void __launch_bounds__(256) linear_group_kernel(const float* part, void* out, int dtype, const int* first, int heads, long long rows, int per, int K) {
     follow_stream();
     const bool vec = K % 4 == 0;
     const int step = vec ? 4 : 1;
     const long long all = rows * (K / step);
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
+    for (long long e = (first ? (long long)*first * heads * (K / step) : 0) + (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
         const long long row = e / (K / step);
         const int c = (int)(e - row * (K / step)) * step;
         const float* p = part + (size_t)row * per * K + c;
@@ -464,11 +464,11 @@ extern "C" int mkda_linear_bwd(const MkdaLinearBwd* q, void* stream) {
     fs.states = bs.states = 1;
     before.kind[0] = fs; before.kind[1] = bs; before.kinds = 2;
     int rc = run_linear(call, before, (cudaStream_t)stream);
-    if (rc != MKDA_OK || !shared || q->end == 0) return rc;
+    if (rc != MKDA_OK || !shared || q->end == 0 || p.S.N == 0) return rc;
     const long long rows = (long long)q->end * p.HK;
     const unsigned blocks = (unsigned)std::min<long long>((rows * p.K + 1023) / 1024, 16ll * sm_count());
     for (int i = 0; i < 2; ++i) {
-        launch(linear_group_kernel, dim3(std::max(1u, blocks)), 256, 0, (cudaStream_t)stream, static_cast<const float*>(i ? q->part_k : q->part_q), i ? q->dk : q->dq, p.dtype, rows, p.HV / p.HK, p.K);
+        launch(linear_group_kernel, dim3(std::max(1u, blocks)), 256, 0, (cudaStream_t)stream, static_cast<const float*>(i ? q->part_k : q->part_q), i ? q->dk : q->dq, p.dtype, p.S.cu, p.HK, rows, p.HV / p.HK, p.K);
         rc = check_launch("linear groups");
         if (rc != MKDA_OK) return rc;
     }

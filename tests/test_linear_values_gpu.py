@@ -110,3 +110,34 @@ def test_steps_of_states_that_are_not_finite(dtype):
     assert (o[0, :, 3].float() == math.inf).all() and torch.isnan(o[0, :, 5]).all()
     rest = [c for c in range(8) if c not in (3, 5)]
     assert torch.isfinite(state[..., rest]).all() and torch.isfinite(o[..., rest]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sums_of_shared_heads_leave_tokens_in_front_of_the_first_sequence_alone(dtype):
+    """The C entry point takes boundaries that begin behind the first token; rows of no sequence are written by nobody."""
+    from mogankda_b200 import _lib
+    lib, S = _lib.load(), _lib.STRUCTS
+    gen = torch.Generator().manual_seed(5)
+    TT, HK, HV, K, first, end = 40, 1, 2, 16, 8, 30
+    x = {n: rand(gen, TT, h, K).to(dtype).cuda() for n, h in (("q", HK), ("k", HK), ("v", HV), ("d_o", HV))}
+    cu, d = torch.tensor([first, end], dtype=torch.int32).cuda(), torch.tensor([-0.1, -0.2]).cuda()
+    got = {n: torch.full_like(x[m], 7.0) for n, m in (("dq", "q"), ("dk", "k"), ("dv", "v"))}
+    part = {n: torch.full((TT, HV, K), 3.0).cuda() for n in ("part_q", "part_k")}
+    p = S["MkdaLinearBwd"]()
+    f = p.f
+    f.S.N, f.S.T, f.S.TT, f.S.cu = 1, TT, TT, cu.data_ptr()
+    f.HK, f.HV, f.K, f.V, f.scale, f.dtype = HK, HV, K, K, 0.25, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    f.q, f.k, f.v, f.log_decay = (t.data_ptr() for t in (x["q"], x["k"], x["v"], d))
+    f.q_stride, f.k_stride, f.v_stride = HK * K, HK * K, HV * K
+    p.d_o, p.end = x["d_o"].data_ptr(), end
+    for n, t in (*got.items(), *part.items()):
+        setattr(p, n, t.data_ptr())
+    import ctypes
+    torch.cuda.synchronize()
+    assert lib.mkda_linear_bwd(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    leaves = [x[n][None, first:end].double().cpu().requires_grad_(True) for n in "qkv"]
+    o, _ = linear_reference(*leaves, d.double().cpu(), 0.25)
+    for n, r in zip(got, torch.autograd.grad(o, leaves, x["d_o"][None, first:end].double().cpu())):
+        near(n, got[n][first:end].cpu(), r[0])
+        assert (got[n][:first] == 7).all() and (got[n][end:] == 7).all(), n
