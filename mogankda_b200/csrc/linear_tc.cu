@@ -36,15 +36,16 @@ static_assert(2 * (LAUNCH_REGS + FACTOR_REGS + STATE_REGS) + ISSUE_REGS <= 7 * L
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
     uint64_t p0_done, p_ready, f_ready[2], f_free[2], s_ready, x_done, in_done, o_scaled, o_done, o_free, o_staged[2], e_ready[2];
+    // of even and odd stretches: which 16 channels of c have values that are not finite (by the warp that made f c of them), and (edge) the first of them in each channel in the order of the walk
+    uint8_t bad[2][8];
+    // of the current part's head, a copy for each group of warps that reads it: f, weights of the pairs by j - i + 128 (0 where a pair does not count), lam^n times the scale
+    float factor[C], pair[2 * C], row[C + 1];
     uint32_t tmem;
-    // of the current part's head, a copy for each group of warps that reads it: weights of the pairs by j - i + 128 (0 where a pair does not count), f, lam^n times the scale
-    __align__(16) float pair[2 * C], factor[C], row[C + 4];
-    // fp16: powers of two that f c and the state are scaled by, of even and odd stretches, and what warps find for them and for the rows of the pairs (half of the columns each)
-    float f_scale[2], s_scale[2], f_top[8], s_top[8];
-    uint8_t p_top[2][C];                                   // as exponents
-    // of even and odd stretches: which 16 channels of c have values that are not finite (by the warp that made f c of them), and the first of them in each channel in the order of the walk
-    __align__(8) uint8_t bad[2][8];
-    __align__(16) uint8_t edge[2][C];
+    // fp16: powers of two that the state and the channels of f c are scaled by, of even and odd stretches, and the largest exponents that warps find for the state and for the rows of the
+    // pairs (of half of the columns each)
+    float s_scale[2];
+    uint8_t f_scale[2][C], s_top[8], p_top[2][C];
+    uint8_t edge[2][C];
 };
 constexpr int SMEM = 2 * TILE + SLOTS * TILE + (int)sizeof(Shared);
 static_assert(SMEM <= 232448, "shared memory of one block");
@@ -145,28 +146,11 @@ __device__ __forceinline__ float warp_top(float v) {
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-__device__ __forceinline__ float top_of(const float (&tops)[8]) {
-    float v = tops[0];
+__device__ __forceinline__ int top_of(const uint8_t (&tops)[8]) {
+    int v = tops[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v = fmaxf(v, tops[i]);
+    for (int i = 1; i < 8; ++i) v = max(v, (int)tops[i]);
     return v;
-}
-// The largest finite magnitude of a fp16 tile's rows [0, len), of this thread's pieces (of 256 threads)
-__device__ __forceinline__ float tile_top(const uint8_t* tile, int me, int len) {
-    __half2 top = __half2half2(__ushort_as_half(0));
-#pragma unroll 2
-    for (int e = me; e < len * 16; e += 256) {
-        const uint4 v = *reinterpret_cast<const uint4*>(tile + umma::tile_chunk_offset(128, e >> 4, e & 15));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t m = w[i] & 0x7fff7fffu;
-            const __half2 v2 = *reinterpret_cast<const __half2*>(&m);
-            top = __hmax2(top, __hfma2(v2, __half2half2(__ushort_as_half(0)), v2));      // infinity becomes NaN, and NaN is no maximum
-        }
-    }
-    const float2 f = __half22float2(top);
-    return fmaxf(f.x, f.y);
 }
 // Four 8 x 8 blocks of 16-bit values, transposed: lane t gets elements (2 (t % 4), t / 4) and (2 (t % 4) + 1, t / 4) of each; lane t gives the address of row t % 8 of block t / 8
 __device__ __forceinline__ void load_transposed(uint32_t addr, uint32_t (&r)[4]) {
@@ -199,7 +183,8 @@ __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES
 // STATES: nothing but what the parts of cut sequences make of a zero state
 // HALF: fp16 rows.  Their products are exact as those of bf16 are, but pair weights, f c and states leave fp16's range where bf16 has fp32's: each is scaled by a power of two that
 // keeps it below 2^15, and its two parts are off by 2^-22 of the value or 2^-40 of the largest that shares the power of two.  That is, for pairs, of one row, found from its accumulator:
-// from the stretch's largest q and k, one large token took the bits of all others, also of those in front of it.  For f c it is the largest c of the stretch, for the state its largest value.
+// from the stretch's largest q and k, one large token took the bits of all others, also of those in front of it.  For f c it is one channel, which is one of the state and of the results,
+// for the state its largest value.
 template <bool STATES, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_constant__ Plan plan, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -575,33 +560,49 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     group_sync(2);
                     __syncwarp();
                 }
-                f32x2 scale = both(1.f);
-                if (HALF) {
-                    const float c_top = warp_top(tile_top(c, me, len));
-                    group_sync(2);                         // what was found for the last stretch has been read
-                    if (lane == 0) sh.f_top[me >> 5] = c_top;
-                    group_sync(2);
-                    const float up = scale_to(top_of(sh.f_top) * fmaxf(1.f, fabsf(k.in_scale)), 15);
-                    scale = both(up);
-                    if (me == 0) sh.f_scale[n & 1] = up;
-                    __syncwarp();
-                }
                 const uint32_t rows = umma::smem_u32(c);
+                // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15), of each this lane's two tokens; and their f
+                auto fetch = [&](int j0, uint32_t (&r)[4]) {
+                    const int j = j0 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * half) / 8 + ((lane >> 3) & 1);
+                    load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
+                };
+                auto f_of = [&](int j0, int m) { return *reinterpret_cast<const f32x2*>(sh.factor + j0 + 8 * (m >> 1) + 2 * (lane & 3)); };
+                float up[2] = {1.f, 1.f};                  // fp16: what this lane's two channels are scaled by
+                if (HALF) {
+                    float top[2] = {0.f, 0.f};
+#pragma unroll 1
+                    for (int j0 = 0; j0 < C; j0 += 16) {
+                        uint32_t r[4];
+                        fetch(j0, r);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            float a, b;
+                            unpack2(mul2(of_part<HALF>(r[m]), f_of(j0, m)), a, b);
+                            top[m & 1] = fmaxf(top[m & 1], fmaxf(fabsf(fmaf(a, 0.f, a)), fabsf(fmaf(b, 0.f, b))));      // finite ones
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        top[m] = fmaxf(top[m], __shfl_xor_sync(0xffffffffu, top[m], 1));
+                        top[m] = fmaxf(top[m], __shfl_xor_sync(0xffffffffu, top[m], 2));
+                        up[m] = scale_to(top[m], 15);
+                        if ((lane & 3) == 0) sh.f_scale[n & 1][32 * w + 16 * half + 8 * m + (lane >> 2)] = (uint8_t)exponent_of(up[m]);
+                    }
+                }
                 uint32_t odd = 0;                          // not 0: a value of this thread is not finite
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
                     const uint32_t use = 2 * n + (q >> 1);         // of this buffer
                     uint32_t part_[3][8];
 #pragma unroll
-                    for (int g2 = 0; g2 < 2; ++g2) {       // 16 tokens: blocks (tokens 0..7, channels 0..7), (0..7, 8..15), (8..15, 0..7), (8..15, 8..15)
+                    for (int g2 = 0; g2 < 2; ++g2) {
                         uint32_t r[4];
-                        const int j = 32 * q + 16 * g2 + ((lane >> 4) << 3) + (lane & 7), k8 = (32 * w + 16 * half) / 8 + ((lane >> 3) & 1);
-                        load_transposed(rows + umma::tile_chunk_offset(128, j, k8), r);
+                        fetch(32 * q + 16 * g2, r);
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) {      // of this lane's two tokens in each 8
+                        for (int m = 0; m < 4; ++m) {
                             if (!STATES) note_not_finite<HALF>(odd, r[m]);
-                            const f32x2 f = *reinterpret_cast<const f32x2*>(sh.factor + 32 * q + 16 * g2 + 8 * (m >> 1) + 2 * (lane & 3));
-                            f32x2 x = mul2(of_part<HALF>(r[m]), HALF ? mul2(f, scale) : f);
+                            f32x2 x = mul2(of_part<HALF>(r[m]), f_of(32 * q + 16 * g2, m));
+                            if (HALF) x = mul2(x, both(up[m & 1]));
                             const int to = 2 * (2 * g2 + (m >> 1)) + (m & 1);
                             part_[0][to] = take_part<HALF>(x);
                             if (exact) {
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                 }
                 if (add) {
                     // what has come from memory into X is not scaled
-                    const f32x2 down = both(HALF && t ? 1.f / sh.f_scale[(n - 1) & 1] : 1.f);
+                    const f32x2 down = both(HALF && t ? __uint_as_float((254u - sh.f_scale[(n - 1) & 1][ch]) << 23) : 1.f);
                     float top = 0.f;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
@@ -726,9 +727,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tc_kernel(const __grid_cons
                     }
                     if (HALF && store) {
                         top = warp_top(top);
-                        if (lane == 0) sh.s_top[warp - WARP_STATE] = top;
+                        if (lane == 0) sh.s_top[warp - WARP_STATE] = (uint8_t)exponent_of(top);
                         group_sync(3);
-                        const float up = scale_to(top_of(sh.s_top), 15);
+                        const float up = scale_of(top_of(sh.s_top), 15);
                         group_sync(3);
                         if (warp == WARP_STATE && lane == 0) sh.s_scale[n & 1] = up;
 #pragma unroll
