@@ -97,9 +97,14 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, outp
     three types, natural logarithm, at most 0) has no gradient: a call that wants one is refused.  ``scale`` is K ** -0.5 by default; ``initial_state`` [N,HV,K,V] float32.
     Returns ``(o, final_state)``: o [B,T,HV,V] in the type of q; the state float32 or None.
 
-    Pairs of tokens up to 128 apart are computed as products of q and k, earlier ones through the state, which is fp32 throughout.  Long sequences of few heads are cut into parts that run
-    side by side, by a rule on sizes: results on both sides of it agree to rounding.  What is not finite stays in its sequence and reaches no
-    token in front of it (in the gradients: behind it); where the definition has an infinity, a result may be NaN."""
+    Pairs of tokens up to 128 apart are computed as products of q and k, earlier ones through the state, which is held in fp32.  In 16 bits the weights of pairs, and the state where it meets q,
+    go into these products as two 16-bit parts each (off by 2^-16 of the value at most in bfloat16; in float16 by 2^-22 of it, or 2^-39 of the largest of a token's pairs or of the state), and what goes into the state
+    as three (bfloat16; two where ``output_final_state`` is not asked for, so that o may differ in its last bit by that flag; float16 always two).  o is rounded once.  Long sequences of few
+    heads are cut into parts that run side by side, by a rule on sizes: results on both sides of it agree to rounding.  What is not finite stays in its sequence and reaches no
+    token in front of it (in the gradients: behind it); where the definition has an infinity, a result may be NaN.
+
+    Workspace: a cut call holds the states that its parts enter with, 4 K V bytes a part and v-head, 256 MB at most, and twice that in the backward pass; with HV > HK the backward pass holds the
+    gradients of q and k per v-head, 8 HV K bytes a token."""
     table, dims = _sequences(q, cu_seqlens, 4)
     return _lib.host().linear(q, k, v, log_decay, initial_state, table, dims, scale, output_final_state)
 

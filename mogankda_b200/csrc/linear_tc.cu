@@ -5,14 +5,15 @@
 //   P0 = a b^T                       pairs; the weights lam^|i - j| and the mask are applied to the accumulator, and P leaves as hi + lo in 16 bits, the left operand of P c
 //   O  = a M                         M: the state in front of the stretch as hi + lo in shared memory; lam^(i + 1) is applied to the accumulator's rows
 //   O += P c
-//   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts (fp16: two), so that the state, fp32 in registers, is exact to 32 bits
+//   X = (f c)^T b                    what goes into the state, f[j] = lam^(L - 1 - j); f c is split in three parts, so that the state, fp32 in registers, is exact to 32 bits; in two
+//                                  where no state leaves, and in fp16
 // a, b and c are exact as they are.  Two halves (2^-16) are enough where the result is rounded to bf16, one would show: P and M in one bf16 each are as far off as the result's own rounding.
 //
 // Roles, joined by mbarriers: a warp that fetches rows into a ring of five tiles, one that issues products, and eight warps each for the pairs' weights and the output, for f c and for
 // the state.  Every accumulator row is a lane: token i of P0 and O, channel of c of X and of the state M^T.
 //
 // Bound by the hand-overs between the products and, in runs that last, by 1000 W: a stretch takes 3.3 us where few SMs are busy, 4.2 (7 k cycles) where all are.  HBM alone would
-// take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 575 us, 0.66 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 271 us, where
+// take 2.9 (128 KB), the products 7 or 8 x 516 cycles, the warps' arithmetic less.  16384 tokens x 148 heads 587 us, 0.64 of HBM; fp16 4 x 2048 x 16 heads with the backward pass 271 us, where
 // the fp32 units (linear.cu) take 2890.
 #include <algorithm>
 #include <cfloat>
@@ -182,7 +183,7 @@ __device__ __forceinline__ bool exact_state(const LinearKind& k) { return STATES
 
 // STATES: nothing but what the parts of cut sequences make of a zero state
 // HALF: fp16 rows.  Their products are exact as those of bf16 are, but pair weights, f c and states leave fp16's range where bf16 has fp32's: each is scaled by a power of two that
-// keeps it below 2^15, and its two parts are off by 2^-22 of the value or 2^-40 of the largest that shares the power of two.  That is, for pairs, of one row, found from its accumulator:
+// keeps it below 2^15, and its two parts are off by 2^-22 of the value or 2^-39 of the largest that shares the power of two.  That is, for pairs, of one row, found from its accumulator:
 // from the stretch's largest q and k, one large token took the bits of all others, also of those in front of it.  For f c it is one channel, which is one of the state and of the results,
 // for the state its largest value.
 template <bool STATES, bool HALF>

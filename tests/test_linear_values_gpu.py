@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mogankda_b200 as mk
-from tests.test_block_gpu import DTYPES, near, rand
+from tests.test_block_gpu import ARITHMETIC, DTYPES, near, rand
 from tests.test_mixer_gpu import linear_reference
 
 pytestmark = pytest.mark.gpu
@@ -56,6 +56,18 @@ def test_one_large_channel(shape, dtype):
         near("last", last[..., c].cpu(), rlast[..., c])
         if dtype != torch.float16 or c == 5:      # the others' results are too small for fp16
             near("o", o[..., c].cpu(), ro[..., c])
+
+
+def test_the_final_state_leaves_results_as_exact():
+    """What goes into a state has three parts where one leaves, else two (2^-16 off at most, 2^-17 in the root mean square): both calls' results round the same number but for that, and
+    those that come out as neighbours, 2^-8 apart at least, are as many as 4 x 2^-17 / 2^-8 of them, four times over for the small ones among them."""
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (rand(gen, 1, 3000, 4, 128).bfloat16().cuda() for _ in range(3))
+    d = -torch.tensor([1e-3, 1e-2, 0.1, 1.0]).cuda()
+    with torch.no_grad():
+        a, b = mk.linear_attention(q, k, v, d)[0].double(), mk.linear_attention(q, k, v, d, output_final_state=True)[0].double()
+    assert (a - b).norm() <= 2 * (ARITHMETIC + 2.0 ** -8) * a.norm()
+    assert (a != b).double().mean() <= 4 * 4 * ARITHMETIC / 2.0 ** -8
 
 
 WEAK = [-1e-6, -3e-7, -1e-7, -1e-4, -0.03, -1.0, -20.0, 0.0]
