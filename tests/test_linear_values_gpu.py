@@ -70,6 +70,27 @@ def test_the_final_state_leaves_results_as_exact():
     assert (a != b).double().mean() <= 4 * 4 * ARITHMETIC / 2.0 ** -8
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_later_tokens_leave_no_trace(dtype):
+    """Not a bit of a result depends on tokens behind it (of a gradient of k or v: in front of it), however large these are, in a call that is not cut."""
+    gen = torch.Generator().manual_seed(7)
+    x = {n: rand(gen, 1, 300, 2, 64).to(dtype) for n in ("q", "k", "v", "up")}
+    d = torch.tensor([-0.01, -0.3]).cuda()
+    got = []
+    for size in (1.0, 30000.0):
+        for side in (slice(171, 300), slice(0, 171)):
+            y = {n: t.clone() for n, t in x.items()}
+            for t in y.values():
+                t[:, side] *= size / 5
+            leaves = [y[n].cuda().requires_grad_(True) for n in "qkv"]
+            o, _ = mk.linear_attention(*leaves, d)
+            g = torch.autograd.grad(o, leaves, y["up"].cuda())
+            other = slice(0, 171) if side.start else slice(171, 300)
+            got.append([t[:, other] for t in ((o, g[0]) if side.start else g[1:])])
+    for a, b in ((got[0], got[2]), (got[1], got[3])):
+        assert all(torch.isfinite(s).all() and torch.equal(s, t) for s, t in zip(a, b))
+
+
 WEAK = [-1e-6, -3e-7, -1e-7, -1e-4, -0.03, -1.0, -20.0, 0.0]
 
 
