@@ -152,7 +152,8 @@ int mkda_norm_bwd_part_rows(int rows, int width);
 
 /* Linear attention with a decay for each head: S[t] = exp(log_decay[h]) S[t - 1] + k[t] v[t]^T, o[t] = scale S[t]^T q[t].  HK heads of q and k [HK,K] and HV of v
  * [HV,V] per token, HV a multiple of HK: v-head h reads head h / (HV / HK) of q and k.  1 <= K, V <= MKDA_LINEAR_MAX_DIM.  Strides are between tokens; the heads of a
- * token lie one behind the other.  S.seg: sequences are cut into parts of so many tokens (a multiple of 128, fp32 64) that run side by side, S.segs of them in the longest. */
+ * token lie one behind the other.  S.seg: sequences are cut into parts of so many tokens (a multiple of 128, fp32 64) that run side by side, S.segs of them in the longest.
+ * Rows of no sequence are left as they are. */
 typedef struct {
     MkdaSeqs S; int HK; int HV; int K; int V; int dtype; float scale;
     const void* q; const void* k; const void* v;
