@@ -12,7 +12,7 @@ namespace mkda {
 // A block carries one part of a sequence and v-head, 64 tokens at a time: their rows and the state in shared memory, every product by fused multiply-adds on tiles of registers.  Bound by
 // the tiles' way out of shared memory, four cycles for a warp's 16 bytes each, whoever shares them: with four rows and four columns a thread twice what its 49 thousand multiply-adds per
 // token at 128 channels take (the older tensor instructions, as compensated TF32, are no faster).  ROWS x COLS: what the channels of b and of c are padded to for the threads' tiles.  64 x 64
-// by 256 threads, two blocks to an SM: 4 x 1000 tokens x 8 heads forward 90 us, by 512 threads of two rows 99, 296 x 512 tokens 196 and 229.  128 channels by 512, in us 279 for 148 x 512
+// by 256 threads, two blocks to an SM: 4 x 1000 tokens x 8 heads forward 90 us, by 512 threads of two rows 99, 296 x 512 tokens 196 and 229 (201 since decays of states have two parts).  128 channels by 512, in us 279 for 148 x 512
 // tokens; 256 threads with eight rows each have too few warps to cover the waits (319).
 namespace ls {
 constexpr int C = 64, PP = C + 4;
